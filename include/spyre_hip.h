@@ -367,6 +367,107 @@ int spyre_sdpa_fwd_own_f16(const void* q, const int64_t* q_strides, const void* 
                            size_t workspace_bytes, int B, int Hq, int Hkv, int Sq, int Skv, int D,
                            void* stream);
 
+/* ------------------------- rotary positions, 8-bit cache, drafted tokens -- */
+
+/* Rotates the positions into q and k: with theta = positions[b, s] *
+ * frequencies[i] (radians), c = amplitude cos(theta), s = amplitude
+ * sin(theta), every head's pair i < pairs becomes
+ *   (x1 c - x2 s, x2 c + x1 s),  (x1, x2) the features (i, i + pairs) or,
+ * interleaved, (2 i, 2 i + 1); features from 2 pairs on are copied.  inverse:
+ * s -> -s, which is also the gradient.  theta is formed and reduced in 64
+ * bits, the rotation in 32, each result rounded once.
+ *   q, q_out : [B, Hq, S, D], feature stride 1, strides {b, h, s} (elements);
+ *              k, k_out likewise with Hkv heads (either may have 0 heads)
+ *   scalar_type : SPYRE_DT_FLOAT16, _BFLOAT16 or _FLOAT32
+ *   positions : int32 or int64 (position_bytes 4 / 8), strides pos_sb, pos_ss
+ *   frequencies : float64 [pairs], pairs <= 512
+ * Any strides and alignment; multiples of 8 elements, 16-byte aligned
+ * pointers and pairs and D - 2 pairs multiples of 8 move as vectors.  No
+ * reference counterpart. */
+int spyre_rotary(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides,
+                 int Hq, const void* k, const int64_t* k_strides, void* k_out,
+                 const int64_t* k_out_strides, int Hkv, int scalar_type, const void* positions,
+                 int position_bytes, int64_t pos_sb, int64_t pos_ss, const double* frequencies,
+                 int pairs, float amplitude, int interleaved, int inverse, int B, int S, int D,
+                 void* stream);
+
+/* What a paged cache holds. */
+#define SPYRE_CACHE_F16 0  /* fp16 pages, as spyre_kv_append_f16 writes them */
+#define SPYRE_CODES_E4M3 1 /* 8-bit codes: OCP e4m3                          */
+#define SPYRE_CODES_INT8 2 /* 8-bit codes: two's complement, -127 .. 127     */
+
+/* Quantises new K and V rows into the 8-bit paged cache.  A row x (token,
+ * KV head) of D features becomes
+ *   scale = amax / TOP,  code = rne(x TOP / amax),  amax = max |x|,
+ * TOP 448 (e4m3) or 127 (int8), in fp32; it reads back as code * scale.  Rows
+ * whose amax is below 2^-100 get zeros and scale 1; a row that holds a NaN or
+ * an infinity reads back as NaN.
+ *   k_new, v_new : [B, T, Hkv, D] fp16, feature stride 1, strides {b, t, h}
+ *                  multiples of 8 elements, 16-byte aligned
+ *   k_cache : [num_pages, Hkv, D/16, 64, 16] codes (units of 16 features)
+ *   v_cache : [num_pages, Hkv, 4, D, 16]     codes (units of 16 tokens)
+ *   k_scale, v_scale : fp32 [num_pages, Hkv, 64]
+ *   slots   : int32 [B, T] (strides slot_sb, slot_st): token (b, t) goes to
+ *             page block_table[b, slots / 64], slot % 64.  Negative ones are
+ *             skipped; those past the table's pages_per_seq and pages outside
+ *             [0, num_pages) are dropped.  Two tokens of a call must not
+ *             share a slot (its codes are then a mix of both).
+ * pairs > 0: K is rotated first, as spyre_rotary does with positions [B, T],
+ * without a rounding between, and the q heads (Hq, 0 for none) are rotated
+ * into q_out [B, T, Hq, D] (contiguous fp16).  pairs is a multiple of 8.
+ * D in {64, 128}.  No reference counterpart. */
+int spyre_kv_quant_append(const void* q, const int64_t* q_strides, void* q_out, int Hq,
+                          const void* k_new, const int64_t* k_strides, const void* v_new,
+                          const int64_t* v_strides, void* k_cache, void* v_cache, float* k_scale,
+                          float* v_scale, int codes, const int32_t* block_table, int64_t bt_stride,
+                          int64_t pages_per_seq, const int32_t* slots, int64_t slot_sb,
+                          int64_t slot_st, const void* positions, int position_bytes,
+                          int64_t pos_sb, int64_t pos_st, const double* frequencies, int pairs,
+                          float amplitude, int interleaved, int B, int T, int Hkv, int D,
+                          int page_size, int64_t num_pages, void* stream);
+
+/* Reads tokens of the 8-bit cache back: row i of k, v [B, Hkv, L, D]
+ * (contiguous fp16) is token start[b] + i (start NULL: 0) while that is below
+ * lens[b], else zeros.  Tokens of a page that the table does not name validly
+ * are NaN.  No reference counterpart. */
+int spyre_kv_quant_read(const void* k_cache, const void* v_cache, const float* k_scale,
+                        const float* v_scale, int codes, const int32_t* block_table,
+                        int64_t bt_stride, int64_t pages_per_seq, const int32_t* lens,
+                        const int32_t* start, void* k, void* v, int B, int Hkv, int L, int D,
+                        int page_size, int64_t num_pages, void* stream);
+
+/* Attention of T drafted tokens a sequence over the paged cache that holds
+ * them behind its context.  Sequence b has ctx = context_lens[b] cached tokens
+ * and n = draft_lens[b] (NULL: T) drafted ones at positions ctx .. ctx + n - 1;
+ * query (i, h), i < n, attends the tokens t < ctx and the drafted j < n with
+ * mask[b, i, j] (NULL mask: j <= i):
+ *   out = softmax(scale q . K^T) V,  lse the natural logarithm of its sum
+ * Rows that attend nothing and rows i >= n are zeros with lse -inf; what a
+ * row does not attend never reaches it, whatever it holds.  draft_keys 0: no
+ * drafted keys, every query attends its ctx tokens (T = 1: a decode step).
+ *   q     : [B, T, Hq, D] fp16, feature stride 1, strides {b, t, h} multiples
+ *           of 8 elements, 16-byte aligned
+ *   cache : SPYRE_CACHE_F16 pages as spyre_paged_decode_attn_f16 reads them
+ *           (scales NULL), or codes and scales as spyre_kv_quant_append writes
+ *   mask  : bool [B, T, T], strides {b, i, j} in bytes, 0 to broadcast
+ *   out   : [B, T, Hq, D] fp16, lse: optional fp32 [B, T, Hq]; contiguous
+ * A context above max_context_len and a page that the table does not name
+ * validly make the sequence's rows NaN.  The workspace holds
+ * spyre_paged_tree_attn_workspace_bytes (asked of the current device; may be
+ * 0), 16-byte aligned, without initialisation; two calls in flight need two.
+ * D in {64, 128}, page_size 64.  No reference counterpart. */
+size_t spyre_paged_tree_attn_workspace_bytes(int cache_kind, int B, int T, int Hq, int Hkv, int D,
+                                             int max_context_len, int draft_keys);
+int spyre_paged_tree_attn(const void* q, const int64_t* q_strides, const void* k_cache,
+                          const void* v_cache, const float* k_scale, const float* v_scale,
+                          int cache_kind, const int32_t* block_table, int64_t bt_stride,
+                          int64_t pages_per_seq, const int32_t* context_lens,
+                          const int32_t* draft_lens, int draft_keys, const void* mask,
+                          const int64_t* mask_strides, void* out, float* lse, void* workspace,
+                          size_t workspace_bytes, int B, int T, int Hq, int Hkv, int D,
+                          int page_size, int64_t num_pages, int max_context_len, float scale,
+                          void* stream);
+
 #ifdef __cplusplus
 }
 #endif

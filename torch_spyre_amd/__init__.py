@@ -1,4 +1,5 @@
-"""MI355X (gfx950) stick relayout and paged split-KV decode attention.
+"""MI355X (gfx950) stick relayout and paged split-KV decode attention,
+with rotary positions, an 8-bit cache and attention of drafted tokens.
 
 A drop-in for torch-spyre's relayout / restickify / overwrite / decode-SDPA
 path: the SpyreTensorLayout descriptor, the host<->device DMA descriptors and
@@ -51,10 +52,18 @@ from .attention import (  # noqa: E402
     paged_decode_attention,
     paged_decode_merge,
     paged_decode_split,
+    paged_tree_attention,
     sdpa_decode,
     v_page_layout,
     workspace_bytes,
 )
+from .quantized import (  # noqa: E402
+    QuantizedKVCache,
+    kv_append_quantized,
+    kv_read_quantized,
+    rotary_kv_append_quantized,
+)
+from .rotary import rotary_embedding, rotary_frequencies  # noqa: E402
 from .sdpa import (  # noqa: E402
     SdpaCall,
     Unsupported,
@@ -75,6 +84,8 @@ __all__ = [
     "as_strided_with_layout", "reinterpret_tensor", "reinterpret_tensor_with_layout",
     "PagedDecode", "PagedKVCache", "dense_to_pages", "k_page_layout", "kv_append", "paged_decode_attention",
     "paged_decode_merge", "paged_decode_split",
-    "sdpa_decode", "v_page_layout", "workspace_bytes",
+    "paged_tree_attention", "sdpa_decode", "v_page_layout", "workspace_bytes",
+    "QuantizedKVCache", "kv_append_quantized", "kv_read_quantized", "rotary_kv_append_quantized",
+    "rotary_embedding", "rotary_frequencies",
     "SdpaCall", "Unsupported", "scaled_dot_product_attention", "sdpa_override", "sdpa_overrideable",
 ]

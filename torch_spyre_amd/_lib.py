@@ -112,6 +112,22 @@ SIGNATURES = {
                                    POINTER(c_int64), c_void_p, c_int, POINTER(c_int64), c_int, c_float,
                                    c_void_p, c_void_p, c_void_p, c_size_t, c_int, c_int, c_int, c_int,
                                    c_int, c_int, c_void_p]),
+    "spyre_rotary": (c_int, [c_void_p, POINTER(c_int64), c_void_p, POINTER(c_int64), c_int] * 2
+                     + [c_int, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int, c_float, c_int, c_int, c_int,
+                        c_int, c_int, c_void_p]),
+    "spyre_kv_quant_append": (c_int, [c_void_p, POINTER(c_int64), c_void_p, c_int, c_void_p, POINTER(c_int64),
+                                      c_void_p, POINTER(c_int64), c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                      c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int,
+                                      c_int64, c_int64, c_void_p, c_int, c_float, c_int, c_int, c_int, c_int,
+                                      c_int, c_int, c_int64, c_void_p]),
+    "spyre_kv_quant_read": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64,
+                                    c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                                    c_int64, c_void_p]),
+    "spyre_paged_tree_attn_workspace_bytes": (c_size_t, [c_int] * 8),
+    "spyre_paged_tree_attn": (c_int, [c_void_p, POINTER(c_int64), c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                      c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p,
+                                      POINTER(c_int64), c_void_p, c_void_p, c_void_p, c_size_t, c_int, c_int,
+                                      c_int, c_int, c_int, c_int, c_int64, c_int, c_float, c_void_p]),
 }
 
 _lib = None

@@ -178,15 +178,32 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
                            scale: Optional[float] = None, split_tokens: int = 512,
                            max_context_len: Optional[int] = None,
                            workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
-                           return_lse: bool = False):
+                           return_lse: bool = False, k_scale: Optional[torch.Tensor] = None,
+                           v_scale: Optional[torch.Tensor] = None):
     """out[b, h] = softmax(scale * q[b, h] . K[b, h // g]^T) V[b, h // g] over
     the first context_lens[b] tokens of sequence b's pages.
+
+    With ``k_scale`` and ``v_scale`` the caches are 8-bit ones
+    (QuantizedKVCache); ``split_tokens``, ``workspace`` and ``out`` are the
+    fp16 cache's alone.
 
     q [B, Hq, D] fp16; caches as PagedKVCache; block_table int32 [B, W];
     context_lens int32 [B].  ``max_context_len`` bounds every context (if
     omitted it is read from context_lens, which synchronises).  One kernel
     when max_context_len <= CHUNK_WAVES * split_tokens, else the split pass
     then the merge pass."""
+    if k_scale is not None or v_scale is not None:
+        if workspace is not None or out is not None:
+            raise ValueError("8-bit caches take no workspace= and no out=")
+        if k_scale is None or v_scale is None:
+            raise ValueError("k_scale and v_scale go together")
+        try:
+            o, lse = torch.ops.spyre.quant_paged_decode_attention.default(
+                q, k_cache, v_cache, k_scale, v_scale, block_table, context_lens,
+                None if scale is None else float(scale), -1 if max_context_len is None else int(max_context_len))
+        except RuntimeError as e:
+            raise _lib.library_error(e) from None
+        return (o, lse) if return_lse else o
     if workspace is None and out is None:  # the C++ kernel of spyre::paged_decode_attention
         if scale is None:
             scale = 1.0 / math.sqrt(q.shape[-1])
@@ -211,6 +228,35 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         a.D, PAGE, a.num_pages, a.max_ctx, a.split, a.scale, a.stream)
     _lib.check("spyre_paged_decode_attn_f16", rc)
     return (out, lse) if return_lse else out
+
+
+def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                         context_lens: torch.Tensor, tree_mask: Optional[torch.Tensor] = None,
+                         draft_lens: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                         max_context_len: Optional[int] = None, return_lse: bool = False,
+                         k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
+    """Attention of drafted tokens over the paged cache that holds them behind
+    their context: sequence b's cache has context_lens[b] tokens (int32 [B]) and
+    then draft_lens[b] (int32 [B], default T) drafted ones, appended by the
+    caller at positions context_lens[b] + j.  Query i of q [B, T, Hq, D]
+    (float16) attends the context and the drafted tokens j with tree_mask[b, i,
+    j] (bool [B, T, T] or [T, T]: a tree gives each token its ancestors and
+    itself); without a mask j <= i, one line of tokens.
+
+    fp16 caches as PagedKVCache, or 8-bit ones with ``k_scale`` and ``v_scale``
+    (QuantizedKVCache).  Returns out [B, T, Hq, D] and, with ``return_lse``, the
+    fp32 logsumexp [B, T, Hq].  Rows i >= draft_lens[b], and rows that attend
+    nothing, are zeros with logsumexp -inf; what a row does not attend does not
+    reach it, even if it is NaN.  ``max_context_len`` bounds context_lens (if
+    omitted it is read from them, which synchronises); longer contexts, and
+    pages that the block table does not name validly, make the sequence NaN."""
+    try:
+        o, lse = torch.ops.spyre.paged_tree_attention.default(
+            q, k_cache, v_cache, block_table, context_lens, tree_mask, draft_lens, k_scale, v_scale,
+            None if scale is None else float(scale), -1 if max_context_len is None else int(max_context_len))
+    except RuntimeError as e:
+        raise _lib.library_error(e) from None
+    return (o, lse) if return_lse else o
 
 
 class PagedDecode:

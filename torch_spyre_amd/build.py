@@ -6,8 +6,8 @@
 
 Objects go to torch_spyre_amd/_build/ (compiled in parallel), the shared
 library to torch_spyre_amd/libspyre_hip.so, and the PyTorch kernels of the
-attention and KV ops (csrc/torch_ops.cpp, against torch's headers, calling
-that library) to torch_spyre_amd/libspyre_torch.so.
+attention, KV, rotary and draft ops (csrc/torch_ops.cpp and
+csrc/serving_ops.cpp, against torch's headers, calling that library) to torch_spyre_amd/libspyre_torch.so.
 """
 
 from __future__ import annotations
@@ -22,8 +22,9 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 OUT = os.path.join(HERE, "libspyre_hip.so")
 TORCH_OUT = os.path.join(HERE, "libspyre_torch.so")
-SOURCES = ["layout.cpp", "dma.hip", "decode_attn.hip", "kv_append.hip", "sdpa_fwd.hip"]
-TORCH_SOURCE = "torch_ops.cpp"
+SOURCES = ["layout.cpp", "dma.hip", "decode_attn.hip", "kv_append.hip", "sdpa_fwd.hip", "rotary.hip",
+           "kv_quant.hip", "tree_attn.hip"]
+TORCH_SOURCES = ["torch_ops.cpp", "serving_ops.cpp"]
 ARCH = os.environ.get("SPYRE_OFFLOAD_ARCH", "gfx950")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -46,7 +47,7 @@ def _compile(src: str, build_dir: str = BUILD, defines=()) -> str:
     path = os.path.join(CSRC, src)
     if src.endswith(".hip"):
         cmd = [HIPCC, *COMMON, *DEVICE, *[f"-D{d}" for d in defines], "-c", path, "-o", obj]
-    elif src == TORCH_SOURCE:
+    elif src in TORCH_SOURCES:
         import torch
 
         incs, _ = _torch_dirs()
@@ -67,10 +68,11 @@ def build(verbose: bool = False, out: str = OUT, build_dir: str = BUILD, defines
     macros for the device sources (kernel variants)."""
     os.makedirs(build_dir, exist_ok=True)
     with_torch = out == OUT
-    srcs = SOURCES + ([TORCH_SOURCE] if with_torch else [])
+    srcs = SOURCES + (TORCH_SOURCES if with_torch else [])
     with ThreadPoolExecutor(max_workers=min(len(srcs), os.cpu_count() or 1)) as ex:
         objs = list(ex.map(lambda f: _compile(f, build_dir, defines), srcs))
-    torch_obj = objs.pop() if with_torch else None
+    torch_objs = objs[len(SOURCES):]
+    objs = objs[:len(SOURCES)]
     tmp = out + ".tmp"
     # --no-undefined: a kernel whose host stub was not emitted fails here,
     # not at the first dlopen.
@@ -86,7 +88,7 @@ def build(verbose: bool = False, out: str = OUT, build_dir: str = BUILD, defines
         # beside them at run time) and torch's own libraries
         _, tlib = _torch_dirs()
         tmp = TORCH_OUT + ".tmp"
-        cmd = [HIPCC, "-shared", "-Wl,--no-undefined", torch_obj, f"-L{HERE}", "-lspyre_hip", f"-L{tlib}",
+        cmd = [HIPCC, "-shared", "-Wl,--no-undefined", *torch_objs, f"-L{HERE}", "-lspyre_hip", f"-L{tlib}",
                "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-Wl,-rpath,$ORIGIN",
                f"-Wl,-rpath,{tlib}", "-o", tmp]
         r = subprocess.run(cmd, capture_output=True, text=True)

@@ -18,28 +18,14 @@
 // SpyreHipError).  Dropout raises NotImplementedError, as the reference's
 // decomposition refuses it (decompositions.py:578-580).
 
-#include <ATen/ATen.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/library.h>
-
 #include <cmath>
 #include <cstdint>
 
-#include "../../include/spyre_hip.h"
+#include "torch_checks.h"
 
 namespace {
 
-void* stream_of(const at::Tensor& t) {
-  return static_cast<void*>(c10::hip::getCurrentHIPStream(t.device().index()).stream());
-}
-
-void check_rc(const char* fn, int rc) {
-  if (rc != SPYRE_OK) {
-    const char* msg = spyre_last_error();
-    TORCH_CHECK(false, "[spyre_hip ", fn, " ", rc, "] ", msg ? msg : "");
-  }
-}
+using namespace spyre_torch;
 
 // fp16 CUDA [B, H, S, D] whose rows the kernels read as 16-byte vectors:
 // feature stride 1, other strides multiples of 8, 16-byte aligned; anything
@@ -128,13 +114,6 @@ sdpa_overrideable(const at::Tensor& query, const at::Tensor& key, const at::Tens
 }
 
 constexpr int64_t kPage = 64;
-
-// t must be a CUDA tensor on `dev`: a kernel launched there reads or writes
-// it through its pointer (a host pointer would fault there).
-void require_on(const at::Tensor& t, const c10::Device& dev, const char* name) {
-  TORCH_CHECK_VALUE(t.is_cuda(), name, " must be a CUDA (HIP) tensor; there is no CPU path");
-  TORCH_CHECK_VALUE(t.device() == dev, name, " is on ", t.device(), "; the call runs on ", dev);
-}
 
 int64_t check_cache(const at::Tensor& kc, const at::Tensor& vc, int64_t Hkv, int64_t D) {
   for (const at::Tensor* t : {&kc, &vc}) {

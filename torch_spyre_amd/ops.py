@@ -25,8 +25,12 @@ an op on CPU tensors raises.  Fake kernels make the ops traceable.
   aten::_scaled_dot_product_fused_attention_overrideable (CUDA kernel)
         the reference's decomposition target (decompositions.py:523-609),
         returning its 9-tuple
-The last four are defined and implemented in C++ (csrc/torch_ops.cpp); this
-module gives them fake kernels.
+  spyre::rotary, spyre::kv_quant_append, spyre::rotary_kv_quant_append,
+  spyre::kv_quant_read, spyre::quant_paged_decode_attention, spyre::paged_tree_attention
+        rotary positions, the 8-bit paged cache and attention of drafted
+        tokens (no reference counterparts)
+Those from spyre::kv_append on are defined and implemented in C++
+(csrc/torch_ops.cpp, csrc/serving_ops.cpp); this module gives them fake kernels.
 """
 
 from __future__ import annotations
@@ -181,6 +185,39 @@ def _(query, key, value, attn_mask=None, is_causal=False, scale=None, enable_gqa
     B, Hq, Sq, D = query.shape
     out = query.new_empty((B, Sq, Hq, D)).transpose(1, 2)
     return out, query.new_empty((B if return_lse else 0, Hq, Sq), dtype=torch.float32)
+
+
+@torch.library.register_fake("spyre::rotary")
+def _(q, k, positions, frequencies, amplitude=1.0, interleaved=False, inverse=False):
+    return torch.empty_like(q), q.new_empty((0,)) if k is None else torch.empty_like(k)
+
+
+@torch.library.register_fake("spyre::kv_quant_append")
+def _(k_new, v_new, k_cache, v_cache, k_scale, v_scale, block_table, slots):
+    return None
+
+
+@torch.library.register_fake("spyre::rotary_kv_quant_append")
+def _(q, k_new, v_new, k_cache, v_cache, k_scale, v_scale, block_table, slots, positions, frequencies,
+      amplitude=1.0, interleaved=False):
+    return q.new_empty(q.shape)
+
+
+@torch.library.register_fake("spyre::kv_quant_read")
+def _(k_cache, v_cache, k_scale, v_scale, block_table, lens, length, start=None):
+    shape = (block_table.shape[0], k_cache.shape[1], length, 16 * k_cache.shape[2])
+    return tuple(k_cache.new_empty(shape, dtype=torch.float16) for _ in range(2))
+
+
+@torch.library.register_fake("spyre::quant_paged_decode_attention")
+def _(q, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, scale=None, max_context_len=-1):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
+@torch.library.register_fake("spyre::paged_tree_attention")
+def _(q, k_cache, v_cache, block_table, context_lens, tree_mask=None, draft_lens=None, k_scale=None, v_scale=None,
+      scale=None, max_context_len=-1):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:3], dtype=torch.float32)
 
 
 device_tensor.register_spyre_ops()
