@@ -28,6 +28,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "cache8.h"
 #include "fast_div.h"
@@ -67,7 +68,8 @@ struct TreeArgs {
   int B, T, Hq, Hkv, g, rows, tiles, max_ctx, draft_keys, chunk_pages, max_chunks;
   float scale_log2;
   uint32_t pairs;  // B Hkv
-  FastDiv by_g, by_hkv, by_tiles, by_pairs;
+  int row_blocks;  // of the wide kernel
+  FastDiv by_g, by_hkv, by_tiles, by_pairs, by_blocks;
 };
 
 __device__ __forceinline__ float xor32_max(float x) {
@@ -152,6 +154,103 @@ __device__ __forceinline__ bool drop_odd(uint32_t& w) {
   return odd != 0;
 }
 
+// A wavefront's pages, one after the other from `first` on, as indexes of their
+// (page, KV head): 64 table entries at a time, one a lane, so that no page's
+// loads wait for its entry.  A page that the table does not name validly is
+// page 0 (in bounds) and poisons the rows.
+struct Pages {
+  const TreeArgs& a;
+  const int32_t* trow;
+  int kvh, lane, first, ids = 0;
+  bool poisoned = false;
+  __device__ __forceinline__ Pages(const TreeArgs& args, int b, int kv_head, int lane_, int first_)
+      : a(args), trow(args.bt + b * args.bt_stride), kvh(kv_head), lane(lane_), first(first_) {}
+  __device__ __forceinline__ int64_t head(int p) {  // p: first, first + 1, ..., each once or again
+    const int at = p - first;
+    if ((at & 63) == 0) ids = p + lane < a.pages_per_seq ? trow[p + lane] : -1;
+    const int64_t phys = __builtin_amdgcn_readlane(ids, at & 63);
+    const bool bad = phys < 0 || phys >= a.num_pages;
+    poisoned |= bad;
+    return (bad ? 0 : phys) * a.Hkv + kvh;
+  }
+};
+
+// A lane's row of the T g rows of a KV head.
+struct Row {
+  int i;      // its drafted token
+  int head;   // its q head
+  bool live;
+  const uint8_t* mask;  // of its token; null: a chain
+  // Which of the 16 tokens from t on the row attends (total: all there are).
+  // Every mask byte is loaded, and none waits for another.
+  __device__ __forceinline__ uint32_t attends16(const TreeArgs& a, const Seq& sq, int t, int total) const {
+    uint32_t seen = 0;
+    const int j0 = t - sq.ctx;
+    if (mask) {
+      uint8_t keep[16];
+#pragma unroll
+      for (int x = 0; x < 16; ++x) keep[x] = mask[min(max(j0 + x, 0), a.T - 1) * a.m_sj];
+#pragma unroll
+      for (int x = 0; x < 16; ++x) seen |= static_cast<uint32_t>(j0 + x < 0 || keep[x] != 0) << x;
+    } else {
+      const int n = i - j0 + 1;  // tokens of the 16 up to i's own
+      seen = n <= 0 ? 0u : n >= 16 ? 0xffffu : (1u << n) - 1;
+    }
+    const int n = total - t;
+    return live && n > 0 ? seen & (n >= 16 ? 0xffffu : (1u << n) - 1) : 0u;
+  }
+};
+
+__device__ __forceinline__ Row row_of(const TreeArgs& a, const Seq& sq, int b, int kvh, int row) {
+  Row r;
+  r.i = static_cast<int>(fdiv(row, a.by_g));
+  r.head = kvh * a.g + row - r.i * a.g;
+  r.live = row < a.rows && r.i < sq.n;
+  r.mask = a.mask ? a.mask + b * a.m_sb + (r.live ? r.i : 0) * a.m_si : nullptr;
+  return r;
+}
+
+// Q^T operands of a lane's row: features 32 s + 16 half + 8 e .. + 7.
+template <int DS>
+__device__ __forceinline__ void load_q(const TreeArgs& a, int b, const Row& r, int half, f16x8 (&qf)[DS][2]) {
+  const _Float16* qp = a.q + b * a.q_sb + r.i * a.q_st + r.head * a.q_sh + 16 * half;
+#pragma unroll
+  for (int s = 0; s < DS; ++s)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      qf[s][e] = f16x8{};
+      if (r.live) qf[s][e] = *reinterpret_cast<const f16x8*>(qp + 32 * s + 8 * e);
+    }
+}
+
+// The infinities and NaNs of tokens t0 .. t1 - 1 that drop_odd left out of O,
+// number by number.
+template <int CT, int D>
+__device__ void add_odd(const TreeArgs& a, const Seq& sq, int b, int kvh, const Row& r, int lane, int t0, int t1,
+                        f32x16 (&o)[D / 32]) {
+  constexpr int KB = CT == kF16 ? 2 : 1;
+  const int half = lane >> 5;
+  Pages pages(a, b, kvh, lane, t0 / kPage);
+  for (int t = t0; t < t1; ++t) {
+    const bool attends = r.attends16(a, sq, t, t + 1);
+    const uint8_t* v = a.v + pages.head(t / kPage) * (static_cast<int64_t>(kPage) * D * KB);
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const int d = 32 * dt + 8 * (x / 4) + 4 * half + x % 4;
+        float f = 0.f;
+        if constexpr (CT == kF16) {
+          f = static_cast<float>(reinterpret_cast<const _Float16*>(v)[d * kPage + t % kPage]);
+          if (__builtin_fabsf(f) <= 65504.f) f = 0.f;
+        } else {
+          if ((v[(t % kPage / 16) * (D * 16) + d * 16 + t % 16] & 0x7f) == 0x7f) f = NAN;
+        }
+        if (attends) o[dt][x] += f;
+      }
+  }
+}
+
 // W wavefronts share a chunk of a (sequence, KV head, row tile): each takes
 // its own steps of it, and they join in LDS.
 template <int CT, int D, int W>
@@ -180,23 +279,11 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
   const int c1 = static_cast<int>(static_cast<int64_t>(chunk + 1) * steps / nch);
   const int s0 = c0 + (c1 - c0) * wave / W, s1 = c0 + (c1 - c0) * (wave + 1) / W;
 
-  const int row = tile * kTile + col;  // of the T g rows: token i, q head kvh g + hg
-  const int i = static_cast<int>(fdiv(row, a.by_g)), hg = row - i * a.g;
-  const bool live = row < a.rows && i < sq.n;
+  const Row row = row_of(a, sq, b, kvh, tile * kTile + col);
   f16x8 qf[DS][2];
-  {
-    const _Float16* qp = a.q + b * a.q_sb + i * a.q_st + (kvh * a.g + hg) * a.q_sh + 16 * half;
-#pragma unroll
-    for (int s = 0; s < DS; ++s)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        qf[s][e] = f16x8{};
-        if (live) qf[s][e] = *reinterpret_cast<const f16x8*>(qp + 32 * s + 8 * e);
-      }
-  }
-  const uint8_t* mrow = a.mask ? a.mask + b * a.m_sb + (live ? i : 0) * a.m_si : nullptr;
-  const int32_t* trow = a.bt + b * a.bt_stride;
-  bool poisoned = sq.bad, odd = false;
+  load_q<DS>(a, b, row, half, qf);
+  Pages pages(a, b, kvh, lane, s0 / PER_PAGE);
+  bool odd = false;
 
   f32x16 o[DS];
 #pragma unroll
@@ -211,13 +298,7 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
   const int v_off = CT == kF16 ? (col * kPage + 16 * half) * 2 : half * (D * 16) + col * 16;
 
   int64_t head = 0;  // physical page * Hkv + KV head, of the step being loaded
-  auto locate = [&](int st) {
-    const int p = st / PER_PAGE;
-    int64_t phys = p < a.pages_per_seq ? trow[p] : -1;
-    const bool bad = phys < 0 || phys >= a.num_pages;
-    poisoned |= bad;
-    head = (bad ? 0 : phys) * a.Hkv + kvh;  // in bounds; the rows are poisoned below
-  };
+  auto locate = [&](int st) { head = pages.head(st / PER_PAGE); };
   Raw<CT, D> kr, vr;
   float scale = 0.f;  // 8-bit: of the step's token `col`, K's in the lower lanes, V's in the upper
   auto load_k = [&](int st) {
@@ -256,6 +337,9 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
 
   auto step = [&](int st, bool more, auto edge_tag) {
     constexpr bool EDGE = decltype(edge_tag)::value;  // some tokens are drafted or do not exist
+    const int tok0 = st * STEP + 16 * half;           // this lane's 16 tokens
+    uint32_t seen = 0;                                // those that its row attends
+    if constexpr (EDGE) seen = row.attends16(a, sq, tok0, total);
     uint32_t odd_scale = 0, inf_scale = 0;  // of this lane's 16 tokens, those whose V has no finite scale
     if constexpr (CT != kF16) {
       __builtin_amdgcn_wave_barrier();
@@ -278,17 +362,6 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
     if (more) {
       if ((st + 1) % PER_PAGE == 0) locate(st + 1);
       load_k(st + 1);
-    }
-    const int tok0 = st * STEP + 16 * half;  // this lane's 16 tokens
-    uint32_t seen = 0;                       // those that its row attends
-    if constexpr (EDGE) {
-#pragma unroll
-      for (int x = 0; x < 16; ++x) {
-        const int j = tok0 + x - sq.ctx;
-        bool s = tok0 + x < total && live;
-        if (s && j >= 0) s = mrow ? mrow[j * a.m_sj] != 0 : j <= i;
-        seen |= static_cast<uint32_t>(s) << x;
-      }
     }
     float mx = -INFINITY;
 #pragma unroll
@@ -376,32 +449,11 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
   const int whole = min(s1, sq.ctx / STEP);
   for (; st < whole; ++st) step(st, st + 1 < s1, std::false_type{});
   for (; st < s1; ++st) step(st, st + 1 < s1, std::true_type{});
-  if (CT != SPYRE_CODES_INT8 && __any(odd)) {
-    // The infinities and NaNs left out above, number by number.
-    for (int t = max(s0, whole) * STEP; t < min(s1 * STEP, total); ++t) {
-      locate(t / STEP);
-      const int j = t - sq.ctx;
-      const bool attends = live && (j < 0 || (mrow ? mrow[j * a.m_sj] != 0 : j <= i));
-      const uint8_t* v = a.v + head * (static_cast<int64_t>(kPage) * D * KB);
-#pragma unroll
-      for (int dt = 0; dt < DS; ++dt)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const int d = 32 * dt + 8 * (x / 4) + 4 * half + x % 4;
-          float f = 0.f;
-          if constexpr (CT == kF16) {
-            f = static_cast<float>(reinterpret_cast<const _Float16*>(v)[d * kPage + t % kPage]);
-            if (__builtin_fabsf(f) <= 65504.f) f = 0.f;
-          } else {
-            if ((v[(t % kPage / 16) * (D * 16) + d * 16 + t % 16] & 0x7f) == 0x7f) f = NAN;
-          }
-          if (attends) o[dt][x] += f;
-        }
-    }
-  }
+  if (CT != SPYRE_CODES_INT8 && __any(odd))
+    add_odd<CT, D>(a, sq, b, kvh, row, lane, max(s0, whole) * STEP, min(s1 * STEP, total), o);
   l = xor32_sum(l);
-  if (!live) m = -INFINITY, l = 0.f;
-  if (poisoned && live) l = NAN;
+  if (!row.live) m = -INFINITY, l = 0.f;
+  if ((pages.poisoned || sq.bad) && row.live) l = NAN;
 
   // Join the wavefronts: O, m and l of the rows that exist, then every thread
   // folds elements in wavefront order.
@@ -462,6 +514,289 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
   }
 }
 
+// ---------------------------------------------------------- wide drafts --
+//
+// W wavefronts, 32 rows each, share every page of a chunk through LDS: K [D/64,
+// 64 tok, 64] and V [D, 64 tok] as fp16, in two slots.  8-bit pages are
+// converted once on the way in.  A 128-byte row is 8 units of 16 bytes; unit u
+// lies at u ^ swz(row), so that the 16 lanes that a read serves at once, and a
+// conversion's 16 stores, meet 16 different bank groups.
+__device__ __forceinline__ int swz_k(int row) { return ((row >> 1) & 3) | ((((row >> 3) ^ (row >> 4)) & 1) << 2); }
+__device__ __forceinline__ int swz_v(int row) { return (row >> 1) & 7; }
+
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+
+template <int CT, int D, int W>
+__global__ __launch_bounds__(W * 64, 2) void tree_wide_kernel(TreeArgs a) {
+  constexpr int DS = D / 32;
+  constexpr int TILE = kPage * D * 2;         // bytes of a K or a V tile
+  constexpr int SLOT = 2 * TILE;
+  constexpr int KU = kPage * D / 16;            // 8-bit: units of a K or a V page
+  constexpr int UNITS = 2 * KU / (W * 64);      // of both, that a thread converts
+  static_assert(CT == kF16 || (UNITS >= 1 && KU % 64 == 0), "every thread has a unit, and a wavefront's are all K or all V");
+  __shared__ __align__(16) char s_kv[2 * SLOT];
+  __shared__ __align__(16) float s_sc[2][3][kPage];  // 8-bit: score factors, V's scales' logarithms and inverses
+  __shared__ uint64_t s_odd[2][2];                   // and which of V's scales are not finite, and infinite
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const int col = lane & 31, half = lane >> 5;
+  const uint32_t blk = blockIdx.x, lo8 = blk & 7, hi = blk >> 3;
+  const uint32_t hi_t = fdiv(hi, a.by_blocks), rb = hi - hi_t * a.row_blocks, item = hi_t * 8 + lo8;
+  const uint32_t chunk = fdiv(item, a.by_pairs), pair = item - chunk * a.pairs;
+  if (chunk >= static_cast<uint32_t>(a.max_chunks)) return;
+  const uint32_t b = fdiv(pair, a.by_hkv), kvh = pair - b * a.Hkv;
+  const Seq sq = seq_of(a, b);
+  const int nch = chunks_of(sq.pages, a.chunk_pages);
+  if (static_cast<int>(chunk) >= nch) return;
+  const int total = sq.ctx + (a.draft_keys ? sq.n : 0);
+  const int p0 = static_cast<int>(static_cast<int64_t>(chunk) * sq.pages / nch);
+  const int p1 = static_cast<int>(static_cast<int64_t>(chunk + 1) * sq.pages / nch);
+  const int tile = rb * W + wave;
+  const Row row = row_of(a, sq, b, kvh, tile * kTile + col);
+  Pages pages(a, b, kvh, lane, p0);
+  bool odd = false;
+  const bool block_live = static_cast<int>(rb) * W * kTile < sq.n * a.g;  // some row of the workgroup is drafted
+  const bool wave_live = tile * kTile < sq.n * a.g;
+  f16x8 qf[DS][2];
+  load_q<DS>(a, b, row, half, qf);
+  f32x16 o[DS];
+#pragma unroll
+  for (int dt = 0; dt < DS; ++dt)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) o[dt][x] = 0.f;
+  float m = -INFINITY, l = 0.f;
+
+  // fp16 pages go straight into LDS: load i of a tile fills its bytes 1024 i
+  // .., lane by lane, so each lane fetches the unit that belongs at its place.
+  const int l8 = lane / 8;
+  const int k_src = 1024 * wave + 128 * l8 + (((lane % 8) ^ swz_k(8 * wave + l8)) * 16);
+  const int v_src = 1024 * wave + 128 * l8 + (((lane % 8) ^ swz_v(8 * wave + l8)) * 16);
+  static_assert(W % 4 == 0, "the loads of a wavefront share their swizzle");
+  // 8-bit: the next page's units and scales, in registers.
+  u32x4 raw[CT == kF16 ? 1 : UNITS];
+  float scale = 0.f;
+  auto fetch = [&](int p, int slot) {
+    const int64_t head = pages.head(p);
+    if constexpr (CT == kF16) {
+      const uint8_t *kp = a.k + head * TILE, *vp = a.v + head * TILE;
+      const Rsrc kr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(kp), 0, TILE, 0x00020000);
+      const Rsrc vr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(vp), 0, TILE, 0x00020000);
+#pragma unroll
+      for (int j = 0; j < TILE / 1024 / W; ++j) {
+        char* dk = s_kv + slot * SLOT + 1024 * (wave + W * j);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (__attribute__((address_space(3))) void*)dk, 16, k_src, 1024 * W * j, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (__attribute__((address_space(3))) void*)(dk + TILE), 16, v_src,
+                                                 1024 * W * j, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < UNITS; ++j) {
+        const int w0 = (wave + j * W) * 64;  // this wavefront's first unit, of K's and then V's
+        const uint8_t* p8 = w0 < KU ? a.k + head * (TILE / 2) + w0 * 16 : a.v + head * (TILE / 2) + (w0 - KU) * 16;
+        raw[j] = *reinterpret_cast<const u32x4*>(p8 + lane * 16);
+      }
+      if (wave < 2) scale = (wave ? a.vs : a.ks)[head * kPage + lane];
+    }
+  };
+  // 8-bit: what fetch() brought, into a slot.
+  auto store = [&](int slot) {
+    if constexpr (CT != kF16) {
+      char* k0 = s_kv + slot * SLOT;
+      auto two = [&](char* at, int u, int sw, const u32x4& w) {  // units u and u + 1 of a row
+        *reinterpret_cast<f16x8*>(at + ((u ^ sw) * 16)) = codes_to_f16x8<CT>(w[0], w[1]);
+        *reinterpret_cast<f16x8*>(at + (((u + 1) ^ sw) * 16)) = codes_to_f16x8<CT>(w[2], w[3]);
+      };
+#pragma unroll
+      for (int j = 0; j < UNITS; ++j) {
+        const int w0 = (wave + j * W) * 64;
+        if (w0 < KU) {  // 16 features un of a token
+          const int un = w0 / kPage, tok = lane;
+          two(k0 + (un / 4) * (kPage * 128) + tok * 128, 2 * (un % 4), swz_k(tok), raw[j]);
+        } else {  // 16 tokens q4 of a feature
+          const int x = w0 - KU + lane, q4 = x / D, d = x % D;
+          two(k0 + TILE + d * 128, 2 * q4, swz_v(d), raw[j]);
+        }
+      }
+      if (wave == 0) s_sc[slot][0][lane] = scale * a.scale_log2;
+      if (wave == 1) {
+        const bool finite = __builtin_fabsf(scale) <= 0x1.fffffep127f;
+        const float vc = !finite ? 1.f : scale < 0x1p-60f ? 0x1p-60f : scale;  // 0: codes of no weight
+        s_sc[slot][1][lane] = __builtin_amdgcn_logf(vc);
+        s_sc[slot][2][lane] = __builtin_amdgcn_rcpf(vc);
+        const uint64_t not_finite = __builtin_amdgcn_ballot_w64(!finite);
+        const uint64_t infinite = __builtin_amdgcn_ballot_w64(scale == INFINITY);
+        if (lane == 0) s_odd[slot][0] = not_finite, s_odd[slot][1] = infinite;
+      }
+    }
+  };
+
+  // Operand addresses in a slot: unit u of a row is (bits of the unroll) ^
+  // (bits of the lane), four of each.
+  const int tok = token_of(col);
+  const int k_row = tok * 128, v_row = col * 128;
+  const int k_x = (2 * half) ^ swz_k(tok), v_x = (2 * half) ^ swz_v(col);
+  int k_at[2][2];
+#pragma unroll
+  for (int y = 0; y < 2; ++y)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) k_at[y][e] = k_row + ((k_x ^ (4 * y + e)) * 16);
+
+  // The 32 tokens from half t of page p on.
+  auto step = [&](int p, int slot, int t, auto edge_tag) {
+    constexpr bool EDGE = decltype(edge_tag)::value;
+    const char* base = s_kv + slot * SLOT;
+    const int s0 = 32 * t + 16 * half, tok0 = p * kPage + s0;  // this lane's 16 tokens
+    uint32_t seen = 0;
+    if constexpr (EDGE) seen = row.attends16(a, sq, tok0, total);
+    f32x16 sc;
+#pragma unroll
+    for (int x = 0; x < 16; ++x) sc[x] = 0.f;
+#pragma unroll
+    for (int s = 0; s < DS; ++s)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const f16x8 k = *reinterpret_cast<const f16x8*>(base + t * (32 * 128) + k_at[s % 2][e] + (s / 2) * (kPage * 128));
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[s][e], sc, 0, 0, 0);
+      }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int x4 = 0; x4 < 4; ++x4) {
+      f32x4 f, lv;
+      if constexpr (CT != kF16) {
+        f = *reinterpret_cast<const f32x4*>(&s_sc[slot][0][s0 + 4 * x4]);
+        lv = *reinterpret_cast<const f32x4*>(&s_sc[slot][1][s0 + 4 * x4]);
+      }
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int x = 4 * x4 + y;
+        float v = CT == kF16 ? sc[x] * a.scale_log2 : __builtin_fmaf(sc[x], f[y], lv[y]);
+        if constexpr (EDGE) v = (seen >> x) & 1 ? v : -INFINITY;
+        sc[x] = v;
+        mx = fmaxf(mx, v);
+      }
+    }
+    mx = xor32_max(mx);
+    if (__any(mx > m + kSlack)) {
+      const float mn = fmaxf(m, mx);
+      const float alpha = m == -INFINITY ? 0.f : exp2_of(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DS; ++dt)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) o[dt][x] *= alpha;
+    }
+    const float mu = m == -INFINITY ? 0.f : m;
+    f16x8 pw[2];
+#pragma unroll
+    for (int x4 = 0; x4 < 4; ++x4) {
+      f32x4 r;
+      if constexpr (CT != kF16) r = *reinterpret_cast<const f32x4*>(&s_sc[slot][2][s0 + 4 * x4]);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int x = 4 * x4 + y;
+        const float w = exp2_of(sc[x] - mu);
+        if constexpr (CT == kF16)
+          l += w;
+        else
+          l = __builtin_fmaf(w, EDGE && !((seen >> x) & 1) ? 0.f : r[y], l);
+        pw[x / 8][x % 8] = static_cast<_Float16>(w);
+      }
+    }
+    if constexpr (CT != kF16) {
+      const uint32_t not_finite = static_cast<uint32_t>(s_odd[slot][0] >> s0) & 0xffffu;
+      if (__any(not_finite != 0)) {
+        const uint32_t infinite = static_cast<uint32_t>(s_odd[slot][1] >> s0) & 0xffffu;
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+          if ((not_finite >> x) & 1 && (!EDGE || (seen >> x) & 1))
+            pw[x / 8][x % 8] = static_cast<_Float16>((infinite >> x) & 1 ? INFINITY : NAN);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const char* v_at = base + TILE + v_row + ((v_x ^ (4 * t + e)) * 16);
+#pragma unroll
+      for (int dt = 0; dt < DS; ++dt) {
+        u32x4 v = *reinterpret_cast<const u32x4*>(v_at + dt * (32 * 128));
+        if constexpr (EDGE) {  // as in the rows kernel
+          const int keep = total - tok0 - 8 * e;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = keep - 2 * i;
+            uint32_t w = v[i] & (k <= 0 ? 0u : k == 1 ? 0xffffu : ~0u);
+            odd = drop_odd<kF16>(w) || odd;
+            v[i] = w;
+          }
+        }
+        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v), pw[e], o[dt], 0, 0, 0);
+      }
+    }
+  };
+
+  if (block_live && p0 < p1) {
+    fetch(p0, 0);
+    if constexpr (CT != kF16) {
+      store(0);
+      if (p0 + 1 < p1) fetch(p0 + 1, 1);
+    }
+    const int whole = min(p1, sq.ctx / kPage);
+    for (int p = p0; p < p1; ++p) {
+      const int slot = (p - p0) & 1;
+      if constexpr (CT == kF16) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();  // page p is in its slot, and every wavefront is done with the other one
+      if constexpr (CT == kF16) {
+        if (p + 1 < p1) fetch(p + 1, slot ^ 1);
+      } else {
+        if (p + 1 < p1) store(slot ^ 1);
+        if (p + 2 < p1) fetch(p + 2, slot);
+      }
+      if (wave_live) {
+        if (p < whole) {
+          step(p, slot, 0, std::false_type{});
+          step(p, slot, 1, std::false_type{});
+        } else {
+#pragma unroll 1
+          for (int t = 0; t < 2; ++t) step(p, slot, t, std::true_type{});
+        }
+      }
+    }
+    if (CT != SPYRE_CODES_INT8 && __any(odd))
+      add_odd<CT, D>(a, sq, b, kvh, row, lane, max(p0, whole) * kPage, min(p1 * kPage, total), o);
+  }
+  l = xor32_sum(l);
+  if (!row.live) m = -INFINITY, l = 0.f;
+  if ((pages.poisoned || sq.bad) && row.live) l = NAN;
+  if (tile * kTile + col >= a.rows) return;
+  if (nch == 1) {
+    const int64_t at = (static_cast<int64_t>(b) * a.T + row.i) * a.Hq + row.head;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int dt = 0; dt < DS; ++dt)
+#pragma unroll
+      for (int x4 = 0; x4 < 4; ++x4) {
+        f16x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = static_cast<_Float16>(l == 0.f ? 0.f : o[dt][4 * x4 + e] * inv);
+        *reinterpret_cast<f16x4*>(a.out + at * D + 32 * dt + 8 * x4 + 4 * half) = y;
+      }
+    if (a.lse && half == 0) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  } else {
+    const int64_t slot = (static_cast<int64_t>(pair) * a.tiles + tile) * a.max_chunks + chunk;
+    const int64_t slots = static_cast<int64_t>(a.pairs) * a.tiles * a.max_chunks;
+    float* x = a.ws + (slot * kTile + col) * D + 4 * half;
+#pragma unroll
+    for (int dt = 0; dt < DS; ++dt)
+#pragma unroll
+      for (int x4 = 0; x4 < 4; ++x4)
+        *reinterpret_cast<f32x4*>(x + 32 * dt + 8 * x4) =
+            f32x4{o[dt][4 * x4], o[dt][4 * x4 + 1], o[dt][4 * x4 + 2], o[dt][4 * x4 + 3]};
+    if (half == 0) {
+      float* ml = a.ws + slots * kTile * D + (slot * kTile + col) * 2;
+      ml[0] = m, ml[1] = l;
+    }
+  }
+}
+
 // Joins the chunks of sequences that have several: a thread 4 features of a row.
 template <int D>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
@@ -503,9 +838,12 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
 }
 
 constexpr int kRowWaves = 4;
+// Rows up to here take the rows kernel: two tiles read a chunk's pages twice.
+constexpr int kNarrowRows = 64;
 
 struct Plan {
-  int tiles, chunk_pages, max_chunks;
+  int tiles, waves, row_blocks;  // waves 0: the rows kernel
+  int chunk_pages, max_chunks;
   size_t ws_bytes;
 };
 
@@ -515,25 +853,40 @@ Plan plan_of(int B, int T, int Hq, int Hkv, int D, int max_tokens) {
   Plan p;
   const int64_t rows = static_cast<int64_t>(T) * (Hq / Hkv);
   p.tiles = static_cast<int>((rows + kTile - 1) / kTile);
+  p.waves = rows <= kNarrowRows ? 0 : rows <= 128 ? 4 : 8;
+  p.row_blocks = p.waves ? (p.tiles + p.waves - 1) / p.waves : p.tiles;
   const int pages = pages_of(max_tokens);
-  const int64_t groups = static_cast<int64_t>(B) * Hkv * p.tiles;
-  int cp = 8 * kRowWaves;
-  while (cp > kRowWaves && groups * chunks_of(pages, cp) < 512) cp /= 2;
-  p.chunk_pages = cp;
-  p.max_chunks = chunks_of(pages, cp);
+  const int64_t groups = static_cast<int64_t>(B) * Hkv * p.row_blocks;
+  if (p.waves == 0) {
+    int cp = 8 * kRowWaves;
+    while (cp > kRowWaves && groups * chunks_of(pages, cp) < 512) cp /= 2;
+    p.chunk_pages = cp;
+  } else {
+    // Rounds of the device times a workgroup's steps, its start counted as
+    // four of them.
+    const int64_t slots = p.waves == 8 ? 256 : 512;
+    int64_t best = INT64_MAX;
+    p.chunk_pages = std::max(pages, 1);
+    for (int n = 1; n <= std::max(pages, 1) && n <= 256; ++n) {
+      const int cp = (pages + n - 1) / n;
+      const int64_t rounds = (groups * n + slots - 1) / slots, cost = rounds * (cp + 4) + (n > 1 ? 4 : 0);
+      if (cost < best) best = cost, p.chunk_pages = std::max(cp, 1);
+    }
+  }
+  p.max_chunks = chunks_of(pages, p.chunk_pages);
   const int64_t width = std::min<int64_t>(kTile, rows);
-  p.ws_bytes = p.max_chunks == 1 ? 0 : static_cast<size_t>(groups * p.max_chunks * width * (D + 2)) * 4;
+  p.ws_bytes = p.max_chunks == 1 ? 0 : static_cast<size_t>(static_cast<int64_t>(B) * Hkv * p.tiles * p.max_chunks * width * (D + 2)) * 4;
   return p;
 }
 
-template <int CT>
-hipError_t launch(const TreeArgs& a, int D, int64_t blocks, hipStream_t st) {
-  const dim3 grid(static_cast<uint32_t>(blocks));
-  if (D == 128)
-    tree_rows_kernel<CT, 128, kRowWaves><<<grid, kRowWaves * 64, 0, st>>>(a);
+template <int CT, int D>
+void launch(const TreeArgs& a, int waves, dim3 grid, hipStream_t st) {
+  if (waves == 8)
+    tree_wide_kernel<CT, D, 8><<<grid, 512, 0, st>>>(a);
+  else if (waves == 4)
+    tree_wide_kernel<CT, D, 4><<<grid, 256, 0, st>>>(a);
   else
-    tree_rows_kernel<CT, 64, kRowWaves><<<grid, kRowWaves * 64, 0, st>>>(a);
-  return hipGetLastError();
+    tree_rows_kernel<CT, D, kRowWaves><<<grid, kRowWaves * 64, 0, st>>>(a);
 }
 
 // T and the tokens of a sequence that a call may hold.
@@ -594,14 +947,24 @@ extern "C" int spyre_paged_tree_attn(const void* q, const int64_t* q_strides, co
   a.scale_log2 = scale * kLog2e;
   const int64_t pairs = static_cast<int64_t>(B) * Hkv;
   const int64_t items = (pairs * p.max_chunks + 7) / 8 * 8;
-  SPYRE_REQUIRE(items * p.tiles < (int64_t{1} << 31), SPYRE_EUNSUPPORTED, "too many workgroups");
+  SPYRE_REQUIRE(items * p.row_blocks < (int64_t{1} << 31), SPYRE_EUNSUPPORTED, "too many workgroups");
   a.pairs = static_cast<uint32_t>(pairs);
   a.by_g = make_fastdiv(static_cast<uint32_t>(a.g)), a.by_hkv = make_fastdiv(static_cast<uint32_t>(Hkv));
+  a.row_blocks = p.row_blocks, a.by_blocks = make_fastdiv(static_cast<uint32_t>(p.row_blocks));
   a.by_tiles = make_fastdiv(static_cast<uint32_t>(p.tiles)), a.by_pairs = make_fastdiv(a.pairs);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  hipError_t e = cache_kind == SPYRE_CACHE_F16    ? launch<SPYRE_CACHE_F16>(a, D, items * p.tiles, st)
-                 : cache_kind == SPYRE_CODES_E4M3 ? launch<SPYRE_CODES_E4M3>(a, D, items * p.tiles, st)
-                                                  : launch<SPYRE_CODES_INT8>(a, D, items * p.tiles, st);
+  const dim3 grid(static_cast<uint32_t>(items * p.row_blocks));
+  auto go = [&](auto kind) {
+    constexpr int CT = decltype(kind)::value;
+    D == 128 ? launch<CT, 128>(a, p.waves, grid, st) : launch<CT, 64>(a, p.waves, grid, st);
+  };
+  if (f16)
+    go(std::integral_constant<int, SPYRE_CACHE_F16>{});
+  else if (cache_kind == SPYRE_CODES_E4M3)
+    go(std::integral_constant<int, SPYRE_CODES_E4M3>{});
+  else
+    go(std::integral_constant<int, SPYRE_CODES_INT8>{});
+  hipError_t e = hipGetLastError();
   SPYRE_REQUIRE(e == hipSuccess, SPYRE_EHIP, "tree attention launch failed: %s", hipGetErrorString(e));
   if (p.max_chunks > 1) {
     const int64_t n = (pairs * a.rows * (D / 4) + 255) / 256;
