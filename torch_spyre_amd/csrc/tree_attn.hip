@@ -65,11 +65,13 @@ struct TreeArgs {
   _Float16* out;  // [B, T, Hq, D]
   float* lse;     // [B, T, Hq] or null
   float* ws;
-  int B, T, Hq, Hkv, g, rows, tiles, max_ctx, draft_keys, chunk_pages, max_chunks;
+  int B, T, Hq, Hkv, g, rows, max_ctx, draft_keys;
   float scale_log2;
-  uint32_t pairs;  // B Hkv
-  int row_blocks;  // of the wide kernel
-  FastDiv by_g, by_hkv, by_tiles, by_pairs, by_blocks;
+  // The rows of a KV head are cut into row_blocks of block_rows; a partial
+  // holds `width` of them, the fewer of block_rows and rows.
+  int row_blocks, block_rows, width;
+  int ranges, min_per;  // see Walk
+  FastDiv by_g, by_hkv, by_blocks, by_ranges;
 };
 
 __device__ __forceinline__ float xor32_max(float x) {
@@ -92,24 +94,161 @@ __device__ __forceinline__ int token_of(int m) {
 }
 
 __host__ __device__ __forceinline__ int pages_of(int tokens) { return tokens / kPage + (tokens % kPage != 0); }
-__host__ __device__ __forceinline__ int chunks_of(int pages, int chunk_pages) {
-  return pages == 0 ? 1 : (pages + chunk_pages - 1) / chunk_pages;
-}
-
 // What a sequence holds.  bad: it breaks the max_context_len contract.
 struct Seq {
   int ctx, n, pages;
   bool bad;
 };
 
-__device__ __forceinline__ Seq seq_of(const TreeArgs& a, int b) {
+__device__ __forceinline__ Seq seq_of(const TreeArgs& a, int raw, int count) {
   Seq s;
-  const int raw = a.ctx[b];
   s.bad = raw > a.max_ctx;
   s.ctx = min(max(raw, 0), a.max_ctx);
-  s.n = a.counts ? min(max(a.counts[b], 0), a.T) : a.T;
+  s.n = min(max(count, 0), a.T);
   s.pages = pages_of(s.ctx + (a.draft_keys ? s.n : 0));
   return s;
+}
+
+// Sequence b, the same for the wavefront (in scalar registers).
+__device__ __forceinline__ Seq seq_at(const TreeArgs& a, int b) {
+  return seq_of(a, __builtin_amdgcn_readfirstlane(a.ctx[b]),
+                a.counts ? __builtin_amdgcn_readfirstlane(a.counts[b]) : a.T);
+}
+
+// Inclusive sums over the lanes of a wavefront.
+__device__ __forceinline__ int scan64(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8: within 16 lanes
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 of a row to the next
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to the upper half
+  return x;
+}
+
+// How the pages are shared out.  Units are the pages of every (sequence, KV
+// head), one after the other (a sequence of none counts one, which writes its
+// zeros); range r of `ranges` is units [r per, (r + 1) per).  The lengths are
+// data of the device, so every wavefront works out the sums itself; ragged
+// batches are then as even as equal ones.  A range that holds only part of a
+// (sequence, KV head) leaves its partial in slot 0 (the range's first piece)
+// or 1 (its last); whole ones are written directly.
+struct Walk {
+  int per, u, end;            // units
+  int b, base, pages;         // the sequence: its first unit / Hkv, its units a KV head
+  __device__ __forceinline__ static int units_of(const TreeArgs& a, int b) {
+    return max(1, seq_of(a, a.ctx[b], a.counts ? a.counts[b] : a.T).pages);
+  }
+  // Units a KV head of all sequences.
+  __device__ __forceinline__ static int total_of(const TreeArgs& a, int lane, int& first64) {
+    int sum = 0;
+    for (int c = 0; c < a.B; c += 256) {
+      int x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = c + 64 * k + lane;
+        x[k] = i < a.B ? units_of(a, i) : 0;
+      }
+      if (c == 0) first64 = x[0];
+      sum += x[0] + x[1] + x[2] + x[3];
+    }
+    return __builtin_amdgcn_readlane(scan64(sum), 63);
+  }
+  __device__ __forceinline__ static int per_of(const TreeArgs& a, int total) {
+    return max(a.min_per, static_cast<int>(fdiv(total * a.Hkv + a.ranges - 1, a.by_ranges)));
+  }
+  // Range r; false if it is empty.
+  __device__ __forceinline__ bool start(const TreeArgs& a, int lane, int r) {
+    int x = 0;
+    const int total = total_of(a, lane, x);
+    per = per_of(a, total);
+    u = r * per;
+    end = min(u + per, total * a.Hkv);
+    if (u >= end) return false;
+    const int target = static_cast<int>(fdiv(u, a.by_hkv));
+    base = 0;
+    for (int c = 0;; c += 64) {  // ends: target < total
+      if (c > 0) x = c + lane < a.B ? units_of(a, c + lane) : 0;
+      const int sum = scan64(x);
+      const uint64_t past = __builtin_amdgcn_ballot_w64(base + sum > target);
+      if (past) {
+        const int i = __builtin_ctzll(past);
+        b = c + i;
+        pages = __builtin_amdgcn_readlane(x, i);
+        base += __builtin_amdgcn_readlane(sum, i) - pages;
+        return true;
+      }
+      base += __builtin_amdgcn_readlane(sum, 63);
+    }
+  }
+  // The first unit / Hkv of sequence `seq`, and `per`.
+  __device__ __forceinline__ void seek(const TreeArgs& a, int lane, int seq) {
+    int x = 0, before = 0;
+    per = per_of(a, total_of(a, lane, x));
+    b = seq;
+    for (int c = 0; c <= seq; c += 64) {
+      if (c > 0) x = c + lane < a.B ? units_of(a, c + lane) : 0;
+      before += c + lane < seq ? x : 0;
+    }
+    base = __builtin_amdgcn_readlane(scan64(before), 63);
+    pages = max(1, seq_at(a, seq).pages);
+  }
+};
+
+// A piece of a range: pages [page0, page1) of a (sequence, KV head).
+struct Piece {
+  int kvh, page0, page1;
+  bool whole;   // all of them
+  int slot;     // else its partial's: 0, or 1
+};
+
+__device__ __forceinline__ Piece piece_of(const TreeArgs& a, const Walk& w, int range) {
+  Piece p;
+  const uint32_t in = w.u - w.base * a.Hkv;
+  p.kvh = in / static_cast<uint32_t>(w.pages);
+  p.page0 = in - p.kvh * w.pages;
+  p.page1 = min(w.pages, p.page0 + w.end - w.u);
+  p.whole = p.page0 == 0 && p.page1 == w.pages;
+  p.slot = w.u == range * w.per ? 0 : 1;
+  return p;
+}
+
+// After it.
+__device__ __forceinline__ void advance(const TreeArgs& a, Walk& w, const Piece& p) {
+  w.u += p.page1 - p.page0;
+  if (w.u < w.end && p.page1 == w.pages && p.kvh == a.Hkv - 1) {
+    w.base += w.pages;
+    w.b += 1;
+    w.pages = max(1, seq_at(a, w.b).pages);
+  }
+}
+
+// The range and the row block of a workgroup.  The row blocks of one range
+// read the same pages: 8 workgroups apart, they meet in one XCD's L2.
+__device__ __forceinline__ void place_of(const TreeArgs& a, int& range, int& rb) {
+  const uint32_t lo8 = blockIdx.x & 7, hi = blockIdx.x >> 3, q = fdiv(hi, a.by_blocks);
+  rb = static_cast<int>(hi - q * a.row_blocks);
+  range = static_cast<int>(q * 8 + lo8);
+}
+
+__device__ __forceinline__ float* partial_o(const TreeArgs& a, int range, int rb, int slot, int row, int D) {
+  return a.ws + (((static_cast<int64_t>(range) * a.row_blocks + rb) * 2 + slot) * a.width + row) * D;
+}
+__device__ __forceinline__ float* partial_ml(const TreeArgs& a, int range, int rb, int slot, int row, int D) {
+  const int64_t slots = static_cast<int64_t>(a.ranges) * a.row_blocks * 2;
+  return a.ws + slots * a.width * D + (((static_cast<int64_t>(range) * a.row_blocks + rb) * 2 + slot) * a.width + row) * 2;
+}
+
+// 4 features of a finished row.
+template <int D>
+__device__ __forceinline__ void store_row4(const TreeArgs& a, int b, int i, int head, int d, f32x4 x, float m, float l) {
+  const int64_t at = (static_cast<int64_t>(b) * a.T + i) * a.Hq + head;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  f16x4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = static_cast<_Float16>(l == 0.f ? 0.f : x[e] * inv);
+  *reinterpret_cast<f16x4*>(a.out + at * D + d) = y;
+  if (a.lse && d == 0) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 // The raw operands of a 32-token step: 8-bit, D / 32 units of 16 codes a lane;
@@ -167,7 +306,10 @@ struct Pages {
       : a(args), trow(args.bt + b * args.bt_stride), kvh(kv_head), lane(lane_), first(first_) {}
   __device__ __forceinline__ int64_t head(int p) {  // p: first, first + 1, ..., each once or again
     const int at = p - first;
-    if ((at & 63) == 0) ids = p + lane < a.pages_per_seq ? trow[p + lane] : -1;
+    if ((at & 63) == 0) {
+      ids = p + lane < a.pages_per_seq ? trow[p + lane] : -1;
+      asm volatile("" : "+v"(ids));  // waits here: behind the branch every page would, for all loads in flight
+    }
     const int64_t phys = __builtin_amdgcn_readlane(ids, at & 63);
     const bool bad = phys < 0 || phys >= a.num_pages;
     poisoned |= bad;
@@ -223,17 +365,24 @@ __device__ __forceinline__ void load_q(const TreeArgs& a, int b, const Row& r, i
     }
 }
 
-// The infinities and NaNs of tokens t0 .. t1 - 1 that drop_odd left out of O,
-// number by number.
+// The infinities and NaNs of tokens t0 .. t1 - 1 (part 0 / 1: of their pages'
+// first / second halves only) that drop_odd left out of O, number by number.
 template <int CT, int D>
 __device__ void add_odd(const TreeArgs& a, const Seq& sq, int b, int kvh, const Row& r, int lane, int t0, int t1,
-                        f32x16 (&o)[D / 32]) {
+                        int part, f32x16 (&o)[D / 32]) {
   constexpr int KB = CT == kF16 ? 2 : 1;
-  const int half = lane >> 5;
+  int half = lane >> 5;
+  asm volatile("" : "+v"(half));  // rare: its addresses are not worth registers of the loops before it
   Pages pages(a, b, kvh, lane, t0 / kPage);
   for (int t = t0; t < t1; ++t) {
-    const bool attends = r.attends16(a, sq, t, t + 1);
-    const uint8_t* v = a.v + pages.head(t / kPage) * (static_cast<int64_t>(kPage) * D * KB);
+    const bool attends = r.attends16(a, sq, t, t + 1) && (part < 0 || part == (t % kPage) / 32);
+    const int64_t head = pages.head(t / kPage);
+    const uint8_t* v = a.v + head * (static_cast<int64_t>(kPage) * D * KB);
+    float vs = 1.f;  // 8-bit: V's scale if it is not finite
+    if constexpr (CT != kF16) {
+      const float x = a.vs[head * kPage + t % kPage];
+      if (!(__builtin_fabsf(x) <= 0x1.fffffep127f)) vs = x;
+    }
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
@@ -244,7 +393,10 @@ __device__ void add_odd(const TreeArgs& a, const Seq& sq, int b, int kvh, const 
           f = static_cast<float>(reinterpret_cast<const _Float16*>(v)[d * kPage + t % kPage]);
           if (__builtin_fabsf(f) <= 65504.f) f = 0.f;
         } else {
-          if ((v[(t % kPage / 16) * (D * 16) + d * 16 + t % 16] & 0x7f) == 0x7f) f = NAN;
+          float x[4];
+          codes_to_f32<CT>(v[(t % kPage / 16) * (D * 16) + d * 16 + t % 16], x);
+          f = x[0] * vs;
+          if (__builtin_fabsf(f) <= 65504.f) f = 0.f;
         }
         if (attends) o[dt][x] += f;
       }
@@ -262,23 +414,18 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
   __shared__ __align__(16) float s_mem[W * kTile * (ROW + 2)];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
   const int col = lane & 31, half = lane >> 5;
-  // Row tiles of one chunk read the same pages: 8 blocks apart, so that they
-  // meet in one XCD's L2.
-  const uint32_t blk = blockIdx.x, lo8 = blk & 7, hi = blk >> 3;
-  const uint32_t hi_t = fdiv(hi, a.by_tiles), tile = hi - hi_t * a.tiles, item = hi_t * 8 + lo8;
-  const uint32_t chunk = fdiv(item, a.by_pairs), pair = item - chunk * a.pairs;
-  if (chunk >= static_cast<uint32_t>(a.max_chunks)) return;
-  const uint32_t b = fdiv(pair, a.by_hkv), kvh = pair - b * a.Hkv;
-  const Seq sq = seq_of(a, b);
-  const int nch = chunks_of(sq.pages, a.chunk_pages);
-  if (static_cast<int>(chunk) >= nch) return;
+  int range, tile;
+  place_of(a, range, tile);
+  Walk walk;
+  if (range >= a.ranges || !walk.start(a, lane, range)) return;
+  for (; walk.u < walk.end;) {
+  const Piece pc = piece_of(a, walk, range);
+  const int b = walk.b, kvh = pc.kvh;
+  const Seq sq = seq_at(a, b);
   const int total = sq.ctx + (a.draft_keys ? sq.n : 0);
-  // Equal shares of the sequence's steps for the chunks, of a chunk's for the wavefronts.
-  const int steps = (total + STEP - 1) / STEP;
-  const int c0 = static_cast<int>(static_cast<int64_t>(chunk) * steps / nch);
-  const int c1 = static_cast<int>(static_cast<int64_t>(chunk + 1) * steps / nch);
+  // The wavefronts take equal shares of the piece's steps; rows of no drafted token none.
+  const int c0 = pc.page0 * PER_PAGE, c1 = tile * kTile < sq.n * a.g ? min(pc.page1 * PER_PAGE, (total + STEP - 1) / STEP) : c0;
   const int s0 = c0 + (c1 - c0) * wave / W, s1 = c0 + (c1 - c0) * (wave + 1) / W;
-
   const Row row = row_of(a, sq, b, kvh, tile * kTile + col);
   f16x8 qf[DS][2];
   load_q<DS>(a, b, row, half, qf);
@@ -450,7 +597,7 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
   for (; st < whole; ++st) step(st, st + 1 < s1, std::false_type{});
   for (; st < s1; ++st) step(st, st + 1 < s1, std::true_type{});
   if (CT != SPYRE_CODES_INT8 && __any(odd))
-    add_odd<CT, D>(a, sq, b, kvh, row, lane, max(s0, whole) * STEP, min(s1 * STEP, total), o);
+    add_odd<CT, D>(a, sq, b, kvh, row, lane, max(s0, whole) * STEP, min(s1 * STEP, total), -1, o);
   l = xor32_sum(l);
   if (!row.live) m = -INFINITY, l = 0.f;
   if ((pages.poisoned || sq.bad) && row.live) l = NAN;
@@ -474,10 +621,6 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
     }
   }
   __syncthreads();
-  const bool single = nch == 1;
-  const int64_t slot = (static_cast<int64_t>(pair) * a.tiles + tile) * a.max_chunks + chunk;
-  const int64_t slots = static_cast<int64_t>(a.pairs) * a.tiles * a.max_chunks;
-  const int width = min(kTile, a.rows);  // rows of a partial
   for (int u = threadIdx.x; u < rows * (D / 4); u += W * 64) {
     const int r = u / (D / 4), d = 4 * (u % (D / 4));
     float M = -INFINITY, L = 0.f;
@@ -495,231 +638,315 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
         for (int e = 0; e < 4; ++e) acc[e] += x[e] * f;
       }
     }
-    if (single) {
-      const int rr = tile * kTile + r, ii = static_cast<int>(fdiv(rr, a.by_g)), hh = kvh * a.g + rr - ii * a.g;
-      const int64_t at = (static_cast<int64_t>(b) * a.T + ii) * a.Hq + hh;
-      const float inv = L == 0.f ? 0.f : 1.f / L;
-      f16x4 y;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = static_cast<_Float16>(L == 0.f ? 0.f : acc[e] * inv);
-      *reinterpret_cast<f16x4*>(a.out + at * D + d) = y;
-      if (a.lse && d == 0) a.lse[at] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+    if (pc.whole) {
+      const int rr = tile * kTile + r, ii = static_cast<int>(fdiv(rr, a.by_g));
+      store_row4<D>(a, b, ii, kvh * a.g + rr - ii * a.g, d, acc, M, L);
     } else {
-      *reinterpret_cast<f32x4*>(a.ws + (slot * width + r) * D + d) = acc;
+      *reinterpret_cast<f32x4*>(partial_o(a, range, tile, pc.slot, r, D) + d) = acc;
       if (d == 0) {
-        float* ml = a.ws + slots * width * D + (slot * width + r) * 2;
+        float* ml = partial_ml(a, range, tile, pc.slot, r, D);
         ml[0] = M, ml[1] = L;
       }
     }
+  }
+  advance(a, walk, pc);
+  __syncthreads();  // LDS is read before the next piece writes it
   }
 }
 
 // ---------------------------------------------------------- wide drafts --
 //
-// W wavefronts, 32 rows each, share every page of a chunk through LDS: K [D/64,
-// 64 tok, 64] and V [D, 64 tok] as fp16, in two slots.  8-bit pages are
-// converted once on the way in.  A 128-byte row is 8 units of 16 bytes; unit u
-// lies at u ^ swz(row), so that the 16 lanes that a read serves at once, and a
+// 8 wavefronts share every page through LDS: RT = 8 row tiles of 32 rows, each
+// wavefront's own, or RT = 4, where a wavefront takes one half of each page's
+// tokens and the two of a tile join at the end.  K [D/64, 64 tok, 64] lies in
+// three slots and V [D, 64 tok] in two, as fp16; 8-bit pages are converted once
+// on the way in.  A 128-byte row is 8 units of 16 bytes; unit u lies at
+// u ^ swz(row), so that the 16 lanes that a read serves at once, and a
 // conversion's 16 stores, meet 16 different bank groups.
+//
+// The matrix products of one 32-token half run beside the softmax of another:
+// while the weights of half i are formed, the scores of half i + 1 are
+// multiplied, and while those weights meet V, the scores' maximum is taken.  K
+// therefore runs one page ahead of V.
 __device__ __forceinline__ int swz_k(int row) { return ((row >> 1) & 3) | ((((row >> 3) ^ (row >> 4)) & 1) << 2); }
 __device__ __forceinline__ int swz_v(int row) { return (row >> 1) & 7; }
 
 typedef __amdgpu_buffer_rsrc_t Rsrc;
+constexpr int kWideWaves = 8;
 
-template <int CT, int D, int W>
-__global__ __launch_bounds__(W * 64, 2) void tree_wide_kernel(TreeArgs a) {
-  constexpr int DS = D / 32;
-  constexpr int TILE = kPage * D * 2;         // bytes of a K or a V tile
-  constexpr int SLOT = 2 * TILE;
-  constexpr int KU = kPage * D / 16;            // 8-bit: units of a K or a V page
-  constexpr int UNITS = 2 * KU / (W * 64);      // of both, that a thread converts
-  static_assert(CT == kF16 || (UNITS >= 1 && KU % 64 == 0), "every thread has a unit, and a wavefront's are all K or all V");
-  __shared__ __align__(16) char s_kv[2 * SLOT];
-  __shared__ __align__(16) float s_sc[2][3][kPage];  // 8-bit: score factors, V's scales' logarithms and inverses
-  __shared__ uint64_t s_odd[2][2];                   // and which of V's scales are not finite, and infinite
+template <int CT, int D, int RT>
+__global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs a) {
+  constexpr int W = kWideWaves, DS = D / 32;
+  constexpr int TILE = kPage * D * 2;  // bytes of a K or a V tile
+  constexpr int KU = kPage * D / 16;   // 8-bit: units of a K or a V page, one for each thread (D 64: K's and V's share them)
+  static_assert(RT == W || 2 * RT == W, "a wavefront takes a page or a half of it");
+  __shared__ __align__(16) char s_kv[5 * TILE];
+  __shared__ __align__(16) float s_sc[3][3][kPage];  // 8-bit: score factors, V's scales' logarithms and inverses
+  __shared__ __align__(16) float s_vs[3][kPage];     // V's scales where they are not finite, else 0
+  __shared__ int s_odd[3];                           // whether any is not
+  __shared__ float s_ml[RT == W ? 1 : RT * 64 * 2];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
   const int col = lane & 31, half = lane >> 5;
-  const uint32_t blk = blockIdx.x, lo8 = blk & 7, hi = blk >> 3;
-  const uint32_t hi_t = fdiv(hi, a.by_blocks), rb = hi - hi_t * a.row_blocks, item = hi_t * 8 + lo8;
-  const uint32_t chunk = fdiv(item, a.by_pairs), pair = item - chunk * a.pairs;
-  if (chunk >= static_cast<uint32_t>(a.max_chunks)) return;
-  const uint32_t b = fdiv(pair, a.by_hkv), kvh = pair - b * a.Hkv;
-  const Seq sq = seq_of(a, b);
-  const int nch = chunks_of(sq.pages, a.chunk_pages);
-  if (static_cast<int>(chunk) >= nch) return;
-  const int total = sq.ctx + (a.draft_keys ? sq.n : 0);
-  const int p0 = static_cast<int>(static_cast<int64_t>(chunk) * sq.pages / nch);
-  const int p1 = static_cast<int>(static_cast<int64_t>(chunk + 1) * sq.pages / nch);
-  const int tile = rb * W + wave;
-  const Row row = row_of(a, sq, b, kvh, tile * kTile + col);
-  Pages pages(a, b, kvh, lane, p0);
-  bool odd = false;
-  const bool block_live = static_cast<int>(rb) * W * kTile < sq.n * a.g;  // some row of the workgroup is drafted
-  const bool wave_live = tile * kTile < sq.n * a.g;
-  f16x8 qf[DS][2];
-  load_q<DS>(a, b, row, half, qf);
-  f32x16 o[DS];
-#pragma unroll
-  for (int dt = 0; dt < DS; ++dt)
-#pragma unroll
-    for (int x = 0; x < 16; ++x) o[dt][x] = 0.f;
-  float m = -INFINITY, l = 0.f;
+  const int part = RT == W ? 0 : wave & 1;  // RT 4: this wavefront's half of a page
+  int range, rb;
+  place_of(a, range, rb);
+  Walk walk;
+  if (range >= a.ranges || !walk.start(a, lane, range)) return;
 
   // fp16 pages go straight into LDS: load i of a tile fills its bytes 1024 i
   // .., lane by lane, so each lane fetches the unit that belongs at its place.
   const int l8 = lane / 8;
   const int k_src = 1024 * wave + 128 * l8 + (((lane % 8) ^ swz_k(8 * wave + l8)) * 16);
   const int v_src = 1024 * wave + 128 * l8 + (((lane % 8) ^ swz_v(8 * wave + l8)) * 16);
-  static_assert(W % 4 == 0, "the loads of a wavefront share their swizzle");
-  // 8-bit: the next page's units and scales, in registers.
-  u32x4 raw[CT == kF16 ? 1 : UNITS];
-  float scale = 0.f;
-  auto fetch = [&](int p, int slot) {
-    const int64_t head = pages.head(p);
-    if constexpr (CT == kF16) {
-      const uint8_t *kp = a.k + head * TILE, *vp = a.v + head * TILE;
-      const Rsrc kr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(kp), 0, TILE, 0x00020000);
-      const Rsrc vr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(vp), 0, TILE, 0x00020000);
-#pragma unroll
-      for (int j = 0; j < TILE / 1024 / W; ++j) {
-        char* dk = s_kv + slot * SLOT + 1024 * (wave + W * j);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (__attribute__((address_space(3))) void*)dk, 16, k_src, 1024 * W * j, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (__attribute__((address_space(3))) void*)(dk + TILE), 16, v_src,
-                                                 1024 * W * j, 0, 0);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < UNITS; ++j) {
-        const int w0 = (wave + j * W) * 64;  // this wavefront's first unit, of K's and then V's
-        const uint8_t* p8 = w0 < KU ? a.k + head * (TILE / 2) + w0 * 16 : a.v + head * (TILE / 2) + (w0 - KU) * 16;
-        raw[j] = *reinterpret_cast<const u32x4*>(p8 + lane * 16);
-      }
-      if (wave < 2) scale = (wave ? a.vs : a.ks)[head * kPage + lane];
-    }
-  };
-  // 8-bit: what fetch() brought, into a slot.
-  auto store = [&](int slot) {
-    if constexpr (CT != kF16) {
-      char* k0 = s_kv + slot * SLOT;
-      auto two = [&](char* at, int u, int sw, const u32x4& w) {  // units u and u + 1 of a row
-        *reinterpret_cast<f16x8*>(at + ((u ^ sw) * 16)) = codes_to_f16x8<CT>(w[0], w[1]);
-        *reinterpret_cast<f16x8*>(at + (((u + 1) ^ sw) * 16)) = codes_to_f16x8<CT>(w[2], w[3]);
-      };
-#pragma unroll
-      for (int j = 0; j < UNITS; ++j) {
-        const int w0 = (wave + j * W) * 64;
-        if (w0 < KU) {  // 16 features un of a token
-          const int un = w0 / kPage, tok = lane;
-          two(k0 + (un / 4) * (kPage * 128) + tok * 128, 2 * (un % 4), swz_k(tok), raw[j]);
-        } else {  // 16 tokens q4 of a feature
-          const int x = w0 - KU + lane, q4 = x / D, d = x % D;
-          two(k0 + TILE + d * 128, 2 * q4, swz_v(d), raw[j]);
-        }
-      }
-      if (wave == 0) s_sc[slot][0][lane] = scale * a.scale_log2;
-      if (wave == 1) {
-        const bool finite = __builtin_fabsf(scale) <= 0x1.fffffep127f;
-        const float vc = !finite ? 1.f : scale < 0x1p-60f ? 0x1p-60f : scale;  // 0: codes of no weight
-        s_sc[slot][1][lane] = __builtin_amdgcn_logf(vc);
-        s_sc[slot][2][lane] = __builtin_amdgcn_rcpf(vc);
-        const uint64_t not_finite = __builtin_amdgcn_ballot_w64(!finite);
-        const uint64_t infinite = __builtin_amdgcn_ballot_w64(scale == INFINITY);
-        if (lane == 0) s_odd[slot][0] = not_finite, s_odd[slot][1] = infinite;
-      }
-    }
-  };
-
-  // Operand addresses in a slot: unit u of a row is (bits of the unroll) ^
-  // (bits of the lane), four of each.
+  // Operand addresses in a tile: unit u of a row is (bits of the unroll) ^
+  // (bits of the lane).
   const int tok = token_of(col);
-  const int k_row = tok * 128, v_row = col * 128;
   const int k_x = (2 * half) ^ swz_k(tok), v_x = (2 * half) ^ swz_v(col);
   int k_at[2][2];
 #pragma unroll
   for (int y = 0; y < 2; ++y)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) k_at[y][e] = k_row + ((k_x ^ (4 * y + e)) * 16);
+    for (int e = 0; e < 2; ++e) k_at[y][e] = tok * 128 + ((k_x ^ (4 * y + e)) * 16);
+  const float c = __builtin_fabsf(a.scale_log2);  // its sign is in q
 
-  // The 32 tokens from half t of page p on.
-  auto step = [&](int p, int slot, int t, auto edge_tag) {
-    constexpr bool EDGE = decltype(edge_tag)::value;
-    const char* base = s_kv + slot * SLOT;
-    const int s0 = 32 * t + 16 * half, tok0 = p * kPage + s0;  // this lane's 16 tokens
-    uint32_t seen = 0;
-    if constexpr (EDGE) seen = row.attends16(a, sq, tok0, total);
-    f32x16 sc;
+  for (; walk.u < walk.end;) {
+    const Piece pc = piece_of(a, walk, range);
+    const int b = walk.b, kvh = pc.kvh;
+    const Seq sq = seq_at(a, b);
+    const int total = sq.ctx + (a.draft_keys ? sq.n : 0);
+    const int p0 = pc.page0, p1 = min(pc.page1, sq.pages);
+    const int local = RT == W ? wave : wave >> 1, tile = rb * RT + local;
+    const Row row = row_of(a, sq, b, kvh, tile * kTile + col);
+    Pages pages(a, b, kvh, lane, p0);
+    bool odd = false;
+    const bool block_live = rb * RT * kTile < sq.n * a.g;  // some row of the workgroup is drafted
+    const bool wave_live = tile * kTile < sq.n * a.g;
+    f16x8 qf[DS][2];
+    load_q<DS>(a, b, row, half, qf);
+    if (a.scale_log2 < 0.f) {
 #pragma unroll
-    for (int x = 0; x < 16; ++x) sc[x] = 0.f;
+      for (int s = 0; s < DS; ++s)
 #pragma unroll
-    for (int s = 0; s < DS; ++s)
+        for (int e = 0; e < 2; ++e) qf[s][e] = -qf[s][e];
+    }
+    f32x16 o[DS];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const f16x8 k = *reinterpret_cast<const f16x8*>(base + t * (32 * 128) + k_at[s % 2][e] + (s / 2) * (kPage * 128));
-        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[s][e], sc, 0, 0, 0);
+    for (int dt = 0; dt < DS; ++dt)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) o[dt][x] = 0.f;
+    float m = -INFINITY, l = 0.f;
+
+    // A page's K or V into its slot: fp16 by loads into LDS; 8-bit by way of
+    // registers (take, then put a step later).
+    auto k_tile = [&](int s3) { return s_kv + s3 * TILE; };
+    auto v_tile = [&](int s2) { return s_kv + (3 + s2) * TILE; };
+    auto dma = [&](const uint8_t* cache, int64_t head, char* to, int src) {
+      const Rsrc r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(cache + head * TILE), 0, TILE, 0x00020000);
+#pragma unroll
+      for (int j = 0; j < TILE / 1024 / W; ++j)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(to + 1024 * (wave + W * j)), 16,
+                                                 src, 1024 * W * j, 0, 0);
+    };
+    // 8-bit: D 128: every thread a unit of K and one of V; D 64: the first
+    // wavefronts K's, the others V's.  Scales: K's by wavefront 0, V's by 1.
+    u32x4 k_raw, v_raw;
+    float scale = 0.f;
+    const bool has_k = wave * 64 < KU, has_v = D == 128 || wave * 64 >= KU;
+    const int v_unit0 = D == 128 ? wave * 64 : wave * 64 - KU;
+    auto take_k = [&](int64_t head) {
+      if (has_k) k_raw = *reinterpret_cast<const u32x4*>(a.k + head * (TILE / 2) + (wave * 64 + lane) * 16);
+      if (wave < 2) scale = (wave ? a.vs : a.ks)[head * kPage + lane];
+    };
+    auto take_v = [&](int64_t head) {
+      if (has_v) v_raw = *reinterpret_cast<const u32x4*>(a.v + head * (TILE / 2) + (v_unit0 + lane) * 16);
+    };
+    auto put = [&](char* at, int u, int sw, const u32x4& w) {  // units u and u + 1 of a row
+      *reinterpret_cast<f16x8*>(at + ((u ^ sw) * 16)) = codes_to_f16x8<CT>(w[0], w[1]);
+      *reinterpret_cast<f16x8*>(at + (((u + 1) ^ sw) * 16)) = codes_to_f16x8<CT>(w[2], w[3]);
+    };
+    auto put_k = [&](int s3) {
+      int ln = lane;
+      asm volatile("" : "+v"(ln));  // its addresses are not worth registers of the products
+      if (has_k) {
+        const int un = wave * 64 / kPage;  // 16 features of token ln
+        put(k_tile(s3) + (un / 4) * (kPage * 128) + ln * 128, 2 * (un % 4), swz_k(ln), k_raw);
       }
-    float mx = -INFINITY;
+      if (wave == 0) s_sc[s3][0][ln] = scale * c;
+      if (wave == 1) {
+        const bool finite = __builtin_fabsf(scale) <= 0x1.fffffep127f;
+        const float vc = !finite ? 1.f : scale < 0x1p-60f ? 0x1p-60f : scale;  // 0: codes of no weight
+        s_sc[s3][1][ln] = __builtin_amdgcn_logf(vc);
+        s_sc[s3][2][ln] = __builtin_amdgcn_rcpf(vc);
+        s_vs[s3][ln] = finite ? 0.f : scale;
+        if (lane == 0) s_odd[s3] = 0;
+        if (!finite) s_odd[s3] = 1;
+      }
+    };
+    auto put_v = [&](int s2) {
+      int ln = lane;
+      asm volatile("" : "+v"(ln));
+      if (has_v) {  // 16 tokens of a feature
+        const int x = v_unit0 + ln, q4 = x / D, d = x % D;
+        put(v_tile(s2) + d * 128, 2 * q4, swz_v(d), v_raw);
+      }
+    };
+    // 8-bit V whose scales are not finite: their numbers as the scales leave them.
+    auto patch_v = [&](int s2, int s3) {
+      for (int i = threadIdx.x; i < kPage * D; i += W * 64) {
+        const int d = i / kPage, t = i % kPage;
+        const float vs = s_vs[s3][t];
+        if (!(vs == 0.f)) {
+          _Float16* at = reinterpret_cast<_Float16*>(v_tile(s2) + d * 128 + (((t / 8) ^ swz_v(d)) * 16)) + t % 8;
+          *at = static_cast<_Float16>(static_cast<float>(*at) * vs);
+        }
+      }
+    };
+
+    // The scores of half t of a K tile.
+    auto scores = [&](f32x16& s, const char* kt, int t) {
 #pragma unroll
-    for (int x4 = 0; x4 < 4; ++x4) {
-      f32x4 f, lv;
+      for (int x = 0; x < 16; ++x) s[x] = 0.f;
+#pragma unroll
+      for (int i = 0; i < DS; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const f16x8 k = *reinterpret_cast<const f16x8*>(kt + t * (32 * 128) + k_at[i % 2][e] + (i / 2) * (kPage * 128));
+          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[i][e], s, 0, 0, 0);
+        }
+    };
+    // 8-bit: scores scaled, V's scales added.  The largest, in log2 units.
+    auto largest = [&](f32x16& s, int s3, int t) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int x4 = 0; x4 < 4; ++x4) {
+        f32x4 f, lv;
+        if constexpr (CT != kF16) {
+          f = *reinterpret_cast<const f32x4*>(&s_sc[s3][0][32 * t + 16 * half + 4 * x4]);
+          lv = *reinterpret_cast<const f32x4*>(&s_sc[s3][1][32 * t + 16 * half + 4 * x4]);
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          if constexpr (CT != kF16) s[4 * x4 + y] = __builtin_fmaf(s[4 * x4 + y], f[y], lv[y]);
+          mx = fmaxf(mx, s[4 * x4 + y]);
+        }
+      }
+      return xor32_max(mx) * (CT == kF16 ? c : 1.f);
+    };
+    auto rescale = [&](float mx) {
+      if (__any(mx > m + kSlack)) {
+        const float mn = fmaxf(m, mx);
+        const float alpha = m == -INFINITY ? 0.f : exp2_of(m - mn);
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DS; ++dt)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) o[dt][x] *= alpha;
+      }
+    };
+    // The step of a half whose scores are `cur` (half t of the page whose V is
+    // vt and whose scales are in slot s3), beside the scores `nxt` of the next
+    // half (tn of kt, slot n3); returns the largest of those.  First the next
+    // scores' products with the weights, then the values' products with the
+    // maximum.  The scheduling barriers keep each product beside its share of
+    // the softmax, and operands three products ahead.
+    auto step = [&](const f32x16& cur, f32x16& nxt, const char* kt, int tn, int n3, const char* vt, int t, int s3) {
+      constexpr int N = 2 * DS, PER = 16 / N, AHEAD = 3;
+      const char* v_at[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) v_at[e] = vt + col * 128 + ((v_x ^ (4 * t + e)) * 16);
+      // operands 0 .. N - 1: K's; N .. 2 N - 1: V's
+      f16x8 x[2 * N];
+      auto read = [&](int i) {
+        if (i < N)
+          x[i] = *reinterpret_cast<const f16x8*>(kt + tn * (32 * 128) + k_at[(i / 2) % 2][i % 2] + (i / 4) * (kPage * 128));
+        else if (i < 2 * N)
+          x[i] = *reinterpret_cast<const f16x8*>(v_at[(i - N) / DS] + (i - N) % DS * (32 * 128));
+      };
+      f32x4 r[4], f[4], lv[4];
+      const float *sc0 = &s_sc[s3][2][32 * t + 16 * half], *sc1 = &s_sc[n3][0][32 * tn + 16 * half];
       if constexpr (CT != kF16) {
-        f = *reinterpret_cast<const f32x4*>(&s_sc[slot][0][s0 + 4 * x4]);
-        lv = *reinterpret_cast<const f32x4*>(&s_sc[slot][1][s0 + 4 * x4]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = *reinterpret_cast<const f32x4*>(sc0 + 4 * i);
       }
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const int x = 4 * x4 + y;
-        float v = CT == kF16 ? sc[x] * a.scale_log2 : __builtin_fmaf(sc[x], f[y], lv[y]);
-        if constexpr (EDGE) v = (seen >> x) & 1 ? v : -INFINITY;
-        sc[x] = v;
-        mx = fmaxf(mx, v);
+      for (int i = 0; i < AHEAD; ++i) read(i);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) nxt[i] = 0.f;
+      f16x8 pw[2];
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        read(i + AHEAD);
+        nxt = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[i], qf[i / 2][i % 2], nxt, 0, 0, 0);
+#pragma unroll
+        for (int y = PER * i; y < PER * (i + 1); ++y) {
+          const float w = exp2_of(CT == kF16 ? __builtin_fmaf(cur[y], c, -m) : cur[y] - m);
+          l = CT == kF16 ? l + w : __builtin_fmaf(w, r[y / 4][y % 4], l);
+          pw[y / 8][y % 8] = static_cast<_Float16>(w);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-    }
-    mx = xor32_max(mx);
-    if (__any(mx > m + kSlack)) {
-      const float mn = fmaxf(m, mx);
-      const float alpha = m == -INFINITY ? 0.f : exp2_of(m - mn);
-      m = mn;
-      l *= alpha;
+      float mx = -INFINITY;
+      auto scale4 = [&](int i) {
+        if constexpr (CT != kF16) {
+          f[i] = *reinterpret_cast<const f32x4*>(sc1 + 4 * i);
+          lv[i] = *reinterpret_cast<const f32x4*>(sc1 + kPage + 4 * i);
+        }
+      };
+      auto max4 = [&](int i) {
 #pragma unroll
-      for (int dt = 0; dt < DS; ++dt)
+        for (int y = 4 * i; y < 4 * i + 4; ++y) {
+          if constexpr (CT != kF16) nxt[y] = __builtin_fmaf(nxt[y], f[i][y % 4], lv[i][y % 4]);
+          mx = fmaxf(mx, nxt[y]);
+        }
+      };
+      if constexpr (N == 4) {
 #pragma unroll
-        for (int x = 0; x < 16; ++x) o[dt][x] *= alpha;
-    }
-    const float mu = m == -INFINITY ? 0.f : m;
-    f16x8 pw[2];
+        for (int i = 0; i < 4; ++i) scale4(i);
+      }
 #pragma unroll
-    for (int x4 = 0; x4 < 4; ++x4) {
-      f32x4 r;
-      if constexpr (CT != kF16) r = *reinterpret_cast<const f32x4*>(&s_sc[slot][2][s0 + 4 * x4]);
+      for (int i = 0; i < N; ++i) {
+        read(N + i + AHEAD);
+        if (N == 8 && i < 4) scale4(i);
+        o[i % DS] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[N + i], pw[i / DS], o[i % DS], 0, 0, 0);
+        if (N == 4 || i >= 4) max4(i % 4);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      return xor32_max(mx) * (CT == kF16 ? c : 1.f);
+    };
+    // Half t of a page with drafted tokens, or the sequence's end: one thing
+    // after the other, each token tested.
+    auto edge = [&](int p, int s3, int s2, int t) {
+      const int tok0 = p * kPage + 32 * t + 16 * half;  // this lane's 16 tokens
+      const uint32_t seen = row.attends16(a, sq, tok0, total);
+      f32x16 s;
+      scores(s, k_tile(s3), t);
+      float mx = -INFINITY;
+      largest(s, s3, t);
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const int x = 4 * x4 + y;
-        const float w = exp2_of(sc[x] - mu);
-        if constexpr (CT == kF16)
-          l += w;
-        else
-          l = __builtin_fmaf(w, EDGE && !((seen >> x) & 1) ? 0.f : r[y], l);
+      for (int x = 0; x < 16; ++x) {
+        const float v = CT == kF16 ? s[x] * c : s[x];
+        s[x] = (seen >> x) & 1 ? v : -INFINITY;
+        mx = fmaxf(mx, s[x]);
+      }
+      rescale(xor32_max(mx));
+      const float mu = m == -INFINITY ? 0.f : m;  // a row that has attended nothing yet: weights 0
+      f16x8 pw[2];
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const float w = exp2_of(s[x] - mu);
+        const float r = CT == kF16 ? 1.f : s_sc[s3][2][32 * t + 16 * half + x];
+        l = __builtin_fmaf(w, (seen >> x) & 1 ? r : 0.f, l);
         pw[x / 8][x % 8] = static_cast<_Float16>(w);
       }
-    }
-    if constexpr (CT != kF16) {
-      const uint32_t not_finite = static_cast<uint32_t>(s_odd[slot][0] >> s0) & 0xffffu;
-      if (__any(not_finite != 0)) {
-        const uint32_t infinite = static_cast<uint32_t>(s_odd[slot][1] >> s0) & 0xffffu;
 #pragma unroll
-        for (int x = 0; x < 16; ++x)
-          if ((not_finite >> x) & 1 && (!EDGE || (seen >> x) & 1))
-            pw[x / 8][x % 8] = static_cast<_Float16>((infinite >> x) & 1 ? INFINITY : NAN);
-      }
-    }
+      for (int e = 0; e < 2; ++e) {
+        const char* v_at = v_tile(s2) + col * 128 + ((v_x ^ (4 * t + e)) * 16);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const char* v_at = base + TILE + v_row + ((v_x ^ (4 * t + e)) * 16);
-#pragma unroll
-      for (int dt = 0; dt < DS; ++dt) {
-        u32x4 v = *reinterpret_cast<const u32x4*>(v_at + dt * (32 * 128));
-        if constexpr (EDGE) {  // as in the rows kernel
-          const int keep = total - tok0 - 8 * e;
+        for (int dt = 0; dt < DS; ++dt) {
+          u32x4 v = *reinterpret_cast<const u32x4*>(v_at + dt * (32 * 128));
+          const int keep = total - tok0 - 8 * e;  // as in the rows kernel
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int k = keep - 2 * i;
@@ -727,114 +954,216 @@ __global__ __launch_bounds__(W * 64, 2) void tree_wide_kernel(TreeArgs a) {
             odd = drop_odd<kF16>(w) || odd;
             v[i] = w;
           }
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v), pw[e], o[dt], 0, 0, 0);
         }
-        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v), pw[e], o[dt], 0, 0, 0);
       }
-    }
-  };
+    };
 
-  if (block_live && p0 < p1) {
-    fetch(p0, 0);
-    if constexpr (CT != kF16) {
-      store(0);
-      if (p0 + 1 < p1) fetch(p0 + 1, 1);
-    }
-    const int whole = min(p1, sq.ctx / kPage);
-    for (int p = p0; p < p1; ++p) {
-      const int slot = (p - p0) & 1;
-      if constexpr (CT == kF16) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();  // page p is in its slot, and every wavefront is done with the other one
+    if (block_live && p0 < p1) {
+      // Page p's K lies in slot (p - p0) % 3 and its V in (p - p0) % 2.  At the
+      // top of page p, K of pages p and p + 1 and V of page p have arrived.
+      const bool two = p0 + 1 < p1;
+      int64_t head = pages.head(p0);
       if constexpr (CT == kF16) {
-        if (p + 1 < p1) fetch(p + 1, slot ^ 1);
+        dma(a.k, head, k_tile(0), k_src);
+        dma(a.v, head, v_tile(0), v_src);
+        if (two) {
+          head = pages.head(p0 + 1);
+          dma(a.k, head, k_tile(1), k_src);
+        }
       } else {
-        if (p + 1 < p1) store(slot ^ 1);
-        if (p + 2 < p1) fetch(p + 2, slot);
+        take_k(head);
+        take_v(head);
+        put_k(0);
+        put_v(0);
+        if (two) {
+          head = pages.head(p0 + 1);
+          take_k(head);
+          take_v(head);
+          put_k(1);
+          if (p0 + 2 < p1) {
+            head = pages.head(p0 + 2);
+            take_k(head);
+          }
+        }
       }
-      if (wave_live) {
-        if (p < whole) {
-          step(p, slot, 0, std::false_type{});
-          step(p, slot, 1, std::false_type{});
+      const int whole = min(p1, sq.ctx / kPage);
+      int s3 = 0, s2 = 0;
+      f32x16 sa, sb;
+      // The top of page p: its arrivals, and the loads of what comes after.
+      auto top = [&](int p) {
+        const int f3 = s3 == 0 ? 2 : s3 - 1;  // page p + 2's slot
+        if constexpr (CT == kF16) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();  // and every wavefront is done with page p - 1
+        if constexpr (CT == kF16) {
+          if (p + 1 < p1) dma(a.v, head, v_tile(s2 ^ 1), v_src);
+          if (p + 2 < p1) {
+            head = pages.head(p + 2);
+            dma(a.k, head, k_tile(f3), k_src);
+          }
         } else {
+          if (p + 1 < p1) put_v(s2 ^ 1);
+          if (p + 2 < p1) {
+            put_k(f3);
+            take_v(head);
+          }
+          if (p + 3 < p1) {
+            head = pages.head(p + 3);
+            take_k(head);
+          }
+          if (s_odd[s3]) {
+            patch_v(s2, s3);
+            __syncthreads();
+          }
+        }
+      };
+      auto next = [&] {
+        s3 = s3 == 2 ? 0 : s3 + 1;
+        s2 ^= 1;
+      };
+      if (wave_live) {
+        int p = p0;
+        if (p < whole) {  // sa: the scores of the page's first (or only) half
+          top(p);
+          scores(sa, k_tile(0), part);
+          rescale(largest(sa, 0, part));
+          for (;;) {
+            // (past the last whole page the scores ahead are of no page, and not used)
+            const int n3 = s3 == 2 ? 0 : s3 + 1;
+            const char *k0 = k_tile(s3), *k1 = k_tile(n3), *v0 = v_tile(s2);
+            float mx;
+            if constexpr (RT == W) {
+              mx = step(sa, sb, k0, 1, s3, v0, 0, s3);
+              rescale(mx);
+              mx = step(sb, sa, k1, 0, n3, v0, 1, s3);
+            } else {
+              mx = step(sa, sb, k1, part, n3, v0, part, s3);
+              sa = sb;
+            }
+            next();
+            if (++p == whole) break;
+            rescale(mx);
+            top(p);
+          }
+        }
+        for (; p < p1; ++p, next()) {
+          top(p);
+          if constexpr (RT == W) {
 #pragma unroll 1
-          for (int t = 0; t < 2; ++t) step(p, slot, t, std::true_type{});
+            for (int t = 0; t < 2; ++t) edge(p, s3, s2, t);
+          } else {
+            edge(p, s3, s2, part);
+          }
+        }
+      } else {
+        for (int p = p0; p < p1; ++p, next()) top(p);
+      }
+      if (__any(odd)) {
+        const int t0 = max(p0, whole) * kPage, t1 = min(p1 * kPage, total);
+        if constexpr (RT == W)
+          add_odd<CT, D>(a, sq, b, kvh, row, lane, t0, t1, -1, o);
+        else
+          add_odd<CT, D>(a, sq, b, kvh, row, lane, t0, t1, part, o);
+      }
+    }
+    l = xor32_sum(l);
+    if (!row.live) m = -INFINITY, l = 0.f;
+    if ((pages.poisoned || sq.bad) && row.live) l = NAN;
+    if constexpr (RT != W) {  // the second half's wavefront hands over
+      f32x4* x = reinterpret_cast<f32x4*>(s_kv) + local * (DS * 4 * 64) + lane;
+      __syncthreads();  // the tiles are read
+      if (part == 1) {
+#pragma unroll
+        for (int i = 0; i < DS * 4; ++i)
+          x[i * 64] = f32x4{o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1], o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]};
+        s_ml[(local * 64 + lane) * 2] = m;
+        s_ml[(local * 64 + lane) * 2 + 1] = l;
+      }
+      __syncthreads();
+      if (part == 0) {
+        const float m1 = s_ml[(local * 64 + lane) * 2], l1 = s_ml[(local * 64 + lane) * 2 + 1];
+        const float M = fmaxf(m, m1);
+        const float f0 = m == -INFINITY ? 0.f : exp2_of(m - M), f1 = m1 == -INFINITY ? 0.f : exp2_of(m1 - M);
+        l = (m == -INFINITY ? l : l * f0) + (m1 == -INFINITY ? l1 : l1 * f1);  // l without a reference is 0, or NaN
+        m = M;
+#pragma unroll
+        for (int i = 0; i < DS * 4; ++i) {
+          const f32x4 y = x[i * 64];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float z = f0 == 0.f ? 0.f : o[i / 4][4 * (i % 4) + e] * f0;
+            if (f1 != 0.f) z += y[e] * f1;
+            o[i / 4][4 * (i % 4) + e] = z;
+          }
         }
       }
     }
-    if (CT != SPYRE_CODES_INT8 && __any(odd))
-      add_odd<CT, D>(a, sq, b, kvh, row, lane, max(p0, whole) * kPage, min(p1 * kPage, total), o);
-  }
-  l = xor32_sum(l);
-  if (!row.live) m = -INFINITY, l = 0.f;
-  if ((pages.poisoned || sq.bad) && row.live) l = NAN;
-  if (tile * kTile + col >= a.rows) return;
-  if (nch == 1) {
-    const int64_t at = (static_cast<int64_t>(b) * a.T + row.i) * a.Hq + row.head;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (part == 0 && tile * kTile + col < a.rows) {
+      float* x = partial_o(a, range, rb, pc.slot, local * kTile + col, D) + 4 * half;
 #pragma unroll
-    for (int dt = 0; dt < DS; ++dt)
+      for (int dt = 0; dt < DS; ++dt)
 #pragma unroll
-      for (int x4 = 0; x4 < 4; ++x4) {
-        f16x4 y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = static_cast<_Float16>(l == 0.f ? 0.f : o[dt][4 * x4 + e] * inv);
-        *reinterpret_cast<f16x4*>(a.out + at * D + 32 * dt + 8 * x4 + 4 * half) = y;
+        for (int x4 = 0; x4 < 4; ++x4) {
+          const f32x4 y = {o[dt][4 * x4], o[dt][4 * x4 + 1], o[dt][4 * x4 + 2], o[dt][4 * x4 + 3]};
+          if (pc.whole)
+            store_row4<D>(a, b, row.i, row.head, 32 * dt + 8 * x4 + 4 * half, y, m, l);
+          else
+            *reinterpret_cast<f32x4*>(x + 32 * dt + 8 * x4) = y;
+        }
+      if (!pc.whole && half == 0) {
+        float* ml = partial_ml(a, range, rb, pc.slot, local * kTile + col, D);
+        ml[0] = m, ml[1] = l;
       }
-    if (a.lse && half == 0) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
-  } else {
-    const int64_t slot = (static_cast<int64_t>(pair) * a.tiles + tile) * a.max_chunks + chunk;
-    const int64_t slots = static_cast<int64_t>(a.pairs) * a.tiles * a.max_chunks;
-    float* x = a.ws + (slot * kTile + col) * D + 4 * half;
-#pragma unroll
-    for (int dt = 0; dt < DS; ++dt)
-#pragma unroll
-      for (int x4 = 0; x4 < 4; ++x4)
-        *reinterpret_cast<f32x4*>(x + 32 * dt + 8 * x4) =
-            f32x4{o[dt][4 * x4], o[dt][4 * x4 + 1], o[dt][4 * x4 + 2], o[dt][4 * x4 + 3]};
-    if (half == 0) {
-      float* ml = a.ws + slots * kTile * D + (slot * kTile + col) * 2;
-      ml[0] = m, ml[1] = l;
     }
+    advance(a, walk, pc);
+    __syncthreads();  // LDS is read before the next piece writes it
   }
 }
 
-// Joins the chunks of sequences that have several: a thread 4 features of a row.
+// Joins the partials of each (sequence, KV head) that several ranges share: a
+// thread 4 features of a row.
 template <int D>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
-  const int64_t u = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t r_all = u / (D / 4);
-  const int d = 4 * static_cast<int>(u % (D / 4));
-  if (r_all >= static_cast<int64_t>(a.pairs) * a.rows) return;
-  const uint32_t pair = static_cast<uint32_t>(r_all / a.rows), row = static_cast<uint32_t>(r_all % a.rows);
-  const uint32_t b = fdiv(pair, a.by_hkv), kvh = pair - b * a.Hkv;
-  const Seq sq = seq_of(a, b);
-  const int nch = chunks_of(sq.pages, a.chunk_pages);
-  if (nch == 1) return;
-  const int tile = row / kTile, r = row % kTile, width = min(kTile, a.rows);
-  const int64_t slot0 = (static_cast<int64_t>(pair) * a.tiles + tile) * a.max_chunks;
-  const int64_t slots = static_cast<int64_t>(a.pairs) * a.tiles * a.max_chunks;
-  const float* ml = a.ws + slots * width * D + (slot0 * width + r) * 2;
-  const float* x = a.ws + (slot0 * width + r) * D + d;
+  const uint32_t pair = blockIdx.x, b = fdiv(pair, a.by_hkv), kvh = pair - b * a.Hkv;
+  const int u = blockIdx.y * 256 + threadIdx.x, row = u / (D / 4), d = 4 * (u % (D / 4));
+  Walk w;
+  w.seek(a, threadIdx.x % 64, b);
+  const int g0 = w.base * a.Hkv + kvh * w.pages, g1 = g0 + w.pages;
+  const int r0 = g0 / w.per, r1 = (g1 - 1) / w.per;
+  if (r0 == r1 || row >= a.rows) return;
+  const Seq sq = seq_at(a, b);
+  const int ii = static_cast<int>(fdiv(row, a.by_g)), rb = row / a.block_rows, rl = row - rb * a.block_rows;
   float M = -INFINITY, L = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int c = 0; c < nch; ++c) M = fmaxf(M, ml[static_cast<int64_t>(c) * width * 2]);
-  for (int c = 0; c < nch; ++c) {
-    const float mc = ml[static_cast<int64_t>(c) * width * 2], lc = ml[static_cast<int64_t>(c) * width * 2 + 1];
-    const float f = mc == -INFINITY ? 0.f : exp2_of(mc - M);
-    L += mc == -INFINITY ? lc : lc * f;
-    if (mc != -INFINITY) {
-      const f32x4 y = *reinterpret_cast<const f32x4*>(x + static_cast<int64_t>(c) * width * D);
+  if (ii < sq.n) {
+    constexpr int G = 8;  // partials in flight
+    for (int c = r0; c <= r1; c += G) {
+      float ml[G][2];
+      f32x4 x[G];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] += y[e] * f;
+      for (int k = 0; k < G; ++k) {
+        const int r = min(c + k, r1), slot = r * w.per < g0 ? 1 : 0;
+        const float* p = partial_ml(a, r, rb, slot, rl, D);
+        ml[k][0] = p[0], ml[k][1] = p[1];
+        x[k] = *reinterpret_cast<const f32x4*>(partial_o(a, r, rb, slot, rl, D) + d);
+      }
+      float mc = M;
+#pragma unroll
+      for (int k = 0; k < G; ++k) mc = fmaxf(mc, ml[k][0]);  // past r1 the last one again
+      const float f0 = M == -INFINITY ? 0.f : exp2_of(M - mc);
+      L *= f0;
+      acc *= f0;
+#pragma unroll
+      for (int k = 0; k < G; ++k) {
+        if (c + k > r1) break;
+        const float f = ml[k][0] == -INFINITY ? 0.f : exp2_of(ml[k][0] - mc);
+        L += ml[k][0] == -INFINITY ? ml[k][1] : ml[k][1] * f;  // l without a reference is 0, or NaN
+        if (ml[k][0] != -INFINITY) acc += x[k] * f;
+      }
+      M = mc;
     }
   }
-  const int ii = static_cast<int>(fdiv(row, a.by_g)), hh = kvh * a.g + row - ii * a.g;
-  const int64_t at = (static_cast<int64_t>(b) * a.T + ii) * a.Hq + hh;
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  f16x4 y;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) y[e] = static_cast<_Float16>(L == 0.f ? 0.f : acc[e] * inv);
-  *reinterpret_cast<f16x4*>(a.out + at * D + d) = y;
-  if (a.lse && d == 0) a.lse[at] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+  store_row4<D>(a, b, ii, kvh * a.g + row - ii * a.g, d, acc, M, L);
 }
 
 constexpr int kRowWaves = 4;
@@ -842,49 +1171,35 @@ constexpr int kRowWaves = 4;
 constexpr int kNarrowRows = 64;
 
 struct Plan {
-  int tiles, waves, row_blocks;  // waves 0: the rows kernel
-  int chunk_pages, max_chunks;
+  int wide;  // row tiles of a workgroup of the wide kernel; 0: the rows kernel
+  int row_blocks, block_rows, width, ranges, min_per;
   size_t ws_bytes;
 };
 
-// Chunks: enough workgroups to fill the device, each wavefront at least a
-// page, at most 8 pages a wavefront.
 Plan plan_of(int B, int T, int Hq, int Hkv, int D, int max_tokens) {
   Plan p;
   const int64_t rows = static_cast<int64_t>(T) * (Hq / Hkv);
-  p.tiles = static_cast<int>((rows + kTile - 1) / kTile);
-  p.waves = rows <= kNarrowRows ? 0 : rows <= 128 ? 4 : 8;
-  p.row_blocks = p.waves ? (p.tiles + p.waves - 1) / p.waves : p.tiles;
-  const int pages = pages_of(max_tokens);
-  const int64_t groups = static_cast<int64_t>(B) * Hkv * p.row_blocks;
-  if (p.waves == 0) {
-    int cp = 8 * kRowWaves;
-    while (cp > kRowWaves && groups * chunks_of(pages, cp) < 512) cp /= 2;
-    p.chunk_pages = cp;
-  } else {
-    // Rounds of the device times a workgroup's steps, its start counted as
-    // four of them.
-    const int64_t slots = p.waves == 8 ? 256 : 512;
-    int64_t best = INT64_MAX;
-    p.chunk_pages = std::max(pages, 1);
-    for (int n = 1; n <= std::max(pages, 1) && n <= 256; ++n) {
-      const int cp = (pages + n - 1) / n;
-      const int64_t rounds = (groups * n + slots - 1) / slots, cost = rounds * (cp + 4) + (n > 1 ? 4 : 0);
-      if (cost < best) best = cost, p.chunk_pages = std::max(cp, 1);
-    }
-  }
-  p.max_chunks = chunks_of(pages, p.chunk_pages);
-  const int64_t width = std::min<int64_t>(kTile, rows);
-  p.ws_bytes = p.max_chunks == 1 ? 0 : static_cast<size_t>(static_cast<int64_t>(B) * Hkv * p.tiles * p.max_chunks * width * (D + 2)) * 4;
+  p.wide = rows <= kNarrowRows ? 0 : rows <= 128 ? 4 : 8;
+  p.block_rows = kTile * std::max(p.wide, 1);
+  p.row_blocks = static_cast<int>((rows + p.block_rows - 1) / p.block_rows);
+  p.width = static_cast<int>(std::min<int64_t>(p.block_rows, rows));
+  p.min_per = 2;
+  // One round of the device, or fewer ranges where each has a few pages.
+  const int64_t units = static_cast<int64_t>(B) * Hkv * std::max(pages_of(max_tokens), 1);
+  const int64_t slots = p.wide ? 256 : 512;
+  const int64_t ranges = std::min((units + p.min_per - 1) / p.min_per, std::max<int64_t>(slots / p.row_blocks, 1));
+  p.ranges = static_cast<int>(std::max<int64_t>(ranges, 1));
+  // With a range for each (sequence, KV head) and no more, none is shared.
+  p.ws_bytes = static_cast<size_t>(static_cast<int64_t>(p.ranges) * p.row_blocks * 2 * p.width * (D + 2)) * 4;
   return p;
 }
 
 template <int CT, int D>
-void launch(const TreeArgs& a, int waves, dim3 grid, hipStream_t st) {
-  if (waves == 8)
-    tree_wide_kernel<CT, D, 8><<<grid, 512, 0, st>>>(a);
-  else if (waves == 4)
-    tree_wide_kernel<CT, D, 4><<<grid, 256, 0, st>>>(a);
+void launch(const TreeArgs& a, int wide, dim3 grid, hipStream_t st) {
+  if (wide == 8)
+    tree_wide_kernel<CT, D, 8><<<grid, kWideWaves * 64, 0, st>>>(a);
+  else if (wide == 4)
+    tree_wide_kernel<CT, D, 4><<<grid, kWideWaves * 64, 0, st>>>(a);
   else
     tree_rows_kernel<CT, D, kRowWaves><<<grid, kRowWaves * 64, 0, st>>>(a);
 }
@@ -943,20 +1258,19 @@ extern "C" int spyre_paged_tree_attn(const void* q, const int64_t* q_strides, co
   if (mask) a.m_sb = mask_strides[0], a.m_si = mask_strides[1], a.m_sj = mask_strides[2];
   a.out = static_cast<_Float16*>(out), a.lse = lse, a.ws = static_cast<float*>(workspace);
   a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.g = Hq / Hkv, a.rows = T * a.g;
-  a.tiles = p.tiles, a.chunk_pages = p.chunk_pages, a.max_chunks = p.max_chunks, a.max_ctx = max_context_len;
-  a.scale_log2 = scale * kLog2e;
-  const int64_t pairs = static_cast<int64_t>(B) * Hkv;
-  const int64_t items = (pairs * p.max_chunks + 7) / 8 * 8;
-  SPYRE_REQUIRE(items * p.row_blocks < (int64_t{1} << 31), SPYRE_EUNSUPPORTED, "too many workgroups");
-  a.pairs = static_cast<uint32_t>(pairs);
+  a.max_ctx = max_context_len, a.scale_log2 = scale * kLog2e;
+  a.row_blocks = p.row_blocks, a.block_rows = p.block_rows, a.width = p.width, a.ranges = p.ranges, a.min_per = p.min_per;
+  const int64_t pairs = static_cast<int64_t>(B) * Hkv, blocks = static_cast<int64_t>((p.ranges + 7) / 8 * 8) * p.row_blocks;
+  SPYRE_REQUIRE(pairs * (pages_of(max_context_len + T) + 1) < (int64_t{1} << 30) && blocks < (int64_t{1} << 31),
+                SPYRE_EUNSUPPORTED, "too many pages or rows");
   a.by_g = make_fastdiv(static_cast<uint32_t>(a.g)), a.by_hkv = make_fastdiv(static_cast<uint32_t>(Hkv));
-  a.row_blocks = p.row_blocks, a.by_blocks = make_fastdiv(static_cast<uint32_t>(p.row_blocks));
-  a.by_tiles = make_fastdiv(static_cast<uint32_t>(p.tiles)), a.by_pairs = make_fastdiv(a.pairs);
+  a.by_blocks = make_fastdiv(static_cast<uint32_t>(p.row_blocks));
+  a.by_ranges = make_fastdiv(static_cast<uint32_t>(p.ranges));
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<uint32_t>(items * p.row_blocks));
+  const dim3 grid(static_cast<uint32_t>(blocks));
   auto go = [&](auto kind) {
     constexpr int CT = decltype(kind)::value;
-    D == 128 ? launch<CT, 128>(a, p.waves, grid, st) : launch<CT, 64>(a, p.waves, grid, st);
+    D == 128 ? launch<CT, 128>(a, p.wide, grid, st) : launch<CT, 64>(a, p.wide, grid, st);
   };
   if (f16)
     go(std::integral_constant<int, SPYRE_CACHE_F16>{});
@@ -966,15 +1280,14 @@ extern "C" int spyre_paged_tree_attn(const void* q, const int64_t* q_strides, co
     go(std::integral_constant<int, SPYRE_CODES_INT8>{});
   hipError_t e = hipGetLastError();
   SPYRE_REQUIRE(e == hipSuccess, SPYRE_EHIP, "tree attention launch failed: %s", hipGetErrorString(e));
-  if (p.max_chunks > 1) {
-    const int64_t n = (pairs * a.rows * (D / 4) + 255) / 256;
-    SPYRE_REQUIRE(n < (int64_t{1} << 31), SPYRE_EUNSUPPORTED, "too many rows");
-    if (D == 128)
-      tree_merge_kernel<128><<<dim3(static_cast<uint32_t>(n)), 256, 0, st>>>(a);
-    else
-      tree_merge_kernel<64><<<dim3(static_cast<uint32_t>(n)), 256, 0, st>>>(a);
-    e = hipGetLastError();
-    SPYRE_REQUIRE(e == hipSuccess, SPYRE_EHIP, "tree attention merge launch failed: %s", hipGetErrorString(e));
-  }
+  const int64_t n = (static_cast<int64_t>(a.rows) * (D / 4) + 255) / 256;
+  SPYRE_REQUIRE(n <= 65535, SPYRE_EUNSUPPORTED, "too many rows");
+  const dim3 merge(static_cast<uint32_t>(pairs), static_cast<uint32_t>(n));
+  if (D == 128)
+    tree_merge_kernel<128><<<merge, 256, 0, st>>>(a);
+  else
+    tree_merge_kernel<64><<<merge, 256, 0, st>>>(a);
+  e = hipGetLastError();
+  SPYRE_REQUIRE(e == hipSuccess, SPYRE_EHIP, "tree attention merge launch failed: %s", hipGetErrorString(e));
   return SPYRE_OK;
 }
