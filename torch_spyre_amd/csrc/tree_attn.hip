@@ -31,6 +31,7 @@
 #include <type_traits>
 
 #include "cache8.h"
+#include "decode_dense.h"
 #include "fast_div.h"
 #include "spyre_common.h"
 
@@ -71,6 +72,7 @@ struct TreeArgs {
   // holds `width` of them, the fewer of block_rows and rows.
   int row_blocks, block_rows, width;
   int ranges, min_per;  // see Walk
+  uint32_t ticket;      // see finish()
   FastDiv by_g, by_hkv, by_blocks, by_ranges;
 };
 
@@ -81,6 +83,17 @@ __device__ __forceinline__ float xor32_max(float x) {
 
 __device__ __forceinline__ float xor32_sum(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+  return __builtin_bit_cast(float, static_cast<unsigned>(r[0])) + __builtin_bit_cast(float, static_cast<unsigned>(r[1]));
+}
+
+// The same over lanes l and l ^ 16.
+__device__ __forceinline__ float xor16_max(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+  return fmaxf(__builtin_bit_cast(float, static_cast<unsigned>(r[0])), __builtin_bit_cast(float, static_cast<unsigned>(r[1])));
+}
+
+__device__ __forceinline__ float xor16_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
   return __builtin_bit_cast(float, static_cast<unsigned>(r[0])) + __builtin_bit_cast(float, static_cast<unsigned>(r[1]));
 }
 
@@ -128,18 +141,20 @@ __device__ __forceinline__ int scan64(int x) {
 
 // How the pages are shared out.  Units are the pages of every (sequence, KV
 // head), one after the other (a sequence of none counts one, which writes its
-// zeros); range r of `ranges` is units [r per, (r + 1) per).  The lengths are
-// data of the device, so every wavefront works out the sums itself; ragged
-// batches are then as even as equal ones.  A range that holds only part of a
-// (sequence, KV head) leaves its partial in slot 0 (the range's first piece)
-// or 1 (its last); whole ones are written directly.
+// zeros); range r of `ranges` is units [r per, (r + 1) per), but for a bound
+// near the start or the end of its (sequence, KV head), which moves there: a
+// part costs its join, ranges are uneven by a few pages instead, and what has
+// no more than `per` <= 8 pages is never cut.  The lengths are data of the device, so every wavefront works
+// out the sums itself; ragged batches are then as even as equal ones.  A range
+// that holds only part of a (sequence, KV head) leaves a partial: in slot 1
+// that of the first part, in slot 0 that of any other.
 struct Walk {
   int per, u, end;            // units
   int b, base, pages;         // the sequence: its first unit / Hkv, its units a KV head
   __device__ __forceinline__ static int units_of(const TreeArgs& a, int b) {
     return max(1, seq_of(a, a.ctx[b], a.counts ? a.counts[b] : a.T).pages);
   }
-  // Units a KV head of all sequences.
+  // Units a KV head of all sequences; the first 64 sequences', one a lane.
   __device__ __forceinline__ static int total_of(const TreeArgs& a, int lane, int& first64) {
     int sum = 0;
     for (int c = 0; c < a.B; c += 256) {
@@ -154,21 +169,19 @@ struct Walk {
     }
     return __builtin_amdgcn_readlane(scan64(sum), 63);
   }
+  // An equal share, but at least min_per pages where (sequence, KV head)s have
+  // as many.
   __device__ __forceinline__ static int per_of(const TreeArgs& a, int total) {
-    return max(a.min_per, static_cast<int>(fdiv(total * a.Hkv + a.ranges - 1, a.by_ranges)));
+    return max(static_cast<int>(fdiv(total * a.Hkv + a.ranges - 1, a.by_ranges)),
+               min(a.min_per, total / a.B));
   }
-  // Range r; false if it is empty.
-  __device__ __forceinline__ bool start(const TreeArgs& a, int lane, int r) {
-    int x = 0;
-    const int total = total_of(a, lane, x);
-    per = per_of(a, total);
-    u = r * per;
-    end = min(u + per, total * a.Hkv);
-    if (u >= end) return false;
-    const int target = static_cast<int>(fdiv(u, a.by_hkv));
+  __device__ __forceinline__ int near() const { return per <= 8 ? per / 2 : 4; }
+  // The sequence of a unit (below the total).
+  __device__ __forceinline__ void find(const TreeArgs& a, int lane, int first64, int unit) {
+    const int target = static_cast<int>(fdiv(unit, a.by_hkv));
     base = 0;
-    for (int c = 0;; c += 64) {  // ends: target < total
-      if (c > 0) x = c + lane < a.B ? units_of(a, c + lane) : 0;
+    for (int c = 0;; c += 64) {  // ends: target is below the total
+      const int x = c == 0 ? first64 : c + lane < a.B ? units_of(a, c + lane) : 0;
       const int sum = scan64(x);
       const uint64_t past = __builtin_amdgcn_ballot_w64(base + sum > target);
       if (past) {
@@ -176,12 +189,41 @@ struct Walk {
         b = c + i;
         pages = __builtin_amdgcn_readlane(x, i);
         base += __builtin_amdgcn_readlane(sum, i) - pages;
-        return true;
+        return;
       }
       base += __builtin_amdgcn_readlane(sum, 63);
     }
   }
-  // The first unit / Hkv of sequence `seq`, and `per`.
+  // A bound where it belongs, after find() of it.
+  __device__ __forceinline__ int snapped(const TreeArgs& a, int unit) const {
+    const uint32_t in = unit - base * a.Hkv, at = in % static_cast<uint32_t>(pages);
+    const int g0 = unit - static_cast<int>(at), g1 = g0 + pages;
+    return unit - g0 <= near() ? g0 : g1 - unit <= near() ? g1 : unit;
+  }
+  // Range r; false if it is empty.
+  __device__ __forceinline__ bool start(const TreeArgs& a, int lane, int r) {
+    int x = 0;
+    const int total = total_of(a, lane, x), units = total * a.Hkv;
+    per = per_of(a, total);
+    u = r * per;
+    if (u >= units) return false;
+    end = units;
+    if (u + per < units) {
+      find(a, lane, x, u + per);
+      end = snapped(a, u + per);
+    }
+    find(a, lane, x, u);
+    u = snapped(a, u);
+    if (u >= end) return false;
+    if (u == (base + pages) * a.Hkv) next_sequence(a);
+    return true;
+  }
+  __device__ __forceinline__ void next_sequence(const TreeArgs& a) {
+    base += pages;
+    b += 1;
+    pages = max(1, seq_at(a, b).pages);
+  }
+  // Sequence `seq` and `per`, for parts_of().
   __device__ __forceinline__ void seek(const TreeArgs& a, int lane, int seq) {
     int x = 0, before = 0;
     per = per_of(a, total_of(a, lane, x));
@@ -193,34 +235,37 @@ struct Walk {
     base = __builtin_amdgcn_readlane(scan64(before), 63);
     pages = max(1, seq_at(a, seq).pages);
   }
+  // The ranges that hold parts of a KV head of the sequence: r0 the first one,
+  // r0 + 1 .. r1 the others; r1 <= r0 where one range holds it whole.
+  __device__ __forceinline__ void parts_of(const TreeArgs& a, int kvh, int& r0, int& r1) const {
+    const int g0 = base * a.Hkv + kvh * pages, g1 = g0 + pages;
+    r0 = (g0 + near()) / per;
+    r1 = (g1 - near() - 1) / per;
+  }
 };
 
 // A piece of a range: pages [page0, page1) of a (sequence, KV head).
 struct Piece {
   int kvh, page0, page1;
   bool whole;   // all of them
-  int slot;     // else its partial's: 0, or 1
+  int slot;     // else its partial's
 };
 
-__device__ __forceinline__ Piece piece_of(const TreeArgs& a, const Walk& w, int range) {
+__device__ __forceinline__ Piece piece_of(const TreeArgs& a, const Walk& w) {
   Piece p;
   const uint32_t in = w.u - w.base * a.Hkv;
   p.kvh = in / static_cast<uint32_t>(w.pages);
   p.page0 = in - p.kvh * w.pages;
   p.page1 = min(w.pages, p.page0 + w.end - w.u);
   p.whole = p.page0 == 0 && p.page1 == w.pages;
-  p.slot = w.u == range * w.per ? 0 : 1;
+  p.slot = p.page0 == 0 ? 1 : 0;
   return p;
 }
 
 // After it.
 __device__ __forceinline__ void advance(const TreeArgs& a, Walk& w, const Piece& p) {
   w.u += p.page1 - p.page0;
-  if (w.u < w.end && p.page1 == w.pages && p.kvh == a.Hkv - 1) {
-    w.base += w.pages;
-    w.b += 1;
-    w.pages = max(1, seq_at(a, w.b).pages);
-  }
+  if (w.u < w.end && p.page1 == w.pages && p.kvh == a.Hkv - 1) w.next_sequence(a);
 }
 
 // The range and the row block of a workgroup.  The row blocks of one range
@@ -231,12 +276,13 @@ __device__ __forceinline__ void place_of(const TreeArgs& a, int& range, int& rb)
   range = static_cast<int>(q * 8 + lo8);
 }
 
-__device__ __forceinline__ float* partial_o(const TreeArgs& a, int range, int rb, int slot, int row, int D) {
-  return a.ws + (((static_cast<int64_t>(range) * a.row_blocks + rb) * 2 + slot) * a.width + row) * D;
+// Partials: O [slots][width][D], then (m, l) [slots][width], then an arrival
+// flag for each slot; slots are (range, row block, slot 0 / 1).
+__device__ __forceinline__ int64_t partial_of(const TreeArgs& a, int range, int rb, int slot, int row) {
+  return ((static_cast<int64_t>(range) * a.row_blocks + rb) * 2 + slot) * a.width + row;
 }
-__device__ __forceinline__ float* partial_ml(const TreeArgs& a, int range, int rb, int slot, int row, int D) {
-  const int64_t slots = static_cast<int64_t>(a.ranges) * a.row_blocks * 2;
-  return a.ws + slots * a.width * D + (((static_cast<int64_t>(range) * a.row_blocks + rb) * 2 + slot) * a.width + row) * 2;
+__device__ __forceinline__ int64_t partials(const TreeArgs& a) {
+  return static_cast<int64_t>(a.ranges) * a.row_blocks * 2 * a.width;
 }
 
 // 4 features of a finished row.
@@ -323,23 +369,24 @@ struct Row {
   int head;   // its q head
   bool live;
   const uint8_t* mask;  // of its token; null: a chain
-  // Which of the 16 tokens from t on the row attends (total: all there are).
-  // Every mask byte is loaded, and none waits for another.
-  __device__ __forceinline__ uint32_t attends16(const TreeArgs& a, const Seq& sq, int t, int total) const {
+  // Which of the 16 tokens t + offset(x) the row attends (total: all there
+  // are).  Every mask byte is loaded, and none waits for another.
+  template <typename Offset>
+  __device__ __forceinline__ uint32_t attends16(const TreeArgs& a, const Seq& sq, int t, int total, Offset offset) const {
     uint32_t seen = 0;
-    const int j0 = t - sq.ctx;
+    const int j0 = t - sq.ctx, n = total - t;
     if (mask) {
       uint8_t keep[16];
 #pragma unroll
-      for (int x = 0; x < 16; ++x) keep[x] = mask[min(max(j0 + x, 0), a.T - 1) * a.m_sj];
+      for (int x = 0; x < 16; ++x) keep[x] = mask[min(max(j0 + offset(x), 0), a.T - 1) * a.m_sj];
 #pragma unroll
-      for (int x = 0; x < 16; ++x) seen |= static_cast<uint32_t>(j0 + x < 0 || keep[x] != 0) << x;
+      for (int x = 0; x < 16; ++x)
+        seen |= static_cast<uint32_t>(offset(x) < n && (j0 + offset(x) < 0 || keep[x] != 0)) << x;
     } else {
-      const int n = i - j0 + 1;  // tokens of the 16 up to i's own
-      seen = n <= 0 ? 0u : n >= 16 ? 0xffffu : (1u << n) - 1;
+#pragma unroll
+      for (int x = 0; x < 16; ++x) seen |= static_cast<uint32_t>(offset(x) < n && j0 + offset(x) <= i) << x;
     }
-    const int n = total - t;
-    return live && n > 0 ? seen & (n >= 16 ? 0xffffu : (1u << n) - 1) : 0u;
+    return live ? seen : 0u;
   }
 };
 
@@ -352,30 +399,34 @@ __device__ __forceinline__ Row row_of(const TreeArgs& a, const Seq& sq, int b, i
   return r;
 }
 
-// Q^T operands of a lane's row: features 32 s + 16 half + 8 e .. + 7.
+// Q^T operands of a lane's row: features 32 s + 16 half + 8 e .. + 7.  (A row
+// that is not live loads another's.)
 template <int DS>
 __device__ __forceinline__ void load_q(const TreeArgs& a, int b, const Row& r, int half, f16x8 (&qf)[DS][2]) {
-  const _Float16* qp = a.q + b * a.q_sb + r.i * a.q_st + r.head * a.q_sh + 16 * half;
+  const _Float16* qp = a.q + b * a.q_sb + (r.live ? r.i * a.q_st + r.head * a.q_sh : 0) + 16 * half;
 #pragma unroll
   for (int s = 0; s < DS; ++s)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      qf[s][e] = f16x8{};
-      if (r.live) qf[s][e] = *reinterpret_cast<const f16x8*>(qp + 32 * s + 8 * e);
-    }
+    for (int e = 0; e < 2; ++e) qf[s][e] = *reinterpret_cast<const f16x8*>(qp + 32 * s + 8 * e);
+#pragma unroll
+  for (int s = 0; s < DS; ++s)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (!r.live) qf[s][e] = f16x8{};
 }
 
 // The infinities and NaNs of tokens t0 .. t1 - 1 (part 0 / 1: of their pages'
 // first / second halves only) that drop_odd left out of O, number by number.
-template <int CT, int D>
-__device__ void add_odd(const TreeArgs& a, const Seq& sq, int b, int kvh, const Row& r, int lane, int t0, int t1,
-                        int part, f32x16 (&o)[D / 32]) {
+// A lane's numbers of O are those of the features feature(x), x < NR; add(x, f)
+// adds to one.
+template <int CT, int D, int NR, typename Feature, typename Add>
+__device__ __forceinline__ void add_odd(const TreeArgs& a, const Seq& sq, int b, int kvh, const Row& r, int lane, int t0, int t1,
+                                        int part, Feature feature, Add add) {
   constexpr int KB = CT == kF16 ? 2 : 1;
-  int half = lane >> 5;
-  asm volatile("" : "+v"(half));  // rare: its addresses are not worth registers of the loops before it
+  asm volatile("" : "+v"(lane));  // rare: its addresses are not worth registers of the loops before it
   Pages pages(a, b, kvh, lane, t0 / kPage);
   for (int t = t0; t < t1; ++t) {
-    const bool attends = r.attends16(a, sq, t, t + 1) && (part < 0 || part == (t % kPage) / 32);
+    const bool attends = r.attends16(a, sq, t, t + 1, [](int x) { return x; }) && (part < 0 || part == (t % kPage) / 32);
     const int64_t head = pages.head(t / kPage);
     const uint8_t* v = a.v + head * (static_cast<int64_t>(kPage) * D * KB);
     float vs = 1.f;  // 8-bit: V's scale if it is not finite
@@ -384,23 +435,129 @@ __device__ void add_odd(const TreeArgs& a, const Seq& sq, int b, int kvh, const 
       if (!(__builtin_fabsf(x) <= 0x1.fffffep127f)) vs = x;
     }
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-      for (int x = 0; x < 16; ++x) {
-        const int d = 32 * dt + 8 * (x / 4) + 4 * half + x % 4;
-        float f = 0.f;
-        if constexpr (CT == kF16) {
-          f = static_cast<float>(reinterpret_cast<const _Float16*>(v)[d * kPage + t % kPage]);
-          if (__builtin_fabsf(f) <= 65504.f) f = 0.f;
-        } else {
-          float x[4];
-          codes_to_f32<CT>(v[(t % kPage / 16) * (D * 16) + d * 16 + t % 16], x);
-          f = x[0] * vs;
-          if (__builtin_fabsf(f) <= 65504.f) f = 0.f;
-        }
-        if (attends) o[dt][x] += f;
+    for (int x = 0; x < NR; ++x) {
+      const int d = feature(x, lane);
+      float f;
+      if constexpr (CT == kF16) {
+        f = static_cast<float>(reinterpret_cast<const _Float16*>(v)[d * kPage + t % kPage]);
+      } else {
+        float c[4];
+        codes_to_f32<CT>(v[(t % kPage / 16) * (D * 16) + d * 16 + t % 16], c);
+        f = c[0] * vs;
       }
+      if (attends && !(__builtin_fabsf(f) <= 65504.f)) add(x, f);
+    }
   }
+}
+
+// Joins the parts r0 .. r1 of 4 features of a row, 8 loads in flight.
+template <typename Load>
+__device__ __forceinline__ void merge_parts(int r0, int r1, float& M, float& L, f32x4& acc, Load load) {
+  constexpr int G = 8;
+  for (int c = r0; c <= r1; c += G) {
+    float m[G], l[G];
+    f32x4 x[G];
+#pragma unroll
+    for (int k = 0; k < G; ++k) load(min(c + k, r1), m[k], l[k], x[k]);  // past r1 the last one again
+    float mc = M;
+#pragma unroll
+    for (int k = 0; k < G; ++k) mc = fmaxf(mc, m[k]);
+    const float f0 = M == -INFINITY ? 0.f : exp2_of(M - mc);
+    L *= f0;
+    acc *= f0;
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+      if (c + k > r1) break;
+      const float f = m[k] == -INFINITY ? 0.f : exp2_of(m[k] - mc);
+      L += m[k] == -INFINITY ? l[k] : l[k] * f;  // l without a reference is 0, or NaN
+      if (m[k] != -INFINITY) acc += x[k] * f;
+    }
+    M = mc;
+  }
+}
+
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+constexpr int kAuxDevice = 16;  // sc1: device scope
+
+// The end of a piece whose wavefronts' partials are in LDS, O [W][rows][D + 4]
+// at s_o and (m, l) [W][rows] at s_ml: every thread folds 4 features of a row
+// over the wavefronts, in their order.  A whole (sequence, KV head) is then
+// finished.  Any other leaves its part in the workspace, then an arrival flag
+// (the call's ticket), and reads the flags of all parts: of two workgroups the
+// one whose flag was stored later sees the other's, so at least one sees them
+// all; those that do join the parts (to the same bits) and clear the flags,
+// so that a replayed call (the same ticket) starts with none.  One launch: a
+// second kernel for it costs a decode step 4 us.
+template <int D, int W>
+__device__ __forceinline__ void finish(const TreeArgs& a, const Walk& walk, const Piece& pc, const Seq& sq, int range, int rb,
+                                       int rows, const float* s_o, const float* s_ml) {
+  constexpr int ROW = D + 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const int row0 = rb * a.block_rows;
+  // The host keeps the workspace below 2^31 bytes here.
+  const Rsrc ws = __builtin_amdgcn_make_buffer_rsrc(a.ws, 0, 0x7ffffff0, 0x00020000);
+  const uint32_t ml0 = static_cast<uint32_t>(partials(a) * D * 4);
+  for (int u = threadIdx.x; u < rows * (D / 4); u += W * 64) {
+    const int r = u / (D / 4), d = 4 * (u % (D / 4));
+    float M = -INFINITY, L = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < W; ++w) M = fmaxf(M, s_ml[(w * rows + r) * 2]);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float mw = s_ml[(w * rows + r) * 2], lw = s_ml[(w * rows + r) * 2 + 1];
+      const float f = mw == -INFINITY ? 0.f : exp2_of(mw - M);
+      L += mw == -INFINITY ? lw : lw * f;  // l without a reference is 0, or NaN
+      if (mw != -INFINITY) acc += *reinterpret_cast<const f32x4*>(s_o + (w * rows + r) * ROW + d) * f;
+    }
+    if (pc.whole) {
+      const int i = static_cast<int>(fdiv(row0 + r, a.by_g));
+      store_row4<D>(a, walk.b, i, pc.kvh * a.g + row0 + r - i * a.g, d, acc, M, L);
+    } else {
+      const uint32_t part = static_cast<uint32_t>(partial_of(a, range, rb, pc.slot, r));
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc), ws, (part * D + d) * 4, 0, kAuxDevice);
+      if (d == 0) {
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__builtin_bit_cast(uint32_t, M), __builtin_bit_cast(uint32_t, L)}, ws,
+                                              ml0 + part * 8, 0, kAuxDevice);
+      }
+    }
+  }
+  if (pc.whole) return;
+  __shared__ int s_merge;
+  int r0, r1;
+  walk.parts_of(a, pc.kvh, r0, r1);
+  const uint32_t fl0 = ml0 + static_cast<uint32_t>(partials(a)) * 8;
+  auto flag_of = [&](int r) { return fl0 + ((r * a.row_blocks + rb) * 2 + (r == r0 ? 1 : 0)) * 4; };
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();  // every part of the row is stored
+  if (wave == 0) {
+    if (lane == 0) __builtin_amdgcn_raw_buffer_store_b32(a.ticket, ws, flag_of(range), 0, kAuxDevice);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    bool seen = true;
+    for (int r = r0 + lane; r <= r1; r += 64)
+      seen = seen && __builtin_amdgcn_raw_buffer_load_b32(ws, flag_of(r), 0, kAuxDevice) == a.ticket;
+    const bool all = __all(seen);
+    if (lane == 0) s_merge = all ? 1 : 0;
+  }
+  __syncthreads();
+  if (!s_merge) return;
+  for (int u = threadIdx.x; u < rows * (D / 4); u += W * 64) {
+    const int r = u / (D / 4), d = 4 * (u % (D / 4)), i = static_cast<int>(fdiv(row0 + r, a.by_g));
+    float M = -INFINITY, L = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    if (i < sq.n)
+      merge_parts(r0, r1, M, L, acc, [&](int p, float& m, float& l, f32x4& x) {
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        const uint32_t part = static_cast<uint32_t>(partial_of(a, p, rb, p == r0 ? 1 : 0, r));
+        const f32x2 ml = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(ws, ml0 + part * 8, 0, kAuxDevice));
+        m = ml[0], l = ml[1];
+        x = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(ws, (part * D + d) * 4, 0, kAuxDevice));
+      });
+    store_row4<D>(a, walk.b, i, pc.kvh * a.g + row0 + r - i * a.g, d, acc, M, L);
+  }
+  for (int r = r0 + static_cast<int>(threadIdx.x); r <= r1; r += W * 64)
+    __builtin_amdgcn_raw_buffer_store_b32(0u, ws, flag_of(r), 0, kAuxDevice);
 }
 
 // W wavefronts share a chunk of a (sequence, KV head, row tile): each takes
@@ -419,7 +576,7 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
   Walk walk;
   if (range >= a.ranges || !walk.start(a, lane, range)) return;
   for (; walk.u < walk.end;) {
-  const Piece pc = piece_of(a, walk, range);
+  const Piece pc = piece_of(a, walk);
   const int b = walk.b, kvh = pc.kvh;
   const Seq sq = seq_at(a, b);
   const int total = sq.ctx + (a.draft_keys ? sq.n : 0);
@@ -428,7 +585,6 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
   const int s0 = c0 + (c1 - c0) * wave / W, s1 = c0 + (c1 - c0) * (wave + 1) / W;
   const Row row = row_of(a, sq, b, kvh, tile * kTile + col);
   f16x8 qf[DS][2];
-  load_q<DS>(a, b, row, half, qf);
   Pages pages(a, b, kvh, lane, s0 / PER_PAGE);
   bool odd = false;
 
@@ -482,11 +638,13 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
   // 8-bit: this wavefront's step: score factors, V's scales' logarithms and inverses.
   float* s_sc = s_mem + wave * 3 * STEP;
 
-  auto step = [&](int st, bool more, auto edge_tag) {
+  // MORE: another step follows (as in the few kernel).
+  auto step = [&](int st, auto more_tag, auto edge_tag) {
+    constexpr bool MORE = decltype(more_tag)::value;
     constexpr bool EDGE = decltype(edge_tag)::value;  // some tokens are drafted or do not exist
     const int tok0 = st * STEP + 16 * half;           // this lane's 16 tokens
     uint32_t seen = 0;                                // those that its row attends
-    if constexpr (EDGE) seen = row.attends16(a, sq, tok0, total);
+    if constexpr (EDGE) seen = row.attends16(a, sq, tok0, total, [](int x) { return x; });
     uint32_t odd_scale = 0, inf_scale = 0;  // of this lane's 16 tokens, those whose V has no finite scale
     if constexpr (CT != kF16) {
       __builtin_amdgcn_wave_barrier();
@@ -506,7 +664,7 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
         sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand<CT>(kr.x[s], e), qf[s][e], sc, 0, 0, 0);
-    if (more) {
+    if constexpr (MORE) {
       if ((st + 1) % PER_PAGE == 0) locate(st + 1);
       load_k(st + 1);
     }
@@ -582,28 +740,49 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
         o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand<CT>(vr.x[dt], e), p[e], o[dt], 0, 0, 0);
-    if (more) load_v(st + 1);
+    if constexpr (MORE) load_v(st + 1);
   };
 
-  if (s0 < s1) {
-    locate(s0);
-    load_k(s0);
-    load_v(s0);
-  }
   // Every row attends every token of a step below ctx (rows without a drafted
   // token drop theirs at the end), so only the last steps test tokens.
-  int st = s0;
   const int whole = min(s1, sq.ctx / STEP);
-  for (; st < whole; ++st) step(st, st + 1 < s1, std::false_type{});
-  for (; st < s1; ++st) step(st, st + 1 < s1, std::true_type{});
+  std::true_type yes;
+  std::false_type no;
+  auto wait_q = [&] {  // behind the first step's loads; waits here, not in every step
+    load_q<DS>(a, b, row, half, qf);
+#pragma unroll
+    for (int s = 0; s < DS; ++s)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) asm volatile("" : "+v"(qf[s][e]));
+  };
+  int st = s0;
+  if (st < whole) {
+    locate(st);
+    load_k(st);
+    load_v(st);
+    wait_q();
+    for (; st < whole - 1; ++st) step(st, yes, no);
+    step(st, no, no);
+    ++st;
+  } else if (st < s1) {
+    wait_q();
+  }
+  for (; st < s1; ++st) {  // the sequence's last steps
+    if (st == s0 || st % PER_PAGE == 0) locate(st);
+    load_k(st);
+    load_v(st);
+    step(st, no, yes);
+  }
   if (CT != SPYRE_CODES_INT8 && __any(odd))
-    add_odd<CT, D>(a, sq, b, kvh, row, lane, max(s0, whole) * STEP, min(s1 * STEP, total), -1, o);
+    add_odd<CT, D, DS * 16>(
+        a, sq, b, kvh, row, lane, max(s0, whole) * STEP, min(s1 * STEP, total), -1,
+        [](int x, int ln) { return 32 * (x / 16) + 8 * (x % 16 / 4) + 4 * (ln >> 5) + x % 4; },
+        [&](int x, float f) { o[x / 16][x % 16] += f; });
   l = xor32_sum(l);
   if (!row.live) m = -INFINITY, l = 0.f;
   if ((pages.poisoned || sq.bad) && row.live) l = NAN;
 
-  // Join the wavefronts: O, m and l of the rows that exist, then every thread
-  // folds elements in wavefront order.
+  // O, m and l of the rows that exist.
   const int rows = min(kTile, a.rows - static_cast<int>(tile) * kTile);
   float* s_o = s_mem;                          // [W][rows][ROW]
   float* s_ml = s_mem + W * rows * ROW;        // [W][rows][2]
@@ -621,36 +800,270 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
     }
   }
   __syncthreads();
-  for (int u = threadIdx.x; u < rows * (D / 4); u += W * 64) {
-    const int r = u / (D / 4), d = 4 * (u % (D / 4));
-    float M = -INFINITY, L = 0.f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < W; ++w) M = fmaxf(M, s_ml[(w * rows + r) * 2]);
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float mw = s_ml[(w * rows + r) * 2], lw = s_ml[(w * rows + r) * 2 + 1];
-      const float f = mw == -INFINITY ? 0.f : exp2_of(mw - M);
-      L += mw == -INFINITY ? lw : lw * f;  // lw without a reference is 0, or NaN
-      if (mw != -INFINITY) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(s_o + (w * rows + r) * ROW + d);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] += x[e] * f;
-      }
-    }
-    if (pc.whole) {
-      const int rr = tile * kTile + r, ii = static_cast<int>(fdiv(rr, a.by_g));
-      store_row4<D>(a, b, ii, kvh * a.g + rr - ii * a.g, d, acc, M, L);
-    } else {
-      *reinterpret_cast<f32x4*>(partial_o(a, range, tile, pc.slot, r, D) + d) = acc;
-      if (d == 0) {
-        float* ml = partial_ml(a, range, tile, pc.slot, r, D);
-        ml[0] = M, ml[1] = L;
-      }
-    }
-  }
+  finish<D, W>(a, walk, pc, sq, range, tile, rows, s_o, s_ml);
   advance(a, walk, pc);
   __syncthreads();  // LDS is read before the next piece writes it
+  }
+}
+
+// ------------------------------------------------------------- few rows --
+//
+// Up to 16 rows to a KV head (a decode step): MFMA 16x16x32, whose 16 columns
+// cost half of what 32 would.  W wavefronts share a piece, each whole pages of
+// it:
+//   S^T[tok, row] = K[tok, :] Q^T[:, row]      4 x D/32 products of 16 tokens
+//   O^T[d, row] += V^T[d, tok] P^T[tok, row]   D/16 x 2
+// The same free orders as above, taken so that every load instruction covers
+// whole runs of memory.  Lane group G = lane / 16; token tile j's row m is
+//   fp16   token 32 (j / 2) + 8 (m / 4) + 4 (j % 2) + m % 4, features 64 s +
+//          8 G + 32 e of products 2 s + e: group G ends with the scores of the
+//          two runs of 8 tokens of V's 16-byte loads; 64-byte runs of a row.
+//   8-bit  token 16 j + m, features 64 s + 16 G + 8 e: 256-byte runs of K's
+//          units.  Group G then holds the scores of the tokens 16 j + 4 G + i;
+//          its V load is the tokens 16 G .. + 15, so the 4 x 4 words (of 4
+//          tokens) of the four groups change places in registers first.
+// Bound by memory: K of the next page is loaded as soon as the scores have used
+// this one's, V as soon as O has.
+template <int CT, int D, int W>
+__global__ __launch_bounds__(W * 64, 2) void tree_few_kernel(TreeArgs a) {
+  constexpr int KB = CT == kF16 ? 2 : 1, KW = KB;  // bytes of an element; 16-byte words of 16 of them
+  constexpr int DQ = D / 64, DV = D / 16;
+  constexpr int ROW = D + 4;
+  __shared__ __align__(16) float s_mem[W * 16 * (ROW + 2)];
+  static_assert(3 * kPage <= 16 * (ROW + 2), "a wavefront's scales fit its share");
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const int col = lane & 15, grp = lane >> 4;
+  const int range = blockIdx.x;
+  Walk walk;
+  if (!walk.start(a, lane, range)) return;
+  // Lane offsets within a page, bytes.
+  const int k_off = CT == kF16 ? (8 * (col >> 2) + (col & 3)) * 128 + grp * 16 : grp * (kPage * 16) + col * 16;
+  const int v_off = CT == kF16 ? col * (kPage * 2) + grp * 16 : grp * (D * 16) + col * 16;
+  // This lane's 16 tokens of a page, in the order of its scores: tok_of(0) + offset(x).
+  auto offset = [](int x) { return CT == kF16 ? 32 * (x / 8) + x % 8 : 16 * (x / 4) + x % 4; };
+  const int tok_of0 = CT == kF16 ? 8 * grp : 4 * grp;
+  float* s_sc = s_mem + wave * 3 * kPage;  // 8-bit: score factors, V's scales' logarithms and inverses
+  for (; walk.u < walk.end;) {
+    const Piece pc = piece_of(a, walk);
+    const int b = walk.b, kvh = pc.kvh;
+    const Seq sq = seq_at(a, b);
+    const int total = sq.ctx + (a.draft_keys ? sq.n : 0);
+    const int c1 = sq.n > 0 ? min(pc.page1, sq.pages) : pc.page0, nc = c1 - pc.page0;
+    const int p0 = pc.page0 + nc * wave / W, p1 = pc.page0 + nc * (wave + 1) / W;
+    const Row row = row_of(a, sq, b, kvh, col);
+    f16x8 qf[DQ][2];
+    auto load_q = [&] {  // behind the first page's loads; waits for all of them
+      const _Float16* qp = a.q + b * a.q_sb + (row.live ? row.i * a.q_st + row.head * a.q_sh : 0) + (CT == kF16 ? 8 : 16) * grp;
+#pragma unroll
+      for (int s = 0; s < DQ; ++s)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) qf[s][e] = *reinterpret_cast<const f16x8*>(qp + 64 * s + (CT == kF16 ? 32 : 8) * e);
+#pragma unroll
+      for (int s = 0; s < DQ; ++s)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (!row.live) qf[s][e] = f16x8{};
+          asm volatile("" : "+v"(qf[s][e]));
+        }
+    };
+    Pages pages(a, b, kvh, lane, p0);
+    bool odd = false;
+    f32x4 o[DV];
+#pragma unroll
+    for (int dt = 0; dt < DV; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    u32x4 kr[4][DQ][KW], vr[DV][KW];
+    float ksc = 0.f, vsc = 0.f;  // 8-bit: of the page's token `lane`
+    auto load_k = [&](int64_t head) {
+      const uint8_t* p = a.k + head * (static_cast<int64_t>(kPage) * D * KB) + k_off;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int s = 0; s < DQ; ++s)
+#pragma unroll
+          for (int e = 0; e < KW; ++e)
+            kr[j][s][e] = *reinterpret_cast<const u32x4*>(
+                p + (CT == kF16 ? s * (kPage * 128) + (32 * (j / 2) + 4 * (j % 2)) * 128 + 64 * e : 4 * s * (kPage * 16) + 16 * j * 16));
+      if constexpr (CT != kF16) {
+        ksc = a.ks[head * kPage + lane];
+        vsc = a.vs[head * kPage + lane];
+      }
+    };
+    auto load_v = [&](int64_t head) {
+      const uint8_t* p = a.v + head * (static_cast<int64_t>(kPage) * D * KB) + v_off;
+#pragma unroll
+      for (int dt = 0; dt < DV; ++dt)
+#pragma unroll
+        for (int e = 0; e < KW; ++e)
+          vr[dt][e] = *reinterpret_cast<const u32x4*>(p + (CT == kF16 ? dt * (16 * kPage * 2) + 64 * e : dt * (16 * 16)));
+    };
+    int64_t head = 0;
+    // MORE: another page follows.  (A test of it at run time would leave the
+    // compiler paths on which K is loaded and V is not, and every page would
+    // wait for its V before its first product.)
+    auto step = [&](int p, auto more_tag, auto edge_tag) {
+      constexpr bool MORE = decltype(more_tag)::value;
+      constexpr bool EDGE = decltype(edge_tag)::value;   // some tokens are drafted or do not exist
+      const int tok0 = p * kPage + tok_of0;
+      uint32_t seen = 0, odd_scale = 0, inf_scale = 0;   // as in the rows kernel
+      if constexpr (EDGE) seen = row.attends16(a, sq, tok0, total, offset);
+      if constexpr (CT != kF16) {
+        __builtin_amdgcn_wave_barrier();
+        const bool finite = __builtin_fabsf(vsc) <= 0x1.fffffep127f;
+        const uint64_t not_finite = __builtin_amdgcn_ballot_w64(!finite), infinite = __builtin_amdgcn_ballot_w64(vsc == INFINITY);
+        if (not_finite) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            odd_scale |= (static_cast<uint32_t>(not_finite >> (16 * j + 4 * grp)) & 0xfu) << (4 * j);
+            inf_scale |= (static_cast<uint32_t>(infinite >> (16 * j + 4 * grp)) & 0xfu) << (4 * j);
+          }
+        }
+        const float vc = !finite ? 1.f : vsc < 0x1p-60f ? 0x1p-60f : vsc;
+        s_sc[lane] = ksc * a.scale_log2;
+        s_sc[kPage + lane] = __builtin_amdgcn_logf(vc);
+        s_sc[2 * kPage + lane] = __builtin_amdgcn_rcpf(vc);
+        __builtin_amdgcn_wave_barrier();
+      }
+      f32x4 sc[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < DQ; ++s)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            sc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand<CT>(kr[j][s], e), qf[s][e], sc[j], 0, 0, 0);
+      }
+      if constexpr (MORE) {
+        head = pages.head(p + 1);
+        load_k(head);
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f32x4 f, lv;
+        if constexpr (CT != kF16) {
+          f = *reinterpret_cast<const f32x4*>(s_sc + 16 * j + 4 * grp);
+          lv = *reinterpret_cast<const f32x4*>(s_sc + kPage + 16 * j + 4 * grp);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v = CT == kF16 ? sc[j][i] * a.scale_log2 : __builtin_fmaf(sc[j][i], f[i], lv[i]);
+          if constexpr (EDGE) v = (seen >> (4 * j + i)) & 1 ? v : -INFINITY;
+          sc[j][i] = v;
+          mx = fmaxf(mx, v);
+        }
+      }
+      mx = xor32_max(mx);
+      mx = xor16_max(mx);
+      if (__any(mx > m + kSlack)) {
+        const float mn = fmaxf(m, mx);
+        const float alpha = m == -INFINITY ? 0.f : exp2_of(m - mn);
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DV; ++dt) o[dt] *= alpha;
+      }
+      const float mu = m == -INFINITY ? 0.f : m;  // a row that has attended nothing yet: weights 0
+      f16x8 pw[2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f32x4 r;
+        if constexpr (CT != kF16) r = *reinterpret_cast<const f32x4*>(s_sc + 2 * kPage + 16 * j + 4 * grp);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float w = exp2_of(sc[j][i] - mu);
+          if constexpr (CT == kF16)
+            l += w;
+          else
+            l = __builtin_fmaf(w, EDGE && !((seen >> (4 * j + i)) & 1) ? 0.f : r[i], l);
+          pw[j / 2][4 * (j % 2) + i] = static_cast<_Float16>(w);
+        }
+      }
+      if (CT != kF16 && __any(odd_scale != 0)) {
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+          if ((odd_scale >> x) & 1 && (!EDGE || (seen >> x) & 1))
+            pw[x / 8][x % 8] = static_cast<_Float16>((inf_scale >> x) & 1 ? INFINITY : NAN);
+      }
+      if constexpr (EDGE) {
+#pragma unroll
+        for (int dt = 0; dt < DV; ++dt) {
+          if constexpr (CT == kF16) {
+            u32x4 lo[1] = {vr[dt][0]}, hi[1] = {vr[dt][1]};  // 8 tokens each
+            drop_tokens<CT>(lo, total - tok0);
+            drop_tokens<CT>(hi, total - tok0 - 32);
+            vr[dt][0] = lo[0], vr[dt][1] = hi[0];
+          } else {
+            drop_tokens<CT>(vr[dt], total - p * kPage - 16 * grp);
+          }
+#pragma unroll
+          for (int e = 0; e < KW; ++e)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              uint32_t y = vr[dt][e][w];
+              odd = drop_odd<CT>(y) || odd;
+              vr[dt][e][w] = y;
+            }
+        }
+      }
+#pragma unroll
+      for (int dt = 0; dt < DV; ++dt) {
+        if constexpr (CT != kF16) {
+          uint32_t w[4] = {vr[dt][0][0], vr[dt][0][1], vr[dt][0][2], vr[dt][0][3]};
+          transpose4x4_groups(w);  // word j: tokens 16 j + 4 grp ..
+          vr[dt][0] = u32x4{w[0], w[1], w[2], w[3]};
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand<CT>(vr[dt], e), pw[e], o[dt], 0, 0, 0);
+      }
+      if constexpr (MORE) load_v(head);
+    };
+    const int whole = min(p1, sq.ctx / kPage);
+    std::true_type yes;
+    std::false_type no;
+    int p = p0;
+    if (p < whole) {
+      head = pages.head(p);
+      load_k(head);
+      load_v(head);
+      load_q();
+      for (; p < whole - 1; ++p) step(p, yes, no);
+      step(p, no, no);
+      ++p;
+    } else if (p < p1) {
+      load_q();
+    }
+    for (; p < p1; ++p) {  // the sequence's last pages
+      head = pages.head(p);
+      load_k(head);
+      load_v(head);
+      step(p, no, yes);
+    }
+    if (CT != SPYRE_CODES_INT8 && __any(odd))
+      add_odd<CT, D, DV * 4>(
+          a, sq, b, kvh, row, lane, max(p0, whole) * kPage, min(p1 * kPage, total), -1,
+          [](int x, int ln) { return 16 * (x / 4) + 4 * (ln >> 4) + x % 4; }, [&](int x, float f) { o[x / 4][x % 4] += f; });
+    l = xor16_sum(xor32_sum(l));
+    if (!row.live) m = -INFINITY, l = 0.f;
+    if ((pages.poisoned || sq.bad) && row.live) l = NAN;
+    const int rows = a.rows;
+    float* s_o = s_mem;
+    float* s_ml = s_mem + W * rows * ROW;
+    __syncthreads();
+    if (col < rows) {
+#pragma unroll
+      for (int dt = 0; dt < DV; ++dt) *reinterpret_cast<f32x4*>(s_o + (wave * rows + col) * ROW + 16 * dt + 4 * grp) = o[dt];
+      if (grp == 0) {
+        s_ml[(wave * rows + col) * 2] = m;
+        s_ml[(wave * rows + col) * 2 + 1] = l;
+      }
+    }
+    __syncthreads();
+    finish<D, W>(a, walk, pc, sq, range, 0, rows, s_o, s_ml);
+    advance(a, walk, pc);
+    __syncthreads();  // LDS is read before the next piece writes it
   }
 }
 
@@ -671,7 +1084,6 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
 __device__ __forceinline__ int swz_k(int row) { return ((row >> 1) & 3) | ((((row >> 3) ^ (row >> 4)) & 1) << 2); }
 __device__ __forceinline__ int swz_v(int row) { return (row >> 1) & 7; }
 
-typedef __amdgpu_buffer_rsrc_t Rsrc;
 constexpr int kWideWaves = 8;
 
 template <int CT, int D, int RT>
@@ -710,7 +1122,7 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
   const float c = __builtin_fabsf(a.scale_log2);  // its sign is in q
 
   for (; walk.u < walk.end;) {
-    const Piece pc = piece_of(a, walk, range);
+    const Piece pc = piece_of(a, walk);
     const int b = walk.b, kvh = pc.kvh;
     const Seq sq = seq_at(a, b);
     const int total = sq.ctx + (a.draft_keys ? sq.n : 0);
@@ -919,7 +1331,7 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
     // after the other, each token tested.
     auto edge = [&](int p, int s3, int s2, int t) {
       const int tok0 = p * kPage + 32 * t + 16 * half;  // this lane's 16 tokens
-      const uint32_t seen = row.attends16(a, sq, tok0, total);
+      const uint32_t seen = row.attends16(a, sq, tok0, total, [](int x) { return x; });
       f32x16 s;
       scores(s, k_tile(s3), t);
       float mx = -INFINITY;
@@ -1060,10 +1472,10 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
       }
       if (__any(odd)) {
         const int t0 = max(p0, whole) * kPage, t1 = min(p1 * kPage, total);
-        if constexpr (RT == W)
-          add_odd<CT, D>(a, sq, b, kvh, row, lane, t0, t1, -1, o);
-        else
-          add_odd<CT, D>(a, sq, b, kvh, row, lane, t0, t1, part, o);
+        add_odd<CT, D, DS * 16>(
+            a, sq, b, kvh, row, lane, t0, t1, RT == W ? -1 : part,
+            [](int x, int ln) { return 32 * (x / 16) + 8 * (x % 16 / 4) + 4 * (ln >> 5) + x % 4; },
+            [&](int x, float f) { o[x / 16][x % 16] += f; });
       }
     }
     l = xor32_sum(l);
@@ -1099,7 +1511,8 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
       }
     }
     if (part == 0 && tile * kTile + col < a.rows) {
-      float* x = partial_o(a, range, rb, pc.slot, local * kTile + col, D) + 4 * half;
+        const int64_t part_row = partial_of(a, range, rb, pc.slot, local * kTile + col);
+      float* x = a.ws + part_row * D + 4 * half;
 #pragma unroll
       for (int dt = 0; dt < DS; ++dt)
 #pragma unroll
@@ -1111,7 +1524,7 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
             *reinterpret_cast<f32x4*>(x + 32 * dt + 8 * x4) = y;
         }
       if (!pc.whole && half == 0) {
-        float* ml = partial_ml(a, range, rb, pc.slot, local * kTile + col, D);
+        float* ml = a.ws + partials(a) * D + part_row * 2;
         ml[0] = m, ml[1] = l;
       }
     }
@@ -1121,76 +1534,62 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
 }
 
 // Joins the partials of each (sequence, KV head) that several ranges share: a
-// thread 4 features of a row.
+// thread 4 features of a row.  For the wide kernel, whose partials are too many
+// for one workgroup.
 template <int D>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   const uint32_t pair = blockIdx.x, b = fdiv(pair, a.by_hkv), kvh = pair - b * a.Hkv;
-  const int u = blockIdx.y * 256 + threadIdx.x, row = u / (D / 4), d = 4 * (u % (D / 4));
   Walk w;
   w.seek(a, threadIdx.x % 64, b);
-  const int g0 = w.base * a.Hkv + kvh * w.pages, g1 = g0 + w.pages;
-  const int r0 = g0 / w.per, r1 = (g1 - 1) / w.per;
-  if (r0 == r1 || row >= a.rows) return;
+  int r0, r1;
+  w.parts_of(a, kvh, r0, r1);
+  if (r1 <= r0) return;
   const Seq sq = seq_at(a, b);
-  const int ii = static_cast<int>(fdiv(row, a.by_g)), rb = row / a.block_rows, rl = row - rb * a.block_rows;
-  float M = -INFINITY, L = 0.f;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  if (ii < sq.n) {
-    constexpr int G = 8;  // partials in flight
-    for (int c = r0; c <= r1; c += G) {
-      float ml[G][2];
-      f32x4 x[G];
-#pragma unroll
-      for (int k = 0; k < G; ++k) {
-        const int r = min(c + k, r1), slot = r * w.per < g0 ? 1 : 0;
-        const float* p = partial_ml(a, r, rb, slot, rl, D);
-        ml[k][0] = p[0], ml[k][1] = p[1];
-        x[k] = *reinterpret_cast<const f32x4*>(partial_o(a, r, rb, slot, rl, D) + d);
-      }
-      float mc = M;
-#pragma unroll
-      for (int k = 0; k < G; ++k) mc = fmaxf(mc, ml[k][0]);  // past r1 the last one again
-      const float f0 = M == -INFINITY ? 0.f : exp2_of(M - mc);
-      L *= f0;
-      acc *= f0;
-#pragma unroll
-      for (int k = 0; k < G; ++k) {
-        if (c + k > r1) break;
-        const float f = ml[k][0] == -INFINITY ? 0.f : exp2_of(ml[k][0] - mc);
-        L += ml[k][0] == -INFINITY ? ml[k][1] : ml[k][1] * f;  // l without a reference is 0, or NaN
-        if (ml[k][0] != -INFINITY) acc += x[k] * f;
-      }
-      M = mc;
-    }
+  for (int u = blockIdx.y * 256 + threadIdx.x; u < a.rows * (D / 4); u += gridDim.y * 256) {
+    const int row = u / (D / 4), d = 4 * (u % (D / 4));
+    const int i = static_cast<int>(fdiv(row, a.by_g)), rb = row / a.block_rows, rl = row - rb * a.block_rows;
+    float M = -INFINITY, L = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    if (i < sq.n)
+      merge_parts(r0, r1, M, L, acc, [&](int r, float& m, float& l, f32x4& x) {
+        const int64_t part = partial_of(a, r, rb, r == r0 ? 1 : 0, rl);
+        const float* ml = a.ws + partials(a) * D + part * 2;
+        m = ml[0], l = ml[1];
+        x = *reinterpret_cast<const f32x4*>(a.ws + part * D + d);
+      });
+    store_row4<D>(a, b, i, kvh * a.g + row - i * a.g, d, acc, M, L);
   }
-  store_row4<D>(a, b, ii, kvh * a.g + row - ii * a.g, d, acc, M, L);
 }
 
-constexpr int kRowWaves = 4;
+constexpr int kWaves = 8;  // of every workgroup
+static_assert(kWaves == kWideWaves, "one workgroup to a compute unit in all three kernels");
+constexpr int kFewRows = 16;
 // Rows up to here take the rows kernel: two tiles read a chunk's pages twice.
 constexpr int kNarrowRows = 64;
 
 struct Plan {
-  int wide;  // row tiles of a workgroup of the wide kernel; 0: the rows kernel
+  int wide;  // row tiles of a workgroup of the wide kernel; 0: the rows kernel, -1: the few
   int row_blocks, block_rows, width, ranges, min_per;
+  bool merge;  // a second kernel joins the parts
   size_t ws_bytes;
 };
 
 Plan plan_of(int B, int T, int Hq, int Hkv, int D, int max_tokens) {
   Plan p;
   const int64_t rows = static_cast<int64_t>(T) * (Hq / Hkv);
-  p.wide = rows <= kNarrowRows ? 0 : rows <= 128 ? 4 : 8;
+  p.wide = rows <= kFewRows ? -1 : rows <= kNarrowRows ? 0 : rows <= 128 ? 4 : 8;
   p.block_rows = kTile * std::max(p.wide, 1);
   p.row_blocks = static_cast<int>((rows + p.block_rows - 1) / p.block_rows);
   p.width = static_cast<int>(std::min<int64_t>(p.block_rows, rows));
-  p.min_per = 2;
-  // One round of the device, or fewer ranges where each has a few pages.
-  const int64_t units = static_cast<int64_t>(B) * Hkv * std::max(pages_of(max_tokens), 1);
-  const int64_t slots = p.wide ? 256 : 512;
-  const int64_t ranges = std::min((units + p.min_per - 1) / p.min_per, std::max<int64_t>(slots / p.row_blocks, 1));
+  p.min_per = 8;
+  // One round of the device.
+  const int64_t pages = std::max(pages_of(max_tokens), 1), units = static_cast<int64_t>(B) * Hkv * pages;
+  const int64_t slots = 256;
+  const int64_t ranges = std::min(units, std::max<int64_t>(slots / p.row_blocks, 1));
   p.ranges = static_cast<int>(std::max<int64_t>(ranges, 1));
-  // With a range for each (sequence, KV head) and no more, none is shared.
-  p.ws_bytes = static_cast<size_t>(static_cast<int64_t>(p.ranges) * p.row_blocks * 2 * p.width * (D + 2)) * 4;
+  const int64_t parts = static_cast<int64_t>(p.ranges) * p.row_blocks * 2;
+  p.ws_bytes = static_cast<size_t>(parts * p.width * (D + 2) + parts) * 4;
+  p.merge = p.wide > 0;
   return p;
 }
 
@@ -1200,8 +1599,10 @@ void launch(const TreeArgs& a, int wide, dim3 grid, hipStream_t st) {
     tree_wide_kernel<CT, D, 8><<<grid, kWideWaves * 64, 0, st>>>(a);
   else if (wide == 4)
     tree_wide_kernel<CT, D, 4><<<grid, kWideWaves * 64, 0, st>>>(a);
+  else if (wide == 0)
+    tree_rows_kernel<CT, D, kWaves><<<grid, kWaves * 64, 0, st>>>(a);
   else
-    tree_rows_kernel<CT, D, kRowWaves><<<grid, kRowWaves * 64, 0, st>>>(a);
+    tree_few_kernel<CT, D, kWaves><<<dim3(a.ranges), kWaves * 64, 0, st>>>(a);
 }
 
 // T and the tokens of a sequence that a call may hold.
@@ -1260,6 +1661,7 @@ extern "C" int spyre_paged_tree_attn(const void* q, const int64_t* q_strides, co
   a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.g = Hq / Hkv, a.rows = T * a.g;
   a.max_ctx = max_context_len, a.scale_log2 = scale * kLog2e;
   a.row_blocks = p.row_blocks, a.block_rows = p.block_rows, a.width = p.width, a.ranges = p.ranges, a.min_per = p.min_per;
+  a.ticket = spyre_hip::next_call_ticket();
   const int64_t pairs = static_cast<int64_t>(B) * Hkv, blocks = static_cast<int64_t>((p.ranges + 7) / 8 * 8) * p.row_blocks;
   SPYRE_REQUIRE(pairs * (pages_of(max_context_len + T) + 1) < (int64_t{1} << 30) && blocks < (int64_t{1} << 31),
                 SPYRE_EUNSUPPORTED, "too many pages or rows");
@@ -1280,14 +1682,17 @@ extern "C" int spyre_paged_tree_attn(const void* q, const int64_t* q_strides, co
     go(std::integral_constant<int, SPYRE_CODES_INT8>{});
   hipError_t e = hipGetLastError();
   SPYRE_REQUIRE(e == hipSuccess, SPYRE_EHIP, "tree attention launch failed: %s", hipGetErrorString(e));
-  const int64_t n = (static_cast<int64_t>(a.rows) * (D / 4) + 255) / 256;
-  SPYRE_REQUIRE(n <= 65535, SPYRE_EUNSUPPORTED, "too many rows");
-  const dim3 merge(static_cast<uint32_t>(pairs), static_cast<uint32_t>(n));
-  if (D == 128)
-    tree_merge_kernel<128><<<merge, 256, 0, st>>>(a);
-  else
-    tree_merge_kernel<64><<<merge, 256, 0, st>>>(a);
-  e = hipGetLastError();
-  SPYRE_REQUIRE(e == hipSuccess, SPYRE_EHIP, "tree attention merge launch failed: %s", hipGetErrorString(e));
+  if (p.merge) {
+    // Workgroups whose rows nobody shared leave at once; too many of those cost
+    // more than a few long loops (8192 of them 23 us).
+    const int64_t n = std::min((static_cast<int64_t>(a.rows) * (D / 4) + 255) / 256, std::max<int64_t>(2048 / pairs, 1));
+    const dim3 merge(static_cast<uint32_t>(pairs), static_cast<uint32_t>(n));
+    if (D == 128)
+      tree_merge_kernel<128><<<merge, 256, 0, st>>>(a);
+    else
+      tree_merge_kernel<64><<<merge, 256, 0, st>>>(a);
+    e = hipGetLastError();
+    SPYRE_REQUIRE(e == hipSuccess, SPYRE_EHIP, "tree attention merge launch failed: %s", hipGetErrorString(e));
+  }
   return SPYRE_OK;
 }
