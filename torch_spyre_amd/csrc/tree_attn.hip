@@ -339,6 +339,16 @@ __device__ __forceinline__ bool drop_odd(uint32_t& w) {
   return odd != 0;
 }
 
+// Pages are read by buffer loads: the base in scalar registers, 32-bit offsets a
+// lane, and every access clamped to the page.
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+constexpr int kAuxDevice = 16;  // sc1: device scope
+constexpr int kAuxOnce = 2;     // non-temporal: read once
+
+__device__ __forceinline__ Rsrc page_rsrc(const void* cache, int64_t head, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(static_cast<const uint8_t*>(cache)) + head * bytes, 0, bytes, 0x00020000);
+}
+
 // A wavefront's pages, one after the other from `first` on, as indexes of their
 // (page, KV head): 64 table entries at a time, one a lane, so that no page's
 // loads wait for its entry.  A page that the table does not name validly is
@@ -476,9 +486,6 @@ __device__ __forceinline__ void merge_parts(int r0, int r1, float& M, float& L, 
   }
 }
 
-typedef __amdgpu_buffer_rsrc_t Rsrc;
-constexpr int kAuxDevice = 16;  // sc1: device scope
-
 // The end of a piece whose wavefronts' partials are in LDS, O [W][rows][D + 4]
 // at s_o and (m, l) [W][rows] at s_ml: every thread folds 4 features of a row
 // over the wavefronts, in their order.  A whole (sequence, KV head) is then
@@ -606,34 +613,25 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
   float scale = 0.f;  // 8-bit: of the step's token `col`, K's in the lower lanes, V's in the upper
   auto load_k = [&](int st) {
     const int hp = st % PER_PAGE;
-    const uint8_t* p = a.k + head * (static_cast<int64_t>(kPage) * D * KB) + k_off;
-    if constexpr (CT == kF16) {
+    const Rsrc r = page_rsrc(a.k, head, kPage * D * KB);
 #pragma unroll
-      for (int s = 0; s < DS; ++s)
+    for (int s = 0; s < DS; ++s)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          kr.x[s][e] = *reinterpret_cast<const u32x4*>(p + hp * (STEP * 128) + (s / 2) * (kPage * 128) + (s % 2) * 64 + 16 * e);
-    } else {
-#pragma unroll
-      for (int s = 0; s < DS; ++s)
-        kr.x[s][0] = *reinterpret_cast<const u32x4*>(p + hp * (STEP * 16) + 2 * s * (kPage * 16));
+      for (int e = 0; e < KB; ++e)
+        kr.x[s][e] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+            r, k_off, CT == kF16 ? hp * (STEP * 128) + (s / 2) * (kPage * 128) + (s % 2) * 64 + 16 * e : hp * (STEP * 16) + 2 * s * (kPage * 16), 0));
+    if constexpr (CT != kF16)
       scale = (half ? a.vs : a.ks)[head * kPage + hp * STEP + col];
-    }
   };
   auto load_v = [&](int st) {
     const int hp = st % PER_PAGE;
-    const uint8_t* p = a.v + head * (static_cast<int64_t>(kPage) * D * KB) + v_off;
-    if constexpr (CT == kF16) {
+    const Rsrc r = page_rsrc(a.v, head, kPage * D * KB);
 #pragma unroll
-      for (int dt = 0; dt < DS; ++dt)
+    for (int dt = 0; dt < DS; ++dt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          vr.x[dt][e] = *reinterpret_cast<const u32x4*>(p + hp * (STEP * 2) + dt * (32 * kPage * 2) + 16 * e);
-    } else {
-#pragma unroll
-      for (int dt = 0; dt < DS; ++dt)
-        vr.x[dt][0] = *reinterpret_cast<const u32x4*>(p + 2 * hp * (D * 16) + dt * (32 * 16));
-    }
+      for (int e = 0; e < KB; ++e)
+        vr.x[dt][e] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+            r, v_off, CT == kF16 ? hp * (STEP * 2) + dt * (32 * kPage * 2) + 16 * e : 2 * hp * (D * 16) + dt * (32 * 16), 0));
   };
   // 8-bit: this wavefront's step: score factors, V's scales' logarithms and inverses.
   float* s_sc = s_mem + wave * 3 * STEP;
@@ -828,6 +826,7 @@ template <int CT, int D, int W>
 __global__ __launch_bounds__(W * 64, 2) void tree_few_kernel(TreeArgs a) {
   constexpr int KB = CT == kF16 ? 2 : 1, KW = KB;  // bytes of an element; 16-byte words of 16 of them
   constexpr int DQ = D / 64, DV = D / 16;
+  constexpr int SETS = D == 128 ? 1 : 2;
   constexpr int ROW = D + 4;
   __shared__ __align__(16) float s_mem[W * 16 * (ROW + 2)];
   static_assert(3 * kPage <= 16 * (ROW + 2), "a wavefront's scales fit its share");
@@ -872,36 +871,43 @@ __global__ __launch_bounds__(W * 64, 2) void tree_few_kernel(TreeArgs a) {
 #pragma unroll
     for (int dt = 0; dt < DV; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
-    u32x4 kr[4][DQ][KW], vr[DV][KW];
-    float ksc = 0.f, vsc = 0.f;  // 8-bit: of the page's token `lane`
-    auto load_k = [&](int64_t head) {
-      const uint8_t* p = a.k + head * (static_cast<int64_t>(kPage) * D * KB) + k_off;
+    // The raw operands of a page.  8-bit pages have two sets, which take turns:
+    // two pages are then in flight.
+    struct Operands {
+      u32x4 k[4][DQ][KW], v[DV][KW];
+      float ks, vs;  // 8-bit: scales of the page's token `lane`
+    };
+    Operands set[SETS];
+    auto load_k = [&](Operands& x, int64_t head) {
+      const Rsrc r = page_rsrc(a.k, head, kPage * D * KB);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int s = 0; s < DQ; ++s)
 #pragma unroll
           for (int e = 0; e < KW; ++e)
-            kr[j][s][e] = *reinterpret_cast<const u32x4*>(
-                p + (CT == kF16 ? s * (kPage * 128) + (32 * (j / 2) + 4 * (j % 2)) * 128 + 64 * e : 4 * s * (kPage * 16) + 16 * j * 16));
+            x.k[j][s][e] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                r, k_off,
+                CT == kF16 ? s * (kPage * 128) + (32 * (j / 2) + 4 * (j % 2)) * 128 + 64 * e : 4 * s * (kPage * 16) + 16 * j * 16,
+                kAuxOnce));
       if constexpr (CT != kF16) {
-        ksc = a.ks[head * kPage + lane];
-        vsc = a.vs[head * kPage + lane];
+        x.ks = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(page_rsrc(a.ks, head, kPage * 4), 4 * lane, 0, kAuxOnce));
+        x.vs = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(page_rsrc(a.vs, head, kPage * 4), 4 * lane, 0, kAuxOnce));
       }
     };
-    auto load_v = [&](int64_t head) {
-      const uint8_t* p = a.v + head * (static_cast<int64_t>(kPage) * D * KB) + v_off;
+    auto load_v = [&](Operands& x, int64_t head) {
+      const Rsrc r = page_rsrc(a.v, head, kPage * D * KB);
 #pragma unroll
       for (int dt = 0; dt < DV; ++dt)
 #pragma unroll
         for (int e = 0; e < KW; ++e)
-          vr[dt][e] = *reinterpret_cast<const u32x4*>(p + (CT == kF16 ? dt * (16 * kPage * 2) + 64 * e : dt * (16 * 16)));
+          x.v[dt][e] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+              r, v_off, CT == kF16 ? dt * (16 * kPage * 2) + 64 * e : dt * (16 * 16), kAuxOnce));
     };
-    int64_t head = 0;
-    // MORE: another page follows.  (A test of it at run time would leave the
+    // MORE: page p + SETS follows in the same registers.  (A test of it at run time would leave the
     // compiler paths on which K is loaded and V is not, and every page would
     // wait for its V before its first product.)
-    auto step = [&](int p, auto more_tag, auto edge_tag) {
+    auto step = [&](Operands& x, int p, auto more_tag, auto edge_tag) {
       constexpr bool MORE = decltype(more_tag)::value;
       constexpr bool EDGE = decltype(edge_tag)::value;   // some tokens are drafted or do not exist
       const int tok0 = p * kPage + tok_of0;
@@ -909,8 +915,8 @@ __global__ __launch_bounds__(W * 64, 2) void tree_few_kernel(TreeArgs a) {
       if constexpr (EDGE) seen = row.attends16(a, sq, tok0, total, offset);
       if constexpr (CT != kF16) {
         __builtin_amdgcn_wave_barrier();
-        const bool finite = __builtin_fabsf(vsc) <= 0x1.fffffep127f;
-        const uint64_t not_finite = __builtin_amdgcn_ballot_w64(!finite), infinite = __builtin_amdgcn_ballot_w64(vsc == INFINITY);
+        const bool finite = __builtin_fabsf(x.vs) <= 0x1.fffffep127f;
+        const uint64_t not_finite = __builtin_amdgcn_ballot_w64(!finite), infinite = __builtin_amdgcn_ballot_w64(x.vs == INFINITY);
         if (not_finite) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -918,8 +924,8 @@ __global__ __launch_bounds__(W * 64, 2) void tree_few_kernel(TreeArgs a) {
             inf_scale |= (static_cast<uint32_t>(infinite >> (16 * j + 4 * grp)) & 0xfu) << (4 * j);
           }
         }
-        const float vc = !finite ? 1.f : vsc < 0x1p-60f ? 0x1p-60f : vsc;
-        s_sc[lane] = ksc * a.scale_log2;
+        const float vc = !finite ? 1.f : x.vs < 0x1p-60f ? 0x1p-60f : x.vs;
+        s_sc[lane] = x.ks * a.scale_log2;
         s_sc[kPage + lane] = __builtin_amdgcn_logf(vc);
         s_sc[2 * kPage + lane] = __builtin_amdgcn_rcpf(vc);
         __builtin_amdgcn_wave_barrier();
@@ -932,11 +938,12 @@ __global__ __launch_bounds__(W * 64, 2) void tree_few_kernel(TreeArgs a) {
         for (int s = 0; s < DQ; ++s)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            sc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand<CT>(kr[j][s], e), qf[s][e], sc[j], 0, 0, 0);
+            sc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand<CT>(x.k[j][s], e), qf[s][e], sc[j], 0, 0, 0);
       }
+      int64_t head = 0;
       if constexpr (MORE) {
-        head = pages.head(p + 1);
-        load_k(head);
+        head = pages.head(p + SETS);
+        load_k(x, head);
       }
       float mx = -INFINITY;
 #pragma unroll
@@ -990,56 +997,76 @@ __global__ __launch_bounds__(W * 64, 2) void tree_few_kernel(TreeArgs a) {
 #pragma unroll
         for (int dt = 0; dt < DV; ++dt) {
           if constexpr (CT == kF16) {
-            u32x4 lo[1] = {vr[dt][0]}, hi[1] = {vr[dt][1]};  // 8 tokens each
+            u32x4 lo[1] = {x.v[dt][0]}, hi[1] = {x.v[dt][1]};  // 8 tokens each
             drop_tokens<CT>(lo, total - tok0);
             drop_tokens<CT>(hi, total - tok0 - 32);
-            vr[dt][0] = lo[0], vr[dt][1] = hi[0];
+            x.v[dt][0] = lo[0], x.v[dt][1] = hi[0];
           } else {
-            drop_tokens<CT>(vr[dt], total - p * kPage - 16 * grp);
+            drop_tokens<CT>(x.v[dt], total - p * kPage - 16 * grp);
           }
 #pragma unroll
           for (int e = 0; e < KW; ++e)
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-              uint32_t y = vr[dt][e][w];
+              uint32_t y = x.v[dt][e][w];
               odd = drop_odd<CT>(y) || odd;
-              vr[dt][e][w] = y;
+              x.v[dt][e][w] = y;
             }
         }
       }
 #pragma unroll
       for (int dt = 0; dt < DV; ++dt) {
         if constexpr (CT != kF16) {
-          uint32_t w[4] = {vr[dt][0][0], vr[dt][0][1], vr[dt][0][2], vr[dt][0][3]};
+          uint32_t w[4] = {x.v[dt][0][0], x.v[dt][0][1], x.v[dt][0][2], x.v[dt][0][3]};
           transpose4x4_groups(w);  // word j: tokens 16 j + 4 grp ..
-          vr[dt][0] = u32x4{w[0], w[1], w[2], w[3]};
+          x.v[dt][0] = u32x4{w[0], w[1], w[2], w[3]};
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand<CT>(vr[dt], e), pw[e], o[dt], 0, 0, 0);
+          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand<CT>(x.v[dt], e), pw[e], o[dt], 0, 0, 0);
       }
-      if constexpr (MORE) load_v(head);
+      if constexpr (MORE) load_v(x, head);
     };
     const int whole = min(p1, sq.ctx / kPage);
     std::true_type yes;
     std::false_type no;
     int p = p0;
+    auto load = [&](Operands& x, int page) {
+      const int64_t head = pages.head(page);
+      load_k(x, head);
+      load_v(x, head);
+    };
     if (p < whole) {
-      head = pages.head(p);
-      load_k(head);
-      load_v(head);
+      load(set[0], p);
+      if constexpr (SETS == 2) {
+        if (p + 1 < whole) load(set[1], p + 1);
+      }
       load_q();
-      for (; p < whole - 1; ++p) step(p, yes, no);
-      step(p, no, no);
-      ++p;
+      if constexpr (SETS == 2) {
+        for (; p + 3 < whole; p += 2) {
+          step(set[0], p, yes, no);
+          step(set[1], p + 1, yes, no);
+        }
+        if (p + 2 < whole) {
+          step(set[0], p, yes, no);
+          step(set[1], p + 1, no, no);
+          step(set[0], p + 2, no, no);
+        } else {
+          step(set[0], p, no, no);
+          if (p + 1 < whole) step(set[1], p + 1, no, no);
+        }
+        p = whole;
+      } else {
+        for (; p < whole - 1; ++p) step(set[0], p, yes, no);
+        step(set[0], p, no, no);
+        ++p;
+      }
     } else if (p < p1) {
       load_q();
     }
     for (; p < p1; ++p) {  // the sequence's last pages
-      head = pages.head(p);
-      load_k(head);
-      load_v(head);
-      step(p, no, yes);
+      load(set[0], p);
+      step(set[0], p, no, yes);
     }
     if (CT != SPYRE_CODES_INT8 && __any(odd))
       add_odd<CT, D, DV * 4>(
