@@ -139,20 +139,24 @@ __device__ __forceinline__ int scan64(int x) {
   return x;
 }
 
-// How the pages are shared out.  Units are the pages of every (sequence, KV
-// head), one after the other (a sequence of none counts one, which writes its
-// zeros); range r of `ranges` is units [r per, (r + 1) per), but for a bound
-// near the start or the end of its (sequence, KV head), which moves there: a
-// part costs its join, ranges are uneven by a few pages instead, and what has
-// no more than `per` <= 8 pages is never cut.  The lengths are data of the device, so every wavefront works
-// out the sums itself; ragged batches are then as even as equal ones.  A range
-// that holds only part of a (sequence, KV head) leaves a partial: in slot 1
-// that of the first part, in slot 0 that of any other.
+// How the pages are shared out.  A (sequence, KV head) counts kStart units, what
+// its beginning and end cost, and then one for each page; range r of `ranges` is
+// the units [r per, (r + 1) per) of all, one (sequence, KV head) after the
+// other.  A bound that would leave a piece of few pages moves to the
+// (sequence, KV head)'s end: a part costs its join.  The lengths are data of
+// the device, so every wavefront works out the sums itself; ragged batches are
+// then as even as equal ones.  A range that holds only part of a (sequence, KV
+// head) leaves a partial: in slot 1 that of the first part, in slot 0 that of
+// any other.
+// kStart: 64 sequences of 128 to 16384 tokens, longest first, took 237 us
+// where pages alone were counted: a workgroup had 60 short ones.
+constexpr int kStart = 4;
+
 struct Walk {
-  int per, u, end;            // units
-  int b, base, pages;         // the sequence: its first unit / Hkv, its units a KV head
-  __device__ __forceinline__ static int units_of(const TreeArgs& a, int b) {
-    return max(1, seq_of(a, a.ctx[b], a.counts ? a.counts[b] : a.T).pages);
+  int per, u, end;      // units
+  int b, base, size;    // the sequence: its first unit / Hkv, its units a KV head
+  __device__ __forceinline__ static int size_of(const TreeArgs& a, int b) {
+    return kStart + seq_of(a, a.ctx[b], a.counts ? a.counts[b] : a.T).pages;
   }
   // Units a KV head of all sequences; the first 64 sequences', one a lane.
   __device__ __forceinline__ static int total_of(const TreeArgs& a, int lane, int& first64) {
@@ -162,43 +166,44 @@ struct Walk {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int i = c + 64 * k + lane;
-        x[k] = i < a.B ? units_of(a, i) : 0;
+        x[k] = i < a.B ? size_of(a, i) : 0;
       }
       if (c == 0) first64 = x[0];
       sum += x[0] + x[1] + x[2] + x[3];
     }
     return __builtin_amdgcn_readlane(scan64(sum), 63);
   }
-  // An equal share, but at least min_per pages where (sequence, KV head)s have
-  // as many.
+  // An equal share, but no smaller than a mean (sequence, KV head) cut into
+  // parts of min_per pages.
   __device__ __forceinline__ static int per_of(const TreeArgs& a, int total) {
-    return max(static_cast<int>(fdiv(total * a.Hkv + a.ranges - 1, a.by_ranges)),
-               min(a.min_per, total / a.B));
+    const int mean = total / a.B, parts = max(1, (mean - kStart) / a.min_per);
+    return max(static_cast<int>(fdiv(total * a.Hkv + a.ranges - 1, a.by_ranges)), (mean + parts - 1) / parts);
   }
-  __device__ __forceinline__ int near() const { return per <= 8 ? per / 2 : 4; }
+  // Pages that are too few for a piece.
+  __device__ __forceinline__ int few() const { return min(max(per - kStart, 0) / 2, 4); }
   // The sequence of a unit (below the total).
   __device__ __forceinline__ void find(const TreeArgs& a, int lane, int first64, int unit) {
     const int target = static_cast<int>(fdiv(unit, a.by_hkv));
     base = 0;
     for (int c = 0;; c += 64) {  // ends: target is below the total
-      const int x = c == 0 ? first64 : c + lane < a.B ? units_of(a, c + lane) : 0;
+      const int x = c == 0 ? first64 : c + lane < a.B ? size_of(a, c + lane) : 0;
       const int sum = scan64(x);
       const uint64_t past = __builtin_amdgcn_ballot_w64(base + sum > target);
       if (past) {
         const int i = __builtin_ctzll(past);
         b = c + i;
-        pages = __builtin_amdgcn_readlane(x, i);
-        base += __builtin_amdgcn_readlane(sum, i) - pages;
+        size = __builtin_amdgcn_readlane(x, i);
+        base += __builtin_amdgcn_readlane(sum, i) - size;
         return;
       }
       base += __builtin_amdgcn_readlane(sum, 63);
     }
   }
   // A bound where it belongs, after find() of it.
-  __device__ __forceinline__ int snapped(const TreeArgs& a, int unit) const {
-    const uint32_t in = unit - base * a.Hkv, at = in % static_cast<uint32_t>(pages);
-    const int g0 = unit - static_cast<int>(at), g1 = g0 + pages;
-    return unit - g0 <= near() ? g0 : g1 - unit <= near() ? g1 : unit;
+  __device__ __forceinline__ int placed(const TreeArgs& a, int unit) const {
+    const uint32_t in = unit - base * a.Hkv, at = in % static_cast<uint32_t>(size);
+    const int g0 = unit - static_cast<int>(at), g1 = g0 + size;
+    return static_cast<int>(at) - kStart <= few() ? g0 : g1 - unit <= few() ? g1 : unit;
   }
   // Range r; false if it is empty.
   __device__ __forceinline__ bool start(const TreeArgs& a, int lane, int r) {
@@ -210,18 +215,18 @@ struct Walk {
     end = units;
     if (u + per < units) {
       find(a, lane, x, u + per);
-      end = snapped(a, u + per);
+      end = placed(a, u + per);
     }
     find(a, lane, x, u);
-    u = snapped(a, u);
+    u = placed(a, u);
     if (u >= end) return false;
-    if (u == (base + pages) * a.Hkv) next_sequence(a);
+    if (u == (base + size) * a.Hkv) next_sequence(a);
     return true;
   }
   __device__ __forceinline__ void next_sequence(const TreeArgs& a) {
-    base += pages;
+    base += size;
     b += 1;
-    pages = max(1, seq_at(a, b).pages);
+    size = kStart + seq_at(a, b).pages;
   }
   // Sequence `seq` and `per`, for parts_of().
   __device__ __forceinline__ void seek(const TreeArgs& a, int lane, int seq) {
@@ -229,18 +234,18 @@ struct Walk {
     per = per_of(a, total_of(a, lane, x));
     b = seq;
     for (int c = 0; c <= seq; c += 64) {
-      if (c > 0) x = c + lane < a.B ? units_of(a, c + lane) : 0;
+      if (c > 0) x = c + lane < a.B ? size_of(a, c + lane) : 0;
       before += c + lane < seq ? x : 0;
     }
     base = __builtin_amdgcn_readlane(scan64(before), 63);
-    pages = max(1, seq_at(a, seq).pages);
+    size = kStart + seq_at(a, seq).pages;
   }
   // The ranges that hold parts of a KV head of the sequence: r0 the first one,
   // r0 + 1 .. r1 the others; r1 <= r0 where one range holds it whole.
   __device__ __forceinline__ void parts_of(const TreeArgs& a, int kvh, int& r0, int& r1) const {
-    const int g0 = base * a.Hkv + kvh * pages, g1 = g0 + pages;
-    r0 = (g0 + near()) / per;
-    r1 = (g1 - near() - 1) / per;
+    const int g0 = base * a.Hkv + kvh * size, g1 = g0 + size;
+    r0 = (g0 + kStart + few()) / per;
+    r1 = (g1 - few() - 1) / per;
   }
 };
 
@@ -253,19 +258,20 @@ struct Piece {
 
 __device__ __forceinline__ Piece piece_of(const TreeArgs& a, const Walk& w) {
   Piece p;
-  const uint32_t in = w.u - w.base * a.Hkv;
-  p.kvh = in / static_cast<uint32_t>(w.pages);
-  p.page0 = in - p.kvh * w.pages;
-  p.page1 = min(w.pages, p.page0 + w.end - w.u);
-  p.whole = p.page0 == 0 && p.page1 == w.pages;
-  p.slot = p.page0 == 0 ? 1 : 0;
+  const int in = w.u - w.base * a.Hkv;
+  p.kvh = static_cast<uint32_t>(in) / static_cast<uint32_t>(w.size);
+  const int at = in - p.kvh * w.size;
+  p.page0 = max(at - kStart, 0);
+  p.page1 = min(w.size, at + w.end - w.u) - kStart;
+  p.whole = at == 0 && p.page1 == w.size - kStart;
+  p.slot = at == 0 ? 1 : 0;
   return p;
 }
 
 // After it.
 __device__ __forceinline__ void advance(const TreeArgs& a, Walk& w, const Piece& p) {
-  w.u += p.page1 - p.page0;
-  if (w.u < w.end && p.page1 == w.pages && p.kvh == a.Hkv - 1) w.next_sequence(a);
+  w.u = w.base * a.Hkv + p.kvh * w.size + kStart + p.page1;
+  if (w.u < w.end && p.kvh == a.Hkv - 1 && p.page1 == w.size - kStart) w.next_sequence(a);
 }
 
 // The range and the row block of a workgroup.  The row blocks of one range
@@ -1595,7 +1601,7 @@ constexpr int kFewRows = 16;
 constexpr int kNarrowRows = 64;
 
 struct Plan {
-  int wide;  // row tiles of a workgroup of the wide kernel; 0: the rows kernel, -1: the few
+  int wide;  // row tiles of a workgroup of the wide kernel; 0: the rows kernel; -1: the few, -2: in half workgroups
   int row_blocks, block_rows, width, ranges, min_per;
   bool merge;  // a second kernel joins the parts
   size_t ws_bytes;
@@ -1604,14 +1610,17 @@ struct Plan {
 Plan plan_of(int B, int T, int Hq, int Hkv, int D, int max_tokens) {
   Plan p;
   const int64_t rows = static_cast<int64_t>(T) * (Hq / Hkv);
-  p.wide = rows <= kFewRows ? -1 : rows <= kNarrowRows ? 0 : rows <= 128 ? 4 : 8;
+  // Half workgroups, two to a compute unit, where each has a (sequence, KV
+  // head) of its own (64 x 8 x 1024 tokens 28.8 -> 25.5 us, x 8192 168.5 -> 165.5);
+  // fewer would be cut for them (32 x 8 x 4096 45.6 -> 50.0).
+  p.wide = rows <= kFewRows ? (static_cast<int64_t>(B) * Hkv >= 512 ? -2 : -1) : rows <= kNarrowRows ? 0 : rows <= 128 ? 4 : 8;
   p.block_rows = kTile * std::max(p.wide, 1);
   p.row_blocks = static_cast<int>((rows + p.block_rows - 1) / p.block_rows);
   p.width = static_cast<int>(std::min<int64_t>(p.block_rows, rows));
   p.min_per = 8;
   // One round of the device.
-  const int64_t pages = std::max(pages_of(max_tokens), 1), units = static_cast<int64_t>(B) * Hkv * pages;
-  const int64_t slots = 256;
+  const int64_t pages = std::max(pages_of(max_tokens), 1), units = static_cast<int64_t>(B) * Hkv * (pages + kStart);
+  const int64_t slots = p.wide == -2 ? 512 : 256;
   const int64_t ranges = std::min(units, std::max<int64_t>(slots / p.row_blocks, 1));
   p.ranges = static_cast<int>(std::max<int64_t>(ranges, 1));
   const int64_t parts = static_cast<int64_t>(p.ranges) * p.row_blocks * 2;
@@ -1628,8 +1637,10 @@ void launch(const TreeArgs& a, int wide, dim3 grid, hipStream_t st) {
     tree_wide_kernel<CT, D, 4><<<grid, kWideWaves * 64, 0, st>>>(a);
   else if (wide == 0)
     tree_rows_kernel<CT, D, kWaves><<<grid, kWaves * 64, 0, st>>>(a);
-  else
+  else if (wide == -1)
     tree_few_kernel<CT, D, kWaves><<<dim3(a.ranges), kWaves * 64, 0, st>>>(a);
+  else
+    tree_few_kernel<CT, D, kWaves / 2><<<dim3(a.ranges), kWaves / 2 * 64, 0, st>>>(a);
 }
 
 // T and the tokens of a sequence that a call may hold.
@@ -1690,7 +1701,7 @@ extern "C" int spyre_paged_tree_attn(const void* q, const int64_t* q_strides, co
   a.row_blocks = p.row_blocks, a.block_rows = p.block_rows, a.width = p.width, a.ranges = p.ranges, a.min_per = p.min_per;
   a.ticket = spyre_hip::next_call_ticket();
   const int64_t pairs = static_cast<int64_t>(B) * Hkv, blocks = static_cast<int64_t>((p.ranges + 7) / 8 * 8) * p.row_blocks;
-  SPYRE_REQUIRE(pairs * (pages_of(max_context_len + T) + 1) < (int64_t{1} << 30) && blocks < (int64_t{1} << 31),
+  SPYRE_REQUIRE(pairs * (pages_of(max_context_len + T) + kStart + 1) < (int64_t{1} << 30) && blocks < (int64_t{1} << 31),
                 SPYRE_EUNSUPPORTED, "too many pages or rows");
   a.by_g = make_fastdiv(static_cast<uint32_t>(a.g)), a.by_hkv = make_fastdiv(static_cast<uint32_t>(Hkv));
   a.by_blocks = make_fastdiv(static_cast<uint32_t>(p.row_blocks));
