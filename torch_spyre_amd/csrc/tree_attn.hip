@@ -71,7 +71,7 @@ struct TreeArgs {
   // The rows of a KV head are cut into row_blocks of block_rows; a partial
   // holds `width` of them, the fewer of block_rows and rows.
   int row_blocks, block_rows, width;
-  int ranges, min_per, each;  // see Walk; each: (sequence, KV head)s a range where that is a whole number, else 0
+  int ranges, min_per, min_cut, each;  // see Walk; each: (sequence, KV head)s a range where that is a whole number, else 0
   uint32_t ticket;      // see finish()
   FastDiv by_g, by_hkv, by_blocks, by_ranges;
 };
@@ -166,22 +166,29 @@ constexpr int kStart = 4;
 struct Walk {
   int per, u, end;      // units
   int b, base, size;    // the sequence: its first unit / Hkv, its units a KV head
+  Seq seq;              // what it holds
   bool uncut;           // range r is the (sequence, KV head)s [r each, (r + 1) each)
-  __device__ __forceinline__ static int size_of(const TreeArgs& a, int b) {
-    return kStart + seq_of(a, a.ctx[b], a.counts ? a.counts[b] : a.T).pages;
+  // A sequence a lane: its lengths as they were given, its units a KV head.
+  struct Lane {
+    int ctx = 0, count = 0, size = 0;
+  };
+  __device__ __forceinline__ static Lane lane_of(const TreeArgs& a, int b) {
+    Lane x;
+    if (b < a.B) {
+      x.ctx = a.ctx[b], x.count = a.counts ? a.counts[b] : a.T;
+      x.size = kStart + seq_of(a, x.ctx, x.count).pages;
+    }
+    return x;
   }
   // Units a KV head of all sequences and the largest one's; the first 64
-  // sequences', one a lane.
-  __device__ __forceinline__ static int total_of(const TreeArgs& a, int lane, int& first64, int& largest) {
+  // sequences, one a lane.
+  __device__ __forceinline__ static int total_of(const TreeArgs& a, int lane, Lane& first64, int& largest) {
     int sum = 0, top = 0;
+    first64 = lane_of(a, lane);
     for (int c = 0; c < a.B; c += 256) {
       int x[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int i = c + 64 * k + lane;
-        x[k] = i < a.B ? size_of(a, i) : 0;
-      }
-      if (c == 0) first64 = x[0];
+      for (int k = 0; k < 4; ++k) x[k] = c == 0 && k == 0 ? first64.size : lane_of(a, c + 64 * k + lane).size;
       sum += x[0] + x[1] + x[2] + x[3];
       top = max(max(top, max(x[0], x[1])), max(x[2], x[3]));
     }
@@ -189,33 +196,38 @@ struct Walk {
     return __builtin_amdgcn_readlane(scan64(sum), 63);
   }
   // An equal share, but no smaller than a mean (sequence, KV head) cut into
-  // parts of min_per pages.  Where a whole number of (sequence, KV head)s to a
+  // parts of min_per pages, or uncut below min_cut.  Where a whole number of (sequence, KV head)s to a
   // range is within an eighth of it, none is cut: 16 x 8 of 8000 to 8192 tokens
   // and 512 rows, whose parts take 20 us to join.
   __device__ __forceinline__ void share(const TreeArgs& a, int total, int largest) {
-    const int mean = total / a.B, parts = max(1, (mean - kStart) / a.min_per);
+    const int mean = total / a.B, pages = mean - kStart, parts = pages < a.min_cut ? 1 : max(1, pages / a.min_per);
     per = max(static_cast<int>(fdiv(total * a.Hkv + a.ranges - 1, a.by_ranges)), (mean + parts - 1) / parts);
     uncut = a.each > 0 && static_cast<int64_t>(largest) * a.each <= per + per / 8;
   }
   // Pages that are too few for a piece.
   __device__ __forceinline__ int few() const { return min(max(per - kStart, 0) / 2, 4); }
   // The sequence of a unit (below the total).
-  __device__ __forceinline__ void find(const TreeArgs& a, int lane, int first64, int unit) {
+  __device__ __forceinline__ void find(const TreeArgs& a, int lane, const Lane& first64, int unit) {
     const int target = static_cast<int>(fdiv(unit, a.by_hkv));
     base = 0;
     for (int c = 0;; c += 64) {  // ends: target is below the total
-      const int x = c == 0 ? first64 : c + lane < a.B ? size_of(a, c + lane) : 0;
-      const int sum = scan64(x);
+      const Lane x = c == 0 ? first64 : lane_of(a, c + lane);
+      const int sum = scan64(x.size);
       const uint64_t past = __builtin_amdgcn_ballot_w64(base + sum > target);
       if (past) {
         const int i = __builtin_ctzll(past);
         b = c + i;
-        size = __builtin_amdgcn_readlane(x, i);
+        take(a, x, i);
         base += __builtin_amdgcn_readlane(sum, i) - size;
         return;
       }
       base += __builtin_amdgcn_readlane(sum, 63);
     }
+  }
+  // The sequence of lane i.
+  __device__ __forceinline__ void take(const TreeArgs& a, const Lane& x, int i) {
+    seq = seq_of(a, __builtin_amdgcn_readlane(x.ctx, i), __builtin_amdgcn_readlane(x.count, i));
+    size = kStart + seq.pages;
   }
   // A bound where it belongs, after find() of it.
   __device__ __forceinline__ int placed(const TreeArgs& a, int unit) const {
@@ -225,16 +237,17 @@ struct Walk {
   }
   // Range r; false if it is empty.
   __device__ __forceinline__ bool start(const TreeArgs& a, int lane, int r) {
-    int x = 0, largest;
+    Lane x;
+    int largest;
     const int total = total_of(a, lane, x, largest), units = total * a.Hkv;
     share(a, total, largest);
     if (uncut) {
-      const int first = r * a.each, seq = static_cast<int>(fdiv(first, a.by_hkv)), kvh = first - seq * a.Hkv;
-      to(a, lane, x, seq);
+      const int first = r * a.each, at0 = static_cast<int>(fdiv(first, a.by_hkv)), kvh = first - at0 * a.Hkv;
+      to(a, lane, x, at0);
       u = base * a.Hkv + kvh * size;
       end = u;
-      for (int k = 0, at = seq, h = kvh; k < a.each; ++k) {
-        end += at == seq ? size : kStart + seq_at(a, at).pages;
+      for (int k = 0, at = at0, h = kvh; k < a.each; ++k) {
+        end += at == at0 ? size : kStart + seq_at(a, at).pages;
         if (++h == a.Hkv) h = 0, ++at;
       }
       return true;
@@ -255,24 +268,28 @@ struct Walk {
   __device__ __forceinline__ void next_sequence(const TreeArgs& a) {
     base += size;
     b += 1;
-    size = kStart + seq_at(a, b).pages;
+    seq = seq_at(a, b);
+    size = kStart + seq.pages;
   }
-  __device__ __forceinline__ void to(const TreeArgs& a, int lane, int first64, int seq) {
+  // To sequence i.
+  __device__ __forceinline__ void to(const TreeArgs& a, int lane, const Lane& first64, int i) {
     int before = 0;
-    for (int c = 0; c <= seq; c += 64) {
-      const int x = c == 0 ? first64 : c + lane < a.B ? size_of(a, c + lane) : 0;
-      before += c + lane < seq ? x : 0;
+    Lane x;
+    for (int c = 0; c <= i; c += 64) {
+      x = c == 0 ? first64 : lane_of(a, c + lane);
+      before += c + lane < i ? x.size : 0;
     }
-    b = seq;
+    b = i;
     base = __builtin_amdgcn_readlane(scan64(before), 63);
-    size = kStart + seq_at(a, seq).pages;
+    take(a, x, i % 64);
   }
-  // Sequence `seq` and the shares, for parts_of().
-  __device__ __forceinline__ void seek(const TreeArgs& a, int lane, int seq) {
-    int x = 0, largest;
+  // Sequence i and the shares, for parts_of().
+  __device__ __forceinline__ void seek(const TreeArgs& a, int lane, int i) {
+    Lane x;
+    int largest;
     const int total = total_of(a, lane, x, largest);
     share(a, total, largest);
-    to(a, lane, x, seq);
+    to(a, lane, x, i);
   }
   // The ranges that hold parts of a KV head of the sequence: r0 the first one,
   // r0 + 1 .. r1 the others; r1 <= r0 where one range holds it whole.
@@ -625,7 +642,7 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
   for (; walk.u < walk.end;) {
   const Piece pc = piece_of(a, walk);
   const int b = walk.b, kvh = pc.kvh;
-  const Seq sq = seq_at(a, b);
+  const Seq sq = walk.seq;
   const int total = sq.ctx + (a.draft_keys ? sq.n : 0);
   // The wavefronts take equal shares of the piece's steps; rows of no drafted token none.
   const int c0 = pc.page0 * PER_PAGE, c1 = tile * kTile < sq.n * a.g ? min(pc.page1 * PER_PAGE, (total + STEP - 1) / STEP) : c0;
@@ -885,7 +902,7 @@ __global__ __launch_bounds__(W * 64, 2) void tree_few_kernel(TreeArgs a) {
   for (; walk.u < walk.end;) {
     const Piece pc = piece_of(a, walk);
     const int b = walk.b, kvh = pc.kvh;
-    const Seq sq = seq_at(a, b);
+    const Seq sq = walk.seq;
     const int total = sq.ctx + (a.draft_keys ? sq.n : 0);
     const int c1 = sq.n > 0 ? min(pc.page1, sq.pages) : pc.page0, nc = c1 - pc.page0;
     const int p0 = pc.page0 + nc * wave / W, p1 = pc.page0 + nc * (wave + 1) / W;
@@ -1191,7 +1208,7 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
   for (; walk.u < walk.end;) {
     const Piece pc = piece_of(a, walk);
     const int b = walk.b, kvh = pc.kvh;
-    const Seq sq = seq_at(a, b);
+    const Seq sq = walk.seq;
     const int total = sq.ctx + (a.draft_keys ? sq.n : 0);
     const int p0 = pc.page0, p1 = min(pc.page1, sq.pages);
     const int local = RT == W ? wave : wave >> 1, tile = rb * RT + local;
@@ -1611,7 +1628,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   int r0, r1;
   w.parts_of(a, kvh, r0, r1);
   if (r1 <= r0) return;
-  const Seq sq = seq_at(a, b);
+  const Seq sq = w.seq;
   for (int u = blockIdx.y * 256 + threadIdx.x; u < a.rows * (D / 4); u += gridDim.y * 256) {
     const int row = u / (D / 4), d = 4 * (u % (D / 4));
     const int i = static_cast<int>(fdiv(row, a.by_g)), rb = row / a.block_rows, rl = row - rb * a.block_rows;
@@ -1636,7 +1653,7 @@ constexpr int kNarrowRows = 64;
 
 struct Plan {
   int wide;  // row tiles of a workgroup of the wide kernel; 0: the rows kernel; -1: the few, -2: in half workgroups
-  int row_blocks, block_rows, width, ranges, min_per;
+  int row_blocks, block_rows, width, ranges, min_per, min_cut;
   bool merge;  // a second kernel joins the parts
   size_t ws_bytes;
 };
@@ -1651,11 +1668,16 @@ Plan plan_of(int B, int T, int Hq, int Hkv, int D, int max_tokens) {
   p.block_rows = kTile * std::max(p.wide, 1);
   p.row_blocks = static_cast<int>((rows + p.block_rows - 1) / p.block_rows);
   p.width = static_cast<int>(std::min<int64_t>(p.block_rows, rows));
-  p.min_per = 8;
-  // One round of the device.
-  const int64_t pages = std::max(pages_of(max_tokens), 1), units = static_cast<int64_t>(B) * Hkv * (pages + kStart);
+  // Parts of fewer pages cost more to join than they save (one sequence of 1024
+  // tokens, us at 2 / 3 / 4 / 8 pages a part: 64 rows 13.2 / 13.5 / 15 / 17;
+  // 256 rows, whose joining is launched in any case, 29 / 31 / 32 / 42).  Few
+  // rows: 12 pages are one or two for each wavefront.
+  p.min_per = p.wide > 0 ? 2 : p.wide == 0 ? 6 : 3;
+  p.min_cut = p.wide < 0 ? 13 : 2 * p.min_per;
+  // One round of the device, or as many parts as there can be.
+  const int64_t pages = std::max(pages_of(max_tokens), 1), parts_of_one = pages < p.min_cut ? 1 : pages / p.min_per;
   const int64_t slots = p.wide == -2 ? 512 : 256;
-  const int64_t ranges = std::min(units, std::max<int64_t>(slots / p.row_blocks, 1));
+  const int64_t ranges = std::min(B * (Hkv * parts_of_one), std::max<int64_t>(slots / p.row_blocks, 1));
   p.ranges = static_cast<int>(std::max<int64_t>(ranges, 1));
   const int64_t parts = static_cast<int64_t>(p.ranges) * p.row_blocks * 2;
   p.ws_bytes = static_cast<size_t>(parts * p.width * (D + 2) + parts) * 4;
@@ -1732,7 +1754,7 @@ extern "C" int spyre_paged_tree_attn(const void* q, const int64_t* q_strides, co
   a.out = static_cast<_Float16*>(out), a.lse = lse, a.ws = static_cast<float*>(workspace);
   a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.g = Hq / Hkv, a.rows = T * a.g;
   a.max_ctx = max_context_len, a.scale_log2 = scale * kLog2e;
-  a.row_blocks = p.row_blocks, a.block_rows = p.block_rows, a.width = p.width, a.ranges = p.ranges, a.min_per = p.min_per;
+  a.row_blocks = p.row_blocks, a.block_rows = p.block_rows, a.width = p.width, a.ranges = p.ranges, a.min_per = p.min_per, a.min_cut = p.min_cut;
   a.each = static_cast<int64_t>(B) * Hkv % p.ranges == 0 ? static_cast<int>(static_cast<int64_t>(B) * Hkv / p.ranges) : 0;
   a.ticket = spyre_hip::next_call_ticket();
   const int64_t pairs = static_cast<int64_t>(B) * Hkv, blocks = static_cast<int64_t>((p.ranges + 7) / 8 * 8) * p.row_blocks;
