@@ -263,7 +263,7 @@ struct ReadArgs {
 // result is token start + i; tokens from lens on are zeros, those of a page
 // that the table does not name validly NaN.
 template <int KIND, int D>
-__global__ __launch_bounds__(kWaves * 64) void read_kernel(ReadArgs a) {
+__global__ __launch_bounds__(kWaves * 64, 6) void read_kernel(ReadArgs a) {
   constexpr int HP = 128 / D;
   const uint32_t u = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   if (u >= a.units) return;
@@ -293,38 +293,33 @@ __global__ __launch_bounds__(kWaves * 64) void read_kernel(ReadArgs a) {
     else if (bad)
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = static_cast<_Float16>(__builtin_nanf(""));
-    __builtin_nontemporal_store(x, reinterpret_cast<f16x8*>(out + i * D + f));
+    *reinterpret_cast<f16x8*>(out + i * D + f) = x;
   };
   auto value = [&](uint32_t w0, uint32_t w1, float s) {
-    float x[8], (&lo)[4] = *reinterpret_cast<float(*)[4]>(x), (&hi)[4] = *reinterpret_cast<float(*)[4]>(x + 4);
-    codes_to_f32<KIND>(w0, lo);
-    codes_to_f32<KIND>(w1, hi);
+    const f16x8 x = codes_to_f16x8<KIND>(w0, w1);
     f16x8 y;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = static_cast<_Float16>(x[e] * s);
+    for (int e = 0; e < 8; ++e) y[e] = static_cast<_Float16>(static_cast<float>(x[e]) * s);
     return y;
   };
   const bool load = !none && !bad;
   if ((u & 1) == 0) {
-    constexpr int U = D / 16, TS = 64 / U, N = kPage / TS;  // units of a row; tokens of an instruction
-    const int un = lane % U, tk = lane / U;
-    const uint8_t* src = a.kc + head * (D * kPage) + un * (kPage * 16);
-    u32x4 x[N];
+    constexpr int LR = D / 8, TS = 64 / LR, N = kPage / TS;  // lanes of a token, 8 features each; tokens of an instruction
+    const int f = 8 * (lane % LR), tk = lane / LR;
+    const uint8_t* src = a.kc + head * (D * kPage) + f / 16 * (kPage * 16) + f % 16;
+    u32x2 x[N];
     float s[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      x[i] = u32x4{0, 0, 0, 0};
+      x[i] = u32x2{0, 0};
       s[i] = 0.f;
       if (load) {
-        x[i] = *reinterpret_cast<const u32x4*>(src + (tk + TS * i) * 16);
+        x[i] = *reinterpret_cast<const u32x2*>(src + (tk + TS * i) * 16);
         s[i] = sc[tk + TS * i];
       }
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      put(tk + TS * i, un * 16, value(x[i][0], x[i][1], s[i]));
-      put(tk + TS * i, un * 16 + 8, value(x[i][2], x[i][3], s[i]));
-    }
+    for (int i = 0; i < N; ++i) put(tk + TS * i, f, value(x[i][0], x[i][1], s[i]));
   } else {
     constexpr int LH = 16 / HP;  // lanes of a 16-token unit's features
     const int rl = lane % 16, g = lane / 16, f = 8 * (rl % LH);
