@@ -31,6 +31,7 @@ constexpr int kLdsPairs = 64;  // R / 2 <= D / 2
 typedef c8_f16x8 f16x8;
 typedef c8_u32x4 u32x4;
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ uint32_t umax_row(uint32_t x, bool sixteen) {
 #define SPYRE_DPP(ctrl) x = max(x, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), ctrl, 0xf, 0xf, false)))
@@ -94,7 +95,7 @@ struct AppendArgs {
 // slice.  A wavefront takes a row of 16 lanes x 8 features for 4 x 4 tokens at
 // once (lane group g: tokens 4 g .. 4 g + 3), so that a whole V unit turns
 // into 16-byte pieces in registers (4 x 4 bytes, then 4 x 4 words over the lane
-// groups); tokens that do not fill a unit are written byte by byte.
+// groups); quarters of a unit are written as words, other tokens byte by byte.
 template <int KIND, int D, bool ROTATE, bool INTERLEAVED>
 __global__ __launch_bounds__(kWaves * 64) void append_kernel(AppendArgs a) {
   constexpr int HP = 128 / D;      // heads of a row
@@ -142,8 +143,12 @@ __global__ __launch_bounds__(kWaves * 64) void append_kernel(AppendArgs a) {
   const int64_t unit0 = __builtin_amdgcn_readfirstlane(static_cast<int>(where[0] & 0xffffffff)) & 0xffffffffll;
   const int64_t unit = unit0 | static_cast<int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(where[0] >> 32))) << 32;
   bool in_unit = unit >= 0 && unit % kGroup == 0;
+  bool quad = where[0] >= 0 && where[0] % 4 == 0;  // this lane's tokens are a quarter of a unit
 #pragma unroll
-  for (int p = 0; p < 4; ++p) in_unit = in_unit && where[p] == unit + 4 * g + p;
+  for (int p = 0; p < 4; ++p) {
+    in_unit = in_unit && where[p] == unit + 4 * g + p;
+    quad = quad && where[p] == where[0] + p;
+  }
   const bool whole = __all(in_unit);
   const int row_end = min(a.q_rows + 2 * a.kv_rows, static_cast<int>(blockIdx.y + 1) * a.rows_per_slice);
   for (int r = blockIdx.y * a.rows_per_slice + wave; r < row_end; r += kWaves) {
@@ -214,17 +219,35 @@ __global__ __launch_bounds__(kWaves * 64) void append_kernel(AppendArgs a) {
     const int64_t hk = static_cast<int64_t>(h) * kPage;
     if (rl % LH == 0 && head) {
       float* sc = what == 1 ? a.ks : a.vs;
+      if (quad) {
+        *reinterpret_cast<f32x4*>(sc + where[0] + hk) = f32x4{scale[0], scale[1], scale[2], scale[3]};
+      } else {
 #pragma unroll
-      for (int p = 0; p < 4; ++p)
-        if (where[p] >= 0) sc[where[p] + hk] = scale[p];
+        for (int p = 0; p < 4; ++p)
+          if (where[p] >= 0) sc[where[p] + hk] = scale[p];
+      }
     }
     if (what == 1) {
+      // Two lanes hold the halves of a token's units: the even one takes those
+      // of its tokens 0 and 1, the odd one those of 2 and 3.
+      const bool odd = lane % 2 != 0;
+      auto unit_of = [&](uint32_t (&even_w)[2], uint32_t (&odd_w)[2], int64_t even_at, int64_t odd_at) {
+        uint32_t mine[2], other[2];
 #pragma unroll
-      for (int p = 0; p < 4; ++p)
-        if (where[p] >= 0 && head) {
-          const int64_t slot = where[p] % kPage, base = (where[p] - slot + hk) * D;
-          *reinterpret_cast<u32x2*>(a.kc + base + (f / 16) * (kPage * 16) + slot * 16 + f % 16) = u32x2{w[p][0], w[p][1]};
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t x = even_w[j], y = odd_w[j];
+          mine[j] = odd ? y : x;
+          other[j] = static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(odd ? x : y), 0xb1, 0xf, 0xf, false));
         }
+        const int64_t at = odd ? odd_at : even_at;
+        if (at >= 0 && head) {
+          const int64_t slot = at % kPage, base = (at - slot + hk) * D;
+          *reinterpret_cast<u32x4*>(a.kc + base + (f / 16) * (kPage * 16) + slot * 16) =
+              odd ? u32x4{other[0], other[1], mine[0], mine[1]} : u32x4{mine[0], mine[1], other[0], other[1]};
+        }
+      };
+      unit_of(w[0], w[2], where[0], where[2]);
+      unit_of(w[1], w[3], where[1], where[3]);
     } else if (whole) {
       const int64_t slot = unit % kPage, base = (unit - slot + hk) * D;
 #pragma unroll
@@ -234,6 +257,16 @@ __global__ __launch_bounds__(kWaves * 64) void append_kernel(AppendArgs a) {
         transpose4x4_groups(z);  // words: tokens 0 .. 15 of feature f + 4 i + g
         if (head)
           *reinterpret_cast<u32x4*>(a.vc + base + (slot / 16) * (D * 16) + (f + 4 * i + g) * 16) = u32x4{z[0], z[1], z[2], z[3]};
+      }
+    } else if (quad) {
+      const int64_t slot = where[0] % kPage, base = (where[0] - slot + hk) * D;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t z[4] = {w[0][i], w[1][i], w[2][i], w[3][i]};
+        transpose4x4_b8(z);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (head) *reinterpret_cast<uint32_t*>(a.vc + base + (slot / 16) * (D * 16) + (f + 4 * i + e) * 16 + slot % 16) = z[e];
       }
     } else {
 #pragma unroll
