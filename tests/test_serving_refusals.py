@@ -133,3 +133,16 @@ def test_fake_shapes(L):
         assert out.shape == (2, 5, 4, 64) and lse.shape == (2, 5, 4) and lse.dtype == f32
         out, lse = torch.ops.spyre.quant_paged_decode_attention(e(2, 4, 64), *cache, e(2, 2, t=i32), e(2, t=i32))
         assert out.shape == (2, 4, 64) and lse.shape == (2, 4)
+
+
+def test_fake_strides_of_rotary(L):
+    """Features lie next to each other in the results, as the kernel leaves them."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    import torch_spyre_amd  # noqa: F401
+
+    with FakeTensorMode():
+        e = lambda *s, t=torch.float16: torch.empty(s, dtype=t, device="cuda")  # noqa: E731
+        q, k = torch.ops.spyre.rotary(e(2, 3, 64, 8).transpose(2, 3), e(2, 1, 8, 64).expand(2, 3, 8, 64), e(8, t=torch.int32),
+                                      e(32, t=torch.float64))
+        assert q.shape == (2, 3, 8, 64) and q.stride(-1) == 1 and k.shape == (2, 3, 8, 64) and k.stride(-1) == 1

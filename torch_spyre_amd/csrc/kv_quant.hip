@@ -31,7 +31,7 @@ constexpr int kLdsPairs = 64;  // R / 2 <= D / 2
 typedef c8_f16x8 f16x8;
 typedef c8_u32x4 u32x4;
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));  // scales may lie anywhere
 
 __device__ __forceinline__ uint32_t umax_row(uint32_t x, bool sixteen) {
 #define SPYRE_DPP(ctrl) x = max(x, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), ctrl, 0xf, 0xf, false)))
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(kWaves * 64) void append_kernel(AppendArgs a) {
   const int32_t* sl = a.slots + b * a.sl_sb;
   const int first = sl[0], last = sl[(a.T - 1) * a.sl_st];
   // Any cut is right; this one meets the units of runs padded on either side.
-  const int off = first >= 0 ? first % kGroup : last >= 0 ? (last + kGroup - (a.T - 1) % kGroup) % kGroup : 0;
+  const int off = first >= 0 ? first % kGroup : last >= 0 ? (last % kGroup + kGroup - (a.T - 1) % kGroup) % kGroup : 0;
   const int t0 = gi * kGroup - off;
   if (t0 >= a.T) return;
   if constexpr (ROTATE) {

@@ -189,7 +189,11 @@ def _(query, key, value, attn_mask=None, is_causal=False, scale=None, enable_gqa
 
 @torch.library.register_fake("spyre::rotary")
 def _(q, k, positions, frequencies, amplitude=1.0, interleaved=False, inverse=False):
-    return torch.empty_like(q), q.new_empty((0,)) if k is None else torch.empty_like(k)
+    def like(x):  # features always have stride 1
+        y = torch.empty_like(x) if x.stride(-1) == 1 else x.new_empty(x.shape)
+        return y if y.stride(-1) == 1 else x.new_empty(x.shape)
+
+    return like(q), q.new_empty((0,)) if k is None else like(k)
 
 
 @torch.library.register_fake("spyre::kv_quant_append")
