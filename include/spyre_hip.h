@@ -453,8 +453,8 @@ int spyre_kv_quant_read(const void* k_cache, const void* v_cache, const float* k
  *   out   : [B, T, Hq, D] fp16, lse: optional fp32 [B, T, Hq]; contiguous
  * A context above max_context_len and a page that the table does not name
  * validly make the sequence's rows NaN.  The workspace holds
- * spyre_paged_tree_attn_workspace_bytes (asked of the current device; may be
- * 0), 16-byte aligned, without initialisation; two calls in flight need two.
+ * spyre_paged_tree_attn_workspace_bytes, 16-byte aligned, without
+ * initialisation; two calls in flight need two.
  * D in {64, 128}, page_size 64.  No reference counterpart. */
 size_t spyre_paged_tree_attn_workspace_bytes(int cache_kind, int B, int T, int Hq, int Hkv, int D,
                                              int max_context_len, int draft_keys);

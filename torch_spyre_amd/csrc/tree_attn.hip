@@ -624,8 +624,15 @@ __device__ __forceinline__ void finish(const TreeArgs& a, const Walk& walk, cons
     __builtin_amdgcn_raw_buffer_store_b32(0u, ws, flag_of(r), 0, kAuxDevice);
 }
 
-// W wavefronts share a chunk of a (sequence, KV head, row tile): each takes
-// its own steps of it, and they join in LDS.
+// Up to 64 rows to a KV head.  W wavefronts share a piece of a (sequence, KV
+// head, tile of 32 rows): each takes steps of 32 tokens of its own, and they
+// join in LDS at its end.  K of the next step is loaded as soon as the scores
+// have used this one's, V as soon as O has.
+// 16 sequences x 4096 tokens, 32 / 8 heads of 128: 8 drafted tokens (32 rows)
+// 36 us over e4m3 (3.7 TB/s), 67 over fp16 (4.1 TB/s); 16 (two tiles, which
+// read the pages twice, the second time from L2) 33 us over e4m3, 527 TFLOP/s.
+// Bound by instruction issue over 8-bit pages (a tile's conversions cost as much
+// as its products) and by the one step in flight over fp16 ones.
 template <int CT, int D, int W>
 __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
   constexpr int STEP = 32, PER_PAGE = kPage / STEP;
@@ -640,224 +647,227 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
   Walk walk;
   if (range >= a.ranges || !walk.start(a, lane, range)) return;
   for (; walk.u < walk.end;) {
-  const Piece pc = piece_of(a, walk);
-  const int b = walk.b, kvh = pc.kvh;
-  const Seq sq = walk.seq;
-  const int total = sq.ctx + (a.draft_keys ? sq.n : 0);
-  // The wavefronts take equal shares of the piece's steps; rows of no drafted token none.
-  const int c0 = pc.page0 * PER_PAGE, c1 = tile * kTile < sq.n * a.g ? min(pc.page1 * PER_PAGE, (total + STEP - 1) / STEP) : c0;
-  const int s0 = c0 + (c1 - c0) * wave / W, s1 = c0 + (c1 - c0) * (wave + 1) / W;
-  const Row row = row_of(a, sq, b, kvh, tile * kTile + col);
-  f16x8 qf[DS][2];
-  Pages pages(a, b, kvh, lane, s0 / PER_PAGE);
-  bool odd = false;
+    const Piece pc = piece_of(a, walk);
+    const int b = walk.b, kvh = pc.kvh;
+    const Seq sq = walk.seq;
+    const int total = sq.ctx + (a.draft_keys ? sq.n : 0);
+    // The wavefronts take equal shares of the piece's steps; rows of no drafted token none.
+    const int c0 = pc.page0 * PER_PAGE, c1 = tile * kTile < sq.n * a.g ? min(pc.page1 * PER_PAGE, (total + STEP - 1) / STEP) : c0;
+    const int s0 = c0 + (c1 - c0) * wave / W, s1 = c0 + (c1 - c0) * (wave + 1) / W;
+    const Row row = row_of(a, sq, b, kvh, tile * kTile + col);
+    f16x8 qf[DS][2];
+    Pages pages(a, b, kvh, lane, s0 / PER_PAGE);
+    bool odd = false;
 
-  f32x16 o[DS];
-#pragma unroll
-  for (int dt = 0; dt < DS; ++dt)
-#pragma unroll
-    for (int x = 0; x < 16; ++x) o[dt][x] = 0.f;
-  float m = -INFINITY, l = 0.f;
-
-  // Lane offsets within a page, bytes.
-  const int tok = token_of(col);
-  const int k_off = CT == kF16 ? (tok * 64 + 16 * half) * 2 : half * (kPage * 16) + tok * 16;
-  const int v_off = CT == kF16 ? (col * kPage + 16 * half) * 2 : half * (D * 16) + col * 16;
-
-  int64_t head = 0;  // physical page * Hkv + KV head, of the step being loaded
-  auto locate = [&](int st) { head = pages.head(st / PER_PAGE); };
-  Raw<CT, D> kr, vr;
-  float scale = 0.f;  // 8-bit: of the step's token `col`, K's in the lower lanes, V's in the upper
-  auto load_k = [&](int st) {
-    const int hp = st % PER_PAGE;
-    const Rsrc r = page_rsrc(a.k, head, kPage * D * KB);
-#pragma unroll
-    for (int s = 0; s < DS; ++s)
-#pragma unroll
-      for (int e = 0; e < KB; ++e)
-        kr.x[s][e] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-            r, k_off, CT == kF16 ? hp * (STEP * 128) + (s / 2) * (kPage * 128) + (s % 2) * 64 + 16 * e : hp * (STEP * 16) + 2 * s * (kPage * 16), 0));
-    if constexpr (CT != kF16)
-      scale = (half ? a.vs : a.ks)[head * kPage + hp * STEP + col];
-  };
-  auto load_v = [&](int st) {
-    const int hp = st % PER_PAGE;
-    const Rsrc r = page_rsrc(a.v, head, kPage * D * KB);
+    f32x16 o[DS];
 #pragma unroll
     for (int dt = 0; dt < DS; ++dt)
 #pragma unroll
-      for (int e = 0; e < KB; ++e)
-        vr.x[dt][e] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-            r, v_off, CT == kF16 ? hp * (STEP * 2) + dt * (32 * kPage * 2) + 16 * e : 2 * hp * (D * 16) + dt * (32 * 16), 0));
-  };
-  // 8-bit: this wavefront's step: score factors, V's scales' logarithms and inverses.
-  float* s_sc = s_mem + wave * 3 * STEP;
+      for (int x = 0; x < 16; ++x) o[dt][x] = 0.f;
+    float m = -INFINITY, l = 0.f;
 
-  // MORE: another step follows (as in the few kernel).
-  auto step = [&](int st, auto more_tag, auto edge_tag) {
-    constexpr bool MORE = decltype(more_tag)::value;
-    constexpr bool EDGE = decltype(edge_tag)::value;  // some tokens are drafted or do not exist
-    const int tok0 = st * STEP + 16 * half;           // this lane's 16 tokens
-    uint32_t seen = 0;                                // those that its row attends
-    if constexpr (EDGE) seen = row.attends16(a, sq, tok0, total, [](int x) { return x; });
-    uint32_t odd_scale = 0, inf_scale = 0;  // of this lane's 16 tokens, those whose V has no finite scale
-    if constexpr (CT != kF16) {
-      __builtin_amdgcn_wave_barrier();
-      const bool finite = __builtin_fabsf(scale) <= 0x1.fffffep127f;
-      odd_scale = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(half && !finite) >> (32 + 16 * half)) & 0xffffu;
-      inf_scale = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(half && scale == INFINITY) >> (32 + 16 * half)) & 0xffffu;
-      const float vc = !finite ? 1.f : scale < 0x1p-60f ? 0x1p-60f : scale;  // V's scale 0: codes of no weight
-      s_sc[lane] = half ? __builtin_amdgcn_logf(vc) : scale * a.scale_log2;
-      if (half) s_sc[2 * STEP + col] = __builtin_amdgcn_rcpf(vc);
-      __builtin_amdgcn_wave_barrier();
-    }
-    f32x16 sc;
+    // Lane offsets within a page, bytes.
+    const int tok = token_of(col);
+    const int k_off = CT == kF16 ? (tok * 64 + 16 * half) * 2 : half * (kPage * 16) + tok * 16;
+    const int v_off = CT == kF16 ? (col * kPage + 16 * half) * 2 : half * (D * 16) + col * 16;
+
+    int64_t head = 0;  // physical page * Hkv + KV head, of the step being loaded
+    auto locate = [&](int st) { head = pages.head(st / PER_PAGE); };
+    Raw<CT, D> kr, vr;
+    float scale = 0.f;  // 8-bit: of the step's token `col`, K's in the lower lanes, V's in the upper
+    auto load_k = [&](int st) {
+      const int hp = st % PER_PAGE;
+      const Rsrc r = page_rsrc(a.k, head, kPage * D * KB);
 #pragma unroll
-    for (int x = 0; x < 16; ++x) sc[x] = 0.f;
+      for (int s = 0; s < DS; ++s)
 #pragma unroll
-    for (int s = 0; s < DS; ++s)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand<CT>(kr.x[s], e), qf[s][e], sc, 0, 0, 0);
-    if constexpr (MORE) {
-      if ((st + 1) % PER_PAGE == 0) locate(st + 1);
-      load_k(st + 1);
-    }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int x4 = 0; x4 < 4; ++x4) {
-      f32x4 f, lv;
-      if constexpr (CT != kF16) {
-        f = *reinterpret_cast<const f32x4*>(s_sc + 16 * half + 4 * x4);
-        lv = *reinterpret_cast<const f32x4*>(s_sc + STEP + 16 * half + 4 * x4);
-      }
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const int x = 4 * x4 + y;
-        float v = CT == kF16 ? sc[x] * a.scale_log2 : __builtin_fmaf(sc[x], f[y], lv[y]);
-        if constexpr (EDGE) v = (seen >> x) & 1 ? v : -INFINITY;
-        sc[x] = v;
-        mx = fmaxf(mx, v);
-      }
-    }
-    mx = xor32_max(mx);
-    if (__any(mx > m + kSlack)) {
-      const float mn = fmaxf(m, mx);
-      const float alpha = m == -INFINITY ? 0.f : exp2_of(m - mn);
-      m = mn;
-      l *= alpha;
+        for (int e = 0; e < KB; ++e)
+          kr.x[s][e] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+              r, k_off,
+              CT == kF16 ? hp * (STEP * 128) + (s / 2) * (kPage * 128) + (s % 2) * 64 + 16 * e
+                         : hp * (STEP * 16) + 2 * s * (kPage * 16), 0));
+      if constexpr (CT != kF16)
+        scale = (half ? a.vs : a.ks)[head * kPage + hp * STEP + col];
+    };
+    auto load_v = [&](int st) {
+      const int hp = st % PER_PAGE;
+      const Rsrc r = page_rsrc(a.v, head, kPage * D * KB);
 #pragma unroll
       for (int dt = 0; dt < DS; ++dt)
 #pragma unroll
-        for (int x = 0; x < 16; ++x) o[dt][x] *= alpha;
+        for (int e = 0; e < KB; ++e)
+          vr.x[dt][e] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+              r, v_off, CT == kF16 ? hp * (STEP * 2) + dt * (32 * kPage * 2) + 16 * e : 2 * hp * (D * 16) + dt * (32 * 16), 0));
+    };
+    // 8-bit: this wavefront's step: score factors, V's scales' logarithms and inverses.
+    float* s_sc = s_mem + wave * 3 * STEP;
+
+    // MORE: another step follows (as in the few kernel).
+    auto step = [&](int st, auto more_tag, auto edge_tag) {
+      constexpr bool MORE = decltype(more_tag)::value;
+      constexpr bool EDGE = decltype(edge_tag)::value;  // some tokens are drafted or do not exist
+      const int tok0 = st * STEP + 16 * half;           // this lane's 16 tokens
+      uint32_t seen = 0;                                // those that its row attends
+      if constexpr (EDGE) seen = row.attends16(a, sq, tok0, total, [](int x) { return x; });
+      uint32_t odd_scale = 0, inf_scale = 0;  // of this lane's 16 tokens, those whose V has no finite scale
+      if constexpr (CT != kF16) {
+        __builtin_amdgcn_wave_barrier();
+        const bool finite = __builtin_fabsf(scale) <= 0x1.fffffep127f;
+        odd_scale = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(half && !finite) >> (32 + 16 * half)) & 0xffffu;
+        inf_scale = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(half && scale == INFINITY) >> (32 + 16 * half)) & 0xffffu;
+        const float vc = !finite ? 1.f : scale < 0x1p-60f ? 0x1p-60f : scale;  // V's scale 0: codes of no weight
+        s_sc[lane] = half ? __builtin_amdgcn_logf(vc) : scale * a.scale_log2;
+        if (half) s_sc[2 * STEP + col] = __builtin_amdgcn_rcpf(vc);
+        __builtin_amdgcn_wave_barrier();
+      }
+      f32x16 sc;
+#pragma unroll
+      for (int x = 0; x < 16; ++x) sc[x] = 0.f;
+#pragma unroll
+      for (int s = 0; s < DS; ++s)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand<CT>(kr.x[s], e), qf[s][e], sc, 0, 0, 0);
+      if constexpr (MORE) {
+        if ((st + 1) % PER_PAGE == 0) locate(st + 1);
+        load_k(st + 1);
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int x4 = 0; x4 < 4; ++x4) {
+        f32x4 f, lv;
+        if constexpr (CT != kF16) {
+          f = *reinterpret_cast<const f32x4*>(s_sc + 16 * half + 4 * x4);
+          lv = *reinterpret_cast<const f32x4*>(s_sc + STEP + 16 * half + 4 * x4);
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int x = 4 * x4 + y;
+          float v = CT == kF16 ? sc[x] * a.scale_log2 : __builtin_fmaf(sc[x], f[y], lv[y]);
+          if constexpr (EDGE) v = (seen >> x) & 1 ? v : -INFINITY;
+          sc[x] = v;
+          mx = fmaxf(mx, v);
+        }
+      }
+      mx = xor32_max(mx);
+      if (__any(mx > m + kSlack)) {
+        const float mn = fmaxf(m, mx);
+        const float alpha = m == -INFINITY ? 0.f : exp2_of(m - mn);
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DS; ++dt)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) o[dt][x] *= alpha;
+      }
+      const float mu = m == -INFINITY ? 0.f : m;  // a row that has attended nothing yet: weights 0
+      f16x8 p[2];
+#pragma unroll
+      for (int x4 = 0; x4 < 4; ++x4) {
+        f32x4 r;
+        if constexpr (CT != kF16) r = *reinterpret_cast<const f32x4*>(s_sc + 2 * STEP + 16 * half + 4 * x4);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int x = 4 * x4 + y;
+          const float w = exp2_of(sc[x] - mu);
+          if constexpr (CT == kF16)
+            l += w;
+          else
+            l = __builtin_fmaf(w, EDGE && !((seen >> x) & 1) ? 0.f : r[y], l);
+          p[x / 8][x % 8] = static_cast<_Float16>(w);
+        }
+      }
+      if (CT != kF16 && __any(odd_scale != 0)) {  // weights that leave the codes as the scale does; lse does not know V
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+          if ((odd_scale >> x) & 1 && (!EDGE || (seen >> x) & 1))
+            p[x / 8][x % 8] = static_cast<_Float16>((inf_scale >> x) & 1 ? INFINITY : NAN);
+      }
+      if constexpr (EDGE) {
+        // Numbers of tokens that do not exist are any bits; those of drafted
+        // tokens that a row does not attend may be infinite or NaN.  Neither
+        // may meet a weight of 0: rows that do attend them take them below.
+#pragma unroll
+        for (int dt = 0; dt < DS; ++dt) {
+          drop_tokens<CT>(vr.x[dt], total - tok0);
+#pragma unroll
+          for (int e = 0; e < Raw<CT, D>::W; ++e)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              uint32_t y = vr.x[dt][e][w];
+              odd = drop_odd<CT>(y) || odd;
+              vr.x[dt][e][w] = y;
+            }
+        }
+      }
+#pragma unroll
+      for (int dt = 0; dt < DS; ++dt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand<CT>(vr.x[dt], e), p[e], o[dt], 0, 0, 0);
+      if constexpr (MORE) load_v(st + 1);
+    };
+
+    // Every row attends every token of a step below ctx (rows without a drafted
+    // token drop theirs at the end), so only the last steps test tokens.
+    const int whole = min(s1, sq.ctx / STEP);
+    std::true_type yes;
+    std::false_type no;
+    auto wait_q = [&] {  // behind the first step's loads; waits here, not in every step
+      load_q<DS>(a, b, row, half, qf);
+#pragma unroll
+      for (int s = 0; s < DS; ++s)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) asm volatile("" : "+v"(qf[s][e]));
+    };
+    int st = s0;
+    if (st < whole) {
+      locate(st);
+      load_k(st);
+      load_v(st);
+      wait_q();
+      for (; st < whole - 1; ++st) step(st, yes, no);
+      step(st, no, no);
+      ++st;
+    } else if (st < s1) {
+      wait_q();
     }
-    const float mu = m == -INFINITY ? 0.f : m;  // a row that has attended nothing yet: weights 0
-    f16x8 p[2];
+    for (; st < s1; ++st) {  // the sequence's last steps
+      if (st == s0 || st % PER_PAGE == 0) locate(st);
+      load_k(st);
+      load_v(st);
+      step(st, no, yes);
+    }
+    if (CT != SPYRE_CODES_INT8 && __any(odd))
+      add_odd<CT, D, DS * 16>(
+          a, sq, b, kvh, row, lane, max(s0, whole) * STEP, min(s1 * STEP, total), -1,
+          [](int x, int ln) { return 32 * (x / 16) + 8 * (x % 16 / 4) + 4 * (ln >> 5) + x % 4; },
+          [&](int x, float f) { o[x / 16][x % 16] += f; });
+    l = xor32_sum(l);
+    if (!row.live) m = -INFINITY, l = 0.f;
+    if ((pages.poisoned || sq.bad) && row.live) l = NAN;
+
+    // O, m and l of the rows that exist.
+    const int rows = min(kTile, a.rows - static_cast<int>(tile) * kTile);
+    float* s_o = s_mem;                          // [W][rows][ROW]
+    float* s_ml = s_mem + W * rows * ROW;        // [W][rows][2]
+    __syncthreads();
+    if (col < rows) {
 #pragma unroll
-    for (int x4 = 0; x4 < 4; ++x4) {
-      f32x4 r;
-      if constexpr (CT != kF16) r = *reinterpret_cast<const f32x4*>(s_sc + 2 * STEP + 16 * half + 4 * x4);
+      for (int dt = 0; dt < DS; ++dt)
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const int x = 4 * x4 + y;
-        const float w = exp2_of(sc[x] - mu);
-        if constexpr (CT == kF16)
-          l += w;
-        else
-          l = __builtin_fmaf(w, EDGE && !((seen >> x) & 1) ? 0.f : r[y], l);
-        p[x / 8][x % 8] = static_cast<_Float16>(w);
+        for (int x4 = 0; x4 < 4; ++x4)
+          *reinterpret_cast<f32x4*>(s_o + (wave * rows + col) * ROW + 32 * dt + 8 * x4 + 4 * half) =
+              f32x4{o[dt][4 * x4], o[dt][4 * x4 + 1], o[dt][4 * x4 + 2], o[dt][4 * x4 + 3]};
+      if (half == 0) {
+        s_ml[(wave * rows + col) * 2] = m;
+        s_ml[(wave * rows + col) * 2 + 1] = l;
       }
     }
-    if (CT != kF16 && __any(odd_scale != 0)) {  // weights that leave the codes as the scale does; lse does not know V
-#pragma unroll
-      for (int x = 0; x < 16; ++x)
-        if ((odd_scale >> x) & 1 && (!EDGE || (seen >> x) & 1)) p[x / 8][x % 8] = static_cast<_Float16>((inf_scale >> x) & 1 ? INFINITY : NAN);
-    }
-    if constexpr (EDGE) {
-      // Numbers of tokens that do not exist are any bits; those of drafted
-      // tokens that a row does not attend may be infinite or NaN.  Neither
-      // may meet a weight of 0: rows that do attend them take them below.
-#pragma unroll
-      for (int dt = 0; dt < DS; ++dt) {
-        drop_tokens<CT>(vr.x[dt], total - tok0);
-#pragma unroll
-        for (int e = 0; e < Raw<CT, D>::W; ++e)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            uint32_t y = vr.x[dt][e][w];
-            odd = drop_odd<CT>(y) || odd;
-            vr.x[dt][e][w] = y;
-          }
-      }
-    }
-#pragma unroll
-    for (int dt = 0; dt < DS; ++dt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(operand<CT>(vr.x[dt], e), p[e], o[dt], 0, 0, 0);
-    if constexpr (MORE) load_v(st + 1);
-  };
-
-  // Every row attends every token of a step below ctx (rows without a drafted
-  // token drop theirs at the end), so only the last steps test tokens.
-  const int whole = min(s1, sq.ctx / STEP);
-  std::true_type yes;
-  std::false_type no;
-  auto wait_q = [&] {  // behind the first step's loads; waits here, not in every step
-    load_q<DS>(a, b, row, half, qf);
-#pragma unroll
-    for (int s = 0; s < DS; ++s)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) asm volatile("" : "+v"(qf[s][e]));
-  };
-  int st = s0;
-  if (st < whole) {
-    locate(st);
-    load_k(st);
-    load_v(st);
-    wait_q();
-    for (; st < whole - 1; ++st) step(st, yes, no);
-    step(st, no, no);
-    ++st;
-  } else if (st < s1) {
-    wait_q();
-  }
-  for (; st < s1; ++st) {  // the sequence's last steps
-    if (st == s0 || st % PER_PAGE == 0) locate(st);
-    load_k(st);
-    load_v(st);
-    step(st, no, yes);
-  }
-  if (CT != SPYRE_CODES_INT8 && __any(odd))
-    add_odd<CT, D, DS * 16>(
-        a, sq, b, kvh, row, lane, max(s0, whole) * STEP, min(s1 * STEP, total), -1,
-        [](int x, int ln) { return 32 * (x / 16) + 8 * (x % 16 / 4) + 4 * (ln >> 5) + x % 4; },
-        [&](int x, float f) { o[x / 16][x % 16] += f; });
-  l = xor32_sum(l);
-  if (!row.live) m = -INFINITY, l = 0.f;
-  if ((pages.poisoned || sq.bad) && row.live) l = NAN;
-
-  // O, m and l of the rows that exist.
-  const int rows = min(kTile, a.rows - static_cast<int>(tile) * kTile);
-  float* s_o = s_mem;                          // [W][rows][ROW]
-  float* s_ml = s_mem + W * rows * ROW;        // [W][rows][2]
-  __syncthreads();
-  if (col < rows) {
-#pragma unroll
-    for (int dt = 0; dt < DS; ++dt)
-#pragma unroll
-      for (int x4 = 0; x4 < 4; ++x4)
-        *reinterpret_cast<f32x4*>(s_o + (wave * rows + col) * ROW + 32 * dt + 8 * x4 + 4 * half) =
-            f32x4{o[dt][4 * x4], o[dt][4 * x4 + 1], o[dt][4 * x4 + 2], o[dt][4 * x4 + 3]};
-    if (half == 0) {
-      s_ml[(wave * rows + col) * 2] = m;
-      s_ml[(wave * rows + col) * 2 + 1] = l;
-    }
-  }
-  __syncthreads();
-  finish<D, W>(a, walk, pc, sq, range, tile, rows, s_o, s_ml);
-  advance(a, walk, pc);
-  __syncthreads();  // LDS is read before the next piece writes it
+    __syncthreads();
+    finish<D, W>(a, walk, pc, sq, range, tile, rows, s_o, s_ml);
+    advance(a, walk, pc);
+    __syncthreads();  // LDS is read before the next piece writes it
   }
 }
 
@@ -878,7 +888,11 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
 //          its V load is the tokens 16 G .. + 15, so the 4 x 4 words (of 4
 //          tokens) of the four groups change places in registers first.
 // Bound by memory: K of the next page is loaded as soon as the scores have used
-// this one's, V as soon as O has.
+// this one's, V as soon as O has; head_dim 64 has the registers for two pages in
+// flight.  A decode step over e4m3, 32 / 8 heads of 128: 32 x 4096 tokens 45.6 us
+// (6.0 TB/s), 64 x 8192 166 us (6.6 TB/s), 64 x 128 to 16384 189 us; one
+// sequence of 700 tokens 10.6 us, which is the chain of its loads (lengths, table,
+// page) and the join.
 template <int CT, int D, int W>
 __global__ __launch_bounds__(W * 64, 2) void tree_few_kernel(TreeArgs a) {
   constexpr int KB = CT == kF16 ? 2 : 1, KW = KB;  // bytes of an element; 16-byte words of 16 of them
@@ -928,8 +942,7 @@ __global__ __launch_bounds__(W * 64, 2) void tree_few_kernel(TreeArgs a) {
 #pragma unroll
     for (int dt = 0; dt < DV; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
-    // The raw operands of a page.  8-bit pages have two sets, which take turns:
-    // two pages are then in flight.
+    // The raw operands of a page, in sets that take turns.
     struct Operands {
       u32x4 k[4][DQ][KW], v[DV][KW];
       float ks, vs;  // 8-bit: scales of the page's token `lane`
@@ -961,9 +974,9 @@ __global__ __launch_bounds__(W * 64, 2) void tree_few_kernel(TreeArgs a) {
           x.v[dt][e] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
               r, v_off, CT == kF16 ? dt * (16 * kPage * 2) + 64 * e : dt * (16 * 16), kAuxOnce));
     };
-    // MORE: page p + SETS follows in the same registers.  (A test of it at run time would leave the
-    // compiler paths on which K is loaded and V is not, and every page would
-    // wait for its V before its first product.)
+    // MORE: page p + SETS follows in the same registers.  (A test of it at run
+    // time would leave the compiler paths on which K is loaded and V is not, and
+    // every page would wait for its V before its first product.)
     auto step = [&](Operands& x, int p, auto more_tag, auto edge_tag) {
       constexpr bool MORE = decltype(more_tag)::value;
       constexpr bool EDGE = decltype(edge_tag)::value;   // some tokens are drafted or do not exist
@@ -1165,6 +1178,16 @@ __global__ __launch_bounds__(W * 64, 2) void tree_few_kernel(TreeArgs a) {
 // while the weights of half i are formed, the scores of half i + 1 are
 // multiplied, and while those weights meet V, the scores' maximum is taken.  K
 // therefore runs one page ahead of V.
+//
+// RT 8: 16 sequences x 8192 tokens, 64 tokens of 64 / 8 heads of 128 (512 rows to
+// a KV head): 305 us over fp16, 901 TFLOP/s where a large matrix product of the
+// same type reaches 1199; 321 us over e4m3.  Bound by the products and the
+// softmax's instructions beside them.
+// RT 4: 25 tokens of 32 / 8 heads x 4096: 64 + 8 us of joining over e4m3, 75 + 8
+// over fp16.  A page takes 1.4 us, 0.9 without its loads and conversions: one
+// step a wavefront between two barriers is too little to hide either.  More
+// pages in flight, as codes in LDS or in a second set of registers, gained
+// nothing (1.9 and 1.3 us).
 __device__ __forceinline__ int swz_k(int row) { return ((row >> 1) & 3) | ((((row >> 3) ^ (row >> 4)) & 1) << 2); }
 __device__ __forceinline__ int swz_v(int row) { return (row >> 1) & 7; }
 
@@ -1619,7 +1642,8 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
 
 // Joins the partials of each (sequence, KV head) that several ranges share: a
 // thread 4 features of a row.  For the wide kernel, whose partials are too many
-// for one workgroup.
+// for one workgroup (100 rows to each of 16 x 8: 8 us, most of it the launch and
+// the chain lengths, references, partials).
 template <int D>
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
   const uint32_t pair = blockIdx.x, b = fdiv(pair, a.by_hkv), kvh = pair - b * a.Hkv;
@@ -1754,7 +1778,8 @@ extern "C" int spyre_paged_tree_attn(const void* q, const int64_t* q_strides, co
   a.out = static_cast<_Float16*>(out), a.lse = lse, a.ws = static_cast<float*>(workspace);
   a.B = B, a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.g = Hq / Hkv, a.rows = T * a.g;
   a.max_ctx = max_context_len, a.scale_log2 = scale * kLog2e;
-  a.row_blocks = p.row_blocks, a.block_rows = p.block_rows, a.width = p.width, a.ranges = p.ranges, a.min_per = p.min_per, a.min_cut = p.min_cut;
+  a.row_blocks = p.row_blocks, a.block_rows = p.block_rows, a.width = p.width;
+  a.ranges = p.ranges, a.min_per = p.min_per, a.min_cut = p.min_cut;
   a.each = static_cast<int64_t>(B) * Hkv % p.ranges == 0 ? static_cast<int>(static_cast<int64_t>(B) * Hkv / p.ranges) : 0;
   a.ticket = spyre_hip::next_call_ticket();
   const int64_t pairs = static_cast<int64_t>(B) * Hkv, blocks = static_cast<int64_t>((p.ranges + 7) / 8 * 8) * p.row_blocks;
