@@ -159,6 +159,9 @@ __device__ __forceinline__ int max64(int x) {
 // then as even as equal ones.  A range that holds only part of a (sequence, KV
 // head) leaves a partial: in slot 1 that of the first part, in slot 0 that of
 // any other.
+// Lengths that another stream changes meanwhile give wrong results, as in any
+// kernel, but no endless walk and no index beyond the buffers: hence the bounds
+// that lengths at rest never meet.
 // kStart: 64 sequences of 128 to 16384 tokens, longest first, took 237 us
 // where pages alone were counted: a workgroup had 60 short ones.
 constexpr int kStart = 4;
@@ -210,12 +213,12 @@ struct Walk {
   __device__ __forceinline__ void find(const TreeArgs& a, int lane, const Lane& first64, int unit) {
     const int target = static_cast<int>(fdiv(unit, a.by_hkv));
     base = 0;
-    for (int c = 0;; c += 64) {  // ends: target is below the total
+    for (int c = 0;; c += 64) {
       const Lane x = c == 0 ? first64 : lane_of(a, c + lane);
       const int sum = scan64(x.size);
       const uint64_t past = __builtin_amdgcn_ballot_w64(base + sum > target);
-      if (past) {
-        const int i = __builtin_ctzll(past);
+      if (past || c + 64 >= a.B) {
+        const int i = past ? __builtin_ctzll(past) : (a.B - 1) % 64;
         b = c + i;
         take(a, x, i);
         base += __builtin_amdgcn_readlane(sum, i) - size;
@@ -267,7 +270,7 @@ struct Walk {
   }
   __device__ __forceinline__ void next_sequence(const TreeArgs& a) {
     base += size;
-    b += 1;
+    b = min(b + 1, a.B - 1);
     seq = seq_at(a, b);
     size = kStart + seq.pages;
   }
@@ -295,8 +298,8 @@ struct Walk {
   // r0 + 1 .. r1 the others; r1 <= r0 where one range holds it whole.
   __device__ __forceinline__ void parts_of(const TreeArgs& a, int kvh, int& r0, int& r1) const {
     const int g0 = base * a.Hkv + kvh * size, g1 = g0 + size;
-    r0 = (g0 + kStart + few()) / per;
-    r1 = uncut ? r0 : (g1 - few() - 1) / per;
+    r0 = min((g0 + kStart + few()) / per, a.ranges - 1);
+    r1 = uncut ? r0 : min((g1 - few() - 1) / per, a.ranges - 1);
   }
 };
 
@@ -310,7 +313,7 @@ struct Piece {
 __device__ __forceinline__ Piece piece_of(const TreeArgs& a, const Walk& w) {
   Piece p;
   const int in = w.u - w.base * a.Hkv;
-  p.kvh = static_cast<uint32_t>(in) / static_cast<uint32_t>(w.size);
+  p.kvh = min(static_cast<uint32_t>(in) / static_cast<uint32_t>(w.size), static_cast<uint32_t>(a.Hkv - 1));
   const int at = in - p.kvh * w.size;
   p.page0 = max(at - kStart, 0);
   p.page1 = min(w.size, at + w.end - w.u) - kStart;
@@ -321,7 +324,7 @@ __device__ __forceinline__ Piece piece_of(const TreeArgs& a, const Walk& w) {
 
 // After it.
 __device__ __forceinline__ void advance(const TreeArgs& a, Walk& w, const Piece& p) {
-  w.u = w.base * a.Hkv + p.kvh * w.size + kStart + p.page1;
+  w.u = max(w.base * a.Hkv + p.kvh * w.size + kStart + p.page1, w.u + 1);
   if (w.u < w.end && p.kvh == a.Hkv - 1 && p.page1 == w.size - kStart) w.next_sequence(a);
 }
 
