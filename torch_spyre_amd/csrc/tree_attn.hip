@@ -1685,7 +1685,7 @@ struct Plan {
   size_t ws_bytes;
 };
 
-Plan plan_of(int B, int T, int Hq, int Hkv, int D, int max_tokens) {
+Plan plan_of(int kind, int B, int T, int Hq, int Hkv, int D, int max_tokens) {
   Plan p;
   const int64_t rows = static_cast<int64_t>(T) * (Hq / Hkv);
   // Half workgroups, two to a compute unit, where each has a (sequence, KV
@@ -1697,10 +1697,12 @@ Plan plan_of(int B, int T, int Hq, int Hkv, int D, int max_tokens) {
   p.width = static_cast<int>(std::min<int64_t>(p.block_rows, rows));
   // Parts of fewer pages cost more to join than they save (one sequence of 1024
   // tokens, us at 2 / 3 / 4 / 8 pages a part: 64 rows 13.2 / 13.5 / 15 / 17;
-  // 256 rows, whose joining is launched in any case, 29 / 31 / 32 / 42).  Few
-  // rows: 12 pages are one or two for each wavefront.
-  p.min_per = p.wide > 0 ? 2 : p.wide == 0 ? 6 : 3;
-  p.min_cut = p.wide < 0 ? 13 : 2 * p.min_per;
+  // 256 rows, whose joining is launched in any case, 29 / 31 / 32 / 42).  Nor is
+  // a sequence cut whose wavefronts have one page each, or two of 16 KiB
+  // (700 tokens, few rows: int8 10.6 whole, 11.7 in parts; fp16 17.8 and 15.2).
+  const bool large = kind == kF16 && D == 128;  // pages of 32 KiB
+  p.min_per = p.wide > 0 ? 2 : p.wide < 0 ? 3 : large ? 4 : 6;
+  p.min_cut = p.wide > 0 ? 4 : p.wide < 0 ? (large ? 9 : 13) : large ? 10 : 12;
   // One round of the device, or as many parts as there can be.
   const int64_t pages = std::max(pages_of(max_tokens), 1), parts_of_one = pages < p.min_cut ? 1 : pages / p.min_per;
   const int64_t slots = p.wide == -2 ? 512 : 256;
@@ -1736,9 +1738,8 @@ bool sizes_ok(int B, int T, int Hq, int Hkv, int D, int max_ctx) {
 
 extern "C" size_t spyre_paged_tree_attn_workspace_bytes(int cache_kind, int B, int T, int Hq, int Hkv, int D, int max_context_len,
                                                         int draft_keys) {
-  (void)cache_kind;
   if (!sizes_ok(B, T, Hq, Hkv, D, max_context_len)) return 0;
-  return plan_of(B, T, Hq, Hkv, D, max_context_len + (draft_keys ? T : 0)).ws_bytes;
+  return plan_of(cache_kind, B, T, Hq, Hkv, D, max_context_len + (draft_keys ? T : 0)).ws_bytes;
 }
 
 extern "C" int spyre_paged_tree_attn(const void* q, const int64_t* q_strides, const void* k_cache, const void* v_cache,
@@ -1768,7 +1769,7 @@ extern "C" int spyre_paged_tree_attn(const void* q, const int64_t* q_strides, co
                 "q, the caches and out must be 16-byte aligned");
   for (int i = 0; i < 3; ++i)
     SPYRE_REQUIRE(q_strides[i] % 8 == 0, SPYRE_EINVAL, "q strides must be multiples of 8 elements");
-  const Plan p = plan_of(B, T, Hq, Hkv, D, max_context_len + (draft_keys ? T : 0));
+  const Plan p = plan_of(cache_kind, B, T, Hq, Hkv, D, max_context_len + (draft_keys ? T : 0));
   SPYRE_REQUIRE(p.ws_bytes == 0 || (workspace && workspace_bytes >= p.ws_bytes && aligned(workspace, 16)), SPYRE_ENOSPC,
                 "workspace holds %zu bytes, need %zu (16-byte aligned)", workspace ? workspace_bytes : 0, p.ws_bytes);
   TreeArgs a{};
