@@ -627,15 +627,15 @@ __device__ __forceinline__ void finish(const TreeArgs& a, const Walk& walk, cons
     __builtin_amdgcn_raw_buffer_store_b32(0u, ws, flag_of(r), 0, kAuxDevice);
 }
 
-// Up to 64 rows to a KV head.  W wavefronts share a piece of a (sequence, KV
+// 17 to 64 rows to a KV head.  W wavefronts share a piece of a (sequence, KV
 // head, tile of 32 rows): each takes steps of 32 tokens of its own, and they
 // join in LDS at its end.  K of the next step is loaded as soon as the scores
 // have used this one's, V as soon as O has.
-// 16 sequences x 4096 tokens, 32 / 8 heads of 128: 8 drafted tokens (32 rows)
-// 36 us over e4m3 (3.7 TB/s), 67 over fp16 (4.1 TB/s); 16 (two tiles, which
-// read the pages twice, the second time from L2) 33 us over e4m3, 527 TFLOP/s.
-// Bound by instruction issue over 8-bit pages (a tile's conversions cost as much
-// as its products) and by the one step in flight over fp16 ones.
+// 16 sequences x 4096 tokens, 32 / 8 heads: 8 drafted tokens (32 rows) 36 us over
+// e4m3 of head_dim 128 (3.7 TB/s), 31 over fp16 of 64 (4.4 TB/s); 16 (two tiles,
+// which read the pages twice, the second time from L2) 33 us over e4m3, 527
+// TFLOP/s.  Bound by instruction issue over 8-bit pages (a tile's conversions
+// cost as much as its products) and by the one step in flight over fp16 ones.
 template <int CT, int D, int W>
 __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
   constexpr int STEP = 32, PER_PAGE = kPage / STEP;
@@ -1675,8 +1675,13 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a) {
 constexpr int kWaves = 8;  // of every workgroup
 static_assert(kWaves == kWideWaves, "one workgroup to a compute unit in all three kernels");
 constexpr int kFewRows = 16;
-// Rows up to here take the rows kernel: two tiles read a chunk's pages twice.
+// Rows up to here take the rows kernel, whose two tiles read a piece's pages
+// twice; but fp16 pages of head_dim 128 (large_pages) go through LDS at once.
+// 16 x 8192 tokens, 32 / 8 heads, 8 and 16 drafted (32 and 64 rows), us by rows
+// and through LDS: fp16 139, 209 and 119, 136; head_dim 64 51, 70 and 75, 79;
+// e4m3 56, 59 and 120 (25 drafted).
 constexpr int kNarrowRows = 64;
+constexpr bool large_pages(int kind, int D) { return kind == kF16 && D == 128; }  // 32 KiB for K and V
 
 struct Plan {
   int wide;  // row tiles of a workgroup of the wide kernel; 0: the rows kernel; -1: the few, -2: in half workgroups
@@ -1691,7 +1696,7 @@ Plan plan_of(int kind, int B, int T, int Hq, int Hkv, int D, int max_tokens) {
   // Half workgroups, two to a compute unit, where each has a (sequence, KV
   // head) of its own (64 x 8 x 1024 tokens 28.8 -> 25.5 us, x 8192 168.5 -> 165.5);
   // fewer would be cut for them (32 x 8 x 4096 45.6 -> 50.0).
-  p.wide = rows <= kFewRows ? (static_cast<int64_t>(B) * Hkv >= 512 ? -2 : -1) : rows <= kNarrowRows ? 0 : rows <= 128 ? 4 : 8;
+  p.wide = rows <= kFewRows ? (static_cast<int64_t>(B) * Hkv >= 512 ? -2 : -1) : rows <= kNarrowRows && !large_pages(kind, D) ? 0 : rows <= 128 ? 4 : 8;
   p.block_rows = kTile * std::max(p.wide, 1);
   p.row_blocks = static_cast<int>((rows + p.block_rows - 1) / p.block_rows);
   p.width = static_cast<int>(std::min<int64_t>(p.block_rows, rows));
@@ -1700,9 +1705,8 @@ Plan plan_of(int kind, int B, int T, int Hq, int Hkv, int D, int max_tokens) {
   // 256 rows, whose joining is launched in any case, 29 / 31 / 32 / 42).  Nor is
   // a sequence cut whose wavefronts have one page each, or two of 16 KiB
   // (700 tokens, few rows: int8 10.6 whole, 11.7 in parts; fp16 17.8 and 15.2).
-  const bool large = kind == kF16 && D == 128;  // pages of 32 KiB
-  p.min_per = p.wide > 0 ? 2 : p.wide < 0 ? 3 : large ? 4 : 6;
-  p.min_cut = p.wide > 0 ? 4 : p.wide < 0 ? (large ? 9 : 13) : large ? 10 : 12;
+  p.min_per = p.wide > 0 ? 2 : p.wide < 0 ? 3 : 6;
+  p.min_cut = p.wide > 0 ? 4 : p.wide == 0 ? 12 : large_pages(kind, D) ? 9 : 13;
   // One round of the device, or as many parts as there can be.
   const int64_t pages = std::max(pages_of(max_tokens), 1), parts_of_one = pages < p.min_cut ? 1 : pages / p.min_per;
   const int64_t slots = p.wide == -2 ? 512 : 256;
@@ -1716,16 +1720,17 @@ Plan plan_of(int kind, int B, int T, int Hq, int Hkv, int D, int max_tokens) {
 
 template <int CT, int D>
 void launch(const TreeArgs& a, int wide, dim3 grid, hipStream_t st) {
-  if (wide == 8)
+  if (wide == 8) {
     tree_wide_kernel<CT, D, 8><<<grid, kWideWaves * 64, 0, st>>>(a);
-  else if (wide == 4)
+  } else if (wide == 4) {
     tree_wide_kernel<CT, D, 4><<<grid, kWideWaves * 64, 0, st>>>(a);
-  else if (wide == 0)
-    tree_rows_kernel<CT, D, kWaves><<<grid, kWaves * 64, 0, st>>>(a);
-  else if (wide == -1)
+  } else if (wide == 0) {
+    if constexpr (!large_pages(CT, D)) tree_rows_kernel<CT, D, kWaves><<<grid, kWaves * 64, 0, st>>>(a);
+  } else if (wide == -1) {
     tree_few_kernel<CT, D, kWaves><<<dim3(a.ranges), kWaves * 64, 0, st>>>(a);
-  else
+  } else {
     tree_few_kernel<CT, D, kWaves / 2><<<dim3(a.ranges), kWaves / 2 * 64, 0, st>>>(a);
+  }
 }
 
 // T and the tokens of a sequence that a call may hold.
