@@ -1172,8 +1172,8 @@ __global__ __launch_bounds__(W * 64, 2) void tree_few_kernel(TreeArgs a) {
 // 8 wavefronts share every page through LDS: RT = 8 row tiles of 32 rows, each
 // wavefront's own, or RT = 4, where a wavefront takes one half of each page's
 // tokens and the two of a tile join at the end.  K [D/64, 64 tok, 64] lies in
-// three slots and V [D, 64 tok] in two, as fp16; 8-bit pages are converted once
-// on the way in.  A 128-byte row is 8 units of 16 bytes; unit u lies at
+// KS slots and V [D, 64 tok] in VS, as fp16: fp16 pages are on their way two
+// pages ahead, 8-bit ones, converted once on the way in, one.  A 128-byte row is 8 units of 16 bytes; unit u lies at
 // u ^ swz(row), so that the 16 lanes that a read serves at once, and a
 // conversion's 16 stores, meet 16 different bank groups.
 //
@@ -1187,10 +1187,10 @@ __global__ __launch_bounds__(W * 64, 2) void tree_few_kernel(TreeArgs a) {
 // same type reaches 1199; 321 us over e4m3.  Bound by the products and the
 // softmax's instructions beside them.
 // RT 4: 25 tokens of 32 / 8 heads x 4096: 64 + 8 us of joining over e4m3, 75 + 8
-// over fp16.  A page takes 1.4 us, 0.9 without its loads and conversions: one
-// step a wavefront between two barriers is too little to hide either.  More
-// pages in flight, as codes in LDS or in a second set of registers, gained
-// nothing (1.9 and 1.3 us).
+// over fp16; 16 tokens x 8192 over fp16 131 us, 4.1 TB/s.  An e4m3 page takes 1.4
+// us, 0.9 without its loads and conversions: one step a wavefront between two
+// barriers is too little to hide either.  More 8-bit pages in flight, as codes
+// in LDS or in a second set of registers, gained nothing (1.9 and 1.3 us).
 __device__ __forceinline__ int swz_k(int row) { return ((row >> 1) & 3) | ((((row >> 3) ^ (row >> 4)) & 1) << 2); }
 __device__ __forceinline__ int swz_v(int row) { return (row >> 1) & 7; }
 
@@ -1202,7 +1202,8 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
   constexpr int TILE = kPage * D * 2;  // bytes of a K or a V tile
   constexpr int KU = kPage * D / 16;   // 8-bit: units of a K or a V page, one for each thread (D 64: K's and V's share them)
   static_assert(RT == W || 2 * RT == W, "a wavefront takes a page or a half of it");
-  __shared__ __align__(16) char s_kv[5 * TILE];
+  constexpr int KS = CT == kF16 ? 4 : 3, VS = KS - 1;  // K and V slots
+  __shared__ __align__(16) char s_kv[(KS + VS) * TILE];
   __shared__ __align__(16) float s_sc[3][3][kPage];  // 8-bit: score factors, V's scales' logarithms and inverses
   __shared__ __align__(16) float s_vs[3][kPage];     // V's scales where they are not finite, else 0
   __shared__ int s_odd[3];                           // whether any is not
@@ -1261,7 +1262,7 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
     // A page's K or V into its slot: fp16 by loads into LDS; 8-bit by way of
     // registers (take, then put a step later).
     auto k_tile = [&](int s3) { return s_kv + s3 * TILE; };
-    auto v_tile = [&](int s2) { return s_kv + (3 + s2) * TILE; };
+    auto v_tile = [&](int s2) { return s_kv + (KS + s2) * TILE; };
     auto dma = [&](const uint8_t* cache, int64_t head, char* to, int src) {
       const Rsrc r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(cache + head * TILE), 0, TILE, 0x00020000);
 #pragma unroll
@@ -1482,7 +1483,7 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
     };
 
     if (block_live && p0 < p1) {
-      // Page p's K lies in slot (p - p0) % 3 and its V in (p - p0) % 2.  At the
+      // Page p's K lies in slot (p - p0) % KS and its V in (p - p0) % VS.  At the
       // top of page p, K of pages p and p + 1 and V of page p have arrived.
       const bool two = p0 + 1 < p1;
       int64_t head = pages.head(p0);
@@ -1492,6 +1493,11 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
         if (two) {
           head = pages.head(p0 + 1);
           dma(a.k, head, k_tile(1), k_src);
+          dma(a.v, head, v_tile(1), v_src);
+        }
+        if (p0 + 2 < p1) {
+          head = pages.head(p0 + 2);
+          dma(a.k, head, k_tile(2), k_src);
         }
       } else {
         take_k(head);
@@ -1514,19 +1520,26 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
       f32x16 sa, sb;
       // The top of page p: its arrivals, and the loads of what comes after.
       auto top = [&](int p) {
-        const int f3 = s3 == 0 ? 2 : s3 - 1;  // page p + 2's slot
-        if constexpr (CT == kF16) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();  // and every wavefront is done with page p - 1
+        const int kf = s3 == 0 ? KS - 1 : s3 - 1, vf = s2 == 0 ? VS - 1 : s2 - 1;  // the slots that page p - 1 had
         if constexpr (CT == kF16) {
-          if (p + 1 < p1) dma(a.v, head, v_tile(s2 ^ 1), v_src);
-          if (p + 2 < p1) {
-            head = pages.head(p + 2);
-            dma(a.k, head, k_tile(f3), k_src);
+          // K of page p + 1 and V of page p have arrived when no more is on its
+          // way than V of p + 1 and K of p + 2.  (__syncthreads() would wait for all.)
+          if (p + 2 < p1)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * (TILE / 1024 / W)) : "memory");
+          else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+          __builtin_amdgcn_s_barrier();  // and every wavefront is done with page p - 1
+          asm volatile("" ::: "memory");
+          if (p + 2 < p1) dma(a.v, head, v_tile(vf), v_src);
+          if (p + 3 < p1) {
+            head = pages.head(p + 3);
+            dma(a.k, head, k_tile(kf), k_src);
           }
         } else {
-          if (p + 1 < p1) put_v(s2 ^ 1);
+          __syncthreads();
+          if (p + 1 < p1) put_v(vf);
           if (p + 2 < p1) {
-            put_k(f3);
+            put_k(kf);
             take_v(head);
           }
           if (p + 3 < p1) {
@@ -1540,8 +1553,8 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
         }
       };
       auto next = [&] {
-        s3 = s3 == 2 ? 0 : s3 + 1;
-        s2 ^= 1;
+        s3 = s3 == KS - 1 ? 0 : s3 + 1;
+        s2 = s2 == VS - 1 ? 0 : s2 + 1;
       };
       if (wave_live) {
         int p = p0;
@@ -1551,7 +1564,7 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
           rescale(largest(sa, 0, part));
           for (;;) {
             // (past the last whole page the scores ahead are of no page, and not used)
-            const int n3 = s3 == 2 ? 0 : s3 + 1;
+            const int n3 = s3 == KS - 1 ? 0 : s3 + 1;
             const char *k0 = k_tile(s3), *k1 = k_tile(n3), *v0 = v_tile(s2);
             float mx;
             if constexpr (RT == W) {
@@ -1678,7 +1691,7 @@ constexpr int kFewRows = 16;
 // Rows up to here take the rows kernel, whose two tiles read a piece's pages
 // twice; but fp16 pages of head_dim 128 (large_pages) go through LDS at once.
 // 16 x 8192 tokens, 32 / 8 heads, 8 and 16 drafted (32 and 64 rows), us by rows
-// and through LDS: fp16 139, 209 and 119, 136; head_dim 64 51, 70 and 75, 79;
+// and through LDS: fp16 139, 209 and 119, 131; head_dim 64 51, 70 and 75, 79;
 // e4m3 56, 59 and 120 (25 drafted).
 constexpr int kNarrowRows = 64;
 constexpr bool large_pages(int kind, int D) { return kind == kF16 && D == 128; }  // 32 KiB for K and V
