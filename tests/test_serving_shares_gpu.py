@@ -170,3 +170,17 @@ def test_rotary_training_step_in_a_graph(cuda):
         torch.cuda.synchronize()
         for x, y in zip(out, step()):
             assert torch.equal(x, y), i
+
+
+@pytest.mark.parametrize("kind", ["f16", "e4m3"])
+@pytest.mark.parametrize("mask", [None, "tree"])
+def test_drafts_longer_than_pages(cuda, kind, mask):
+    """Drafted tokens over several pages, in ten row blocks."""
+    run(cuda, kind, [37, 0, 500], 200, 12, 1, 128, [200, 130, 1], mask=mask, seed=1900)
+
+
+@pytest.mark.parametrize("kind", ["f16", "int8"])
+@pytest.mark.parametrize("Hq,Hkv", [(20, 1), (64, 1), (71, 1), (140, 1), (300, 1), (17, 17)])
+def test_many_heads_to_a_kv_head(cuda, kind, Hq, Hkv):
+    """One drafted token, but as many rows as any."""
+    run(cuda, kind, [700, 64, 0], 1, Hq, Hkv, 64, [1, 1, 0], mask=None, seed=2000)
