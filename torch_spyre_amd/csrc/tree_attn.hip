@@ -1717,12 +1717,16 @@ Plan plan_of(int kind, int B, int T, int Hq, int Hkv, int D, int max_tokens) {
   // tokens, us at 2 / 3 / 4 / 8 pages a part: 64 rows 13.2 / 13.5 / 15 / 17;
   // 256 rows, whose joining is launched in any case, 29 / 31 / 32 / 42).  Nor is
   // a sequence cut whose wavefronts have one page each, or two of 16 KiB
-  // (700 tokens, few rows: int8 10.6 whole, 11.7 in parts; fp16 17.8 and 15.2).
+  // (700 tokens, few rows: int8 10.6 whole, 11.7 in parts; fp16 17.8 and 15.2),
+  // nor one in LDS whose pages are few where whole ones fill half the device (16 x
+  // 25 drafted tokens x 32 / 8 heads over 1000, e4m3: 41.9 whole, 46.4 in parts;
+  // over 1500 49.1 and 39.9).
   p.min_per = p.wide > 0 ? 2 : p.wide < 0 ? 3 : 6;
-  p.min_cut = p.wide > 0 ? 4 : p.wide == 0 ? 12 : large_pages(kind, D) ? 9 : 13;
+  const int64_t slots = p.wide == -2 ? 512 : 256;
+  const bool half = 2 * p.row_blocks * (static_cast<int64_t>(B) * Hkv) >= slots;
+  p.min_cut = p.wide > 0 ? (half ? 20 : 4) : p.wide == 0 ? 12 : large_pages(kind, D) ? 9 : 13;
   // One round of the device, or as many parts as there can be.
   const int64_t pages = std::max(pages_of(max_tokens), 1), parts_of_one = pages < p.min_cut ? 1 : pages / p.min_per;
-  const int64_t slots = p.wide == -2 ? 512 : 256;
   const int64_t ranges = std::min(B * (Hkv * parts_of_one), std::max<int64_t>(slots / p.row_blocks, 1));
   p.ranges = static_cast<int>(std::max<int64_t>(ranges, 1));
   const int64_t parts = static_cast<int64_t>(p.ranges) * p.row_blocks * 2;
