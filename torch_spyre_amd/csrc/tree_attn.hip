@@ -23,6 +23,10 @@
 // 8-bit V carries a scale for each token.  It is added to the score as its
 // logarithm, so the weights that meet the codes are p * scale relative to the
 // largest such, whatever the scales' range; the row sum divides it out again.
+// A V row of zeros is stored with scale 1, far above that of ordinary rows (2^-7
+// for e4m3): attended with 0.999, as an attention sink is, it would press all
+// weights that count below fp16's range.  Where a scale is 1 the codes are looked
+// at, and a row of zeros then weighs as little as a scale of 0 (2^-60).
 
 #include <hip/hip_runtime.h>
 
@@ -387,6 +391,23 @@ __device__ __forceinline__ void drop_tokens(u32x4 (&x)[W], int n) {
     }
 }
 
+// x or-ed over the 16 lanes of a row.
+__device__ __forceinline__ uint32_t or16(uint32_t x) {
+  x |= static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), 0xb1, 0xf, 0xf, false));   // quad_perm 1 0 3 2
+  x |= static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x4e, 0xf, 0xf, false));   // quad_perm 2 3 0 1
+  x |= static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x141, 0xf, 0xf, false));  // row_half_mirror
+  x |= static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x140, 0xf, 0xf, false));  // row_mirror
+  return x;
+}
+
+// A unit of V's codes (16 tokens of a feature), or-ed over all features: whether
+// token t's are all zero (e4m3 has a negative one).
+template <int CT>
+__device__ __forceinline__ bool zero_row(const u32x4& w, int t) {
+  const uint32_t x = t < 8 ? t < 4 ? w[0] : w[1] : t < 12 ? w[2] : w[3];
+  return ((x >> (8 * (t % 4))) & (CT == SPYRE_CODES_E4M3 ? 0x7fu : 0xffu)) == 0;
+}
+
 // Zeroes a word's infinities and NaNs (int8 has none); whether it held any.
 template <int CT>
 __device__ __forceinline__ bool drop_odd(uint32_t& w) {
@@ -718,7 +739,22 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
         const bool finite = __builtin_fabsf(scale) <= 0x1.fffffep127f;
         odd_scale = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(half && !finite) >> (32 + 16 * half)) & 0xffffu;
         inf_scale = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(half && scale == INFINITY) >> (32 + 16 * half)) & 0xffffu;
-        const float vc = !finite ? 1.f : scale < 0x1p-60f ? 0x1p-60f : scale;  // V's scale 0: codes of no weight
+        bool none = scale < 0x1p-60f;  // codes of no weight
+        if (__any(half && scale == 1.f && (!EDGE || st * STEP + col < total))) {  // rows of zeros?
+          u32x4 w = vr.x[0][0];
+#pragma unroll
+          for (int dt = 1; dt < DS; ++dt) w |= vr.x[dt][0];
+          u32x4 w0, w1;  // tokens 0 .. 15 and 16 .. 31 of the step
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t x = or16(w[i]);
+            const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+            const auto h = __builtin_amdgcn_permlane32_swap(r[0] | r[1], r[0] | r[1], false, false);
+            w0[i] = h[0], w1[i] = h[1];
+          }
+          none = none || (scale == 1.f && zero_row<CT>(col < 16 ? w0 : w1, col % 16));
+        }
+        const float vc = !finite ? 1.f : none ? 0x1p-60f : scale;
         s_sc[lane] = half ? __builtin_amdgcn_logf(vc) : scale * a.scale_log2;
         if (half) s_sc[2 * STEP + col] = __builtin_amdgcn_rcpf(vc);
         __builtin_amdgcn_wave_barrier();
@@ -997,7 +1033,16 @@ __global__ __launch_bounds__(W * 64, 2) void tree_few_kernel(TreeArgs a) {
             inf_scale |= (static_cast<uint32_t>(infinite >> (16 * j + 4 * grp)) & 0xfu) << (4 * j);
           }
         }
-        const float vc = !finite ? 1.f : x.vs < 0x1p-60f ? 0x1p-60f : x.vs;
+        bool none = x.vs < 0x1p-60f;  // as in the rows kernel
+        if (__any(x.vs == 1.f && (!EDGE || p * kPage + lane < total))) {
+          u32x4 w = x.v[0][0];
+#pragma unroll
+          for (int dt = 1; dt < DV; ++dt) w |= x.v[dt][0];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = or16(w[i]);
+          none = none || (x.vs == 1.f && zero_row<CT>(w, col));
+        }
+        const float vc = !finite ? 1.f : none ? 0x1p-60f : x.vs;
         s_sc[lane] = x.ks * a.scale_log2;
         s_sc[kPage + lane] = __builtin_amdgcn_logf(vc);
         s_sc[2 * kPage + lane] = __builtin_amdgcn_rcpf(vc);
@@ -1287,7 +1332,7 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
       *reinterpret_cast<f16x8*>(at + ((u ^ sw) * 16)) = codes_to_f16x8<CT>(w[0], w[1]);
       *reinterpret_cast<f16x8*>(at + (((u + 1) ^ sw) * 16)) = codes_to_f16x8<CT>(w[2], w[3]);
     };
-    auto put_k = [&](int s3) {
+    auto put_k = [&](int s3, int page, int64_t head) {  // those of `page`, which lies at `head`
       int ln = lane;
       asm volatile("" : "+v"(ln));  // its addresses are not worth registers of the products
       if (has_k) {
@@ -1297,7 +1342,17 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
       if (wave == 0) s_sc[s3][0][ln] = scale * c;
       if (wave == 1) {
         const bool finite = __builtin_fabsf(scale) <= 0x1.fffffep127f;
-        const float vc = !finite ? 1.f : scale < 0x1p-60f ? 0x1p-60f : scale;  // 0: codes of no weight
+        bool none = scale < 0x1p-60f;  // codes of no weight
+        if (__any(scale == 1.f && page * kPage + ln < total)) {  // rows of zeros?
+          const u32x4* v = reinterpret_cast<const u32x4*>(a.v + head * (TILE / 2)) + ln / 16 * D + ln % 16;
+          u32x4 w = v[0];
+#pragma unroll 1
+          for (int f = 16; f < D; f += 16) w |= v[f];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = or16(w[i]);
+          none = none || (scale == 1.f && zero_row<CT>(w, ln % 16));
+        }
+        const float vc = !finite ? 1.f : none ? 0x1p-60f : scale;
         s_sc[s3][1][ln] = __builtin_amdgcn_logf(vc);
         s_sc[s3][2][ln] = __builtin_amdgcn_rcpf(vc);
         s_vs[s3][ln] = finite ? 0.f : scale;
@@ -1502,13 +1557,13 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
       } else {
         take_k(head);
         take_v(head);
-        put_k(0);
+        put_k(0, p0, head);
         put_v(0);
         if (two) {
           head = pages.head(p0 + 1);
           take_k(head);
           take_v(head);
-          put_k(1);
+          put_k(1, p0 + 1, head);
           if (p0 + 2 < p1) {
             head = pages.head(p0 + 2);
             take_k(head);
@@ -1539,7 +1594,7 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
           __syncthreads();
           if (p + 1 < p1) put_v(vf);
           if (p + 2 < p1) {
-            put_k(kf);
+            put_k(kf, p + 2, head);
             take_v(head);
           }
           if (p + 3 < p1) {
