@@ -1430,6 +1430,7 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
     // the softmax, and operands three products ahead.
     auto step = [&](const f32x16& cur, f32x16& nxt, const char* kt, int tn, int n3, const char* vt, int t, int s3) {
       constexpr int N = 2 * DS, PER = 16 / N, AHEAD = 3;
+      const float mu = m == -INFINITY ? 0.f : m;  // scores of -inf only so far: weights 0
       const char* v_at[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) v_at[e] = vt + col * 128 + ((v_x ^ (4 * t + e)) * 16);
@@ -1459,7 +1460,7 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
         nxt = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[i], qf[i / 2][i % 2], nxt, 0, 0, 0);
 #pragma unroll
         for (int y = PER * i; y < PER * (i + 1); ++y) {
-          const float w = exp2_of(CT == kF16 ? __builtin_fmaf(cur[y], c, -m) : cur[y] - m);
+          const float w = exp2_of(CT == kF16 ? __builtin_fmaf(cur[y], c, -mu) : cur[y] - mu);
           l = CT == kF16 ? l + w : __builtin_fmaf(w, r[y / 4][y % 4], l);
           pw[y / 8][y % 8] = static_cast<_Float16>(w);
         }
