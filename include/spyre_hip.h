@@ -455,7 +455,9 @@ int spyre_kv_quant_read(const void* k_cache, const void* v_cache, const float* k
  * validly make the sequence's rows NaN.  The workspace holds
  * spyre_paged_tree_attn_workspace_bytes, 16-byte aligned, without
  * initialisation; two calls in flight need two.
- * D in {64, 128}, page_size 64.  No reference counterpart. */
+ * D in {64, 128}, page_size 64, T (Hq / Hkv) D / 4 < 2^31 - 2^19; with P the
+ * pages of max_context_len + T tokens, B Hkv (P + 5) < 2^30.  Sizes beyond
+ * the rows' limit need 0 bytes.  No reference counterpart. */
 size_t spyre_paged_tree_attn_workspace_bytes(int cache_kind, int B, int T, int Hq, int Hkv, int D,
                                              int max_context_len, int draft_keys);
 int spyre_paged_tree_attn(const void* q, const int64_t* q_strides, const void* k_cache,

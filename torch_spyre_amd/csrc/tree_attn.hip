@@ -1806,10 +1806,15 @@ void launch(const TreeArgs& a, int wide, dim3 grid, hipStream_t st) {
   }
 }
 
-// T and the tokens of a sequence that a call may hold.
+// T and the tokens of a sequence that a call may hold.  The merge kernel indexes
+// rows x D / 4 in 32 bits, and its loop passes the last by up to kMergeBlocks
+// workgroups of 256.
+constexpr int kMergeBlocks = 2048;
+
 bool sizes_ok(int B, int T, int Hq, int Hkv, int D, int max_ctx) {
   return B >= 0 && T > 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && (D == 64 || D == 128) && max_ctx >= 0 &&
-         static_cast<int64_t>(T) * (Hq / Hkv) < (int64_t{1} << 30) && static_cast<int64_t>(max_ctx) + T < (int64_t{1} << 31) - kPage;
+         static_cast<int64_t>(T) * (Hq / Hkv) * (D / 4) < (int64_t{1} << 31) - 256 * kMergeBlocks &&
+         static_cast<int64_t>(max_ctx) + T < (int64_t{1} << 31) - kPage;
 }
 
 }  // namespace
@@ -1887,7 +1892,7 @@ extern "C" int spyre_paged_tree_attn(const void* q, const int64_t* q_strides, co
   if (p.merge) {
     // Workgroups whose rows nobody shared leave at once; too many of those cost
     // more than a few long loops (8192 of them 23 us).
-    const int64_t n = std::min((static_cast<int64_t>(a.rows) * (D / 4) + 255) / 256, std::max<int64_t>(2048 / pairs, 1));
+    const int64_t n = std::min((static_cast<int64_t>(a.rows) * (D / 4) + 255) / 256, std::max<int64_t>(kMergeBlocks / pairs, 1));
     const dim3 merge(static_cast<uint32_t>(pairs), static_cast<uint32_t>(n));
     if (D == 128)
       tree_merge_kernel<128><<<merge, 256, 0, st>>>(a);
