@@ -115,7 +115,8 @@ std::tuple<at::Tensor, at::Tensor> call_rotary(const at::Tensor& q, const std::o
 }
 
 // The rotation is orthogonal but for the amplitude, so the gradient is the
-// rotation back, by the same kernel.
+// rotation back, by the same kernel; in forward mode (rotary_autograd) the
+// tangent is rotated as the operand is.
 struct Rotary : torch::autograd::Function<Rotary> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q,
                                                 const std::optional<at::Tensor>& k, const at::Tensor& positions,
@@ -154,6 +155,28 @@ struct Rotary : torch::autograd::Function<Rotary> {
 std::tuple<at::Tensor, at::Tensor> rotary_autograd(const at::Tensor& q, const std::optional<at::Tensor>& k,
                                                    const at::Tensor& positions, const at::Tensor& frequencies,
                                                    double amplitude, bool interleaved, bool inverse) {
+  TORCH_CHECK_VALUE(!frequencies._fw_grad(0).defined(), "frequencies take no gradient");
+  const at::Tensor tq = q._fw_grad(0), tk = k.has_value() ? k->_fw_grad(0) : at::Tensor();
+  if (tq.defined() || tk.defined()) {
+    // Forward mode: the rotation is linear, so a result's tangent is the
+    // rotation of its operand's.
+    auto plain = [](const at::Tensor& t) { return t._fw_primal(0); };
+    auto [qo, ko] = rotary_autograd(plain(q), k.has_value() ? std::make_optional(plain(*k)) : std::nullopt, positions,
+                                    frequencies, amplitude, interleaved, inverse);
+    auto along = [&](const at::Tensor& x, const std::optional<at::Tensor>& y) {
+      return rotary_autograd(x, y, positions, frequencies, amplitude, interleaved, inverse);
+    };
+    at::Tensor dq, dk;
+    if (tq.defined() && tk.defined())
+      std::tie(dq, dk) = along(tq, tk);
+    else if (tq.defined())
+      dq = std::get<0>(along(tq, std::nullopt));
+    else
+      dk = std::get<0>(along(tk, std::nullopt));
+    if (dq.defined()) qo._set_fw_grad(dq, 0, false);
+    if (dk.defined()) ko._set_fw_grad(dk, 0, false);
+    return {qo, ko};
+  }
   if (!at::GradMode::is_enabled() || !(q.requires_grad() || (k.has_value() && k->requires_grad()))) {
     at::AutoDispatchBelowADInplaceOrView below;
     return call_rotary(q, k, positions, frequencies, amplitude, interleaved, inverse);

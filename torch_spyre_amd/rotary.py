@@ -84,7 +84,8 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
     their transposes); positions int32 or int64 [B, S] or [S]; frequencies
     float64, as ``rotary_frequencies`` gives them.  Returns (q, k) with the
     operands' strides where these are dense, or q alone without k.
-    Differentiable in q and k (any number of times)."""
+    Differentiable in q and k, in reverse (any number of times) and forward
+    mode."""
     try:
         yq, yk = _ROTARY(q, k, positions, frequencies, float(amplitude), interleaved, inverse)
     except RuntimeError as e:
