@@ -1,6 +1,7 @@
 """GPU: attention over the 8-bit cache, and of drafted tokens, where the tokens
 with the largest weights add little or nothing to the result: V rows of zeros
-(stored with scale 1 whatever the others' are), in every kernel of it."""
+(stored with scale 1 whatever the others' are), and of one feature, in every
+kernel of it."""
 
 import math
 
@@ -31,12 +32,12 @@ def put(cache, kind, table, token, k, v):
         cache.append(k[None], v[None], table, torch.tensor([token], dtype=torch.int32, device=k.device))
 
 
-def check_small(out, lse, q, kl, vl, table, ctx, T, draft_keys=True, headroom=1.0):
+def check_small(out, lse, q, kl, vl, table, ctx, T, draft_keys=True, headroom=1.0, f16=False):
     """Each row within half a step (2^-11) of its rounding to fp16 and of each
     weight's, and sums, scores and exponentials in fp32 as elsewhere.  Weights
     below fp16's normal range are off by 2^-25 of a unit that is at most
-    1 / headroom of the largest weight times V row: rows of zeros count nothing
-    there.  lse is a sum of up to two numbers below 2^7 and of its logarithm."""
+    1 / headroom of the largest weight times V row (rows of zeros count nothing
+    there; fp16 pages: of the largest weight, times the largest V).  lse is a sum of up to two numbers below 2^7 and of its logarithm."""
     D = q.shape[-1]
     total = ctx + (T if draft_keys else 0)
     q64, o64, l64 = (x.double().cpu().numpy() for x in (q, out, lse))
@@ -53,7 +54,8 @@ def check_small(out, lse, q, kl, vl, table, ctx, T, draft_keys=True, headroom=1.
             ref, size = p @ vv, p @ np.abs(vv)
             ds = (D + 4) * 2.0 ** -24 / math.sqrt(D) * (np.abs(kk) @ np.abs(q64[i, h])).max()
             tol = (size * (2 * 2.0 ** -11 + n * 2.0 ** -24 + 2 * ds + 2.0 ** -18)
-                   + n * 2.0 ** -25 / headroom * (p * amax[h // g, :n]).max() + 2.0 ** -25)
+                   + n * 2.0 ** -25 / headroom * (p.max() * amax[h // g, :n].max() if f16 else (p * amax[h // g, :n]).max())
+                   + 2.0 ** -25)
             err = np.abs(o64[i, h] - ref)
             assert (err <= tol).all(), f"row {i} head {h}: worst {(err / tol).max():.1f} of the tolerance, " \
                                        f"result {np.abs(ref).max():.2e}, off by {err.max():.2e}"
@@ -133,3 +135,35 @@ def test_values_all_zero_or_all_of_scale_one(cuda, kind, shape):
     nothing, same = tsa.paged_tree_attention(q, cache.k, cache.v, table, lens, **args)
     assert not nothing.any()
     check_small(nothing[0], same[0], q[0], kl, np.zeros_like(vl), table.cpu().numpy(), ctx, T)
+
+
+@pytest.mark.parametrize("kind", ["f16", "e4m3", "int8"])
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("ctx,token", [(120, 0), (120, 119), (190, 64), (2050, 1000)])
+def test_small_weights_beside_one_that_takes_all(cuda, kind, shape, ctx, token):
+    """One token takes nearly all of every row and has V in one feature only
+    (fp16: none); what the others add to the rest, with weights of 2^-27 each,
+    is there.  The reference of the weights is 2^7 below the largest."""
+    import torch_spyre_amd as tsa
+
+    T, Hq, Hkv, D = shape
+    W = (ctx + T + 63) // 64
+    cache = make_cache(kind, W, Hkv, D, cuda, SEED + 7)
+    table = table_of(1, W, W, cuda, SEED + 8)
+    if kind == "f16":
+        cache.v.abs_().mul_(64)  # results that fp16 holds
+    else:
+        cache.v_scale.mul_(64)
+        codes = cache.v.view(torch.uint8 if kind == "e4m3" else torch.int8)
+        codes.copy_(codes & 0x7f if kind == "e4m3" else codes.abs())
+    v = torch.zeros((Hkv, D), dtype=torch.float16, device=cuda)
+    v[:, D - 1] = 0.0 if kind == "f16" else 128.0
+    put(cache, kind, table, token, key(Hkv, D, 18.8, cuda), v)
+    q = queries(T, Hq, D, cuda, SEED + 9)
+    q[..., 1:] *= 0.0625
+    lens = torch.tensor([ctx], dtype=torch.int32, device=cuda)
+    kl, vl = logical(cache, kind)
+    out, lse = tsa.paged_tree_attention(q, cache.k, cache.v, table, lens, max_context_len=ctx, return_lse=True,
+                                        **scales(cache, kind))
+    check_small(out[0], lse[0], q[0], kl, vl, table.cpu().numpy(), ctx, T, headroom=2.0 ** 7, f16=kind == "f16")
+    assert (out[..., :D - 1] > 0).all()

@@ -54,10 +54,13 @@ constexpr int kTile = 32;  // query rows of a tile, and tokens of an MFMA
 constexpr int kF16 = SPYRE_CACHE_F16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-// The running reference of a row's exponents moves only when a score passes it
-// by more than this (log2 units): weights up to 2^8 are as exact in fp16 as
-// those up to 1, and most steps then skip the rescaling of O.
-constexpr float kSlack = 8.f;
+// The running reference of a row's exponents is put kBelow under its largest score
+// (log2 units) and moves only when a score passes it by more than kAbove: weights
+// up to 2^15 are as exact in fp16 as those up to 1, most steps then skip the
+// rescaling of O, and a weight is a normal number of fp16 (a relative 2^-11) down
+// to 2^-21 of the largest: many small ones count beside one that takes nearly all
+// of a row and whose V adds little, as an attention sink's.
+constexpr float kBelow = 7.f, kAbove = 15.f;
 
 struct TreeArgs {
   const _Float16* q;
@@ -789,8 +792,8 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
         }
       }
       mx = xor32_max(mx);
-      if (__any(mx > m + kSlack)) {
-        const float mn = fmaxf(m, mx);
+      if (__any(mx > m + kAbove)) {
+        const float mn = fmaxf(m, mx - kBelow);
         const float alpha = m == -INFINITY ? 0.f : exp2_of(m - mn);
         m = mn;
         l *= alpha;
@@ -1081,8 +1084,8 @@ __global__ __launch_bounds__(W * 64, 2) void tree_few_kernel(TreeArgs a) {
       }
       mx = xor32_max(mx);
       mx = xor16_max(mx);
-      if (__any(mx > m + kSlack)) {
-        const float mn = fmaxf(m, mx);
+      if (__any(mx > m + kAbove)) {
+        const float mn = fmaxf(m, mx - kBelow);
         const float alpha = m == -INFINITY ? 0.f : exp2_of(m - mn);
         m = mn;
         l *= alpha;
@@ -1411,8 +1414,8 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
       return xor32_max(mx) * (CT == kF16 ? c : 1.f);
     };
     auto rescale = [&](float mx) {
-      if (__any(mx > m + kSlack)) {
-        const float mn = fmaxf(m, mx);
+      if (__any(mx > m + kAbove)) {
+        const float mn = fmaxf(m, mx - kBelow);
         const float alpha = m == -INFINITY ? 0.f : exp2_of(m - mn);
         m = mn;
         l *= alpha;
