@@ -238,7 +238,8 @@ def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     """Attention of drafted tokens over the paged cache that holds them behind
     their context: sequence b's cache has context_lens[b] tokens (int32 [B]) and
     then draft_lens[b] (int32 [B], default T) drafted ones, appended by the
-    caller at positions context_lens[b] + j.  Query i of q [B, T, Hq, D]
+    caller at positions context_lens[b] + j (8-bit caches: in one launch; an fp16
+    one takes a ``kv_append`` for each j).  Query i of q [B, T, Hq, D]
     (float16) attends the context and the drafted tokens j with tree_mask[b, i,
     j] (bool [B, T, T] or [T, T]: a tree gives each token its ancestors and
     itself); without a mask j <= i, one line of tokens.

@@ -8,11 +8,11 @@
 // of scale 1; a NaN or an infinity makes the scale NaN or infinite, and the whole
 // row reads back as NaN.
 //
-// Both directions are bound by memory (a large copy 4.86 TB/s).  3 x 2500 tokens
-// of 32 heads of 128, int8: written in 46 us, 4.0 TB/s (58 where K and V come
-// from memory and the last reader's rows are still on their way there), read
-// in 30 to 37.  8 x 8500 rows of 8 heads, 4500 of them held, e4m3: 74 us,
-// 4.8 TB/s.  A decode step of 32 tokens: 6.5 and 4.4 us, the chains of their loads.
+// Both directions are bound by memory (a large copy 4.88 TB/s).  3 x 2500 tokens
+// of 32 heads of 128, int8: written in 48 to 56 us, 3.3 to 3.9 TB/s (54 where the
+// last reader's rows are still on their way to memory), read in 30 to 34.  8 x
+// 8500 rows of 8 heads, 4500 of them held, e4m3: 73 us, 4.8 TB/s.  A decode step
+// of 32 tokens: 6.5 and 4.5 us, the chains of their loads.
 
 #include <hip/hip_runtime.h>
 

@@ -10,7 +10,7 @@
 // more than the rotation, and all heads of a token share them), leaves cos and
 // sin in LDS, then moves (token, head, unit) items of 8 pairs, two 16-byte
 // loads and stores of fp16 a lane.  8192 tokens of 64 + 8 heads of 128, fp16:
-// 57.5 us, 5.25 TB/s (a large copy 4.86); 32 tokens of 32 + 8 heads 3.9 us, the
+// 52.4 us, 5.8 TB/s (a large copy 4.88); 32 tokens of 32 + 8 heads 3.9 us, the
 // chain of its loads.
 #include <hip/hip_runtime.h>
 

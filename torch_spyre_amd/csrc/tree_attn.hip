@@ -657,7 +657,7 @@ __device__ __forceinline__ void finish(const TreeArgs& a, const Walk& walk, cons
 // have used this one's, V as soon as O has.
 // 16 sequences x 4096 tokens, 32 / 8 heads: 8 drafted tokens (32 rows) 36 us over
 // e4m3 of head_dim 128 (3.7 TB/s), 31 over fp16 of 64 (4.4 TB/s); 16 (two tiles,
-// which read the pages twice, the second time from L2) 33 us over e4m3, 527
+// which read the pages twice, the second time from L2) 34 us over e4m3, 501
 // TFLOP/s.  Bound by instruction issue over 8-bit pages (a tile's conversions
 // cost as much as its products) and by the one step in flight over fp16 ones.
 template <int CT, int D, int W>
@@ -931,8 +931,8 @@ __global__ __launch_bounds__(W * 64, 2) void tree_rows_kernel(TreeArgs a) {
 //          tokens) of the four groups change places in registers first.
 // Bound by memory: K of the next page is loaded as soon as the scores have used
 // this one's, V as soon as O has; head_dim 64 has the registers for two pages in
-// flight.  A decode step over e4m3, 32 / 8 heads of 128: 32 x 4096 tokens 45.6 us
-// (6.0 TB/s), 64 x 8192 166 us (6.6 TB/s), 64 x 128 to 16384 189 us; one
+// flight.  A decode step over e4m3, 32 / 8 heads of 128: 32 x 4096 tokens 45 us
+// (6.1 TB/s), 64 x 8192 165 us (6.7 TB/s), 64 x 128 to 16384 185 us; one
 // sequence of 700 tokens 10.6 us, which is the chain of its loads (lengths, table,
 // page) and the join.
 template <int CT, int D, int W>
@@ -1231,10 +1231,10 @@ __global__ __launch_bounds__(W * 64, 2) void tree_few_kernel(TreeArgs a) {
 // therefore runs one page ahead of V.
 //
 // RT 8: 16 sequences x 8192 tokens, 64 tokens of 64 / 8 heads of 128 (512 rows to
-// a KV head): 305 us over fp16, 901 TFLOP/s where a large matrix product of the
-// same type reaches 1199; 321 us over e4m3.  Bound by the products and the
+// a KV head): 314 to 320 us over fp16, 865 to 880 TFLOP/s where a large matrix
+// product of the same type reaches 1200; 328 us over e4m3.  Bound by the products and the
 // softmax's instructions beside them.
-// RT 4: 25 tokens of 32 / 8 heads x 4096: 64 + 8 us of joining over e4m3, 75 + 8
+// RT 4: 25 tokens of 32 / 8 heads x 4096: 67 + 8 us of joining over e4m3, 77 + 8
 // over fp16; 16 tokens x 8192 over fp16 131 us, 4.1 TB/s.  An e4m3 page takes 1.4
 // us, 0.9 without its loads and conversions: one step a wavefront between two
 // barriers is too little to hide either.  More 8-bit pages in flight, as codes
@@ -1693,7 +1693,7 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void tree_wide_kernel(TreeArgs 
       }
     }
     if (part == 0 && tile * kTile + col < a.rows) {
-        const int64_t part_row = partial_of(a, range, rb, pc.slot, local * kTile + col);
+      const int64_t part_row = partial_of(a, range, rb, pc.slot, local * kTile + col);
       float* x = a.ws + part_row * D + 4 * half;
 #pragma unroll
       for (int dt = 0; dt < DS; ++dt)
