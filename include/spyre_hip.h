@@ -470,6 +470,135 @@ int spyre_paged_tree_attn(const void* q, const int64_t* q_strides, const void* k
                           int page_size, int64_t num_pages, int max_context_len, float scale,
                           void* stream);
 
+/* Block tables and slots from the sequences' lengths.  Sequence b holds the
+ * first held[b] pages of its row of the table; with context_lens[b] cached and
+ * new_lens[b] further tokens it gets as many more as it lacks, sequence after
+ * sequence, from a ring of free pages between two counters that only grow,
+ *   cursor : int64 {taken, returned}; the free pages are
+ *            free_pages[c mod num_free], taken <= c < returned
+ * and no more than there are, nor than pages_per_seq.  New entries of
+ * block_table (int32 [B, pages_per_seq], row stride bt_stride) are written, all
+ * others are left as they are; held_out [B] and cursor_out [2] are the new
+ * values.  A call repeated with the same inputs writes the same.
+ *   length >= 0 (tokens -1) : positions int32, slots int64 [B, length], row t
+ *             of sequence b its new token t; -1 for t >= new_lens[b]
+ *   tokens >= 0 (length -1) : [tokens], the sequences' new tokens one after the
+ *             other, sequence b's from starts[b] (int32 [B + 1]) on; -1 behind
+ *             the last
+ * A token's position is context_lens[b] + t, its slot 64 page + position mod
+ * 64, or -1 where it has no page.  B <= 4096.  No reference counterpart. */
+int spyre_plan_pages(int32_t* block_table, int64_t bt_stride, int64_t pages_per_seq,
+                     const int32_t* held, const int32_t* context_lens, const int32_t* new_lens,
+                     const int32_t* free_pages, int64_t num_free, const int64_t* cursor, int length,
+                     int64_t tokens, int32_t* positions, int64_t* slots, int32_t* starts,
+                     int32_t* held_out, int64_t* cursor_out, int B, void* stream);
+
+/* Pages back to the ring: sequence b keeps those of its first lens[b] tokens,
+ * the others of its held[b] go behind the last returned one.  The table is
+ * left as it is (entries from held_out[b] on are stale).  No reference
+ * counterpart. */
+int spyre_release_pages(const int32_t* block_table, int64_t bt_stride, int64_t pages_per_seq,
+                        const int32_t* held, const int32_t* lens, int32_t* free_pages,
+                        int64_t num_free, const int64_t* cursor, int32_t* held_out,
+                        int64_t* cursor_out, int B, void* stream);
+
+/* Drafted tokens accepted or replaced.  Sequence b has n = draft_lens[b] (NULL:
+ * T) drafted tokens; tokens[b, i] continues tokens[b, parents[b, i]] (-1: the
+ * context's end; NULL parents: i - 1, a chain; a parent that is not below i is
+ * never reached).  target row r is the target's probabilities behind the context
+ * (0) or behind drafted token r - 1.  From the context's end on, the children
+ * of the last accepted token c (-1 at first) are tried in their order; x = tokens[b, i] is
+ * accepted if
+ *   uniforms[b, i] * limit < target[b, c + 1, x]
+ * limit the draft's probability draft[b, i, x], or without draft 1 less those of
+ * c's rejected children (a token rejected there once has probability 0).  When
+ * no child is accepted, one more token is drawn: the lowest j at which the running sum of
+ *   w = max(target[b, c + 1] - draft[b, i], 0)  behind a rejection of i by draft,
+ *       else target[b, c + 1] without the rejected tokens;
+ *       target[b, c + 1] if that has no weight
+ * exceeds uniforms[b, T] times its total; -1 if there is no weight at all.
+ * Sums and tests are in 64 bits.  Probabilities that are negative, NaN or infinite
+ * count as 0, tokens outside of [0, V) have none.
+ *   tokens : int32 or int64 [B, T]; target [B, T + 1, V], draft [B, T, V] (NULL
+ *            with parents): SPYRE_DT_FLOAT32, _FLOAT16 or _BFLOAT16, feature stride 1,
+ *            strides {b, row} in elements; uniforms fp32 [B, T + 1]; parents int32
+ *   out_tokens [B, T + 1] (contiguous, of the tokens' type): the accepted ones, the
+ *            drawn one, then -1; accepted int32 [B]; path int32 [B, T]: the
+ *            accepted ones' indices, then -1
+ * The workspace needs no initialisation; two calls in flight need two.
+ * T <= 1024, B <= 65535.  No reference counterpart. */
+size_t spyre_verify_drafts_workspace_bytes(int B, int V);
+int spyre_verify_drafts(const void* tokens, int token_bytes, int64_t tok_sb, int64_t tok_st,
+                        const void* target, const int64_t* target_strides, const void* draft,
+                        const int64_t* draft_strides, int scalar_type, const float* uniforms,
+                        int64_t u_sb, int64_t u_st, const int32_t* parents, int64_t par_sb,
+                        int64_t par_st, const int32_t* draft_lens, void* out_tokens,
+                        int32_t* accepted, int32_t* path, void* workspace, size_t workspace_bytes,
+                        int B, int T, int V, void* stream);
+
+/* The paged latent cache: one row a token for all heads, its latent vector (rank
+ * features) and its rotated key (64), fp16, in pages of 64 tokens
+ *   cache : [num_pages, (rank + 64) / 64, 64 tokens, 64]   sticks along features
+ * rank in {256, 512}.
+ * Append: rows of latent and k_rope (feature stride 1, row strides multiples of
+ * 8 elements, 16-byte aligned) into slots[i] = 64 page + token (int64); slots
+ * outside of the cache are dropped.  Two rows of a call must not share a slot.
+ * Read: row i of latent [B, length, rank] and k_rope [B, length, 64] is token
+ * start[b] + i (start NULL: 0) while that is below lens[b], else zeros; tokens of
+ * pages that the table does not name validly are NaN.  No reference
+ * counterpart. */
+int spyre_latent_append_f16(const void* latent, int64_t latent_stride, const void* k_rope,
+                            int64_t k_rope_stride, void* cache, const int64_t* slots, int64_t rows,
+                            int rank, int64_t num_pages, void* stream);
+int spyre_latent_read_f16(const void* cache, const int32_t* block_table, int64_t bt_stride,
+                          int64_t pages_per_seq, const int32_t* lens, const int32_t* start,
+                          void* latent, void* k_rope, int B, int length, int rank,
+                          int64_t num_pages, void* stream);
+
+/* Attention over the latent cache: keys and values of all H heads are a token's
+ * one row (c, r).  Sequence b has context_lens[b] tokens and, behind them, n =
+ * draft_lens[b] (NULL: T) new ones; query i < n attends the context and the new
+ * tokens j < n with mask[b, i, j] (NULL: j <= i):
+ *   out = softmax(scale (q . c + q_rope . r)) c,  lse the logarithm of its sum
+ * Rows that attend nothing and rows i >= n are zeros with lse -inf.  What a row
+ * does not attend does not reach it, whatever it holds; a row that attends a new
+ * token with a NaN or an infinity is NaN.
+ *   q [B, T, H, rank], q_rope [B, T, H, 64] : fp16, feature stride 1, strides {b, t, h}
+ *           multiples of 8 elements, 16-byte aligned
+ *   mask  : bool [B, T, T], strides {b, i, j} in bytes, 0 to broadcast
+ *   out   : [B, T, H, rank] fp16, lse: optional fp32 [B, T, H]; contiguous
+ * A context above max_context_len and a page that the table does not name
+ * validly make the sequence's rows NaN.  The workspace needs no initialisation;
+ * two calls in flight need two.  rank in {256, 512}.  No reference counterpart. */
+size_t spyre_paged_latent_attn_workspace_bytes(int B, int T, int H, int rank, int max_context_len);
+int spyre_paged_latent_attn(const void* q, const int64_t* q_strides, const void* q_rope,
+                            const int64_t* q_rope_strides, const void* cache,
+                            const int32_t* block_table, int64_t bt_stride, int64_t pages_per_seq,
+                            const int32_t* context_lens, const int32_t* draft_lens,
+                            const void* mask, const int64_t* mask_strides, void* out, float* lse,
+                            void* workspace, size_t workspace_bytes, int B, int T, int H, int rank,
+                            int64_t num_pages, int max_context_len, float scale, void* stream);
+
+/* Causal attention with keys and values expanded from latent vectors: head h's
+ * keys are k [B, keys, H, D] and behind them k_rope [B, keys, 64], which all heads
+ * share; v [B, keys, H, D].  Sequence b has context_lens[b] keys before its n =
+ * new_lens[b] (NULL: T) queries, query i < n attends keys t <= context_lens[b] + i:
+ *   out = softmax(scale (q . k + q_rope . k_rope)) v,  lse the logarithm of its sum
+ * Rows i >= n are zeros with lse -inf; keys from context_lens[b] + n on, and keys
+ * that a row does not attend, do not reach it.  A sequence whose lengths exceed
+ * `keys` is NaN.
+ *   q [B, T, H, D], q_rope [B, T, H, 64], k, v : fp16, feature stride 1, strides {b, t, h},
+ *   k_rope {b, t}; multiples of 8 elements, 16-byte aligned; token strides of k, k_rope
+ *   and v below 2^23
+ *   out [B, T, H, D] fp16, lse optional fp32 [B, T, H]; contiguous
+ * D in {64, 128}.  No reference counterpart. */
+int spyre_latent_attn(const void* q, const int64_t* q_strides, const void* q_rope,
+                      const int64_t* q_rope_strides, const void* k, const int64_t* k_strides,
+                      const void* k_rope, const int64_t* k_rope_strides, const void* v,
+                      const int64_t* v_strides, const int32_t* context_lens,
+                      const int32_t* new_lens, void* out, float* lse, int B, int T, int H, int D,
+                      int keys, float scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,5 +1,6 @@
 """MI355X (gfx950) stick relayout and paged split-KV decode attention,
-with rotary positions, an 8-bit cache and attention of drafted tokens.
+with rotary positions, an 8-bit cache, attention and verification of drafted
+tokens, block tables built on the device and latent attention.
 
 A drop-in for torch-spyre's relayout / restickify / overwrite / decode-SDPA
 path: the SpyreTensorLayout descriptor, the host<->device DMA descriptors and
@@ -57,6 +58,14 @@ from .attention import (  # noqa: E402
     v_page_layout,
     workspace_bytes,
 )
+from .latent import (  # noqa: E402
+    LatentKVCache,
+    latent_append,
+    latent_attention,
+    latent_read,
+    paged_latent_attention,
+)
+from .paging import PagePlan, PagePool, plan_pages, release_pages  # noqa: E402
 from .quantized import (  # noqa: E402
     QuantizedKVCache,
     kv_append_quantized,
@@ -71,6 +80,7 @@ from .sdpa import (  # noqa: E402
     sdpa_override,
     sdpa_overrideable,
 )
+from .verify import verify_drafts  # noqa: E402
 from . import ops  # noqa: E402,F401  (registers the spyre:: ops)
 from . import _torch_patch  # noqa: E402
 
@@ -87,5 +97,7 @@ __all__ = [
     "paged_tree_attention", "sdpa_decode", "v_page_layout", "workspace_bytes",
     "QuantizedKVCache", "kv_append_quantized", "kv_read_quantized", "rotary_kv_append_quantized",
     "rotary_embedding", "rotary_frequencies",
+    "LatentKVCache", "latent_append", "latent_attention", "latent_read", "paged_latent_attention",
+    "PagePlan", "PagePool", "plan_pages", "release_pages", "verify_drafts",
     "SdpaCall", "Unsupported", "scaled_dot_product_attention", "sdpa_override", "sdpa_overrideable",
 ]

@@ -128,6 +128,26 @@ SIGNATURES = {
                                       c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p,
                                       POINTER(c_int64), c_void_p, c_void_p, c_void_p, c_size_t, c_int, c_int,
                                       c_int, c_int, c_int, c_int, c_int64, c_int, c_float, c_void_p]),
+    "spyre_plan_pages": (c_int, [c_void_p, c_int64, c_int64] + [c_void_p] * 4
+                         + [c_int64, c_void_p, c_int, c_int64] + [c_void_p] * 5 + [c_int, c_void_p]),
+    "spyre_release_pages": (c_int, [c_void_p, c_int64, c_int64] + [c_void_p] * 3
+                            + [c_int64] + [c_void_p] * 3 + [c_int, c_void_p]),
+    "spyre_verify_drafts_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "spyre_verify_drafts": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, POINTER(c_int64), c_void_p,
+                                    POINTER(c_int64), c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_int, c_int, c_int,
+                                    c_void_p]),
+    "spyre_latent_append_f16": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int,
+                                        c_int64, c_void_p]),
+    "spyre_latent_read_f16": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                      c_int, c_int, c_int, c_int64, c_void_p]),
+    "spyre_paged_latent_attn_workspace_bytes": (c_size_t, [c_int] * 5),
+    "spyre_paged_latent_attn": (c_int, [c_void_p, POINTER(c_int64), c_void_p, POINTER(c_int64), c_void_p, c_void_p,
+                                        c_int64, c_int64, c_void_p, c_void_p, c_void_p, POINTER(c_int64), c_void_p,
+                                        c_void_p, c_void_p, c_size_t, c_int, c_int, c_int, c_int, c_int64, c_int,
+                                        c_float, c_void_p]),
+    "spyre_latent_attn": (c_int, [c_void_p, POINTER(c_int64)] * 5 + [c_void_p] * 4 + [c_int] * 5
+                          + [c_float, c_void_p]),
 }
 
 _lib = None

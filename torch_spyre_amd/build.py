@@ -6,8 +6,8 @@
 
 Objects go to torch_spyre_amd/_build/ (compiled in parallel), the shared
 library to torch_spyre_amd/libspyre_hip.so, and the PyTorch kernels of the
-attention, KV, rotary and draft ops (csrc/torch_ops.cpp and
-csrc/serving_ops.cpp, against torch's headers, calling that library) to torch_spyre_amd/libspyre_torch.so.
+attention, KV, rotary, draft, page and latent ops (csrc/torch_ops.cpp, csrc/serving_ops.cpp
+and csrc/step_ops.cpp, against torch's headers, calling that library) to torch_spyre_amd/libspyre_torch.so.
 """
 
 from __future__ import annotations
@@ -23,8 +23,9 @@ BUILD = os.path.join(HERE, "_build")
 OUT = os.path.join(HERE, "libspyre_hip.so")
 TORCH_OUT = os.path.join(HERE, "libspyre_torch.so")
 SOURCES = ["layout.cpp", "dma.hip", "decode_attn.hip", "kv_append.hip", "sdpa_fwd.hip", "rotary.hip",
-           "kv_quant.hip", "tree_attn.hip"]
-TORCH_SOURCES = ["torch_ops.cpp", "serving_ops.cpp"]
+           "kv_quant.hip", "tree_attn.hip", "pages.hip", "verify.hip", "latent_cache.hip", "latent_attn.hip",
+           "latent_prompt.hip"]
+TORCH_SOURCES = ["torch_ops.cpp", "serving_ops.cpp", "step_ops.cpp"]
 ARCH = os.environ.get("SPYRE_OFFLOAD_ARCH", "gfx950")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

@@ -15,20 +15,12 @@
 
 #include <cmath>
 #include <cstdint>
-#include <limits>
 
 #include "torch_checks.h"
 
 namespace {
 
 using namespace spyre_torch;
-
-constexpr int64_t kPage = 64;
-
-int as_int(int64_t x, const char* name) {
-  TORCH_CHECK_VALUE(x >= 0 && x <= std::numeric_limits<int>::max(), name, " ", x, " does not fit 31 bits");
-  return static_cast<int>(x);
-}
 
 // ---------------------------------------------------------------- rotary --
 
@@ -211,30 +203,6 @@ Cache check_cache8(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor&
     TORCH_CHECK_VALUE(s->sizes() == at::IntArrayRef({P, H, kPage}) && s->is_contiguous(),
                       "k_scale and v_scale must be contiguous [", P, ", ", H, ", 64] (got ", s->sizes(), ")");
   return {kc.scalar_type() == at::kChar ? SPYRE_CODES_INT8 : SPYRE_CODES_E4M3, P, H, D};
-}
-
-void check_table(const at::Tensor& t, int64_t B, const c10::Device& dev) {
-  require_on(t, dev, "block_table");
-  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.dim() == 2 && t.size(0) == B && (t.size(1) <= 1 || t.stride(1) == 1),
-                    "block_table must be int32 [B, pages_per_seq] with unit column stride");
-}
-
-void check_lens(const at::Tensor& t, int64_t B, const c10::Device& dev, const char* name) {
-  require_on(t, dev, name);
-  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == B && t.is_contiguous(), name,
-                    " must be contiguous int32 [B]");
-}
-
-// fp16 rows that the kernels read as 16-byte vectors: feature stride 1, other
-// strides multiples of 8, 16-byte aligned; anything else is copied into that form.
-at::Tensor rows_operand(const at::Tensor& t, const char* name) {
-  TORCH_CHECK_VALUE(t.is_cuda(), name, " must be a CUDA (HIP) tensor; there is no CPU path");
-  TORCH_CHECK_TYPE(t.scalar_type() == at::kHalf, name, " must be float16 (got ", t.scalar_type(), ")");
-  TORCH_CHECK_VALUE(t.dim() == 4, name, " must be 4-D [B, T, H, D]");
-  const auto st = t.strides();
-  const bool ready = st[3] == 1 && st[0] % 8 == 0 && st[1] % 8 == 0 && st[2] % 8 == 0 &&
-                     reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-  return ready ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 at::Tensor quant_append(const std::optional<at::Tensor>& query, const at::Tensor& k_new, const at::Tensor& v_new,

@@ -29,8 +29,14 @@ an op on CPU tensors raises.  Fake kernels make the ops traceable.
   spyre::kv_quant_read, spyre::quant_paged_decode_attention, spyre::paged_tree_attention
         rotary positions, the 8-bit paged cache and attention of drafted
         tokens (no reference counterparts)
+  spyre::plan_pages, spyre::release_pages, spyre::verify_drafts,
+  spyre::latent_append, spyre::latent_read, spyre::paged_latent_attention,
+  spyre::latent_attention
+        block tables from lengths, verification of drafted tokens, the paged
+        latent cache and its attention (no reference counterparts)
 Those from spyre::kv_append on are defined and implemented in C++
-(csrc/torch_ops.cpp, csrc/serving_ops.cpp); this module gives them fake kernels.
+(csrc/torch_ops.cpp, csrc/serving_ops.cpp, csrc/step_ops.cpp); this module
+gives them fake kernels.
 """
 
 from __future__ import annotations
@@ -221,6 +227,47 @@ def _(q, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, scale=No
 @torch.library.register_fake("spyre::paged_tree_attention")
 def _(q, k_cache, v_cache, block_table, context_lens, tree_mask=None, draft_lens=None, k_scale=None, v_scale=None,
       scale=None, max_context_len=-1):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:3], dtype=torch.float32)
+
+
+@torch.library.register_fake("spyre::plan_pages")
+def _(block_table, held, context_lens, new_lens, free_pages, cursor, length=-1, tokens=-1):
+    shape = (tokens,) if tokens >= 0 else (block_table.shape[0], length)
+    positions = held.new_empty(shape)
+    return (positions, cursor.new_empty(shape), held.new_empty(held.shape), cursor.new_empty((2,)),
+            held.new_empty((block_table.shape[0] + 1 if tokens >= 0 else 0,)))
+
+
+@torch.library.register_fake("spyre::release_pages")
+def _(block_table, held, lens, free_pages, cursor):
+    return held.new_empty(held.shape), cursor.new_empty((2,))
+
+
+@torch.library.register_fake("spyre::verify_drafts")
+def _(draft_tokens, target_probs, uniforms, draft_probs=None, parents=None, draft_lens=None):
+    B, T = draft_tokens.shape
+    return (draft_tokens.new_empty((B, T + 1)), draft_tokens.new_empty((B,), dtype=torch.int32),
+            draft_tokens.new_empty((B, T), dtype=torch.int32))
+
+
+@torch.library.register_fake("spyre::latent_append")
+def _(latent, k_rope, cache, slots):
+    return None
+
+
+@torch.library.register_fake("spyre::latent_read")
+def _(cache, block_table, lens, length, start=None):
+    B = block_table.shape[0]
+    return cache.new_empty((B, length, 64 * cache.shape[1] - 64)), cache.new_empty((B, length, 64))
+
+
+@torch.library.register_fake("spyre::paged_latent_attention")
+def _(q, q_rope, cache, block_table, context_lens, scale, tree_mask=None, draft_lens=None, max_context_len=-1):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:3], dtype=torch.float32)
+
+
+@torch.library.register_fake("spyre::latent_attention")
+def _(q, q_rope, k, k_rope, v, context_lens, new_lens=None, scale=None):
     return q.new_empty(q.shape), q.new_empty(q.shape[:3], dtype=torch.float32)
 
 
