@@ -28,6 +28,7 @@
 #include <cmath>
 
 #include "fast_div.h"
+#include "lds_dma.h"
 #include "page_walk.h"
 #include "spyre_common.h"
 
@@ -41,7 +42,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __amdgpu_buffer_rsrc_t Rsrc;
 
 constexpr int kRope = 64;
 constexpr int kTile = 32;   // rows of a wavefront
@@ -115,6 +115,13 @@ struct Pages {
   }
 };
 
+// A lane index that the compiler forms addresses from where they are used: kept in
+// registers through the loops, those of rare paths would spill.
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // Rows of a page in LDS are 128 bytes for each stick; unit u (16 bytes) of token t
 // lies at u ^ (t & 7).  Neither 8 lanes that read a unit of 8 tokens nor 16 that read
 // 2 units of 4 tokens, transposed, then meet in a bank.
@@ -134,6 +141,7 @@ __global__ __launch_bounds__(RG * kSplit * 64, 2) void latent_kernel(LatentArgs 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
   const int col = lane & 31, half = lane >> 5, l16 = lane & 15, g16 = lane >> 4;
   const int rg = wave / kSplit, part = wave % kSplit;
+  const uint32_t lds0 = lds_address(s_mem);
   int range, rb;
   place_of(a, range, rb);
   Walk walk;
@@ -143,11 +151,9 @@ __global__ __launch_bounds__(RG * kSplit * 64, 2) void latent_kernel(LatentArgs 
   // 8 half + l16 / 4 (and 4 tokens further) of C^T's tiles.
   const int k_tok = 16 * part + l16;
   const int k_off[2] = {k_tok * 128 + ((g16 ^ (k_tok & 7)) * 16), k_tok * 128 + (((4 + g16) ^ (k_tok & 7)) * 16)};
-  auto v_off = [&](int dt, int t) {  // dt: tile of this wavefront
-    const int tile = DT * part + dt, tok = t + 8 * half + l16 / 4;
-    const int u = 4 * (tile & 1) + 2 * (g16 & 1) + ((lane >> 1) & 1);
-    return (tile / 2) * kStick + tok * 128 + ((u ^ (tok & 7)) * 16) + 8 * (lane & 1);
-  };
+  // The unit's key is that of token l16 / 4, its bit 2 turned by odd tiles and by tokens 4
+  // further: two lane offsets, the rest of an address is constant.
+  const int v_lane = DT / 2 * part * kStick + (8 * half + l16 / 4) * 128 + (((2 * (g16 & 1) + ((lane >> 1) & 1)) ^ (l16 / 4)) * 16) + 8 * (lane & 1);
   auto tr = [&](int at) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(s_mem + at));
   };
@@ -164,48 +170,51 @@ __global__ __launch_bounds__(RG * kSplit * 64, 2) void latent_kernel(LatentArgs 
 
     // A page on its way into buffer `buf`; tokens that do not exist as zeros.
     auto load = [&](int p, int buf) {
-      const Rsrc r = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<_Float16*>(a.pages) + pages.at(p) * (NS * (kStick / 2)), 0, BUF, 0x00020000);
+      const dma_rsrc r = dma_buffer(a.pages + pages.at(p) * (NS * (kStick / 2)), BUF);
       const int n = total - p * kPage;
-      const int off = lane / 8 * 128 + (((lane & 7) ^ (lane / 8)) * 16);
+      const int t = here(lane) / 8;
+      const uint32_t off = t * 128 + (((lane & 7) ^ t) * 16);
+      // a wavefront's chunks (8 tokens of a stick): the same tokens in every stick, RG 1 two runs of them
+      uint32_t voff[8 / WAVES];
+#pragma unroll
+      for (int c = 0; c < 8 / WAVES; ++c) voff[c] = (c * WAVES + wave) * 8 + t < n ? off : BUF;
 #pragma unroll
       for (int c = 0; c < NS * 8 / WAVES; ++c) {
-        const int chunk = c * WAVES + wave;  // 8 tokens of a stick
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(s_mem + buf * BUF + chunk * 1024), 16,
-                                                 (chunk & 7) * 8 + lane / 8 < n ? off : 0x7fffff00, chunk * 1024, 0, 0);
+        const int chunk = c * WAVES + wave;
+        dma16(r, lds0 + buf * BUF + chunk * 1024, voff[c % (8 / WAVES)], chunk * 1024);
       }
     };
     static_assert(NS * 8 % WAVES == 0, "equal shares of a page's chunks");
     if (p0 < p1) load(p0, 0);
 
-    // Rows l16 and 16 + l16 of the tile: their query, and the mask of its new token.
+    // Queries of rows l16 and 16 + l16 of the tile.  (One that is not there is another's.)
     f16x8 qf[2][NQ];
-    int qi[2];
-    bool live[2];
+    auto token_of_row = [&](int row) {  // its new token; sq.n or more: none
+      return row < a.rows ? static_cast<int>(fdiv(row, a.by_h)) : sq.n;
+    };
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      const int row = row0 + 16 * n + l16;
-      const int i = static_cast<int>(fdiv(row, a.by_h));
-      live[n] = row < a.rows && i < sq.n;
-      qi[n] = live[n] ? i : 0;
-      const int h = live[n] ? row - i * a.H : 0;
-      const _Float16* x = a.q + b * a.q_sb + qi[n] * a.q_st + h * a.q_sh + 8 * g16;
-      const _Float16* xr = a.qr + b * a.qr_sb + qi[n] * a.qr_st + h * a.qr_sh + 8 * g16;
+      const int row = row0 + 16 * n + here(l16), i = token_of_row(row);
+      const bool live = i < sq.n;
+      const int64_t qi = live ? i : 0, h = live ? row - i * a.H : 0;
+      const _Float16* x = a.q + b * a.q_sb + qi * a.q_st + h * a.q_sh + 8 * g16;
+      const _Float16* xr = a.qr + b * a.qr_sb + qi * a.qr_st + h * a.qr_sh + 8 * g16;
 #pragma unroll
       for (int s = 0; s < NQ; ++s) qf[n][s] = *reinterpret_cast<const f16x8*>(32 * s < RANK ? x + 32 * s : xr + 32 * s - RANK);
     }
+#pragma unroll
+    for (int s = 0; s < NQ; ++s) asm volatile("" : "+v"(qf[0][s]), "+v"(qf[1][s]));  // waits here: in the loop it would for the page on its way
     f32x16 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int x = 0; x < 16; ++x) o[dt][x] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // of rows l16 and 16 + l16; l: of this lane's tokens
-    __syncthreads();
     if (part == 0 && half == 0) s_ref[rg][col] = -INFINITY;
 
     for (int p = p0; p < p1; ++p) {
       const int buf = BUFS == 1 ? 0 : (p - p0) & 1;
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      dma_wait();
       __syncthreads();  // the page is there, and the other buffer is read
       if (BUFS == 2 && p + 1 < p1) load(p + 1, buf ^ 1);
       const bool edge = (p + 1) * kPage > sq.ctx;  // some tokens are new or do not exist
@@ -214,8 +223,8 @@ __global__ __launch_bounds__(RG * kSplit * 64, 2) void latent_kernel(LatentArgs 
         // What a row does not attend must not meet its weight of 0: such tokens become
         // zeros, and the rows that attend them NaN.
         constexpr int PER = WAVES * 64 / kPage;  // threads of a token
-        const int t = threadIdx.x / PER;
-        uint8_t* x = s_mem + buf * BUF + t * 128 + (threadIdx.x % PER) * (128 / PER);
+        const int th = here(threadIdx.x), t = th / PER;
+        uint8_t* x = s_mem + buf * BUF + t * 128 + (th % PER) * (128 / PER);
         uint32_t found = 0;
         if (p * kPage + t >= sq.ctx && p * kPage + t < total)
           for (int s = 0; s < NS; ++s)
@@ -249,16 +258,26 @@ __global__ __launch_bounds__(RG * kSplit * 64, 2) void latent_kernel(LatentArgs 
 #pragma unroll
         for (int n = 0; n < 2; ++n) sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[n][s], sc[n], 0, 0, 0);
       }
+      // kAhead operands on their way at a time
+      constexpr int kAhead = 4;
+      __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+      for (int x = 0; x < NQ - kAhead; ++x) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 2 * kAhead, 0);
       // sc[n][e]: row 16 n + l16, token 16 part + 4 g16 + e
       float mx[2];
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         uint32_t seen = 15;
         if (edge) {
-          const int j0 = p * kPage + 16 * part + 4 * g16 - sq.ctx;
+          const int ln = here(lane), j0 = p * kPage + 16 * part + 4 * (ln / 16) - sq.ctx;
+          const int i = min(token_of_row(row0 + 16 * n + ln % 16), sq.n - 1);
           seen = 0;
           if (a.mask) {
-            const uint8_t* mask = a.mask + b * a.m_sb + qi[n] * a.m_si;
+            const uint8_t* mask = a.mask + b * a.m_sb + max(i, 0) * a.m_si;
             uint8_t keep[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) keep[e] = mask[min(max(j0 + e, 0), a.T - 1) * a.m_sj];
@@ -266,7 +285,7 @@ __global__ __launch_bounds__(RG * kSplit * 64, 2) void latent_kernel(LatentArgs 
             for (int e = 0; e < 4; ++e) seen |= static_cast<uint32_t>(j0 + e < 0 || (j0 + e < sq.n && keep[e] != 0)) << e;
           } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) seen |= static_cast<uint32_t>(j0 + e <= min(qi[n], sq.n - 1)) << e;
+            for (int e = 0; e < 4; ++e) seen |= static_cast<uint32_t>(j0 + e <= i) << e;
           }
         }
         mx[n] = -INFINITY;
@@ -283,6 +302,7 @@ __global__ __launch_bounds__(RG * kSplit * 64, 2) void latent_kernel(LatentArgs 
       // Weights relative to the reference as it is.  They round to fp16 for the product (a
       // relative 2^-12 on average); their sum stays in fp32.
       float add[2];
+      const int ln = here(lane), p_write = (ln & 15) * kPage + (((2 * part + ln / 32) ^ (ln & 7)) * 8) + (ln / 16 & 1) * 4;
       auto weigh = [&] {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
@@ -295,8 +315,7 @@ __global__ __launch_bounds__(RG * kSplit * 64, 2) void latent_kernel(LatentArgs 
             add[n] += w;
             w4[e] = static_cast<_Float16>(w);
           }
-          const int u = 2 * part + g16 / 2;
-          *reinterpret_cast<f16x4*>(&s_p[rg][(16 * n + l16) * kPage + ((u ^ (l16 & 7)) * 8) + 4 * (g16 & 1)]) = w4;
+          *reinterpret_cast<f16x4*>(&s_p[rg][p_write + 16 * n * kPage]) = w4;
         }
       };
       weigh();
@@ -305,21 +324,22 @@ __global__ __launch_bounds__(RG * kSplit * 64, 2) void latent_kernel(LatentArgs 
       bool moves = false;
 #pragma unroll
       for (int r = 0; r < RG; ++r) {
-        const int k = 2 * half;
-        moves = moves || fmaxf(s_max[r][k][col], s_max[r][k + 1][col]) > s_ref[r][col] + kAbove;
+        const int k = 2 * (ln / 32), c = ln & 31;
+        moves = moves || fmaxf(s_max[r][k][c], s_max[r][k + 1][c]) > s_ref[r][c] + kAbove;
       }
       if (__any(moves)) {
-        float top = s_max[rg][0][col];
+        const int c = here(col);
+        float top = s_max[rg][0][c];
 #pragma unroll
-        for (int k = 1; k < kSplit; ++k) top = fmaxf(top, s_max[rg][k][col]);
-        const float old = s_ref[rg][col], ref = fmaxf(old, top - kBelow);
+        for (int k = 1; k < kSplit; ++k) top = fmaxf(top, s_max[rg][k][c]);
+        const float old = s_ref[rg][c], ref = fmaxf(old, top - kBelow);
         const float alpha = old == -INFINITY ? 0.f : exp2_of(old - ref);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
           for (int x = 0; x < 16; ++x) o[dt][x] *= alpha;
         __syncthreads();  // the old references and the weights are read
-        if (part == 0 && half == 0) s_ref[rg][col] = ref;
+        if (part == 0 && half == 0) s_ref[rg][c] = ref;
         const float r0 = __shfl(ref, l16, 64), r1 = __shfl(ref, 16 + l16, 64);
         l[0] *= m[0] == -INFINITY ? 0.f : exp2_of(m[0] - r0);
         l[1] *= m[1] == -INFINITY ? 0.f : exp2_of(m[1] - r1);
@@ -328,12 +348,15 @@ __global__ __launch_bounds__(RG * kSplit * 64, 2) void latent_kernel(LatentArgs 
         __syncthreads();
       }
       l[0] += add[0], l[1] += add[1];
+      const int v_at[2] = {buf * BUF + v_lane, (buf * BUF + v_lane) ^ 64};
+      const int p_read = (ln & 31) * kPage + ((ln / 32) ^ (ln & 7)) * 8;
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        const f16x8 w = *reinterpret_cast<const f16x8*>(&s_p[rg][col * kPage + (((2 * s + half) ^ (col & 7)) * 8)]);
+        const f16x8 w = *reinterpret_cast<const f16x8*>(&s_p[rg][p_read ^ (16 * s)]);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          const s16x4 lo = tr(buf * BUF + v_off(dt, 16 * s)), hi = tr(buf * BUF + v_off(dt, 16 * s + 4));
+          const int at = dt / 2 * kStick + 16 * s * 128;
+          const s16x4 lo = tr(v_at[dt & 1] + at), hi = tr(v_at[(dt & 1) ^ 1] + at + 4 * 128);
           o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
               __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), w, o[dt], 0, 0, 0);
         }
@@ -345,10 +368,12 @@ __global__ __launch_bounds__(RG * kSplit * 64, 2) void latent_kernel(LatentArgs 
     }
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
+      const int r = 16 * n + here(l16);
+      const bool live = token_of_row(row0 + r) < sq.n;
       l[n] = xor32_sum(xor16_sum(l[n]));
-      if (!live[n]) l[n] = 0.f;
-      if ((pages.poisoned || sq.bad) && live[n]) l[n] = NAN;
-      if (g16 == n) s_sum[rg][part][16 * n + l16] = l[n];
+      if (!live) l[n] = 0.f;
+      if ((pages.poisoned || sq.bad) && live) l[n] = NAN;
+      if (g16 == n) s_sum[rg][part][r] = l[n];
     }
     __syncthreads();
     float L = 0.f;

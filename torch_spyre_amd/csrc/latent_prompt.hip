@@ -18,6 +18,7 @@
 #include <cmath>
 
 #include "fast_div.h"
+#include "lds_dma.h"
 #include "page_walk.h"
 #include "spyre_common.h"
 
@@ -30,7 +31,6 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __amdgpu_buffer_rsrc_t Rsrc;
 
 constexpr int kRope = 64;
 constexpr int kRows = 32;      // query rows of a wavefront
@@ -89,23 +89,20 @@ __global__ __launch_bounds__(W * 64, W / 4) void prompt_kernel(PromptArgs a) {
   const int all = min(ctx + block0 + 1, total);
   const int tiles = (most + kKeys - 1) / kKeys;
 
+  const uint32_t lds0 = lds_address(s_mem);
   auto load = [&](int t, int buf) {
     const int64_t t0 = static_cast<int64_t>(t) * kKeys;
     const int left = total - t * kKeys;
-    auto rsrc = [](const _Float16* p) {
-      return __builtin_amdgcn_make_buffer_rsrc(const_cast<_Float16*>(p), 0, kNoWhere, 0x00020000);
-    };
-    const Rsrc rk = rsrc(a.k + b * a.k_sb + h * a.k_sh + t0 * a.k_st), rr = rsrc(a.kr + b * a.kr_sb + t0 * a.kr_st),
-               rv = rsrc(a.v + b * a.v_sb + h * a.v_sh + t0 * a.v_st);
+    const dma_rsrc rk = dma_buffer(a.k + b * a.k_sb + h * a.k_sh + t0 * a.k_st, kNoWhere),
+                   rr = dma_buffer(a.kr + b * a.kr_sb + t0 * a.kr_st, kNoWhere),
+                   rv = dma_buffer(a.v + b * a.v_sb + h * a.v_sh + t0 * a.v_st, kNoWhere);
 #pragma unroll
     for (int c = 0; c < (KS + VS) * 8 / W; ++c) {
-      const int chunk = c * W + wave, stick = chunk / 8;  // 8 tokens of a stick (a wavefront's chunks: one tokens' place)
+      const int chunk = c * W + wave, stick = c * W / 8;  // 8 tokens of a stick
       const int tok = (chunk & 7) * 8 + lane / 8;
-      const int unit = ((lane & 7) ^ key_of(tok)) * 16;
-      uint8_t* dst = s_mem + buf * TILE + chunk * 1024;
-      auto go = [&](Rsrc r, int64_t st, int feature) {
-        const int off = tok < left ? tok * static_cast<int>(st) * 2 + feature * 2 + unit : kNoWhere;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)dst, 16, off, 0, 0, 0);
+      const uint32_t unit = ((lane & 7) ^ key_of(tok)) * 16;
+      auto go = [&](dma_rsrc r, int64_t st, int feature) {
+        dma16(r, lds0 + buf * TILE + chunk * 1024, tok < left ? tok * static_cast<uint32_t>(st) * 2 + unit : kNoWhere, feature * 2);
       };
       if (stick < D / 64)
         go(rk, a.k_st, stick * 64);
@@ -115,6 +112,7 @@ __global__ __launch_bounds__(W * 64, W / 4) void prompt_kernel(PromptArgs a) {
         go(rv, a.v_st, (stick - KS) * 64);
     }
   };
+  static_assert(W == 4 || W == 8, "a step of the workgroup's chunks lies in one stick");
   static_assert((KS + VS) * 8 % W == 0, "equal shares of a tile's chunks");
   if (tiles) load(0, 0);
 
@@ -125,17 +123,17 @@ __global__ __launch_bounds__(W * 64, W / 4) void prompt_kernel(PromptArgs a) {
     const _Float16* xr = a.qr + b * a.qr_sb + qi * a.qr_st + h * a.qr_sh + 8 * half;
 #pragma unroll
     for (int s = 0; s < NQ; ++s) qf[s] = *reinterpret_cast<const f16x8*>(16 * s < D ? x + 16 * s : xr + 16 * s - D);
+#pragma unroll
+    for (int s = 0; s < NQ; ++s) asm volatile("" : "+v"(qf[s]));  // waits here: in the loop it would for the tile on its way
   }
   const int k_tok = token_of(col);
   int k_off[4];
 #pragma unroll
   for (int u = 0; u < 4; ++u) k_off[u] = k_tok * 128 + (((2 * u + half) ^ key_of(k_tok)) * 16);
-  // V^T: 4 features of token tv (and 4 tokens further)
+  // V^T: 4 features of token 16 half + lane % 16 / 4; the key of tokens 4, 8, 12 and 32 further
+  // is the same, odd tiles turn bit 2 of the unit.
   const int tv = 16 * half + (lane & 15) / 4;
-  auto v_off = [&](int dt, int t) {
-    const int u = 4 * (dt & 1) + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1), tok = tv + t;
-    return (KS + dt / 2) * kStick + tok * 128 + ((u ^ key_of(tok)) * 16) + 8 * (lane & 1);
-  };
+  const int v_lane = KS * kStick + tv * 128 + (((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ key_of(tv)) * 16) + 8 * (lane & 1);
   auto tr = [&](int at) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(s_mem + at));
   };
@@ -149,7 +147,7 @@ __global__ __launch_bounds__(W * 64, W / 4) void prompt_kernel(PromptArgs a) {
 
   for (int t = 0; t < tiles; ++t) {
     const int buf = t & 1, t0 = t * kKeys;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    dma_wait();
     __syncthreads();  // the tile is there, and the other one is read
     if (t + 1 < tiles) load(t + 1, buf ^ 1);
     const bool edge = t0 + kKeys > all;  // some rows do not attend some of its keys
@@ -186,18 +184,26 @@ __global__ __launch_bounds__(W * 64, W / 4) void prompt_kernel(PromptArgs a) {
     }
     if (t0 >= mine) continue;  // none of its rows' keys (the barriers above are all of a step's)
 
+    f32x16 s16[2] = {};
+#pragma unroll
+    for (int s = 0; s < NQ; ++s)
+#pragma unroll
+      for (int tb = 0; tb < 2; ++tb) {
+        const f16x8 k = *reinterpret_cast<const f16x8*>(s_mem + buf * TILE + k_off[s % 4] + (s / 4) * kStick + tb * (32 * 128));
+        s16[tb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[s], s16[tb], 0, 0, 0);
+      }
+    // kAhead operands on their way at a time
+    constexpr int kAhead = 6;
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+    for (int x = 0; x < 2 * NQ - kAhead; ++x) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
     float sc[32];
 #pragma unroll
-    for (int tb = 0; tb < 2; ++tb) {
-      f32x16 s16 = {};
-#pragma unroll
-      for (int s = 0; s < NQ; ++s) {
-        const f16x8 k = *reinterpret_cast<const f16x8*>(s_mem + buf * TILE + k_off[s % 4] + (s / 4) * kStick + tb * (32 * 128));
-        s16 = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[s], s16, 0, 0, 0);
-      }
-#pragma unroll
-      for (int x = 0; x < 16; ++x) sc[16 * tb + x] = s16[x];
-    }
+    for (int x = 0; x < 32; ++x) sc[x] = s16[x / 16][x % 16];
     float mx = -INFINITY;
 #pragma unroll
     for (int x = 0; x < 32; ++x) {
@@ -224,6 +230,7 @@ __global__ __launch_bounds__(W * 64, W / 4) void prompt_kernel(PromptArgs a) {
     // Weights round to fp16 for the product (a relative 2^-12 on average); their sum
     // stays in fp32.
     f16x8 w[4];
+    const int v_at[2] = {buf * TILE + v_lane, (buf * TILE + v_lane) ^ 64};
 #pragma unroll
     for (int x = 0; x < 32; ++x) {
       const float e = exp2_of(sc[x] - mu);
@@ -234,8 +241,8 @@ __global__ __launch_bounds__(W * 64, W / 4) void prompt_kernel(PromptArgs a) {
     for (int s = 0; s < 4; ++s)
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        const int at = 32 * (s / 2) + 8 * (s % 2);
-        const s16x4 lo = tr(buf * TILE + v_off(dt, at)), hi = tr(buf * TILE + v_off(dt, at + 4));
+        const int at = v_at[dt & 1] + dt / 2 * kStick + (32 * (s / 2) + 8 * (s % 2)) * 128;
+        const s16x4 lo = tr(at), hi = tr(at + 4 * 128);
         o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
             __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), w[s], o[dt], 0, 0, 0);
       }
