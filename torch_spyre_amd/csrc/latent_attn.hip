@@ -14,18 +14,17 @@
 // them: a page is read once, into LDS, and serves both products of all rows.
 //   S^T[tok, row] = K[tok, :] Q^T[:, row]      K as it lies: rows of features
 //   O^T[d, row] += C^T[d, tok] P^T[tok, row]   C^T by transposing reads of the same rows
-// Four wavefronts have 32 rows.  Each has all of their Q in registers (rank 512: 144
-// of them) and takes the scores of 16 of a page's tokens; the weights meet in LDS, and
-// each then takes all 64 tokens of a quarter of O's features (64 registers).  With
-// O whole in one wavefront (256 registers) two of them do not fit a SIMD, and one
-// spills.  Up to 32 rows a workgroup is four wavefronts with one page in LDS, two
-// workgroups to a compute unit, one of which loads while the other computes; beyond
-// it is eight, 64 rows, and two pages in LDS, the next one on its way.
+// A workgroup has RG x 32 rows (RG 1 up to 32 rows, else 2), 4 RG wavefronts and two
+// pages in LDS.  In the first product a wavefront has 16 x 16 tiles: 32 rows x 16 tokens of a
+// page (RG 1), or 16 rows x 32 tokens (RG 2: half the registers for Q, so that two
+// wavefronts fit a SIMD), with Q in registers.  The weights meet in LDS, and each then takes
+// all 64 tokens of 32 rows x a quarter of O's features, which stay in 64 registers.
 
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "fast_div.h"
 #include "lds_dma.h"
@@ -45,7 +44,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kRope = 64;
 constexpr int kTile = 32;   // rows of a wavefront
-constexpr int kSplit = 4;   // wavefronts that share them
+constexpr int kParts = 4;   // of O's features, one to a wavefront
 constexpr int kStick = kPage * 64 * 2;  // bytes of 64 features of a page
 // The reference of a row's exponents lies kBelow under its largest score (log2
 // units) and moves when a score passes it by kAbove: most pages then leave O as
@@ -122,38 +121,58 @@ __device__ __forceinline__ int here(int x) {
   return x;
 }
 
+__device__ __forceinline__ int uniform_here(int x) {
+  asm volatile("" : "+s"(x));
+  return x;
+}
+
+// Waits until no more than N of the wavefront's loads are on their way.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
 // Rows of a page in LDS are 128 bytes for each stick; unit u (16 bytes) of token t
-// lies at u ^ (t & 7).  Neither 8 lanes that read a unit of 8 tokens nor 16 that read
-// 2 units of 4 tokens, transposed, then meet in a bank.
+// lies at u ^ key(t).  Neither 16 lanes that read a unit of 16 tokens nor 32 that read 4
+// units of 4 tokens, transposed, then meet in one of the 64 banks.
+__device__ __forceinline__ int key_of(int t) { return ((t >> 1) & 1) << 2 | ((t >> 2) & 3); }
+
 template <int RANK, int RG>
-__global__ __launch_bounds__(RG * kSplit * 64, 2) void latent_kernel(LatentArgs a) {
-  constexpr int WAVES = RG * kSplit;
-  constexpr int NS = (RANK + kRope) / 64;  // sticks
-  constexpr int DT = RANK / 32 / kSplit;   // tiles of O of a wavefront
-  constexpr int NQ = (RANK + kRope) / 32;  // operands of Q of 16 rows
+__global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs a) {
+  constexpr int WAVES = RG * kParts;
+  constexpr int ROWS = RG * kTile;
+  constexpr int NS = (RANK + kRope) / 64;     // sticks
+  constexpr int OS = RANK / 64 / kParts;      // sticks of O of a wavefront
+  constexpr int DT = 2 * OS;                  // tiles of it, 32 features each
+  constexpr int NQ = (RANK + kRope) / 32;     // steps of the first product
+  constexpr int NR = RG == 1 ? 2 : 1, TB = RG == 1 ? 1 : 2;  // its tiles of 16 rows, 16 tokens
+  constexpr int TG = 4 / TB;                  // wavefronts that share a row's tokens in it
+  constexpr int NT = 4 * TB;                  // scores of a lane's row
   constexpr int BUF = NS * kStick;
-  constexpr int BUFS = RG == 1 ? 1 : 2;
-  __shared__ __align__(16) uint8_t s_mem[BUFS * BUF];
-  __shared__ __align__(16) _Float16 s_p[RG][kTile * kPage];  // weights: 8 units of 8 tokens a row, unit u at u ^ (row & 7)
-  __shared__ float s_max[RG][kSplit][kTile];                 // of a page's scores
-  __shared__ float s_ref[RG][kTile], s_sum[RG][kSplit][kTile];
+  constexpr int SHARE = 8 * NS / WAVES;       // loads of a wavefront for a page
+  static_assert(ROWS * (RANK + kRope) * 2 <= BUF, "the rows' queries fit a page's buffer");
+  __shared__ __align__(16) uint8_t s_mem[2 * BUF];
+  __shared__ __align__(16) _Float16 s_p[ROWS * kPage];  // weights: 8 units of 8 tokens a row, unit u at u ^ (row / 2 & 7)
+  __shared__ float s_max[TG * ROWS], s_sum[TG * ROWS];  // of a page's scores; of all weights
+  __shared__ float s_ref[ROWS];
   __shared__ uint32_t s_odd[WAVES];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
   const int col = lane & 31, half = lane >> 5, l16 = lane & 15, g16 = lane >> 4;
-  const int rg = wave / kSplit, part = wave % kSplit;
+  const int part = wave % kParts, rg = wave / kParts;  // second product: features, rows 32 rg ..
+  const int tg = wave % TG, rq = wave / TG;            // first: tokens 16 TB tg .., rows 16 NR rq ..
   const uint32_t lds0 = lds_address(s_mem);
   int range, rb;
   place_of(a, range, rb);
   Walk walk;
   if (range >= a.ranges || !walk.start(a, lane, range)) return;
 
-  // Lane offsets: unit g16 (and 4 + g16) of K's row 16 part + l16; 4 features of token
-  // 8 half + l16 / 4 (and 4 tokens further) of C^T's tiles.
-  const int k_tok = 16 * part + l16;
-  const int k_off[2] = {k_tok * 128 + ((g16 ^ (k_tok & 7)) * 16), k_tok * 128 + (((4 + g16) ^ (k_tok & 7)) * 16)};
-  // The unit's key is that of token l16 / 4, its bit 2 turned by odd tiles and by tokens 4
-  // further: two lane offsets, the rest of an address is constant.
-  const int v_lane = DT / 2 * part * kStick + (8 * half + l16 / 4) * 128 + (((2 * (g16 & 1) + ((lane >> 1) & 1)) ^ (l16 / 4)) * 16) + 8 * (lane & 1);
+  // K's row of a lane (16 tokens further its key is the same), units g16 and 4 + g16.  C^T: 4 features
+  // of token 8 half + l16 / 4 of the wavefront's first tile; odd tiles and tokens 4 further turn
+  // the unit's bits 2 and 0.
+  const int k_tok = 16 * TB * tg + l16;
+  const int k_lane = k_tok * 128 + ((g16 ^ key_of(k_tok)) * 16);
+  const int v_tok = 8 * half + l16 / 4;
+  const int v_lane = OS * part * kStick + v_tok * 128 + (((2 * (g16 & 1) + ((lane >> 1) & 1)) ^ key_of(v_tok)) * 16) + 8 * (lane & 1);
   auto tr = [&](int at) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(s_mem + at));
   };
@@ -163,63 +182,117 @@ __global__ __launch_bounds__(RG * kSplit * 64, 2) void latent_kernel(LatentArgs 
     const int b = walk.b;
     const Seq sq = walk.seq;
     const int total = sq.ctx + sq.n;
-    const int row0 = rb * a.block_rows + kTile * rg;
+    const int row0 = rb * a.block_rows;
     // (a workgroup whose rows are all of no new token has nothing to do)
-    const int p0 = pc.page0, p1 = rb * a.block_rows < sq.n * a.H ? pc.page1 : pc.page0;
+    const int p0 = pc.page0, p1 = row0 < sq.n * a.H ? pc.page1 : pc.page0;
     Pages pages(a, b, lane, p0);
 
-    // A page on its way into buffer `buf`; tokens that do not exist as zeros.
-    auto load = [&](int p, int buf) {
-      const dma_rsrc r = dma_buffer(a.pages + pages.at(p) * (NS * (kStick / 2)), BUF);
-      const int n = total - p * kPage;
-      const int t = here(lane) / 8;
-      const uint32_t off = t * 128 + (((lane & 7) ^ t) * 16);
-      // a wavefront's chunks (8 tokens of a stick): the same tokens in every stick, RG 1 two runs of them
-      uint32_t voff[8 / WAVES];
+    // `sticks` sticks of a page from s0 on, on their way into buffer `buf`: of their chunks (8
+    // tokens of a stick) one of SHARES.  Tokens that do not exist are zeros.
+    auto load = [&](int64_t page, int p, int buf, auto sticks, int s0, int share, auto shares) {
+      constexpr int STICKS = decltype(sticks)::value, SHARES = decltype(shares)::value;
+      const dma_rsrc r = dma_buffer(a.pages + page * (NS * (kStick / 2)), BUF);
+      const int t = here(lane) / 8, n = total - p * kPage - 8 * share - t;
+      // a chunk's 8 tokens; in odd chunks the key's bit 1 is set
+      const uint32_t off = t * 128 + (((lane & 7) ^ key_of(t + 8 * share)) * 16);
+      const uint32_t at = uniform_here(s0 * kStick + share * 1024), to = lds0 + buf * BUF + at;
+      auto go = [&](auto whole) {
 #pragma unroll
-      for (int c = 0; c < 8 / WAVES; ++c) voff[c] = (c * WAVES + wave) * 8 + t < n ? off : BUF;
+        for (int c = 0; c < 8 / SHARES; ++c)
 #pragma unroll
-      for (int c = 0; c < NS * 8 / WAVES; ++c) {
-        const int chunk = c * WAVES + wave;
-        dma16(r, lds0 + buf * BUF + chunk * 1024, voff[c % (8 / WAVES)], chunk * 1024);
+          for (int s = 0; s < STICKS; ++s)
+            dma16(r, to + s * kStick + c * SHARES * 1024, decltype(whole)::value || c * SHARES * 8 < n ? off ^ (c * SHARES & 1) * 32 : BUF,
+                  at + s * kStick + c * SHARES * 1024);
+      };
+      if ((p + 1) * kPage <= total)
+        go(std::true_type{});
+      else
+        go(std::false_type{});
+    };
+    typedef std::integral_constant<int, 1> One;
+    typedef std::integral_constant<int, WAVES> Shared;
+    // RG 1: a wavefront loads the sticks of its features, which only it reads in the second
+    // product, and its share of the rotated keys; else one of eight chunks of every stick.
+    auto load_page = [&](int64_t page, int p, int buf) {
+      if constexpr (RG == 1) {
+        load(page, p, buf, std::integral_constant<int, OS>{}, OS * part, 0, One{});
+        load(page, p, buf, One{}, NS - 1, wave, Shared{});
+      } else {
+        load(page, p, buf, std::integral_constant<int, NS>{}, 0, wave, Shared{});
       }
     };
-    static_assert(NS * 8 % WAVES == 0, "equal shares of a page's chunks");
-    if (p0 < p1) load(p0, 0);
-
-    // Queries of rows l16 and 16 + l16 of the tile.  (One that is not there is another's.)
-    f16x8 qf[2][NQ];
+    // Queries, whole rows into the second buffer: the latent features [ROWS][RANK], then the
+    // rotated ones, unit u of row r at u ^ (r & 15), u ^ (r / 2 & 7); rows that are not there
+    // are zeros.
     auto token_of_row = [&](int row) {  // its new token; sq.n or more: none
       return row < a.rows ? static_cast<int>(fdiv(row, a.by_h)) : sq.n;
     };
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int row = row0 + 16 * n + here(l16), i = token_of_row(row);
-      const bool live = i < sq.n;
-      const int64_t qi = live ? i : 0, h = live ? row - i * a.H : 0;
-      const _Float16* x = a.q + b * a.q_sb + qi * a.q_st + h * a.q_sh + 8 * g16;
-      const _Float16* xr = a.qr + b * a.qr_sb + qi * a.qr_st + h * a.qr_sh + 8 * g16;
-#pragma unroll
-      for (int s = 0; s < NQ; ++s) qf[n][s] = *reinterpret_cast<const f16x8*>(32 * s < RANK ? x + 32 * s : xr + 32 * s - RANK);
+    int64_t next = 0;  // the page after the ones on their way
+    if (p0 < p1) {
+#pragma unroll 2
+      for (int k = 0; k < ROWS / WAVES; ++k) {
+        const int r = k * WAVES + wave, row = row0 + r, i = token_of_row(row);
+        const int64_t h = row - i * a.H;
+        const bool there = i < sq.n;
+        if (lane < RANK / 8)
+          dma16(dma_buffer(a.q + (there ? b * a.q_sb + i * a.q_st + h * a.q_sh : 0), RANK * 2), lds0 + BUF + r * RANK * 2,
+                there ? (lane ^ (r & 15)) * 16 : RANK * 2, 0);
+        if (lane < kRope / 8)
+          dma16(dma_buffer(a.qr + (there ? b * a.qr_sb + i * a.qr_st + h * a.qr_sh : 0), kRope * 2),
+                lds0 + BUF + ROWS * RANK * 2 + r * kRope * 2,
+                there ? (lane ^ (r / 2 & 7)) * 16 : kRope * 2, 0);
+      }
+      load_page(pages.at(p0), p0, 0);
+      if (p0 + 1 < p1) next = pages.at(p0 + 1);
+      wait_loads<SHARE>();
     }
+    __syncthreads();
+    f16x8 qf[NR][NQ];
 #pragma unroll
-    for (int s = 0; s < NQ; ++s) asm volatile("" : "+v"(qf[0][s]), "+v"(qf[1][s]));  // waits here: in the loop it would for the page on its way
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int s = 0; s < NQ; ++s) {
+        const int r = 16 * (NR * rq + n) + here(l16);
+        const int at = 32 * s < RANK ? r * RANK * 2 + ((4 * s + g16) ^ (r & 15)) * 16
+                                     : ROWS * RANK * 2 + r * kRope * 2 + ((4 * s - RANK / 8 + g16) ^ (r / 2 & 7)) * 16;
+        qf[n][s] = *reinterpret_cast<const f16x8*>(s_mem + BUF + at);
+      }
+#pragma unroll
+    for (int s = 0; s < NQ; ++s)
+#pragma unroll
+      for (int n = 0; n < NR; ++n) asm volatile("" : "+v"(qf[n][s]));  // they are read
+    if (threadIdx.x < ROWS) s_ref[threadIdx.x] = -INFINITY;
+    if (RG == 1) {
+      __syncthreads();
+      if (p0 + 1 < p1) load_page(next, p0 + 1, 1);
+    }
     f32x16 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int x = 0; x < 16; ++x) o[dt][x] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // of rows l16 and 16 + l16; l: of this lane's tokens
-    if (part == 0 && half == 0) s_ref[rg][col] = -INFINITY;
+    float m[NR], l[NR];  // of a lane's rows in the first product; l: of this lane's tokens
+#pragma unroll
+    for (int n = 0; n < NR; ++n) m[n] = -INFINITY, l[n] = 0.f;
 
-    for (int p = p0; p < p1; ++p) {
-      const int buf = BUFS == 1 ? 0 : (p - p0) & 1;
-      dma_wait();
-      __syncthreads();  // the page is there, and the other buffer is read
-      if (BUFS == 2 && p + 1 < p1) load(p + 1, buf ^ 1);
-      const bool edge = (p + 1) * kPage > sq.ctx;  // some tokens are new or do not exist
-      uint32_t odd = 0;                            // of this wavefront's 16 tokens, new ones that hold a NaN or an infinity
-      if (edge && a.T > 1) {
+    // EDGE: some of the page's tokens are new or do not exist.  (In a copy of its own: its loads of
+    // masks would make every page wait for the ones on their way.)
+    auto step = [&](int p, auto edge_tag) {
+      constexpr bool EDGE = decltype(edge_tag)::value;
+      const int buf = (p - p0) & 1;
+      if (RG == 1 && p + 1 < p1)
+        wait_loads<SHARE>();  // the next page's
+      else
+        wait_loads<0>();
+      __syncthreads();  // the page is there; RG 2: the other buffer is read
+      const bool more = p + (RG == 1 ? 2 : 1) < p1;
+      if (RG == 1 && more) next = pages.at(p + 2);
+      if (RG == 2 && more) {
+        load_page(next, p + 1, buf ^ 1);
+        if (p + 2 < p1) next = pages.at(p + 2);
+      }
+      uint32_t odd = 0;                            // of this wavefront's tokens, new ones that hold a NaN or an infinity
+      if (EDGE && a.T > 1) {
         // What a row does not attend must not meet its weight of 0: such tokens become
         // zeros, and the rows that attend them NaN.
         constexpr int PER = WAVES * 64 / kPage;  // threads of a token
@@ -246,76 +319,100 @@ __global__ __launch_bounds__(RG * kSplit * 64, 2) void latent_kernel(LatentArgs 
         for (int k = 0; k < 64 / PER; ++k) bits |= static_cast<uint32_t>((all >> (PER * k)) & 1) << k;
         if (lane == 0) s_odd[wave] = bits;
         __syncthreads();
-        // wavefront w looked at tokens 64 / PER * w on
-        odd = RG == 1 ? s_odd[part] : s_odd[2 * part] | s_odd[2 * part + 1] << 8;
-        static_assert(RG <= 2, "see odd");
+        // (wavefront w looked at tokens 64 / WAVES w .. )
+        if constexpr (RG == 1) {
+          odd = s_odd[wave];
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) odd |= s_odd[4 * tg + k] << (8 * k);
+        }
       }
 
-      f32x4 sc[2] = {};
+      // The scores: sc[n][x] of row 16 (NR rq + n) + l16, token 16 TB tg + tok(x).
+      float sc[NR][NT];
+      auto tok = [&](int x, int ln) { return 16 * (x / 4) + 4 * (ln / 16) + x % 4; };
+      {
+        const uint8_t* kb = s_mem + buf * BUF;
+        const int k_at[2] = {k_lane, k_lane ^ 64};
+        // kAhead operands on their way; in this order, the scheduler would read each when it is due
+        constexpr int kAhead = 8, NK = NQ * TB;
+        f16x8 kf[kAhead];
+        auto k_of = [&](int x) {
+          const int s = x / TB;
+          return *reinterpret_cast<const f16x8*>(kb + k_at[s % 2] + s / 2 * kStick + x % TB * (16 * 128));
+        };
 #pragma unroll
-      for (int s = 0; s < NQ; ++s) {
-        const f16x8 k = *reinterpret_cast<const f16x8*>(s_mem + buf * BUF + k_off[s % 2] + (s / 2) * kStick);
+        for (int x = 0; x < kAhead; ++x) kf[x] = k_of(x);
+        f32x4 acc[NR][TB] = {};
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int n = 0; n < 2; ++n) sc[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[n][s], sc[n], 0, 0, 0);
+        for (int x = 0; x < NK; ++x) {
+#pragma unroll
+          for (int n = 0; n < NR; ++n)
+            acc[n][x % TB] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[x % kAhead], qf[n][x / TB], acc[n][x % TB], 0, 0, 0);
+          if (x + kAhead < NK) kf[x % kAhead] = k_of(x + kAhead);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int x = 0; x < NT; ++x) sc[n][x] = acc[n][x / 4][x % 4];
       }
-      // kAhead operands on their way at a time
-      constexpr int kAhead = 4;
-      __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+      const int ln = here(lane);
 #pragma unroll
-      for (int x = 0; x < NQ - kAhead; ++x) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x008, 2 * kAhead, 0);
-      // sc[n][e]: row 16 n + l16, token 16 part + 4 g16 + e
-      float mx[2];
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        uint32_t seen = 15;
-        if (edge) {
-          const int ln = here(lane), j0 = p * kPage + 16 * part + 4 * (ln / 16) - sq.ctx;
-          const int i = min(token_of_row(row0 + 16 * n + ln % 16), sq.n - 1);
+      for (int n = 0; n < NR; ++n) {
+        uint32_t seen = ~0u;
+        if constexpr (EDGE) {
+          const int j0 = p * kPage + 16 * TB * tg - sq.ctx;
+          const int i = min(token_of_row(row0 + 16 * (NR * rq + n) + ln % 16), sq.n - 1);
           seen = 0;
           if (a.mask) {
             const uint8_t* mask = a.mask + b * a.m_sb + max(i, 0) * a.m_si;
-            uint8_t keep[4];
+            uint8_t keep[NT];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) keep[e] = mask[min(max(j0 + e, 0), a.T - 1) * a.m_sj];
+            for (int x = 0; x < NT; ++x) keep[x] = mask[min(max(j0 + tok(x, ln), 0), a.T - 1) * a.m_sj];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) seen |= static_cast<uint32_t>(j0 + e < 0 || (j0 + e < sq.n && keep[e] != 0)) << e;
+            for (int x = 0; x < NT; ++x) {
+              const int j = j0 + tok(x, ln);
+              seen |= static_cast<uint32_t>(j < 0 || (j < sq.n && keep[x] != 0)) << x;
+            }
           } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) seen |= static_cast<uint32_t>(j0 + e <= i) << e;
+            for (int x = 0; x < NT; ++x) seen |= static_cast<uint32_t>(j0 + tok(x, ln) <= i) << x;
           }
         }
-        mx[n] = -INFINITY;
+        float mx = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = sc[n][e] * a.scale_log2;
-          if (edge) v = !((seen >> e) & 1) ? -INFINITY : (odd >> (4 * g16 + e)) & 1 ? NAN : v;
-          sc[n][e] = v;
-          mx[n] = fmaxf(mx[n], v);
+        for (int x = 0; x < NT; ++x) {
+          float v = sc[n][x] * a.scale_log2;
+          if (EDGE) v = !((seen >> x) & 1) ? -INFINITY : (odd >> tok(x, ln)) & 1 ? NAN : v;
+          sc[n][x] = v;
+          mx = fmaxf(mx, v);
         }
-        mx[n] = xor32_max(xor16_max(mx[n]));
-        if (g16 == n) s_max[rg][part][16 * n + l16] = mx[n];
+        mx = xor32_max(xor16_max(mx));
+        if (ln / 16 == n) s_max[tg * ROWS + 16 * (NR * rq + n) + ln % 16] = mx;
       }
       // Weights relative to the reference as it is.  They round to fp16 for the product (a
       // relative 2^-12 on average); their sum stays in fp32.
-      float add[2];
-      const int ln = here(lane), p_write = (ln & 15) * kPage + (((2 * part + ln / 32) ^ (ln & 7)) * 8) + (ln / 16 & 1) * 4;
+      float add[NR];
       auto weigh = [&] {
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
+        for (int n = 0; n < NR; ++n) {
           const float mu = m[n] == -INFINITY ? 0.f : m[n];  // a row that has attended nothing yet: weights 0
-          f16x4 w4;
           add[n] = 0.f;
+          const int row = 16 * (NR * rq + n) + ln % 16;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float w = exp2_of(sc[n][e] - mu);
-            add[n] += w;
-            w4[e] = static_cast<_Float16>(w);
+          for (int x = 0; x < NT; x += 4) {
+            f16x4 w4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float w = exp2_of(sc[n][x + e] - mu);
+              add[n] += w;
+              w4[e] = static_cast<_Float16>(w);
+            }
+            const int t = 16 * TB * tg + tok(x, ln);  // of 4
+            *reinterpret_cast<f16x4*>(&s_p[row * kPage + (((t / 8) ^ (row / 2 & 7)) * 8) + t % 8]) = w4;
           }
-          *reinterpret_cast<f16x4*>(&s_p[rg][p_write + 16 * n * kPage]) = w4;
         }
       };
       weigh();
@@ -323,65 +420,83 @@ __global__ __launch_bounds__(RG * kSplit * 64, 2) void latent_kernel(LatentArgs 
       // Where a row's scores pass its reference too far, all move.
       bool moves = false;
 #pragma unroll
-      for (int r = 0; r < RG; ++r) {
-        const int k = 2 * (ln / 32), c = ln & 31;
-        moves = moves || fmaxf(s_max[r][k][c], s_max[r][k + 1][c]) > s_ref[r][c] + kAbove;
-      }
+      for (int k = 0; k < 2; ++k) moves = moves || s_max[64 * k + ln] > s_ref[(64 * k + ln) % ROWS] + kAbove;
       if (__any(moves)) {
-        const int c = here(col);
-        float top = s_max[rg][0][c];
+        auto ref_of = [&](int r) {  // a row's new reference
+          float top = s_max[r];
 #pragma unroll
-        for (int k = 1; k < kSplit; ++k) top = fmaxf(top, s_max[rg][k][c]);
-        const float old = s_ref[rg][c], ref = fmaxf(old, top - kBelow);
-        const float alpha = old == -INFINITY ? 0.f : exp2_of(old - ref);
+          for (int k = 1; k < TG; ++k) top = fmaxf(top, s_max[k * ROWS + r]);
+          return fmaxf(s_ref[r], top - kBelow);
+        };
+        auto factor = [](float from, float to) { return from == -INFINITY ? 0.f : exp2_of(from - to); };
+        const int c = kTile * rg + here(col), th = here(threadIdx.x) % ROWS;
+        const float alpha = factor(s_ref[c], ref_of(c)), ref = ref_of(th);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
           for (int x = 0; x < 16; ++x) o[dt][x] *= alpha;
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          const float to = ref_of(16 * (NR * rq + n) + ln % 16);
+          l[n] *= factor(m[n], to);
+          m[n] = to;
+        }
         __syncthreads();  // the old references and the weights are read
-        if (part == 0 && half == 0) s_ref[rg][c] = ref;
-        const float r0 = __shfl(ref, l16, 64), r1 = __shfl(ref, 16 + l16, 64);
-        l[0] *= m[0] == -INFINITY ? 0.f : exp2_of(m[0] - r0);
-        l[1] *= m[1] == -INFINITY ? 0.f : exp2_of(m[1] - r1);
-        m[0] = r0, m[1] = r1;
+        if (threadIdx.x < ROWS) s_ref[th] = ref;
         weigh();
         __syncthreads();
       }
-      l[0] += add[0], l[1] += add[1];
+#pragma unroll
+      for (int n = 0; n < NR; ++n) l[n] += add[n];
       const int v_at[2] = {buf * BUF + v_lane, (buf * BUF + v_lane) ^ 64};
-      const int p_read = (ln & 31) * kPage + ((ln / 32) ^ (ln & 7)) * 8;
+      // RG 1: sticks that no wavefront reads any more take the page after the next.
+      if (RG == 1 && more) load(next, p + 2, buf, One{}, NS - 1, wave, Shared{});
+      f16x8 w[4];
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const f16x8 w = *reinterpret_cast<const f16x8*>(&s_p[rg][p_read ^ (16 * s)]);
+      for (int s = 0; s < 4; ++s) w[s] = *reinterpret_cast<const f16x8*>(&s_p[(kTile * rg + ln % 32) * kPage + (((2 * s + ln / 32) ^ (ln / 2 & 7)) * 8)]);
+      // Operand x of C^T: stick x / 8 of the wavefront, tokens 16 (x / 2 % 4) .. + 15, tile x % 2
+      // of the stick.
+      constexpr int kAhead = 6, NV = 8 * OS;
+      f16x8 vf[kAhead];
+      auto v_of = [&](int x) {
+        const int at = x / 8 * kStick + x / 2 % 4 * 16 * 128;
+        const s16x4 lo = tr(v_at[x & 1] + at), hi = tr((v_at[x & 1] ^ 16) + at + 4 * 128);
+        return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      };
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          const int at = dt / 2 * kStick + 16 * s * 128;
-          const s16x4 lo = tr(v_at[dt & 1] + at), hi = tr(v_at[(dt & 1) ^ 1] + at + 4 * 128);
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-              __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), w, o[dt], 0, 0, 0);
-        }
+      for (int x = 0; x < kAhead; ++x) vf[x] = v_of(x);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int x = 0; x < NV; ++x) {
+        f32x16& y = o[x / 8 * 2 + x % 2];
+        y = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[x % kAhead], w[x / 2 % 4], y, 0, 0, 0);
+        if (x + kAhead < NV) vf[x % kAhead] = v_of(x + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
+        // RG 1: a stick is read: this wavefront alone reads it, in this product
+        if (RG == 1 && x % 8 == 7 && more) load(next, p + 2, buf, One{}, OS * part + x / 8, 0, One{});
       }
-      if (BUFS == 1) {
-        __syncthreads();
-        if (p + 1 < p1) load(p + 1, 0);
-      }
-    }
+    };
+    // Every row attends every token below ctx.
+    const int whole = min(max(sq.ctx / kPage, p0), p1);
+    for (int p = p0; p < whole; ++p) step(p, std::false_type{});
+    for (int p = whole; p < p1; ++p) step(p, std::true_type{});
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int r = 16 * n + here(l16);
+    for (int n = 0; n < NR; ++n) {
+      const int r = 16 * (NR * rq + n) + here(l16);
       const bool live = token_of_row(row0 + r) < sq.n;
       l[n] = xor32_sum(xor16_sum(l[n]));
       if (!live) l[n] = 0.f;
       if ((pages.poisoned || sq.bad) && live) l[n] = NAN;
-      if (g16 == n) s_sum[rg][part][r] = l[n];
+      if (g16 == n) s_sum[tg * ROWS + r] = l[n];
     }
     __syncthreads();
+    const int out_row = kTile * rg + col;
     float L = 0.f;
 #pragma unroll
-    for (int k = 0; k < kSplit; ++k) L += s_sum[rg][k][col];
-    const float M = L == 0.f ? -INFINITY : s_ref[rg][col];
-    if (row0 + col < a.rows) {
-      const int64_t at = partial_of(a, range, rb, pc.slot, kTile * rg + col);
+    for (int k = 0; k < TG; ++k) L += s_sum[k * ROWS + out_row];
+    const float M = L == 0.f ? -INFINITY : s_ref[out_row];
+    if (row0 + out_row < a.rows) {
+      const int64_t at = partial_of(a, range, rb, pc.slot, out_row);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -389,7 +504,7 @@ __global__ __launch_bounds__(RG * kSplit * 64, 2) void latent_kernel(LatentArgs 
           const f32x4 y = {o[dt][4 * x], o[dt][4 * x + 1], o[dt][4 * x + 2], o[dt][4 * x + 3]};
           const int d = 32 * (DT * part + dt) + 8 * x + 4 * half;
           if (pc.whole)
-            store_row4<RANK>(a, b, row0 + col, d, y, M, L);
+            store_row4<RANK>(a, b, row0 + out_row, d, y, M, L);
           else
             *reinterpret_cast<f32x4*>(a.ws + at * RANK + d) = y;
         }
@@ -445,7 +560,7 @@ Plan plan_of(int B, int T, int H, int rank, int max_tokens) {
   p.width = static_cast<int>(std::min<int64_t>(p.block_rows, rows));
   p.min_per = 2, p.min_cut = 4;
   const int64_t pages = std::max(pages_of(max_tokens), 1), parts_of_one = pages < p.min_cut ? 1 : pages / p.min_per;
-  const int64_t ranges = std::min(B * parts_of_one, std::max<int64_t>((p.groups == 1 ? 512 : 256) / p.row_blocks, 1));
+  const int64_t ranges = std::min(B * parts_of_one, std::max<int64_t>(256 / p.row_blocks, 1));
   p.ranges = static_cast<int>(std::max<int64_t>(ranges, 1));
   p.ws_bytes = static_cast<size_t>(p.ranges) * p.row_blocks * 2 * p.width * (rank + 2) * 4;
   return p;
@@ -461,9 +576,9 @@ bool sizes_ok(int B, int T, int H, int max_ctx) {
 template <int RANK>
 void launch(const LatentArgs& a, int groups, dim3 grid, hipStream_t st) {
   if (groups == 1)
-    latent_kernel<RANK, 1><<<grid, kSplit * 64, 0, st>>>(a);
+    latent_kernel<RANK, 1><<<grid, kParts * 64, 0, st>>>(a);
   else
-    latent_kernel<RANK, 2><<<grid, 2 * kSplit * 64, 0, st>>>(a);
+    latent_kernel<RANK, 2><<<grid, 2 * kParts * 64, 0, st>>>(a);
 }
 
 }  // namespace
