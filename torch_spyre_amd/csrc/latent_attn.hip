@@ -63,19 +63,21 @@ struct LatentArgs {
   float* ws;
   int B, T, H, Hkv, rows, max_ctx, draft_keys;
   float scale_log2;
-  int row_blocks, block_rows, width;
+  int row_blocks, block_rows;
   int ranges, min_per, min_cut, each;  // see PageWalk
   FastDiv by_h, by_hkv, by_blocks, by_ranges;
 };
 typedef PageWalk<LatentArgs> Walk;
 
-// Partials: O [slots][width][rank], then (m, l) [slots][width]; slots are (range,
-// row block, slot 0 / 1).
-__device__ __forceinline__ int64_t partial_of(const LatentArgs& a, int range, int rb, int slot, int row) {
-  return ((static_cast<int64_t>(range) * a.row_blocks + rb) * 2 + slot) * a.width + row;
-}
-__device__ __forceinline__ int64_t partials(const LatentArgs& a) {
-  return static_cast<int64_t>(a.ranges) * a.row_blocks * 2 * a.width;
+// The parts of a sequence that several ranges share, joined by a second kernel (in this
+// one, by the last workgroup to arrive, each step of the exchange is a way to memory and
+// back: 8 us more for one short sequence, 60 for 32 x 4 parts of 128 rows).  Slot
+// (range, row block, 0 / 1) of the workspace holds a part: O as the wavefronts' registers
+// have it, [wave][tile, 4 features][lane] of 4 floats, so that stores and loads are whole
+// lines, then (m, l) of its rows.
+__host__ __device__ constexpr int64_t slot_floats(int rows, int rank) { return static_cast<int64_t>(rows) * (rank + 2); }
+__device__ __forceinline__ float* slot_of(const LatentArgs& a, int range, int rb, int slot, int rank) {
+  return a.ws + ((static_cast<int64_t>(range) * a.row_blocks + rb) * 2 + slot) * slot_floats(a.block_rows, rank);
 }
 
 // 4 features of a finished row.
@@ -133,9 +135,12 @@ __device__ __forceinline__ void wait_loads() {
 }
 
 // Rows of a page in LDS are 128 bytes for each stick; unit u (16 bytes) of token t
-// lies at u ^ key(t).  Neither 16 lanes that read a unit of 16 tokens nor 32 that read 4
-// units of 4 tokens, transposed, then meet in one of the 64 banks.
-__device__ __forceinline__ int key_of(int t) { return ((t >> 1) & 1) << 2 | ((t >> 2) & 3); }
+// lies at u ^ key(t).  Of the keys that are linear in t's bits this is the simplest with which
+// neither the reads of K's rows (16 tokens x 4 units) nor the transposing ones (4 tokens x 4
+// units twice) meet in a bank: 4 and 2 cycles a read (measured; t & 7: 4 and 4).
+__device__ __forceinline__ int key_of(int t) { return (t & 2) << 1 | (t & 4) >> 1; }
+// That of the weights' rows, whose reads are 32 rows x 2 units.
+__device__ __forceinline__ int row_key(int r) { return (r & 2) << 1 | ((r >> 2) & 3); }
 
 template <int RANK, int RG>
 __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs a) {
@@ -152,7 +157,7 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
   constexpr int SHARE = 8 * NS / WAVES;       // loads of a wavefront for a page
   static_assert(ROWS * (RANK + kRope) * 2 <= BUF, "the rows' queries fit a page's buffer");
   __shared__ __align__(16) uint8_t s_mem[2 * BUF];
-  __shared__ __align__(16) _Float16 s_p[ROWS * kPage];  // weights: 8 units of 8 tokens a row, unit u at u ^ (row / 2 & 7)
+  __shared__ __align__(16) _Float16 s_p[ROWS * kPage];  // weights: 8 units of 8 tokens a row, unit u at u ^ row_key
   __shared__ float s_max[TG * ROWS], s_sum[TG * ROWS];  // of a page's scores; of all weights
   __shared__ float s_ref[ROWS];
   __shared__ uint32_t s_odd[WAVES];
@@ -168,7 +173,7 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
 
   // K's row of a lane (16 tokens further its key is the same), units g16 and 4 + g16.  C^T: 4 features
   // of token 8 half + l16 / 4 of the wavefront's first tile; odd tiles and tokens 4 further turn
-  // the unit's bits 2 and 0.
+  // the unit's bits 2 and 1.
   const int k_tok = 16 * TB * tg + l16;
   const int k_lane = k_tok * 128 + ((g16 ^ key_of(k_tok)) * 16);
   const int v_tok = 8 * half + l16 / 4;
@@ -193,15 +198,14 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
       constexpr int STICKS = decltype(sticks)::value, SHARES = decltype(shares)::value;
       const dma_rsrc r = dma_buffer(a.pages + page * (NS * (kStick / 2)), BUF);
       const int t = here(lane) / 8, n = total - p * kPage - 8 * share - t;
-      // a chunk's 8 tokens; in odd chunks the key's bit 1 is set
-      const uint32_t off = t * 128 + (((lane & 7) ^ key_of(t + 8 * share)) * 16);
+      const uint32_t off = t * 128 + (((lane & 7) ^ key_of(t)) * 16);
       const uint32_t at = uniform_here(s0 * kStick + share * 1024), to = lds0 + buf * BUF + at;
       auto go = [&](auto whole) {
 #pragma unroll
         for (int c = 0; c < 8 / SHARES; ++c)
 #pragma unroll
           for (int s = 0; s < STICKS; ++s)
-            dma16(r, to + s * kStick + c * SHARES * 1024, decltype(whole)::value || c * SHARES * 8 < n ? off ^ (c * SHARES & 1) * 32 : BUF,
+            dma16(r, to + s * kStick + c * SHARES * 1024, decltype(whole)::value || c * SHARES * 8 < n ? off : BUF,
                   at + s * kStick + c * SHARES * 1024);
       };
       if ((p + 1) * kPage <= total)
@@ -411,7 +415,7 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
               w4[e] = static_cast<_Float16>(w);
             }
             const int t = 16 * TB * tg + tok(x, ln);  // of 4
-            *reinterpret_cast<f16x4*>(&s_p[row * kPage + (((t / 8) ^ (row / 2 & 7)) * 8) + t % 8]) = w4;
+            *reinterpret_cast<f16x4*>(&s_p[row * kPage + (((t / 8) ^ row_key(row)) * 8) + t % 8]) = w4;
           }
         }
       };
@@ -453,14 +457,14 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
       if (RG == 1 && more) load(next, p + 2, buf, One{}, NS - 1, wave, Shared{});
       f16x8 w[4];
 #pragma unroll
-      for (int s = 0; s < 4; ++s) w[s] = *reinterpret_cast<const f16x8*>(&s_p[(kTile * rg + ln % 32) * kPage + (((2 * s + ln / 32) ^ (ln / 2 & 7)) * 8)]);
+      for (int s = 0; s < 4; ++s) w[s] = *reinterpret_cast<const f16x8*>(&s_p[(kTile * rg + ln % 32) * kPage + (((2 * s + ln / 32) ^ row_key(ln)) * 8)]);
       // Operand x of C^T: stick x / 8 of the wavefront, tokens 16 (x / 2 % 4) .. + 15, tile x % 2
       // of the stick.
       constexpr int kAhead = 6, NV = 8 * OS;
       f16x8 vf[kAhead];
       auto v_of = [&](int x) {
         const int at = x / 8 * kStick + x / 2 % 4 * 16 * 128;
-        const s16x4 lo = tr(v_at[x & 1] + at), hi = tr((v_at[x & 1] ^ 16) + at + 4 * 128);
+        const s16x4 lo = tr(v_at[x & 1] + at), hi = tr((v_at[x & 1] ^ 32) + at + 4 * 128);
         return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
       };
 #pragma unroll
@@ -495,21 +499,25 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
 #pragma unroll
     for (int k = 0; k < TG; ++k) L += s_sum[k * ROWS + out_row];
     const float M = L == 0.f ? -INFINITY : s_ref[out_row];
-    if (row0 + out_row < a.rows) {
-      const int64_t at = partial_of(a, range, rb, pc.slot, out_row);
+    if (pc.whole) {
+      if (row0 + out_row < a.rows)
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const f32x4 y = {o[dt][4 * x], o[dt][4 * x + 1], o[dt][4 * x + 2], o[dt][4 * x + 3]};
-          const int d = 32 * (DT * part + dt) + 8 * x + 4 * half;
-          if (pc.whole)
-            store_row4<RANK>(a, b, row0 + out_row, d, y, M, L);
-          else
-            *reinterpret_cast<f32x4*>(a.ws + at * RANK + d) = y;
-        }
-      if (!pc.whole && part == 0 && half == 0) {
-        float* ml = a.ws + partials(a) * RANK + at * 2;
+          for (int x = 0; x < 4; ++x)
+            store_row4<RANK>(a, b, row0 + out_row, 32 * (DT * part + dt) + 8 * x + 4 * half,
+                             f32x4{o[dt][4 * x], o[dt][4 * x + 1], o[dt][4 * x + 2], o[dt][4 * x + 3]}, M, L);
+    } else {
+      float* slot = slot_of(a, range, rb, pc.slot, RANK);
+      if (row0 + out_row < a.rows)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            *reinterpret_cast<f32x4*>(slot + ((wave * DT + dt) * 4 + x) * 256 + lane * 4) =
+              f32x4{o[dt][4 * x], o[dt][4 * x + 1], o[dt][4 * x + 2], o[dt][4 * x + 3]};
+      if (part == 0 && half == 0) {
+        float* ml = slot + ROWS * RANK + out_row * 2;
         ml[0] = M, ml[1] = L;
       }
     }
@@ -518,36 +526,39 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
   }
 }
 
-// Joins the partials of each sequence that several ranges share: a thread 4
-// features of a row.
-template <int RANK>
+// Joins the parts of each sequence that several ranges share: a thread 4 features of a
+// row, numbered as they lie in a slot.
+template <int RANK, int RG>
 __global__ __launch_bounds__(256) void latent_join_kernel(LatentArgs a) {
+  constexpr int ROWS = RG * kTile, DT = RANK / 32 / kParts;
   const int b = blockIdx.x;
   Walk w;
   w.seek(a, threadIdx.x % 64, b);
   int r0, r1;
   w.parts_of(a, 0, r0, r1);
   if (r1 <= r0) return;
-  const Seq sq = w.seq;
-  for (int64_t u = blockIdx.y * 256 + threadIdx.x; u < static_cast<int64_t>(a.rows) * (RANK / 4); u += gridDim.y * 256) {
-    const int row = static_cast<int>(u / (RANK / 4)), d = 4 * static_cast<int>(u % (RANK / 4));
-    const int rb = row / a.block_rows, rl = row - rb * a.block_rows;
+  const int live = w.seq.n * a.H;
+  for (int64_t u = blockIdx.y * 256 + threadIdx.x; u < static_cast<int64_t>(a.row_blocks) * (ROWS * RANK / 4); u += gridDim.y * 256) {
+    const int rb = static_cast<int>(u / (ROWS * RANK / 4)), at = static_cast<int>(u % (ROWS * RANK / 4)), lane = at % 64;
+    const int wave = at / (DT * 256), tile = wave % kParts * DT + at / 256 % DT;
+    const int r = wave / kParts * kTile + lane % 32, row = rb * ROWS + r;
+    if (row >= a.rows) continue;
     float M = -INFINITY, L = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    if (row < sq.n * a.H)
-      merge_parts(r0, r1, M, L, acc, [&](int r, float& m, float& l, f32x4& x) {
-        const int64_t part = partial_of(a, r, rb, r == r0 ? 1 : 0, rl);
-        const float* ml = a.ws + partials(a) * RANK + part * 2;
+    if (row < live)
+      merge_parts(r0, r1, M, L, acc, [&](int p, float& m, float& l, f32x4& x) {
+        const float* slot = slot_of(a, p, rb, p == r0 ? 1 : 0, RANK);
+        const float* ml = slot + ROWS * RANK + r * 2;
         m = ml[0], l = ml[1];
-        x = *reinterpret_cast<const f32x4*>(a.ws + part * RANK + d);
+        x = *reinterpret_cast<const f32x4*>(slot + at * 4);
       });
-    store_row4<RANK>(a, b, row, d, acc, M, L);
+    store_row4<RANK>(a, b, row, 32 * tile + 8 * (at / 64 % 4) + 4 * (lane / 32), acc, M, L);
   }
 }
 
 struct Plan {
   int groups;  // RG
-  int row_blocks, block_rows, width, ranges, min_per, min_cut;
+  int row_blocks, block_rows, ranges, min_per, min_cut;
   size_t ws_bytes;
 };
 
@@ -557,12 +568,11 @@ Plan plan_of(int B, int T, int H, int rank, int max_tokens) {
   p.groups = rows <= kTile ? 1 : 2;
   p.block_rows = kTile * p.groups;
   p.row_blocks = static_cast<int>((rows + p.block_rows - 1) / p.block_rows);
-  p.width = static_cast<int>(std::min<int64_t>(p.block_rows, rows));
   p.min_per = 2, p.min_cut = 4;
   const int64_t pages = std::max(pages_of(max_tokens), 1), parts_of_one = pages < p.min_cut ? 1 : pages / p.min_per;
   const int64_t ranges = std::min(B * parts_of_one, std::max<int64_t>(256 / p.row_blocks, 1));
   p.ranges = static_cast<int>(std::max<int64_t>(ranges, 1));
-  p.ws_bytes = static_cast<size_t>(p.ranges) * p.row_blocks * 2 * p.width * (rank + 2) * 4;
+  p.ws_bytes = p.ranges == 1 ? 0 : static_cast<size_t>(p.ranges) * p.row_blocks * 2 * slot_floats(p.block_rows, rank) * 4;
   return p;
 }
 
@@ -609,7 +619,7 @@ extern "C" int spyre_paged_latent_attn(const void* q, const int64_t* q_strides, 
   for (int i = 0; i < 3; ++i)
     SPYRE_REQUIRE(q_strides[i] % 8 == 0 && q_rope_strides[i] % 8 == 0, SPYRE_EINVAL, "q strides must be multiples of 8 elements");
   const Plan p = plan_of(B, T, H, rank, max_context_len + T);
-  SPYRE_REQUIRE(workspace && workspace_bytes >= p.ws_bytes && aligned(workspace), SPYRE_ENOSPC,
+  SPYRE_REQUIRE(p.ws_bytes == 0 || (workspace && workspace_bytes >= p.ws_bytes && aligned(workspace)), SPYRE_ENOSPC,
                 "workspace holds %zu bytes, need %zu (16-byte aligned)", workspace ? workspace_bytes : 0, p.ws_bytes);
   LatentArgs a{};
   a.q = static_cast<const _Float16*>(q), a.q_sb = q_strides[0], a.q_st = q_strides[1], a.q_sh = q_strides[2];
@@ -622,7 +632,7 @@ extern "C" int spyre_paged_latent_attn(const void* q, const int64_t* q_strides, 
   a.out = static_cast<_Float16*>(out), a.lse = lse, a.ws = static_cast<float*>(workspace);
   a.B = B, a.T = T, a.H = H, a.Hkv = 1, a.rows = T * H;
   a.max_ctx = max_context_len, a.scale_log2 = scale * kLog2e;
-  a.row_blocks = p.row_blocks, a.block_rows = p.block_rows, a.width = p.width;
+  a.row_blocks = p.row_blocks, a.block_rows = p.block_rows;
   a.ranges = p.ranges, a.min_per = p.min_per, a.min_cut = p.min_cut;
   a.each = B % p.ranges == 0 ? B / p.ranges : 0;
   const int64_t blocks = static_cast<int64_t>((p.ranges + 7) / 8 * 8) * p.row_blocks;
@@ -636,9 +646,13 @@ extern "C" int spyre_paged_latent_attn(const void* q, const int64_t* q_strides, 
   hipError_t e = hipGetLastError();
   SPYRE_REQUIRE(e == hipSuccess, SPYRE_EHIP, "latent attention launch failed: %s", hipGetErrorString(e));
   if (p.ranges > 1) {  // no sequence is cut where one range has them all
-    const int64_t n = std::min((static_cast<int64_t>(a.rows) * (rank / 4) + 255) / 256, std::max<int64_t>(kJoinBlocks / B, 1));
+    const int64_t n = std::min(static_cast<int64_t>(p.row_blocks) * p.block_rows * (rank / 4) / 256, std::max<int64_t>(kJoinBlocks / B, 1));
     const dim3 join(static_cast<uint32_t>(B), static_cast<uint32_t>(n));
-    rank == 512 ? latent_join_kernel<512><<<join, 256, 0, st>>>(a) : latent_join_kernel<256><<<join, 256, 0, st>>>(a);
+    auto go = [&](auto r) {
+      constexpr int R = decltype(r)::value;
+      p.groups == 1 ? latent_join_kernel<R, 1><<<join, 256, 0, st>>>(a) : latent_join_kernel<R, 2><<<join, 256, 0, st>>>(a);
+    };
+    rank == 512 ? go(std::integral_constant<int, 512>{}) : go(std::integral_constant<int, 256>{});
     e = hipGetLastError();
     SPYRE_REQUIRE(e == hipSuccess, SPYRE_EHIP, "latent attention join launch failed: %s", hipGetErrorString(e));
   }

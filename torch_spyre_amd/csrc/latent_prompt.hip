@@ -55,10 +55,10 @@ __device__ __forceinline__ int token_of(int m) {
   return 16 * ((m >> 2) & 1) + 8 * (m >> 4) + 4 * ((m >> 3) & 1) + (m & 3);
 }
 
-// Unit u (16 bytes) of token t lies at u ^ key(t) of its 128 bytes in LDS: the 8 lanes
-// that read a unit of tokens 4 x .. + 3 and 16 further, and the 16 that read 2
-// units of 4 tokens, transposed, do not meet in a bank.
-__device__ __forceinline__ int key_of(int t) { return (t & 3) | ((t >> 2) & 4); }
+// Unit u (16 bytes) of token t lies at u ^ key(t) of its 128 bytes in LDS: neither the
+// reads of K's rows (32 tokens in token_of's order x 2 units) nor the transposing ones of V's (2
+// x 4 tokens x 4 units) then meet in a bank: 4 and 2 cycles a read (measured).
+__device__ __forceinline__ int key_of(int t) { return (t & 2) << 1 | ((t >> 2) & 1) | ((t >> 3) & 2); }
 
 template <int D, int W>
 __global__ __launch_bounds__(W * 64, W / 4) void prompt_kernel(PromptArgs a) {
@@ -130,8 +130,8 @@ __global__ __launch_bounds__(W * 64, W / 4) void prompt_kernel(PromptArgs a) {
   int k_off[4];
 #pragma unroll
   for (int u = 0; u < 4; ++u) k_off[u] = k_tok * 128 + (((2 * u + half) ^ key_of(k_tok)) * 16);
-  // V^T: 4 features of token 16 half + lane % 16 / 4; the key of tokens 4, 8, 12 and 32 further
-  // is the same, odd tiles turn bit 2 of the unit.
+  // V^T: 4 features of token 16 half + lane % 16 / 4; the key of tokens 8 and 32 further is the
+  // same, odd tiles and tokens 4 further turn the unit's bits 2 and 0.
   const int tv = 16 * half + (lane & 15) / 4;
   const int v_lane = KS * kStick + tv * 128 + (((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ key_of(tv)) * 16) + 8 * (lane & 1);
   auto tr = [&](int at) {
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(W * 64, W / 4) void prompt_kernel(PromptArgs a) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const int at = v_at[dt & 1] + dt / 2 * kStick + (32 * (s / 2) + 8 * (s % 2)) * 128;
-        const s16x4 lo = tr(at), hi = tr(at + 4 * 128);
+        const s16x4 lo = tr(at), hi = tr((at ^ 16) + 4 * 128);
         o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
             __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), w[s], o[dt], 0, 0, 0);
       }
