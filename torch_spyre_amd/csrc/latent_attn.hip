@@ -291,8 +291,16 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
       __syncthreads();  // the page is there; RG 2: the other buffer is read
       const bool more = p + (RG == 1 ? 2 : 1) < p1;
       if (RG == 1 && more) next = pages.at(p + 2);
-      if (RG == 2 && more) {
-        load_page(next, p + 1, buf ^ 1);
+      // RG 2: the next page's chunks go out between the products below, one of eight to a
+      // wavefront: at once they would take the address unit 1100 cycles, with every wavefront
+      // waiting its turn.  (Behind the last page they read nowhere, into a buffer that nobody reads.)
+      dma_rsrc ahead;
+      uint32_t ahead_off = BUF, ahead_at = 0, ahead_to = 0;
+      if constexpr (RG == 2) {
+        ahead = dma_buffer(a.pages + next * (NS * (kStick / 2)), BUF);
+        const int t = here(lane) / 8;
+        if (more && (p + 1) * kPage + 8 * wave + t < total) ahead_off = t * 128 + (((lane & 7) ^ key_of(t)) * 16);
+        ahead_at = uniform_here(wave * 1024), ahead_to = lds0 + (buf ^ 1) * BUF + ahead_at;
         if (p + 2 < p1) next = pages.at(p + 2);
       }
       uint32_t odd = 0;                            // of this wavefront's tokens, new ones that hold a NaN or an infinity
@@ -340,6 +348,7 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
         const int k_at[2] = {k_lane, k_lane ^ 64};
         // kAhead operands on their way; in this order, the scheduler would read each when it is due
         constexpr int kAhead = 8, NK = NQ * TB;
+        static_assert(RG == 1 || NK % NS == 0, "a stick of the next page every so many products");
         f16x8 kf[kAhead];
         auto k_of = [&](int x) {
           const int s = x / TB;
@@ -347,20 +356,22 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
         };
 #pragma unroll
         for (int x = 0; x < kAhead; ++x) kf[x] = k_of(x);
-        f32x4 acc[NR][TB] = {};
+        f32x4 acc[2][NR][TB] = {};  // four chains: a product waits 64 cycles for the one before it and takes 16
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int x = 0; x < NK; ++x) {
 #pragma unroll
           for (int n = 0; n < NR; ++n)
-            acc[n][x % TB] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[x % kAhead], qf[n][x / TB], acc[n][x % TB], 0, 0, 0);
+            acc[x / TB % 2][n][x % TB] =
+                __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[x % kAhead], qf[n][x / TB], acc[x / TB % 2][n][x % TB], 0, 0, 0);
           if (x + kAhead < NK) kf[x % kAhead] = k_of(x + kAhead);
+          if (RG == 2 && x % (NK / NS) == 0) dma16(ahead, ahead_to + x / (NK / NS) * kStick, ahead_off, ahead_at + x / (NK / NS) * kStick);
           __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int n = 0; n < NR; ++n)
 #pragma unroll
-          for (int x = 0; x < NT; ++x) sc[n][x] = acc[n][x / 4][x % 4];
+          for (int x = 0; x < NT; ++x) sc[n][x] = acc[0][n][x / 4][x % 4] + acc[1][n][x / 4][x % 4];
       }
       const int ln = here(lane);
 #pragma unroll
@@ -458,13 +469,16 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
       f16x8 w[4];
 #pragma unroll
       for (int s = 0; s < 4; ++s) w[s] = *reinterpret_cast<const f16x8*>(&s_p[(kTile * rg + ln % 32) * kPage + (((2 * s + ln / 32) ^ row_key(ln)) * 8)]);
-      // Operand x of C^T: stick x / 8 of the wavefront, tokens 16 (x / 2 % 4) .. + 15, tile x % 2
-      // of the stick.
+      // Operand x of C^T: tile v_tile(x) of the wavefront (two to a stick), tokens 16 v_step(x) .. +
+      // 15.  RG 1: stick after stick; else tiles take turns, so that none waits for its last
+      // product.
+      auto v_tile = [](int x) { return RG == 1 ? x / 8 * 2 + x % 2 : x % DT; };
+      auto v_step = [](int x) { return RG == 1 ? x / 2 % 4 : x / DT; };
       constexpr int kAhead = 6, NV = 8 * OS;
       f16x8 vf[kAhead];
       auto v_of = [&](int x) {
-        const int at = x / 8 * kStick + x / 2 % 4 * 16 * 128;
-        const s16x4 lo = tr(v_at[x & 1] + at), hi = tr((v_at[x & 1] ^ 32) + at + 4 * 128);
+        const int at = v_tile(x) / 2 * kStick + v_step(x) * 16 * 128, odd_tile = v_tile(x) & 1;
+        const s16x4 lo = tr(v_at[odd_tile] + at), hi = tr((v_at[odd_tile] ^ 32) + at + 4 * 128);
         return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
       };
 #pragma unroll
@@ -472,8 +486,8 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int x = 0; x < NV; ++x) {
-        f32x16& y = o[x / 8 * 2 + x % 2];
-        y = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[x % kAhead], w[x / 2 % 4], y, 0, 0, 0);
+        f32x16& y = o[v_tile(x)];
+        y = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[x % kAhead], w[v_step(x)], y, 0, 0, 0);
         if (x + kAhead < NV) vf[x % kAhead] = v_of(x + kAhead);
         __builtin_amdgcn_sched_barrier(0);
         // RG 1: a stick is read: this wavefront alone reads it, in this product
@@ -522,6 +536,7 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
       }
     }
     advance(a, walk, pc);
+    wait_loads<0>();  // (those behind the last page, too)
     __syncthreads();  // LDS is read before the next piece writes it
   }
 }
