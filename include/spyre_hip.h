@@ -591,13 +591,16 @@ int spyre_paged_latent_attn(const void* q, const int64_t* q_strides, const void*
  *   k_rope {b, t}; multiples of 8 elements, 16-byte aligned; token strides of k, k_rope
  *   and v below 2^23
  *   out [B, T, H, D] fp16, lse optional fp32 [B, T, H]; contiguous
- * D in {64, 128}.  No reference counterpart. */
+ * The workspace (16-byte aligned) needs no initialisation; two calls in flight
+ * need two.  D in {64, 128}.  No reference counterpart. */
+size_t spyre_latent_attn_workspace_bytes(int B, int T, int H, int D, int keys);
 int spyre_latent_attn(const void* q, const int64_t* q_strides, const void* q_rope,
                       const int64_t* q_rope_strides, const void* k, const int64_t* k_strides,
                       const void* k_rope, const int64_t* k_rope_strides, const void* v,
                       const int64_t* v_strides, const int32_t* context_lens,
-                      const int32_t* new_lens, void* out, float* lse, int B, int T, int H, int D,
-                      int keys, float scale, void* stream);
+                      const int32_t* new_lens, void* out, float* lse, void* workspace,
+                      size_t workspace_bytes, int B, int T, int H, int D, int keys, float scale,
+                      void* stream);
 
 #ifdef __cplusplus
 }

@@ -373,12 +373,24 @@ def test_not_attended_keys_are_not_reached(cuda, D, bad):
     kv[1, T + 70:], kr[1, T + 70:] = bad, bad
     for a, b in zip(call(), clean):
         assert torch.equal(a, b)
-    for x in (kv[0, 200, 1, 3:4], kv[0, 200, 1, D + 5:D + 6]):  # a key's, a value's feature
+    for x, key in ((kv[0, 200, 1, 3:4], True), (kv[0, 200, 1, D + 5:D + 6], False)):  # a key's, a value's feature
         old = x.clone()
         x.fill_(bad)
         out, lse = call()
         assert torch.equal(out[0, :200], clean[0][0, :200]) and torch.equal(out[1], clean[0][1]) and torch.equal(out[0, :, 0], clean[0][0, :, 0])
-        assert not out[0, 200:256, 1].isfinite().all(-1).any()
+        # A key at infinity has a score of q x inf: where that is -inf its weight is exp(-inf) = 0, so
+        # the row is what it is without the key; +inf and NaN make it NaN, as a value does.
+        reached = torch.full((T - 200,), True, device=cuda)
+        if key and not math.isnan(bad):
+            reached = (q[0, 200:, 1, 3] > 0) == (bad > 0)
+        assert (out[0, 200:, 1].isfinite().all(-1) == ~reached).all()
+        if key:
+            assert (lse[0, 200:, 1].isfinite() == ~reached).all()
+            K = torch.cat((kv[0, :T, 1, :D], kr[0, :T]), -1).double().cpu().numpy()
+            keep = keep_of(T, 1, 0, T) & (np.arange(T) != 200)
+            rows = [200 + r for r in torch.nonzero(~reached).flatten().tolist()]
+            ref = O.attend(q[0, rows, 1].double().cpu().numpy(), K, kv[0, :T, 1, D:].double().cpu().numpy(), keep[rows], (D + 64) ** -0.5)
+            close(out[0, rows, 1], lse[0, rows, 1], ref, T, float(kv[0, :T, 1, D:].abs().max()))
         x.copy_(old)
 
 

@@ -146,7 +146,8 @@ SIGNATURES = {
                                         c_int64, c_int64, c_void_p, c_void_p, c_void_p, POINTER(c_int64), c_void_p,
                                         c_void_p, c_void_p, c_size_t, c_int, c_int, c_int, c_int, c_int64, c_int,
                                         c_float, c_void_p]),
-    "spyre_latent_attn": (c_int, [c_void_p, POINTER(c_int64)] * 5 + [c_void_p] * 4 + [c_int] * 5
+    "spyre_latent_attn_workspace_bytes": (c_size_t, [c_int] * 5),
+    "spyre_latent_attn": (c_int, [c_void_p, POINTER(c_int64)] * 5 + [c_void_p] * 5 + [c_size_t] + [c_int] * 5
                           + [c_float, c_void_p]),
 }
 

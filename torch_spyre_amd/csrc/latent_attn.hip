@@ -432,7 +432,7 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
       };
       weigh();
       __syncthreads();
-      // Where a row's scores pass its reference too far, all move.
+      // Where a row's scores pass its reference too far, it moves.
       bool moves = false;
 #pragma unroll
       for (int k = 0; k < 2; ++k) moves = moves || s_max[64 * k + ln] > s_ref[(64 * k + ln) % ROWS] + kAbove;
@@ -441,7 +441,7 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
           float top = s_max[r];
 #pragma unroll
           for (int k = 1; k < TG; ++k) top = fmaxf(top, s_max[k * ROWS + r]);
-          return fmaxf(s_ref[r], top - kBelow);
+          return top > s_ref[r] + kAbove ? top - kBelow : s_ref[r];  // its own: what others attend does not turn its roundings
         };
         auto factor = [](float from, float to) { return from == -INFINITY ? 0.f : exp2_of(from - to); };
         const int c = kTile * rg + here(col), th = here(threadIdx.x) % ROWS;

@@ -285,12 +285,15 @@ std::tuple<at::Tensor, at::Tensor> latent_attention(const at::Tensor& query, con
   at::Tensor lse = at::empty({B, T, H}, q.options().dtype(at::kFloat));
   auto st = [](const at::Tensor& t) { return std::array<int64_t, 3>{t.stride(0), t.stride(1), t.stride(2)}; };
   const auto qs = st(q), qrs = st(qr), ks = st(k), krs = st(kr), vs = st(v);
+  const int iB = as_int(B, "batch"), iT = as_int(T, "tokens"), iH = as_int(H, "heads"), iD = as_int(D, "head_dim"),
+            iN = as_int(n, "keys");
+  const size_t need = spyre_latent_attn_workspace_bytes(iB, iT, iH, iD, iN);
+  const at::Tensor ws = need ? at::empty({static_cast<int64_t>(need)}, q.options().dtype(at::kByte)) : at::Tensor();
   check_rc("spyre_latent_attn",
            spyre_latent_attn(q.data_ptr(), qs.data(), qr.data_ptr(), qrs.data(), k.data_ptr(), ks.data(), kr.data_ptr(), krs.data(),
                              v.data_ptr(), vs.data(), context_lens.data_ptr<int32_t>(),
                              new_lens.has_value() ? new_lens->data_ptr<int32_t>() : nullptr, out.data_ptr(), lse.data_ptr<float>(),
-                             as_int(B, "batch"), as_int(T, "tokens"), as_int(H, "heads"), as_int(D, "head_dim"), as_int(n, "keys"),
-                             static_cast<float>(s), stream_of(q)));
+                             need ? ws.data_ptr() : nullptr, need, iB, iT, iH, iD, iN, static_cast<float>(s), stream_of(q)));
   return {out, lse};
 }
 
