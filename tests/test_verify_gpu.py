@@ -55,6 +55,22 @@ def test_kinds(cuda, dtype, kind, B, T, V):
 
 
 @pytest.mark.parametrize("kind", ["chain, q", "chain", "tree"])
+@pytest.mark.parametrize("B,T,V", [(64, 2, 40001), (290, 1, 61441)])
+def test_many_sequences_of_large_vocabularies(cuda, kind, B, T, V):
+    x, p, u, q, parents = inputs(cuda, B, T, V, "f16", SEED + V, kind == "chain, q", kind == "tree")
+    check(x, p, u, q, parents)
+
+
+@pytest.mark.parametrize("T", [64, 65, 150, 1024])
+def test_many_siblings(cuda, T):
+    """All of them continue the context, most are rejected, tokens occur again."""
+    x, p, _, _, _ = inputs(cuda, 3, T, 3 * T, "f32", SEED + T, False, True)
+    u = torch.rand((3, T + 1), device=cuda)
+    u[:, :T] = u[:, :T].clamp(min=0.02)
+    check(x, p, u, None, torch.full((3, T), -1, dtype=torch.int32, device=cuda))
+
+
+@pytest.mark.parametrize("kind", ["chain, q", "chain", "tree"])
 def test_uneven_drafts_and_int32(cuda, kind):
     x, p, u, q, parents = inputs(cuda, 9, 6, 777, "f32", SEED, kind == "chain, q", kind == "tree", torch.int32)
     lens = torch.tensor([0, 1, 2, 3, 4, 5, 6, 7, -1], dtype=torch.int32, device=cuda)
