@@ -19,6 +19,11 @@
 // page (RG 1), or 16 rows x 32 tokens (RG 2: half the registers for Q, so that two
 // wavefronts fit a SIMD), with Q in registers.  The weights meet in LDS, and each then takes
 // all 64 tokens of 32 rows x a quarter of O's features, which stay in 64 registers.
+//
+// Measured, rank 512: 32 sequences x 4096 tokens x 128 heads 76 us (36.5 GFLOP, 480 TFLOP/s; a page
+// of 64 rows takes 3 us where its products alone take 1.9, the parts' way to memory and back
+// with the second launch 17); 64 x 128-16384 tokens x 16 heads 127 us (601 MB, 4.7 TB/s: memory);
+// 16 x 500-6000 tokens x 1-7 new x 32 heads 57; 1 x 700 x 16 heads 18.4, of which two launches 9.
 
 #include <hip/hip_runtime.h>
 
@@ -61,23 +66,156 @@ struct LatentArgs {
   _Float16* out;  // [B, T, H, rank]
   float* lse;     // [B, T, H] or null
   float* ws;
-  int B, T, H, Hkv, rows, max_ctx, draft_keys;
+  int B, T, H, rows, max_ctx, draft_keys;
   float scale_log2;
-  int row_blocks, block_rows;
-  int ranges, min_per, min_cut, each;  // see PageWalk
-  FastDiv by_h, by_hkv, by_blocks, by_ranges;
+  int row_blocks, block_rows;  // of a sequence with T new tokens; a block's
+  int ranges, each;            // at most; row blocks of a range where none is cut
+  FastDiv by_h, by_blocks, by_ranges;
 };
-typedef PageWalk<LatentArgs> Walk;
 
-// The parts of a sequence that several ranges share, joined by a second kernel (in this
+// How the work is shared out, as in PageWalk, with row blocks in the place of KV heads: a row
+// block that has rows counts kStart units and one for each page, one behind the sequence's
+// new tokens (zeros) one unit.  Range r is the units [r per, (r + 1) per) of all, row block
+// after row block, sequence after sequence: with a workgroup to each row block of a range of
+// pages half of them had no rows where sequences had 1 to 7 new tokens (16 x 7 x 32 heads 64 us,
+// so 57).
+struct Walk {
+  // Units of a range, at least: one sequence of 700 tokens and 16 heads 18.4 us (4: 21.4, 6: 25),
+  // 4 of 3000 23.0 (23.8, 26.2).
+  static constexpr int kLeast = 3;
+  int per, used;      // units of a range, ranges that have any
+  int u, end;         // units
+  int b, base;        // the sequence, its first unit
+  Seq seq;            // what it holds
+  int size, live;     // units of a row block that has rows; such row blocks
+
+  __device__ __forceinline__ static int live_of(const LatentArgs& a, int n) { return (n * a.H + a.block_rows - 1) / a.block_rows; }
+  struct Lane {  // a sequence a lane
+    int ctx = 0, count = 0, units = 0, top = 0;
+  };
+  __device__ __forceinline__ static Lane lane_of(const LatentArgs& a, int b) {
+    Lane x;
+    if (b < a.B) {
+      x.ctx = a.ctx[b], x.count = a.counts ? a.counts[b] : a.T;
+      const Seq s = seq_of(a, x.ctx, x.count);
+      const int live = live_of(a, s.n);
+      x.top = kStart + s.pages;
+      x.units = live * x.top + a.row_blocks - live;
+      if (live < a.row_blocks) x.top = 1 << 29;
+    }
+    return x;
+  }
+  __device__ __forceinline__ void take(const LatentArgs& a, int ctx, int count) {
+    seq = seq_of(a, ctx, count);
+    live = live_of(a, seq.n), size = kStart + seq.pages;
+  }
+  __device__ __forceinline__ int units(const LatentArgs& a) const { return live * size + a.row_blocks - live; }
+  __device__ __forceinline__ void find(const LatentArgs& a, int lane, const Lane& first64, int unit) {
+    base = 0;
+    for (int c = 0;; c += 64) {
+      const Lane x = c == 0 ? first64 : lane_of(a, c + lane);
+      const int sum = scan64(x.units);
+      const uint64_t past = __builtin_amdgcn_ballot_w64(base + sum > unit);
+      if (past || c + 64 >= a.B) {
+        const int i = past ? __builtin_ctzll(past) : (a.B - 1) % 64;
+        b = c + i;
+        take(a, __builtin_amdgcn_readlane(x.ctx, i), __builtin_amdgcn_readlane(x.count, i));
+        base += __builtin_amdgcn_readlane(sum, i) - units(a);
+        return;
+      }
+      base += __builtin_amdgcn_readlane(sum, 63);
+    }
+  }
+  // A bound where it belongs, after find() of it: no piece of few pages.
+  __device__ __forceinline__ int placed(int unit) const {
+    const int in = unit - base, few = min(max(per - kStart, 0) / 2, 4);
+    if (in >= live * size) return unit;
+    const int at = static_cast<int>(static_cast<uint32_t>(in) % static_cast<uint32_t>(size));
+    const int g0 = unit - at, g1 = g0 + size;
+    return at - kStart <= few ? g0 : g1 - unit <= few ? g1 : unit;
+  }
+  // This workgroup's range; -1: none.  Those that follow one another run in one XCD.
+  __device__ __forceinline__ int start(const LatentArgs& a, int lane) {
+    const Lane x = lane_of(a, lane);
+    int total = 0, largest = 0;
+    for (int c = 0; c < a.B; c += 64) {
+      const Lane y = c == 0 ? x : lane_of(a, c + lane);
+      total += y.units, largest = max(largest, y.top);
+    }
+    total = __builtin_amdgcn_readlane(scan64(total), 63), largest = max64(largest);
+    per = max(static_cast<int>(fdiv(total + a.ranges - 1, a.by_ranges)), kLeast);
+    // Where a whole number of row blocks to a range is within an eighth of it, none is cut.
+    const bool uncut = a.each > 0 && static_cast<int64_t>(largest) * a.each <= per + per / 8;
+    used = uncut ? a.ranges : min((total + per - 1) / per, a.ranges);
+    const int xcd = blockIdx.x & 7, i = blockIdx.x >> 3;
+    if (i >= used / 8 + (xcd < used % 8)) return -1;
+    const int r = xcd * (used / 8) + min(xcd, used % 8) + i;
+    if (uncut) {
+      const int first = r * a.each, at = static_cast<int>(fdiv(first, a.by_blocks));
+      base = 0;
+      for (int c = 0; c <= at; c += 64) {
+        const Lane y = c == 0 ? x : lane_of(a, c + lane);
+        base += __builtin_amdgcn_readlane(scan64(c + lane < at ? y.units : 0), 63);
+      }
+      b = at;
+      take(a, __builtin_amdgcn_readfirstlane(a.ctx[b]), a.counts ? __builtin_amdgcn_readfirstlane(a.counts[b]) : a.T);
+      u = end = base + (first - at * a.row_blocks) * size;
+      for (int k = 0; k < a.each; ++k) end += kStart + seq_at(a, static_cast<int>(fdiv(first + k, a.by_blocks))).pages;
+      return r;
+    }
+    u = r * per;
+    end = total;
+    if (u + per < total) {
+      find(a, lane, x, u + per);
+      end = placed(u + per);
+    }
+    find(a, lane, x, u);
+    u = placed(u);
+    if (u < end && u == base + units(a)) next_sequence(a);
+    return r;
+  }
+  __device__ __forceinline__ void next_sequence(const LatentArgs& a) {
+    base += units(a);
+    b = min(b + 1, a.B - 1);
+    const Seq s = seq_at(a, b);
+    seq = s, live = live_of(a, s.n), size = kStart + s.pages;
+  }
+  // Pages [page0, page1) of a row block.
+  struct Piece {
+    int rb, page0, page1;
+    bool begins, ends;
+  };
+  __device__ __forceinline__ Piece piece(const LatentArgs& a) const {
+    const int in = u - base, of_live = live * size;
+    if (in >= of_live) return {min(live + in - of_live, a.row_blocks - 1), 0, 0, true, true};
+    Piece p;
+    p.rb = min(static_cast<int>(static_cast<uint32_t>(in) / static_cast<uint32_t>(size)), a.row_blocks - 1);
+    const int at = in - p.rb * size;
+    p.page0 = max(at - kStart, 0), p.page1 = min(size, at + end - u) - kStart;
+    p.begins = at == 0, p.ends = p.page1 == size - kStart;
+    return p;
+  }
+  // After it.
+  __device__ __forceinline__ void advance(const LatentArgs& a, const Piece& p) {
+    u = max(p.rb < live ? base + p.rb * size + kStart + p.page1 : u + 1, u + 1);
+    if (u < end && p.ends && p.rb == a.row_blocks - 1) next_sequence(a);
+  }
+};
+
+// The parts of a row block that several ranges share, joined by a second kernel (in this
 // one, by the last workgroup to arrive, each step of the exchange is a way to memory and
-// back: 8 us more for one short sequence, 60 for 32 x 4 parts of 128 rows).  Slot
-// (range, row block, 0 / 1) of the workspace holds a part: O as the wavefronts' registers
-// have it, [wave][tile, 4 features][lane] of 4 floats, so that stores and loads are whole
-// lines, then (m, l) of its rows.
+// back: 8 us more for one short sequence, 60 for 32 x 4 parts of 128 rows).  A range leaves
+// the part of the row block that it ends in at slot 2 r + 1, that of the one that it begins
+// in at 2 r: O as the wavefronts' registers have it, [wave][tile, 4 features][lane] of 4
+// floats, so that stores and loads are whole lines, then (m, l) of its rows.  Behind the slots a
+// range has the (sequence, row block) that it began and did not end (-1: none) and whether it
+// ended the one that it began within; behind those lies the number of ranges.
 __host__ __device__ constexpr int64_t slot_floats(int rows, int rank) { return static_cast<int64_t>(rows) * (rank + 2); }
-__device__ __forceinline__ float* slot_of(const LatentArgs& a, int range, int rb, int slot, int rank) {
-  return a.ws + ((static_cast<int64_t>(range) * a.row_blocks + rb) * 2 + slot) * slot_floats(a.block_rows, rank);
+__device__ __forceinline__ float* slot_of(const LatentArgs& a, int slot, int rank) {
+  return a.ws + slot * slot_floats(a.block_rows, rank);
+}
+__device__ __forceinline__ int32_t* bounds_of(const LatentArgs& a, int range, int rank) {
+  return reinterpret_cast<int32_t*>(slot_of(a, 2 * a.ranges, rank)) + 4 * range;
 }
 
 // 4 features of a finished row.
@@ -166,10 +304,11 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
   const int part = wave % kParts, rg = wave / kParts;  // second product: features, rows 32 rg ..
   const int tg = wave % TG, rq = wave / TG;            // first: tokens 16 TB tg .., rows 16 NR rq ..
   const uint32_t lds0 = lds_address(s_mem);
-  int range, rb;
-  place_of(a, range, rb);
   Walk walk;
-  if (range >= a.ranges || !walk.start(a, lane, range)) return;
+  const int range = walk.start(a, lane);
+  if (range < 0) return;
+  if (threadIdx.x == 0 && range == 0) *bounds_of(a, a.ranges, RANK) = walk.used;
+  int open_b = -1, open_rb = 0, ended = 0;
 
   // K's row of a lane (16 tokens further its key is the same), units g16 and 4 + g16.  C^T: 4 features
   // of token 8 half + l16 / 4 of the wavefront's first tile; odd tiles and tokens 4 further turn
@@ -183,13 +322,11 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
   };
 
   for (; walk.u < walk.end;) {
-    const Piece pc = piece_of(a, walk);
+    const Walk::Piece pc = walk.piece(a);
     const int b = walk.b;
     const Seq sq = walk.seq;
     const int total = sq.ctx + sq.n;
-    const int row0 = rb * a.block_rows;
-    // (a workgroup whose rows are all of no new token has nothing to do)
-    const int p0 = pc.page0, p1 = row0 < sq.n * a.H ? pc.page1 : pc.page0;
+    const int row0 = pc.rb * a.block_rows, p0 = pc.page0, p1 = pc.page1;
     Pages pages(a, b, lane, p0);
 
     // `sticks` sticks of a page from s0 on, on their way into buffer `buf`: of their chunks (8
@@ -513,7 +650,7 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
 #pragma unroll
     for (int k = 0; k < TG; ++k) L += s_sum[k * ROWS + out_row];
     const float M = L == 0.f ? -INFINITY : s_ref[out_row];
-    if (pc.whole) {
+    if (pc.begins && pc.ends) {
       if (row0 + out_row < a.rows)
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
@@ -522,7 +659,9 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
             store_row4<RANK>(a, b, row0 + out_row, 32 * (DT * part + dt) + 8 * x + 4 * half,
                              f32x4{o[dt][4 * x], o[dt][4 * x + 1], o[dt][4 * x + 2], o[dt][4 * x + 3]}, M, L);
     } else {
-      float* slot = slot_of(a, range, rb, pc.slot, RANK);
+      float* slot = slot_of(a, 2 * range + (pc.begins ? 1 : 0), RANK);
+      if (pc.begins) open_b = b, open_rb = pc.rb;
+      if (pc.ends) ended = 1;
       if (row0 + out_row < a.rows)
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
@@ -535,45 +674,52 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
         ml[0] = M, ml[1] = L;
       }
     }
-    advance(a, walk, pc);
+    walk.advance(a, pc);
     wait_loads<0>();  // (those behind the last page, too)
     __syncthreads();  // LDS is read before the next piece writes it
   }
+  if (threadIdx.x == 0) {
+    int32_t* x = bounds_of(a, range, RANK);
+    x[0] = open_b, x[1] = open_rb, x[2] = ended;
+  }
 }
 
-// Joins the parts of each sequence that several ranges share: a thread 4 features of a
+// Joins the parts of the row block that a range began and did not end: a thread 4 features of a
 // row, numbered as they lie in a slot.
 template <int RANK, int RG>
 __global__ __launch_bounds__(256) void latent_join_kernel(LatentArgs a) {
-  constexpr int ROWS = RG * kTile, DT = RANK / 32 / kParts;
-  const int b = blockIdx.x;
-  Walk w;
-  w.seek(a, threadIdx.x % 64, b);
-  int r0, r1;
-  w.parts_of(a, 0, r0, r1);
-  if (r1 <= r0) return;
-  const int live = w.seq.n * a.H;
-  for (int64_t u = blockIdx.y * 256 + threadIdx.x; u < static_cast<int64_t>(a.row_blocks) * (ROWS * RANK / 4); u += gridDim.y * 256) {
-    const int rb = static_cast<int>(u / (ROWS * RANK / 4)), at = static_cast<int>(u % (ROWS * RANK / 4)), lane = at % 64;
-    const int wave = at / (DT * 256), tile = wave % kParts * DT + at / 256 % DT;
-    const int r = wave / kParts * kTile + lane % 32, row = rb * ROWS + r;
-    if (row >= a.rows) continue;
-    float M = -INFINITY, L = 0.f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    if (row < live)
-      merge_parts(r0, r1, M, L, acc, [&](int p, float& m, float& l, f32x4& x) {
-        const float* slot = slot_of(a, p, rb, p == r0 ? 1 : 0, RANK);
-        const float* ml = slot + ROWS * RANK + r * 2;
-        m = ml[0], l = ml[1];
-        x = *reinterpret_cast<const f32x4*>(slot + at * 4);
-      });
-    store_row4<RANK>(a, b, row, 32 * tile + 8 * (at / 64 % 4) + 4 * (lane / 32), acc, M, L);
+  constexpr int ROWS = RG * kTile, DT = RANK / 32 / kParts, BLOCKS = ROWS * RANK / 1024;
+  const int range = static_cast<int>(blockIdx.x / BLOCKS), at = static_cast<int>(blockIdx.x % BLOCKS) * 256 + threadIdx.x, lane = at % 64;
+  const int used = *bounds_of(a, a.ranges, RANK);
+  if (range >= used) return;
+  const int32_t* open = bounds_of(a, range, RANK);
+  const int b = open[0], rb = open[1];
+  if (b < 0) return;
+  int last = range + 1;  // the range that it ends in
+  for (;; last += 64) {
+    const uint64_t ended = __ballot(last + lane >= used - 1 || bounds_of(a, last + lane, RANK)[2] != 0);
+    if (ended != 0) {
+      last += __builtin_ctzll(ended);
+      break;
+    }
   }
+  const int wave = at / (DT * 256), tile = wave % kParts * DT + at / 256 % DT;
+  const int r = wave / kParts * kTile + lane % 32, row = rb * ROWS + r;
+  if (row >= a.rows) return;
+  float M = -INFINITY, L = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  merge_parts(range, min(last, used - 1), M, L, acc, [&](int p, float& m, float& l, f32x4& x) {
+    const float* slot = slot_of(a, 2 * p + (p == range ? 1 : 0), RANK);
+    const float* ml = slot + ROWS * RANK + r * 2;
+    m = ml[0], l = ml[1];
+    x = *reinterpret_cast<const f32x4*>(slot + at * 4);
+  });
+  store_row4<RANK>(a, b, row, 32 * tile + 8 * (at / 64 % 4) + 4 * (lane / 32), acc, M, L);
 }
 
 struct Plan {
   int groups;  // RG
-  int row_blocks, block_rows, ranges, min_per, min_cut;
+  int row_blocks, block_rows, ranges;
   size_t ws_bytes;
 };
 
@@ -583,15 +729,12 @@ Plan plan_of(int B, int T, int H, int rank, int max_tokens) {
   p.groups = rows <= kTile ? 1 : 2;
   p.block_rows = kTile * p.groups;
   p.row_blocks = static_cast<int>((rows + p.block_rows - 1) / p.block_rows);
-  p.min_per = 2, p.min_cut = 4;
-  const int64_t pages = std::max(pages_of(max_tokens), 1), parts_of_one = pages < p.min_cut ? 1 : pages / p.min_per;
-  const int64_t ranges = std::min(B * parts_of_one, std::max<int64_t>(256 / p.row_blocks, 1));
-  p.ranges = static_cast<int>(std::max<int64_t>(ranges, 1));
-  p.ws_bytes = p.ranges == 1 ? 0 : static_cast<size_t>(p.ranges) * p.row_blocks * 2 * slot_floats(p.block_rows, rank) * 4;
+  // One workgroup to a CU, and no more than there could be work for.
+  const double most = static_cast<double>(B) * p.row_blocks * (kStart + std::max(pages_of(max_tokens), 1));
+  p.ranges = static_cast<int>(std::max(1., std::min(256., most / Walk::kLeast)));
+  p.ws_bytes = static_cast<size_t>(2 * p.ranges) * slot_floats(p.block_rows, rank) * 4 + 16 * (static_cast<size_t>(p.ranges) + 1);
   return p;
 }
-
-constexpr int kJoinBlocks = 2048;
 
 bool sizes_ok(int B, int T, int H, int max_ctx) {
   return B >= 0 && T > 0 && H > 0 && max_ctx >= 0 && static_cast<int64_t>(T) * H < (int64_t{1} << 31) - 256 &&
@@ -634,7 +777,7 @@ extern "C" int spyre_paged_latent_attn(const void* q, const int64_t* q_strides, 
   for (int i = 0; i < 3; ++i)
     SPYRE_REQUIRE(q_strides[i] % 8 == 0 && q_rope_strides[i] % 8 == 0, SPYRE_EINVAL, "q strides must be multiples of 8 elements");
   const Plan p = plan_of(B, T, H, rank, max_context_len + T);
-  SPYRE_REQUIRE(p.ws_bytes == 0 || (workspace && workspace_bytes >= p.ws_bytes && aligned(workspace)), SPYRE_ENOSPC,
+  SPYRE_REQUIRE(workspace && workspace_bytes >= p.ws_bytes && aligned(workspace), SPYRE_ENOSPC,
                 "workspace holds %zu bytes, need %zu (16-byte aligned)", workspace ? workspace_bytes : 0, p.ws_bytes);
   LatentArgs a{};
   a.q = static_cast<const _Float16*>(q), a.q_sb = q_strides[0], a.q_st = q_strides[1], a.q_sh = q_strides[2];
@@ -645,24 +788,23 @@ extern "C" int spyre_paged_latent_attn(const void* q, const int64_t* q_strides, 
   a.mask = static_cast<const uint8_t*>(mask);
   if (mask) a.m_sb = mask_strides[0], a.m_si = mask_strides[1], a.m_sj = mask_strides[2];
   a.out = static_cast<_Float16*>(out), a.lse = lse, a.ws = static_cast<float*>(workspace);
-  a.B = B, a.T = T, a.H = H, a.Hkv = 1, a.rows = T * H;
+  a.B = B, a.T = T, a.H = H, a.rows = T * H;
   a.max_ctx = max_context_len, a.scale_log2 = scale * kLog2e;
   a.row_blocks = p.row_blocks, a.block_rows = p.block_rows;
-  a.ranges = p.ranges, a.min_per = p.min_per, a.min_cut = p.min_cut;
-  a.each = B % p.ranges == 0 ? B / p.ranges : 0;
-  const int64_t blocks = static_cast<int64_t>((p.ranges + 7) / 8 * 8) * p.row_blocks;
-  SPYRE_REQUIRE(static_cast<int64_t>(B) * (pages_of(max_context_len + T) + kStart + 1) < (int64_t{1} << 30) && blocks < (int64_t{1} << 31),
-                SPYRE_EUNSUPPORTED, "too many pages or rows");
-  a.by_h = make_fastdiv(static_cast<uint32_t>(H)), a.by_hkv = make_fastdiv(1);
+  a.ranges = p.ranges;
+  const int64_t of_all = static_cast<int64_t>(B) * p.row_blocks;
+  a.each = of_all % p.ranges == 0 ? static_cast<int>(of_all / p.ranges) : 0;
+  SPYRE_REQUIRE(static_cast<double>(of_all) * (pages_of(max_context_len + T) + kStart + 1) < (1 << 30), SPYRE_EUNSUPPORTED,
+                "too many pages or rows");
+  a.by_h = make_fastdiv(static_cast<uint32_t>(H));
   a.by_blocks = make_fastdiv(static_cast<uint32_t>(p.row_blocks)), a.by_ranges = make_fastdiv(static_cast<uint32_t>(p.ranges));
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid(static_cast<uint32_t>(blocks));
+  const dim3 grid(static_cast<uint32_t>((p.ranges + 7) / 8 * 8));
   rank == 512 ? launch<512>(a, p.groups, grid, st) : launch<256>(a, p.groups, grid, st);
   hipError_t e = hipGetLastError();
   SPYRE_REQUIRE(e == hipSuccess, SPYRE_EHIP, "latent attention launch failed: %s", hipGetErrorString(e));
-  if (p.ranges > 1) {  // no sequence is cut where one range has them all
-    const int64_t n = std::min(static_cast<int64_t>(p.row_blocks) * p.block_rows * (rank / 4) / 256, std::max<int64_t>(kJoinBlocks / B, 1));
-    const dim3 join(static_cast<uint32_t>(B), static_cast<uint32_t>(n));
+  if (p.ranges > 1) {  // nothing is cut where one range has it all
+    const dim3 join(static_cast<uint32_t>(p.ranges * (p.block_rows * rank / 1024)));
     auto go = [&](auto r) {
       constexpr int R = decltype(r)::value;
       p.groups == 1 ? latent_join_kernel<R, 1><<<join, 256, 0, st>>>(a) : latent_join_kernel<R, 2><<<join, 256, 0, st>>>(a);
