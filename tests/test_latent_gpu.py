@@ -203,6 +203,13 @@ def test_batches(cuda, B, H, ctx):
     check_paged(out[:, :, some], lse[:, :, some], q[:, :, some], qr[:, :, some], cache, table, lens.tolist(), [1] * B, 0.07)
 
 
+@pytest.mark.parametrize("counts", [[1, 7, 0, 3], [0, 0, 0, 7], [7, 7, 7, 7]])
+@pytest.mark.parametrize("rank", [256, 512])
+def test_rows_of_uneven_drafts_and_parts(cuda, rank, counts):
+    """Row blocks without rows between others that several ranges share."""
+    paged(cuda, 4, 7, 33, rank, [4000, 130, 700, 1], counts=counts, seed=70)
+
+
 def test_one_token_operands(cuda):
     import torch_spyre_amd as tsa
 
@@ -348,6 +355,13 @@ def test_prompts(cuda, D, T, ctx):
 @pytest.mark.parametrize("D", [64, 128])
 def test_ragged_prompts(cuda, D):
     expanded(cuda, 5, 270, 9, D, [0, 100, 0, 64, 7], [270, 0, 1, 129, 64], seed=3)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_few_rows_of_many_keys(cuda, D):
+    """Split over the keys, one split of the short sequence is empty."""
+    expanded(cuda, 2, 2, 2, D, [6000, 3], counts=[2, 1], seed=60)
+    expanded(cuda, 1, 1, 1, D, [9000], seed=61)
 
 
 def test_many_heads(cuda):
