@@ -14,16 +14,15 @@
 // them: a page is read once, into LDS, and serves both products of all rows.
 //   S^T[tok, row] = K[tok, :] Q^T[:, row]      K as it lies: rows of features
 //   O^T[d, row] += C^T[d, tok] P^T[tok, row]   C^T by transposing reads of the same rows
-// A workgroup has RG x 32 rows (RG 1 up to 32 rows, else 2), 4 RG wavefronts and two
-// pages in LDS.  In the first product a wavefront has 16 x 16 tiles: 32 rows x 16 tokens of a
-// page (RG 1), or 16 rows x 32 tokens (RG 2: half the registers for Q, so that two
-// wavefronts fit a SIMD), with Q in registers.  The weights meet in LDS, and each then takes
-// all 64 tokens of 32 rows x a quarter of O's features, which stay in 64 registers.
+// Up to 32 rows of a sequence are one workgroup's, more are split into blocks of 64; pages, and 32
+// tokens of them, come into LDS while the ones before are used.  The first product has 16 x 16 tiles
+// with Q in registers, the weights meet in LDS, and the second has 32 x 32 tiles of O in registers.
 //
-// Measured, rank 512: 32 sequences x 4096 tokens x 128 heads 76 us (36.5 GFLOP, 480 TFLOP/s; a page
-// of 64 rows takes 3 us where its products alone take 1.9, the parts' way to memory and back
-// with the second launch 17); 64 x 128-16384 tokens x 16 heads 127 us (601 MB, 4.7 TB/s: memory);
-// 16 x 500-6000 tokens x 1-7 new x 32 heads 57; 1 x 700 x 16 heads 18.4, of which two launches 9.
+// Measured, rank 512: 32 sequences x 4096 tokens x 128 heads 67 us (36.5 GFLOP, 550 TFLOP/s; 32
+// tokens of 64 rows take 0.85 us, of which the matrix cores 0.45 and the loads' way into LDS as much;
+// the start of a range 6 us, the parts' way to memory and back with the second launch 17); 64 x
+// 128-16384 tokens x 16 heads 125 us (629 MB, 5.0 TB/s: memory); 16 x 500-6000 tokens x 1-7 new x 32
+// heads 52; 1 x 700 x 16 heads 18.4, of which two launches 9.
 
 #include <hip/hip_runtime.h>
 
@@ -74,16 +73,17 @@ struct LatentArgs {
 };
 
 // How the work is shared out, as in PageWalk, with row blocks in the place of KV heads: a row
-// block that has rows counts kStart units and one for each page, one behind the sequence's
-// new tokens (zeros) one unit.  Range r is the units [r per, (r + 1) per) of all, row block
+// block that has rows counts kOpen units and one for each page, one behind the sequence's
+// new tokens (zeros) one unit.  Range r of R is the units [all r / R, all (r + 1) / R), row block
 // after row block, sequence after sequence: with a workgroup to each row block of a range of
-// pages half of them had no rows where sequences had 1 to 7 new tokens (16 x 7 x 32 heads 64 us,
-// so 57).
+// pages half of them had no rows where sequences had 1 to 7 new tokens (16 x 7 x 32 heads 64 us, so
+// 57).  A bound that would leave kFew pages or less of a row block moves to its end.
 struct Walk {
-  // Units of a range, at least: one sequence of 700 tokens and 16 heads 18.4 us (4: 21.4, 6: 25),
-  // 4 of 3000 23.0 (23.8, 26.2).
-  static constexpr int kLeast = 3;
-  int per, used;      // units of a range, ranges that have any
+  // kLeast: units of a range, at least: one sequence of 700 tokens and 16 heads 18.4 us (4: 21.4, 6:
+  // 25), 4 of 3000 23.0 (23.8, 26.2).  kOpen: 32 x 4096 tokens x 128 heads 66 us with 1, 2 and 4; the
+  // drafts above 56, 54, 52.  kFew: 300 x 10-900 tokens x 64 heads 68 us (4: 72).
+  static constexpr int kLeast = 3, kOpen = 4, kFew = 2;
+  int used;           // ranges that have any units
   int u, end;         // units
   int b, base;        // the sequence, its first unit
   Seq seq;            // what it holds
@@ -99,7 +99,7 @@ struct Walk {
       x.ctx = a.ctx[b], x.count = a.counts ? a.counts[b] : a.T;
       const Seq s = seq_of(a, x.ctx, x.count);
       const int live = live_of(a, s.n);
-      x.top = kStart + s.pages;
+      x.top = kOpen + s.pages;
       x.units = live * x.top + a.row_blocks - live;
       if (live < a.row_blocks) x.top = 1 << 29;
     }
@@ -107,7 +107,7 @@ struct Walk {
   }
   __device__ __forceinline__ void take(const LatentArgs& a, int ctx, int count) {
     seq = seq_of(a, ctx, count);
-    live = live_of(a, seq.n), size = kStart + seq.pages;
+    live = live_of(a, seq.n), size = kOpen + seq.pages;
   }
   __device__ __forceinline__ int units(const LatentArgs& a) const { return live * size + a.row_blocks - live; }
   __device__ __forceinline__ void find(const LatentArgs& a, int lane, const Lane& first64, int unit) {
@@ -127,12 +127,12 @@ struct Walk {
     }
   }
   // A bound where it belongs, after find() of it: no piece of few pages.
-  __device__ __forceinline__ int placed(int unit) const {
-    const int in = unit - base, few = min(max(per - kStart, 0) / 2, 4);
+  __device__ __forceinline__ int placed(int unit, int few) const {
+    const int in = unit - base;
     if (in >= live * size) return unit;
     const int at = static_cast<int>(static_cast<uint32_t>(in) % static_cast<uint32_t>(size));
     const int g0 = unit - at, g1 = g0 + size;
-    return at - kStart <= few ? g0 : g1 - unit <= few ? g1 : unit;
+    return at - kOpen <= few ? g0 : g1 - unit <= few ? g1 : unit;
   }
   // This workgroup's range; -1: none.  Those that follow one another run in one XCD.
   __device__ __forceinline__ int start(const LatentArgs& a, int lane) {
@@ -143,10 +143,10 @@ struct Walk {
       total += y.units, largest = max(largest, y.top);
     }
     total = __builtin_amdgcn_readlane(scan64(total), 63), largest = max64(largest);
-    per = max(static_cast<int>(fdiv(total + a.ranges - 1, a.by_ranges)), kLeast);
+    const int per = max(static_cast<int>(fdiv(total, a.by_ranges)), kLeast);
     // Where a whole number of row blocks to a range is within an eighth of it, none is cut.
     const bool uncut = a.each > 0 && static_cast<int64_t>(largest) * a.each <= per + per / 8;
-    used = uncut ? a.ranges : min((total + per - 1) / per, a.ranges);
+    used = uncut ? a.ranges : min(max(total / kLeast, 1), a.ranges);
     const int xcd = blockIdx.x & 7, i = blockIdx.x >> 3;
     if (i >= used / 8 + (xcd < used % 8)) return -1;
     const int r = xcd * (used / 8) + min(xcd, used % 8) + i;
@@ -160,17 +160,19 @@ struct Walk {
       b = at;
       take(a, __builtin_amdgcn_readfirstlane(a.ctx[b]), a.counts ? __builtin_amdgcn_readfirstlane(a.counts[b]) : a.T);
       u = end = base + (first - at * a.row_blocks) * size;
-      for (int k = 0; k < a.each; ++k) end += kStart + seq_at(a, static_cast<int>(fdiv(first + k, a.by_blocks))).pages;
+      for (int k = 0; k < a.each; ++k) end += kOpen + seq_at(a, static_cast<int>(fdiv(first + k, a.by_blocks))).pages;
       return r;
     }
-    u = r * per;
-    end = total;
-    if (u + per < total) {
-      find(a, lane, x, u + per);
-      end = placed(u + per);
+    // (total below 2^30: products of 40 bits)
+    u = static_cast<int>(static_cast<int64_t>(total) * r / used);
+    end = static_cast<int>(static_cast<int64_t>(total) * (r + 1) / used);
+    const int few = min(max(per - kOpen, 0) / 2, kFew);
+    if (end < total) {
+      find(a, lane, x, end);
+      end = placed(end, few);
     }
     find(a, lane, x, u);
-    u = placed(u);
+    u = placed(u, few);
     if (u < end && u == base + units(a)) next_sequence(a);
     return r;
   }
@@ -178,7 +180,7 @@ struct Walk {
     base += units(a);
     b = min(b + 1, a.B - 1);
     const Seq s = seq_at(a, b);
-    seq = s, live = live_of(a, s.n), size = kStart + s.pages;
+    seq = s, live = live_of(a, s.n), size = kOpen + s.pages;
   }
   // Pages [page0, page1) of a row block.
   struct Piece {
@@ -191,13 +193,13 @@ struct Walk {
     Piece p;
     p.rb = min(static_cast<int>(static_cast<uint32_t>(in) / static_cast<uint32_t>(size)), a.row_blocks - 1);
     const int at = in - p.rb * size;
-    p.page0 = max(at - kStart, 0), p.page1 = min(size, at + end - u) - kStart;
-    p.begins = at == 0, p.ends = p.page1 == size - kStart;
+    p.page0 = max(at - kOpen, 0), p.page1 = min(size, at + end - u) - kOpen;
+    p.begins = at == 0, p.ends = p.page1 == size - kOpen;
     return p;
   }
   // After it.
   __device__ __forceinline__ void advance(const LatentArgs& a, const Piece& p) {
-    u = max(p.rb < live ? base + p.rb * size + kStart + p.page1 : u + 1, u + 1);
+    u = max(p.rb < live ? base + p.rb * size + kOpen + p.page1 : u + 1, u + 1);
     if (u < end && p.ends && p.rb == a.row_blocks - 1) next_sequence(a);
   }
 };
@@ -280,17 +282,18 @@ __device__ __forceinline__ int key_of(int t) { return (t & 2) << 1 | (t & 4) >> 
 // That of the weights' rows, whose reads are 32 rows x 2 units.
 __device__ __forceinline__ int row_key(int r) { return (r & 2) << 1 | ((r >> 2) & 3); }
 
-template <int RANK, int RG>
-__global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs a) {
-  constexpr int WAVES = RG * kParts;
-  constexpr int ROWS = RG * kTile;
+// Up to 32 rows: four wavefronts, each a SIMD's alone, have 32 rows x 16 tokens of a page of scores,
+// and then all 64 tokens of 32 rows x a quarter of O's features, which stay in 64 registers.
+template <int RANK>
+__global__ __launch_bounds__(kParts * 64, 1) void latent_kernel(LatentArgs a) {
+  constexpr int WAVES = kParts, ROWS = kTile;
   constexpr int NS = (RANK + kRope) / 64;     // sticks
   constexpr int OS = RANK / 64 / kParts;      // sticks of O of a wavefront
   constexpr int DT = 2 * OS;                  // tiles of it, 32 features each
   constexpr int NQ = (RANK + kRope) / 32;     // steps of the first product
-  constexpr int NR = RG == 1 ? 2 : 1, TB = RG == 1 ? 1 : 2;  // its tiles of 16 rows, 16 tokens
-  constexpr int TG = 4 / TB;                  // wavefronts that share a row's tokens in it
-  constexpr int NT = 4 * TB;                  // scores of a lane's row
+  constexpr int NR = 2;                       // its tiles of 16 rows
+  constexpr int TG = kParts;                  // wavefronts that share a row's tokens in it
+  constexpr int NT = 4;                       // scores of a lane's row
   constexpr int BUF = NS * kStick;
   constexpr int SHARE = 8 * NS / WAVES;       // loads of a wavefront for a page
   static_assert(ROWS * (RANK + kRope) * 2 <= BUF, "the rows' queries fit a page's buffer");
@@ -301,8 +304,7 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
   __shared__ uint32_t s_odd[WAVES];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
   const int col = lane & 31, half = lane >> 5, l16 = lane & 15, g16 = lane >> 4;
-  const int part = wave % kParts, rg = wave / kParts;  // second product: features, rows 32 rg ..
-  const int tg = wave % TG, rq = wave / TG;            // first: tokens 16 TB tg .., rows 16 NR rq ..
+  const int part = wave;  // first product: tokens 16 part ..; second: features
   const uint32_t lds0 = lds_address(s_mem);
   Walk walk;
   const int range = walk.start(a, lane);
@@ -313,7 +315,7 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
   // K's row of a lane (16 tokens further its key is the same), units g16 and 4 + g16.  C^T: 4 features
   // of token 8 half + l16 / 4 of the wavefront's first tile; odd tiles and tokens 4 further turn
   // the unit's bits 2 and 1.
-  const int k_tok = 16 * TB * tg + l16;
+  const int k_tok = 16 * part + l16;
   const int k_lane = k_tok * 128 + ((g16 ^ key_of(k_tok)) * 16);
   const int v_tok = 8 * half + l16 / 4;
   const int v_lane = OS * part * kStick + v_tok * 128 + (((2 * (g16 & 1) + ((lane >> 1) & 1)) ^ key_of(v_tok)) * 16) + 8 * (lane & 1);
@@ -352,15 +354,11 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
     };
     typedef std::integral_constant<int, 1> One;
     typedef std::integral_constant<int, WAVES> Shared;
-    // RG 1: a wavefront loads the sticks of its features, which only it reads in the second
-    // product, and its share of the rotated keys; else one of eight chunks of every stick.
+    // A wavefront loads the sticks of its features, which only it reads in the second product, and
+    // its share of the rotated keys.
     auto load_page = [&](int64_t page, int p, int buf) {
-      if constexpr (RG == 1) {
-        load(page, p, buf, std::integral_constant<int, OS>{}, OS * part, 0, One{});
-        load(page, p, buf, One{}, NS - 1, wave, Shared{});
-      } else {
-        load(page, p, buf, std::integral_constant<int, NS>{}, 0, wave, Shared{});
-      }
+      load(page, p, buf, std::integral_constant<int, OS>{}, OS * part, 0, One{});
+      load(page, p, buf, One{}, NS - 1, wave, Shared{});
     };
     // Queries, whole rows into the second buffer: the latent features [ROWS][RANK], then the
     // rotated ones, unit u of row r at u ^ (r & 15), u ^ (r / 2 & 7); rows that are not there
@@ -393,7 +391,7 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
     for (int n = 0; n < NR; ++n)
 #pragma unroll
       for (int s = 0; s < NQ; ++s) {
-        const int r = 16 * (NR * rq + n) + here(l16);
+        const int r = 16 * (n) + here(l16);
         const int at = 32 * s < RANK ? r * RANK * 2 + ((4 * s + g16) ^ (r & 15)) * 16
                                      : ROWS * RANK * 2 + r * kRope * 2 + ((4 * s - RANK / 8 + g16) ^ (r / 2 & 7)) * 16;
         qf[n][s] = *reinterpret_cast<const f16x8*>(s_mem + BUF + at);
@@ -403,10 +401,8 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
 #pragma unroll
       for (int n = 0; n < NR; ++n) asm volatile("" : "+v"(qf[n][s]));  // they are read
     if (threadIdx.x < ROWS) s_ref[threadIdx.x] = -INFINITY;
-    if (RG == 1) {
-      __syncthreads();
-      if (p0 + 1 < p1) load_page(next, p0 + 1, 1);
-    }
+    __syncthreads();
+    if (p0 + 1 < p1) load_page(next, p0 + 1, 1);
     f32x16 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -421,25 +417,13 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
     auto step = [&](int p, auto edge_tag) {
       constexpr bool EDGE = decltype(edge_tag)::value;
       const int buf = (p - p0) & 1;
-      if (RG == 1 && p + 1 < p1)
+      if (p + 1 < p1)
         wait_loads<SHARE>();  // the next page's
       else
         wait_loads<0>();
-      __syncthreads();  // the page is there; RG 2: the other buffer is read
-      const bool more = p + (RG == 1 ? 2 : 1) < p1;
-      if (RG == 1 && more) next = pages.at(p + 2);
-      // RG 2: the next page's chunks go out between the products below, one of eight to a
-      // wavefront: at once they would take the address unit 1100 cycles, with every wavefront
-      // waiting its turn.  (Behind the last page they read nowhere, into a buffer that nobody reads.)
-      dma_rsrc ahead;
-      uint32_t ahead_off = BUF, ahead_at = 0, ahead_to = 0;
-      if constexpr (RG == 2) {
-        ahead = dma_buffer(a.pages + next * (NS * (kStick / 2)), BUF);
-        const int t = here(lane) / 8;
-        if (more && (p + 1) * kPage + 8 * wave + t < total) ahead_off = t * 128 + (((lane & 7) ^ key_of(t)) * 16);
-        ahead_at = uniform_here(wave * 1024), ahead_to = lds0 + (buf ^ 1) * BUF + ahead_at;
-        if (p + 2 < p1) next = pages.at(p + 2);
-      }
+      __syncthreads();  // the page is there
+      const bool more = p + 2 < p1;
+      if (more) next = pages.at(p + 2);
       uint32_t odd = 0;                            // of this wavefront's tokens, new ones that hold a NaN or an infinity
       if (EDGE && a.T > 1) {
         // What a row does not attend must not meet its weight of 0: such tokens become
@@ -468,13 +452,7 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
         for (int k = 0; k < 64 / PER; ++k) bits |= static_cast<uint32_t>((all >> (PER * k)) & 1) << k;
         if (lane == 0) s_odd[wave] = bits;
         __syncthreads();
-        // (wavefront w looked at tokens 64 / WAVES w .. )
-        if constexpr (RG == 1) {
-          odd = s_odd[wave];
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) odd |= s_odd[4 * tg + k] << (8 * k);
-        }
+        odd = s_odd[wave];  // (wavefront w looked at tokens 16 w ..)
       }
 
       // The scores: sc[n][x] of row 16 (NR rq + n) + l16, token 16 TB tg + tok(x).
@@ -484,39 +462,33 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
         const uint8_t* kb = s_mem + buf * BUF;
         const int k_at[2] = {k_lane, k_lane ^ 64};
         // kAhead operands on their way; in this order, the scheduler would read each when it is due
-        constexpr int kAhead = 8, NK = NQ * TB;
-        static_assert(RG == 1 || NK % NS == 0, "a stick of the next page every so many products");
+        constexpr int kAhead = 8;
         f16x8 kf[kAhead];
-        auto k_of = [&](int x) {
-          const int s = x / TB;
-          return *reinterpret_cast<const f16x8*>(kb + k_at[s % 2] + s / 2 * kStick + x % TB * (16 * 128));
-        };
+        auto k_of = [&](int x) { return *reinterpret_cast<const f16x8*>(kb + k_at[x % 2] + x / 2 * kStick); };
 #pragma unroll
         for (int x = 0; x < kAhead; ++x) kf[x] = k_of(x);
-        f32x4 acc[2][NR][TB] = {};  // four chains: a product waits 64 cycles for the one before it and takes 16
+        f32x4 acc[2][NR] = {};  // four chains: a product waits 64 cycles for the one before it and takes 16
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int x = 0; x < NK; ++x) {
+        for (int x = 0; x < NQ; ++x) {
 #pragma unroll
           for (int n = 0; n < NR; ++n)
-            acc[x / TB % 2][n][x % TB] =
-                __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[x % kAhead], qf[n][x / TB], acc[x / TB % 2][n][x % TB], 0, 0, 0);
-          if (x + kAhead < NK) kf[x % kAhead] = k_of(x + kAhead);
-          if (RG == 2 && x % (NK / NS) == 0) dma16(ahead, ahead_to + x / (NK / NS) * kStick, ahead_off, ahead_at + x / (NK / NS) * kStick);
+            acc[x % 2][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[x % kAhead], qf[n][x], acc[x % 2][n], 0, 0, 0);
+          if (x + kAhead < NQ) kf[x % kAhead] = k_of(x + kAhead);
           __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int n = 0; n < NR; ++n)
 #pragma unroll
-          for (int x = 0; x < NT; ++x) sc[n][x] = acc[0][n][x / 4][x % 4] + acc[1][n][x / 4][x % 4];
+          for (int x = 0; x < NT; ++x) sc[n][x] = acc[0][n][x] + acc[1][n][x];
       }
       const int ln = here(lane);
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
         uint32_t seen = ~0u;
         if constexpr (EDGE) {
-          const int j0 = p * kPage + 16 * TB * tg - sq.ctx;
-          const int i = min(token_of_row(row0 + 16 * (NR * rq + n) + ln % 16), sq.n - 1);
+          const int j0 = p * kPage + 16 * part - sq.ctx;
+          const int i = min(token_of_row(row0 + 16 * (n) + ln % 16), sq.n - 1);
           seen = 0;
           if (a.mask) {
             const uint8_t* mask = a.mask + b * a.m_sb + max(i, 0) * a.m_si;
@@ -542,7 +514,7 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
           mx = fmaxf(mx, v);
         }
         mx = xor32_max(xor16_max(mx));
-        if (ln / 16 == n) s_max[tg * ROWS + 16 * (NR * rq + n) + ln % 16] = mx;
+        if (ln / 16 == n) s_max[part * ROWS + 16 * (n) + ln % 16] = mx;
       }
       // Weights relative to the reference as it is.  They round to fp16 for the product (a
       // relative 2^-12 on average); their sum stays in fp32.
@@ -552,7 +524,7 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
         for (int n = 0; n < NR; ++n) {
           const float mu = m[n] == -INFINITY ? 0.f : m[n];  // a row that has attended nothing yet: weights 0
           add[n] = 0.f;
-          const int row = 16 * (NR * rq + n) + ln % 16;
+          const int row = 16 * (n) + ln % 16;
 #pragma unroll
           for (int x = 0; x < NT; x += 4) {
             f16x4 w4;
@@ -562,7 +534,7 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
               add[n] += w;
               w4[e] = static_cast<_Float16>(w);
             }
-            const int t = 16 * TB * tg + tok(x, ln);  // of 4
+            const int t = 16 * part + tok(x, ln);  // of 4
             *reinterpret_cast<f16x4*>(&s_p[row * kPage + (((t / 8) ^ row_key(row)) * 8) + t % 8]) = w4;
           }
         }
@@ -581,7 +553,7 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
           return top > s_ref[r] + kAbove ? top - kBelow : s_ref[r];  // its own: what others attend does not turn its roundings
         };
         auto factor = [](float from, float to) { return from == -INFINITY ? 0.f : exp2_of(from - to); };
-        const int c = kTile * rg + here(col), th = here(threadIdx.x) % ROWS;
+        const int c = here(col), th = here(threadIdx.x) % ROWS;
         const float alpha = factor(s_ref[c], ref_of(c)), ref = ref_of(th);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
@@ -589,7 +561,7 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
           for (int x = 0; x < 16; ++x) o[dt][x] *= alpha;
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-          const float to = ref_of(16 * (NR * rq + n) + ln % 16);
+          const float to = ref_of(16 * (n) + ln % 16);
           l[n] *= factor(m[n], to);
           m[n] = to;
         }
@@ -601,16 +573,15 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
 #pragma unroll
       for (int n = 0; n < NR; ++n) l[n] += add[n];
       const int v_at[2] = {buf * BUF + v_lane, (buf * BUF + v_lane) ^ 64};
-      // RG 1: sticks that no wavefront reads any more take the page after the next.
-      if (RG == 1 && more) load(next, p + 2, buf, One{}, NS - 1, wave, Shared{});
+      // Sticks that no wavefront reads any more take the page after the next.
+      if (more) load(next, p + 2, buf, One{}, NS - 1, wave, Shared{});
       f16x8 w[4];
 #pragma unroll
-      for (int s = 0; s < 4; ++s) w[s] = *reinterpret_cast<const f16x8*>(&s_p[(kTile * rg + ln % 32) * kPage + (((2 * s + ln / 32) ^ row_key(ln)) * 8)]);
+      for (int s = 0; s < 4; ++s) w[s] = *reinterpret_cast<const f16x8*>(&s_p[(ln % 32) * kPage + (((2 * s + ln / 32) ^ row_key(ln)) * 8)]);
       // Operand x of C^T: tile v_tile(x) of the wavefront (two to a stick), tokens 16 v_step(x) .. +
-      // 15.  RG 1: stick after stick; else tiles take turns, so that none waits for its last
-      // product.
-      auto v_tile = [](int x) { return RG == 1 ? x / 8 * 2 + x % 2 : x % DT; };
-      auto v_step = [](int x) { return RG == 1 ? x / 2 % 4 : x / DT; };
+      // 15, stick after stick.
+      auto v_tile = [](int x) { return x / 8 * 2 + x % 2; };
+      auto v_step = [](int x) { return x / 2 % 4; };
       constexpr int kAhead = 6, NV = 8 * OS;
       f16x8 vf[kAhead];
       auto v_of = [&](int x) {
@@ -627,8 +598,8 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
         y = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[x % kAhead], w[v_step(x)], y, 0, 0, 0);
         if (x + kAhead < NV) vf[x % kAhead] = v_of(x + kAhead);
         __builtin_amdgcn_sched_barrier(0);
-        // RG 1: a stick is read: this wavefront alone reads it, in this product
-        if (RG == 1 && x % 8 == 7 && more) load(next, p + 2, buf, One{}, OS * part + x / 8, 0, One{});
+        // a stick is read: this wavefront alone reads it, in this product
+        if (x % 8 == 7 && more) load(next, p + 2, buf, One{}, OS * part + x / 8, 0, One{});
       }
     };
     // Every row attends every token below ctx.
@@ -637,15 +608,15 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
     for (int p = whole; p < p1; ++p) step(p, std::true_type{});
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      const int r = 16 * (NR * rq + n) + here(l16);
+      const int r = 16 * (n) + here(l16);
       const bool live = token_of_row(row0 + r) < sq.n;
       l[n] = xor32_sum(xor16_sum(l[n]));
       if (!live) l[n] = 0.f;
       if ((pages.poisoned || sq.bad) && live) l[n] = NAN;
-      if (g16 == n) s_sum[tg * ROWS + r] = l[n];
+      if (g16 == n) s_sum[part * ROWS + r] = l[n];
     }
     __syncthreads();
-    const int out_row = kTile * rg + col;
+    const int out_row = col;
     float L = 0.f;
 #pragma unroll
     for (int k = 0; k < TG; ++k) L += s_sum[k * ROWS + out_row];
@@ -676,6 +647,348 @@ __global__ __launch_bounds__(RG * kParts * 64, RG) void latent_kernel(LatentArgs
     }
     walk.advance(a, pc);
     wait_loads<0>();  // (those behind the last page, too)
+    __syncthreads();  // LDS is read before the next piece writes it
+  }
+  if (threadIdx.x == 0) {
+    int32_t* x = bounds_of(a, range, RANK);
+    x[0] = open_b, x[1] = open_rb, x[2] = ended;
+  }
+}
+
+// 64 rows, in two groups of four wavefronts, one of each on a SIMD: while one group has the scores
+// and weights of a tile of 32 tokens, the other multiplies the weights of the tile before it with C,
+// so that neither's waits leave the matrix cores idle (in step, 8 wavefronts took 76 us for 32 x 4096
+// tokens x 128 heads, so 72).
+//   scores: a wavefront has 16 rows x the tile, Q in registers
+//   sums:   a wavefront has 64 rows x a quarter of O's features, in 128 registers
+// Four tiles lie in LDS: one in each product, two on their way.  A load into LDS of 1 KiB holds up
+// its wavefront 25 cycles times those in line, so that the second group has two thirds of them, before
+// its products, and the first one the others, behind its weights (between the products 85 us, all
+// in the second group 79).
+template <int RANK>
+__global__ __launch_bounds__(2 * kParts * 64, 2) void latent_rows_kernel(LatentArgs a) {
+  constexpr int ROWS = 64, WAVES = 2 * kParts, TOKS = 32;
+  constexpr int NS = (RANK + kRope) / 64;     // sticks
+  constexpr int OS = RANK / 64 / kParts;      // sticks of O of a wavefront
+  constexpr int DT = 2 * OS;                  // tiles of it, 32 features each
+  constexpr int NQ = (RANK + kRope) / 32;     // steps of the first product
+  constexpr int STICK = TOKS * 128, TILE = NS * STICK;
+  constexpr int LOADS_A = NS / 3, LOADS = NS - LOADS_A;  // of a wavefront of the first group for a tile, of the second
+  static_assert(ROWS * (RANK + kRope) * 2 == 2 * TILE, "the rows' queries fit the buffers of two tiles");
+  __shared__ __align__(16) uint8_t s_mem[4 * TILE];
+  __shared__ __align__(16) _Float16 s_p[ROWS * 64];  // weights of two tiles: 4 units of 8 tokens each, unit u of a row at u ^ row_key
+  __shared__ float s_alpha[2][ROWS];                 // of two tiles: what O is to be multiplied with before
+  __shared__ int s_moved[2][4];                      // whether any of 16 rows is
+  __shared__ float s_ref[ROWS], s_sum[ROWS];         // at the end
+  __shared__ uint32_t s_odd[WAVES];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const int col = lane & 31, half = lane >> 5, l16 = lane & 15, g16 = lane >> 4;
+  const bool first = wave < kParts;
+  const int part = wave % kParts;  // first group: rows 16 part ..; second: features
+  const uint32_t lds0 = lds_address(s_mem);
+  Walk walk;
+  const int range = walk.start(a, lane);
+  if (range < 0) return;
+  if (threadIdx.x == 0 && range == 0) *bounds_of(a, a.ranges, RANK) = walk.used;
+  int open_b = -1, open_rb = 0, ended = 0;
+
+  for (; walk.u < walk.end;) {
+    const Walk::Piece pc = walk.piece(a);
+    const int b = walk.b;
+    const Seq sq = walk.seq;
+    const int total = sq.ctx + sq.n, row0 = pc.rb * ROWS;
+    const int t0 = 2 * pc.page0, n = max(min(2 * pc.page1, (total + TOKS - 1) / TOKS) - t0, 0);  // tiles t0 .. t0 + n
+    Pages pages(a, b, lane, pc.page0);
+    int64_t page = 0;  // of the tile that is loaded next
+    auto token_of_row = [&](int row) {  // its new token; sq.n or more: none
+      return row < a.rows ? static_cast<int>(fdiv(row, a.by_h)) : sq.n;
+    };
+    // A group's loads of tile t0 + i: sticks, 8 tokens to a wavefront.  Tokens that do not exist are
+    // zeros.
+    auto load_tile = [&](int i) {
+      if ((t0 + i) % 2 == 0) page = pages.at((t0 + i) / 2);
+      const int ln = here(lane), t = ln / 8, at = (t0 + i) % 2 * TOKS + 8 * part;
+      const uint32_t off = (t0 + i) * TOKS + 8 * part + t < total ? t * 128 + (((ln & 7) ^ key_of(t)) * 16) : NS * kStick;
+      const dma_rsrc r = dma_buffer(a.pages + page * (NS * (kStick / 2)), NS * kStick);
+      const uint32_t to = lds0 + (i & 3) * TILE + part * 1024;
+      if (first)
+#pragma unroll
+        for (int k = LOADS; k < NS; ++k) dma16(r, to + k * STICK, off, k * kStick + at * 128);
+      else
+#pragma unroll
+        for (int k = 0; k < LOADS; ++k) dma16(r, to + k * STICK, off, k * kStick + at * 128);
+    };
+    // Queries, whole rows into the last two buffers: the latent features [ROWS][RANK], then the
+    // rotated ones, unit u of row r at u ^ (r & 15), u ^ (r / 2 & 7); rows that are not there
+    // are zeros.
+    constexpr int Q_AT = 2 * TILE;
+    if (n > 0) {
+#pragma unroll 2
+      for (int k = 0; k < ROWS / WAVES; ++k) {
+        const int r = k * WAVES + wave, row = row0 + r, i = token_of_row(row);
+        const int64_t h = row - i * a.H;
+        const bool there = i < sq.n;
+        if (lane < RANK / 8)
+          dma16(dma_buffer(a.q + (there ? b * a.q_sb + i * a.q_st + h * a.q_sh : 0), RANK * 2), lds0 + Q_AT + r * RANK * 2,
+                there ? (lane ^ (r & 15)) * 16 : RANK * 2, 0);
+        if (lane < kRope / 8)
+          dma16(dma_buffer(a.qr + (there ? b * a.qr_sb + i * a.qr_st + h * a.qr_sh : 0), kRope * 2),
+                lds0 + Q_AT + ROWS * RANK * 2 + r * kRope * 2, there ? (lane ^ (r / 2 & 7)) * 16 : kRope * 2, 0);
+      }
+      load_tile(0);
+      if (n > 1) load_tile(1);
+    }
+    wait_loads<0>();
+    __syncthreads();
+
+    // What a row does not attend must not meet its weight of 0: new tokens that hold a NaN or an
+    // infinity become zeros, and the rows that attend them NaN.  All wavefronts, before a tile's first
+    // product; bit t of the result: token t.
+    auto odd_of = [&](int i) -> uint32_t {
+      const int th = here(threadIdx.x), t = th / 16, at = (t0 + i) * TOKS + t;
+      uint8_t* x = s_mem + (i & 3) * TILE + t * 128 + (th % 8) * 16;
+      uint32_t found = 0;
+      const bool fresh = at >= sq.ctx && at < total;
+      for (int s = th / 8 % 2; s < NS && fresh; s += 2) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(x + s * STICK);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) found |= (w[e] & 0x7c007c00u) + 0x04000400u;
+      }
+      const uint64_t lanes = __ballot((found & 0x80008000u) != 0);
+      const bool bad = (lanes >> (lane & 48)) & 0xffff;
+      for (int s = th / 8 % 2; s < NS && bad; s += 2) *reinterpret_cast<u32x4*>(x + s * STICK) = u32x4{0, 0, 0, 0};
+      const uint64_t all = __ballot(bad);
+      if (lane == 0) s_odd[wave] = (all & 1) | (all >> 15 & 2) | (all >> 30 & 4) | (all >> 45 & 8);
+      __syncthreads();
+      uint32_t odd = 0;
+#pragma unroll
+      for (int k = 0; k < WAVES; ++k) odd |= s_odd[k] << (4 * k);
+      return odd;
+    };
+    // Every row attends every token below ctx.
+    auto edge_at = [&](int i) { return (t0 + i + 1) * TOKS > sq.ctx; };
+
+    if (first) {
+      f16x8 qf[NQ];
+#pragma unroll
+      for (int s = 0; s < NQ; ++s) {
+        const int r = 16 * part + here(l16);
+        const int at = 32 * s < RANK ? r * RANK * 2 + ((4 * s + g16) ^ (r & 15)) * 16
+                                     : ROWS * RANK * 2 + r * kRope * 2 + ((4 * s - RANK / 8 + g16) ^ (r / 2 & 7)) * 16;
+        qf[s] = *reinterpret_cast<const f16x8*>(s_mem + Q_AT + at);
+      }
+#pragma unroll
+      for (int s = 0; s < NQ; ++s) asm volatile("" : "+v"(qf[s]));  // they are read
+      __syncthreads();
+      const int k_lane = l16 * 128 + ((g16 ^ key_of(l16)) * 16);
+      float m = -INFINITY, l = 0.f;  // of a lane's row; l: of this lane's tokens
+      auto step = [&](int i, auto edge_tag) {
+        constexpr bool EDGE = decltype(edge_tag)::value;
+        uint32_t odd = 0;
+        if (EDGE && a.T > 1) odd = odd_of(i);
+        // The scores: sc[x] of row 16 part + l16, token tok(x).
+        auto tok = [&](int x, int ln) { return 16 * (x / 4) + 4 * (ln / 16) + x % 4; };
+        float sc[8];
+        {
+          const int kb = (i & 3) * TILE + k_lane, k_at[2] = {kb, kb ^ 64};
+          // kAhead operands on their way; in this order, the scheduler would read each when it is due
+          constexpr int kAhead = 8, NK = 2 * NQ;
+          f16x8 kf[kAhead];
+          auto k_of = [&](int x) { return *reinterpret_cast<const f16x8*>(s_mem + k_at[x / 2 % 2] + x / 4 * STICK + x % 2 * (16 * 128)); };
+#pragma unroll
+          for (int x = 0; x < kAhead; ++x) kf[x] = k_of(x);
+          f32x4 acc[2][2] = {};  // four chains: a product waits 64 cycles for the one before it and takes 16
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int x = 0; x < NK; ++x) {
+            acc[x / 2 % 2][x % 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[x % kAhead], qf[x / 2], acc[x / 2 % 2][x % 2], 0, 0, 0);
+            if (x + kAhead < NK) kf[x % kAhead] = k_of(x + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+#pragma unroll
+          for (int x = 0; x < 8; ++x) sc[x] = acc[0][x / 4][x % 4] + acc[1][x / 4][x % 4];
+        }
+        const int ln = here(lane);
+        uint32_t seen = ~0u;
+        if constexpr (EDGE) {
+          const int j0 = (t0 + i) * TOKS - sq.ctx, q = min(token_of_row(row0 + 16 * part + ln % 16), sq.n - 1);
+          seen = 0;
+          if (a.mask) {
+            const uint8_t* mask = a.mask + b * a.m_sb + max(q, 0) * a.m_si;
+            uint8_t keep[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) keep[x] = mask[min(max(j0 + tok(x, ln), 0), a.T - 1) * a.m_sj];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              const int j = j0 + tok(x, ln);
+              seen |= static_cast<uint32_t>(j < 0 || (j < sq.n && keep[x] != 0)) << x;
+            }
+          } else {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) seen |= static_cast<uint32_t>(j0 + tok(x, ln) <= q) << x;
+          }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          float v = sc[x] * a.scale_log2;
+          if (EDGE) v = !((seen >> x) & 1) ? -INFINITY : (odd >> tok(x, ln)) & 1 ? NAN : v;
+          sc[x] = v;
+          mx = fmaxf(mx, v);
+        }
+        mx = xor32_max(xor16_max(mx));
+        // Where a row's scores pass its reference too far, it moves.
+        const bool moves = mx > m + kAbove;
+        float alpha = 1.f;
+        if (moves) {
+          const float to = mx - kBelow;
+          alpha = m == -INFINITY ? 0.f : exp2_of(m - to);
+          m = to;
+        }
+        const int any = __any(moves);
+        if (ln < 16) s_alpha[i & 1][16 * part + ln] = alpha;
+        if (ln == 0) s_moved[i & 1][part] = any;
+        // Weights round to fp16 for the product (a relative 2^-12 on average); their sum stays in fp32.
+        const float mu = m == -INFINITY ? 0.f : m;  // a row that has attended nothing yet: weights 0
+        float add = 0.f;
+        const int row = 16 * part + ln % 16;
+#pragma unroll
+        for (int x = 0; x < 8; x += 4) {
+          f16x4 w4;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float w = exp2_of(sc[x + e] - mu);
+            add += w;
+            w4[e] = static_cast<_Float16>(w);
+          }
+          const int t = TOKS * (i & 1) + tok(x, ln);  // of 4
+          *reinterpret_cast<f16x4*>(&s_p[row * 64 + (((t / 8) ^ row_key(row)) * 8) + t % 8]) = w4;
+        }
+        l = l * alpha + add;
+        if (i + 2 < n) {
+          load_tile(i + 2);
+          wait_loads<LOADS_A>();  // tile i + 1 is there
+        } else {
+          wait_loads<0>();
+        }
+        __syncthreads();
+      };
+      int i = 0;
+      for (; i < n && !edge_at(i); ++i) step(i, std::false_type{});
+      for (; i < n; ++i) step(i, std::true_type{});
+      const int r = 16 * part + here(l16);
+      const bool live = token_of_row(row0 + r) < sq.n;
+      l = xor32_sum(xor16_sum(l));
+      if (!live) l = 0.f;
+      if ((pages.poisoned || sq.bad) && live) l = NAN;
+      if (g16 == 0) s_sum[r] = l, s_ref[r] = l == 0.f ? -INFINITY : m;
+      if (n > 0) __syncthreads();  // the second group's last tile
+      __syncthreads();
+    } else {
+      __syncthreads();  // the queries are read
+      const int v_tok = 8 * half + l16 / 4;
+      const int v_lane = OS * part * STICK + v_tok * 128 + (((2 * (g16 & 1) + ((lane >> 1) & 1)) ^ key_of(v_tok)) * 16) + 8 * (lane & 1);
+      auto tr = [&](int at) {
+        return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(s_mem + at));
+      };
+      f32x16 o[2][DT];
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) o[g][dt][x] = 0.f;
+      if (n > 0) {
+        if (edge_at(0) && a.T > 1) odd_of(0);
+        if (n > 2) load_tile(2);
+        n > 2 ? wait_loads<LOADS>() : wait_loads<0>();  // tile 1 is there
+        __syncthreads();
+      }
+      for (int i = 1; i <= n; ++i) {
+        if (i < n && edge_at(i) && a.T > 1) odd_of(i);
+        const bool more = i + 2 < n;
+        {
+          const int j = i - 1, ln = here(lane), c = ln % 32;
+          int moved = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) moved |= s_moved[j & 1][k];
+          if (__any(moved)) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const float alpha = s_alpha[j & 1][32 * g + c];
+#pragma unroll
+              for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) o[g][dt][x] *= alpha;
+            }
+          }
+          f16x8 w[2][2];
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+              w[g][s] = *reinterpret_cast<const f16x8*>(&s_p[(32 * g + c) * 64 + (((4 * (j & 1) + 2 * s + ln / 32) ^ row_key(c)) * 8)]);
+          // Operand x of C^T: tile x % DT of the wavefront (two to a stick), tokens 16 (x / DT) .. + 15.
+          const int vb = (j & 3) * TILE + v_lane;
+          constexpr int kAhead = 4, NV = 2 * DT;
+          f16x8 vf[kAhead];
+          auto v_of = [&](int x) {
+            const int at = x % DT / 2 * STICK + x / DT * 16 * 128, turn = x & 1 ? 64 : 0;
+            const s16x4 lo = tr((vb ^ turn) + at), hi = tr((vb ^ turn ^ 32) + at + 4 * 128);
+            return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+          };
+#pragma unroll
+          for (int x = 0; x < kAhead; ++x) vf[x] = v_of(x);
+          __builtin_amdgcn_sched_barrier(0);
+          if (more) load_tile(i + 2);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int x = 0; x < NV; ++x) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+              o[g][x % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[x % kAhead], w[g][x / DT], o[g][x % DT], 0, 0, 0);
+            if (x + kAhead < NV) vf[x % kAhead] = v_of(x + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        more ? wait_loads<LOADS>() : wait_loads<0>();  // tile i + 1 is there
+        __syncthreads();
+      }
+      __syncthreads();  // the rows' sums
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int out_row = 32 * g + col;
+        const float L = s_sum[out_row], M = s_ref[out_row];
+        if (pc.begins && pc.ends) {
+          if (row0 + out_row < a.rows)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                store_row4<RANK>(a, b, row0 + out_row, 32 * (DT * part + dt) + 8 * x + 4 * half,
+                                 f32x4{o[g][dt][4 * x], o[g][dt][4 * x + 1], o[g][dt][4 * x + 2], o[g][dt][4 * x + 3]}, M, L);
+        } else {
+          float* slot = slot_of(a, 2 * range + (pc.begins ? 1 : 0), RANK);
+          if (row0 + out_row < a.rows)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                *reinterpret_cast<f32x4*>(slot + (((g * kParts + part) * DT + dt) * 4 + x) * 256 + lane * 4) =
+                    f32x4{o[g][dt][4 * x], o[g][dt][4 * x + 1], o[g][dt][4 * x + 2], o[g][dt][4 * x + 3]};
+          if (part == 0 && half == 0) {
+            float* ml = slot + ROWS * RANK + out_row * 2;
+            ml[0] = M, ml[1] = L;
+          }
+        }
+      }
+    }
+    if (!(pc.begins && pc.ends)) {
+      if (pc.begins) open_b = b, open_rb = pc.rb;
+      if (pc.ends) ended = 1;
+    }
+    walk.advance(a, pc);
+    wait_loads<0>();
     __syncthreads();  // LDS is read before the next piece writes it
   }
   if (threadIdx.x == 0) {
@@ -718,7 +1031,7 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentArgs a) {
 }
 
 struct Plan {
-  int groups;  // RG
+  int groups;  // of 32 rows to a workgroup
   int row_blocks, block_rows, ranges;
   size_t ws_bytes;
 };
@@ -730,7 +1043,7 @@ Plan plan_of(int B, int T, int H, int rank, int max_tokens) {
   p.block_rows = kTile * p.groups;
   p.row_blocks = static_cast<int>((rows + p.block_rows - 1) / p.block_rows);
   // One workgroup to a CU, and no more than there could be work for.
-  const double most = static_cast<double>(B) * p.row_blocks * (kStart + std::max(pages_of(max_tokens), 1));
+  const double most = static_cast<double>(B) * p.row_blocks * (Walk::kOpen + std::max(pages_of(max_tokens), 1));
   p.ranges = static_cast<int>(std::max(1., std::min(256., most / Walk::kLeast)));
   p.ws_bytes = static_cast<size_t>(2 * p.ranges) * slot_floats(p.block_rows, rank) * 4 + 16 * (static_cast<size_t>(p.ranges) + 1);
   return p;
@@ -744,9 +1057,9 @@ bool sizes_ok(int B, int T, int H, int max_ctx) {
 template <int RANK>
 void launch(const LatentArgs& a, int groups, dim3 grid, hipStream_t st) {
   if (groups == 1)
-    latent_kernel<RANK, 1><<<grid, kParts * 64, 0, st>>>(a);
+    latent_kernel<RANK><<<grid, kParts * 64, 0, st>>>(a);
   else
-    latent_kernel<RANK, 2><<<grid, 2 * kParts * 64, 0, st>>>(a);
+    latent_rows_kernel<RANK><<<grid, 2 * kParts * 64, 0, st>>>(a);
 }
 
 }  // namespace
@@ -794,7 +1107,7 @@ extern "C" int spyre_paged_latent_attn(const void* q, const int64_t* q_strides, 
   a.ranges = p.ranges;
   const int64_t of_all = static_cast<int64_t>(B) * p.row_blocks;
   a.each = of_all % p.ranges == 0 ? static_cast<int>(of_all / p.ranges) : 0;
-  SPYRE_REQUIRE(static_cast<double>(of_all) * (pages_of(max_context_len + T) + kStart + 1) < (1 << 30), SPYRE_EUNSUPPORTED,
+  SPYRE_REQUIRE(static_cast<double>(of_all) * (pages_of(max_context_len + T) + Walk::kOpen + 1) < (1 << 30), SPYRE_EUNSUPPORTED,
                 "too many pages or rows");
   a.by_h = make_fastdiv(static_cast<uint32_t>(H));
   a.by_blocks = make_fastdiv(static_cast<uint32_t>(p.row_blocks)), a.by_ranges = make_fastdiv(static_cast<uint32_t>(p.ranges));
