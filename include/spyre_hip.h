@@ -564,7 +564,8 @@ int spyre_latent_read_f16(const void* cache, const int32_t* block_table, int64_t
  * does not attend does not reach it, whatever it holds; a row that attends a new
  * token with a NaN or an infinity is NaN.
  *   q [B, T, H, rank], q_rope [B, T, H, 64] : fp16, feature stride 1, strides {b, t, h}
- *           multiples of 8 elements, 16-byte aligned
+ *           multiples of 8 elements, 16-byte aligned; {t, h} not negative, 64 of a
+ *           sequence's (t, h) within 2^30 elements
  *   mask  : bool [B, T, T], strides {b, i, j} in bytes, 0 to broadcast
  *   out   : [B, T, H, rank] fp16, lse: optional fp32 [B, T, H]; contiguous
  * A context above max_context_len and a page that the table does not name

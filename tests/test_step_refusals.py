@@ -98,7 +98,8 @@ PAGED = dict(q=PTR, qs=ST, qr=PTR, qrs=ST, cache=PTR, bt=PTR, bts=4, pps=4, ctx=
 @pytest.mark.parametrize("change,code", [
     ({"q": None}, EINVAL), ({"qr": None}, EINVAL), ({"cache": None}, EINVAL), ({"bt": None}, EINVAL), ({"ctx": None}, EINVAL),
     ({"out": None}, EINVAL), ({"mask": PTR}, EINVAL), ({"q": PTR + 8}, EINVAL), ({"out": PTR + 2}, EINVAL),
-    ({"qs": strides(64, 4, 64)}, EINVAL), ({"H": 0}, EINVAL), ({"pages": 0}, EINVAL), ({"max": -1}, EINVAL), ({"B": -1}, EINVAL),
+    ({"qs": strides(64, 4, 64)}, EINVAL), ({"qs": strides(64, 1 << 30, 64)}, EUNSUPPORTED),
+    ({"qrs": strides(64, 64, -64)}, EUNSUPPORTED), ({"H": 0}, EINVAL), ({"pages": 0}, EINVAL), ({"max": -1}, EINVAL), ({"B": -1}, EINVAL),
     ({"rank": 384}, EUNSUPPORTED), ({"T": 1 << 30}, EUNSUPPORTED), ({"max": (1 << 31) - 66}, EUNSUPPORTED),
     ({"B": 1 << 20, "max": 1 << 20}, EUNSUPPORTED), ({"ws": None}, ENOSPC), ({"wsb": 64}, ENOSPC), ({"ws": PTR + 4}, ENOSPC),
     ({"B": 0, "q": None}, 0), ({"T": 0, "q": None}, 0)])

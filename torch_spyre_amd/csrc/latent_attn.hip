@@ -22,7 +22,7 @@
 // tokens of 64 rows take 0.85 us, of which the matrix cores 0.45 and the loads' way into LDS as much;
 // the start of a range 6 us, the parts' way to memory and back with the second launch 17); 64 x
 // 128-16384 tokens x 16 heads 125 us (629 MB, 5.0 TB/s: memory); 16 x 500-6000 tokens x 1-7 new x 32
-// heads 52; 1 x 700 x 16 heads 18.4, of which two launches 9.
+// heads 52; 1 x 700 x 16 heads 17.4, of which two launches 9.
 
 #include <hip/hip_runtime.h>
 
@@ -67,9 +67,9 @@ struct LatentArgs {
   float* ws;
   int B, T, H, rows, max_ctx, draft_keys;
   float scale_log2;
-  int row_blocks, block_rows;  // of a sequence with T new tokens; a block's
-  int ranges, each;            // at most; row blocks of a range where none is cut
-  FastDiv by_h, by_blocks, by_ranges;
+  int row_blocks, block_rows, block_shift;  // of a sequence with T new tokens; a block's
+  int ranges;                               // at most
+  FastDiv by_h, by_ranges;
 };
 
 // How the work is shared out, as in PageWalk, with row blocks in the place of KV heads: a row
@@ -77,10 +77,11 @@ struct LatentArgs {
 // new tokens (zeros) one unit.  Range r of R is the units [all r / R, all (r + 1) / R), row block
 // after row block, sequence after sequence: with a workgroup to each row block of a range of
 // pages half of them had no rows where sequences had 1 to 7 new tokens (16 x 7 x 32 heads 64 us, so
-// 57).  A bound that would leave kFew pages or less of a row block moves to its end.
+// 57).  A bound that would leave kFew pages or less of a row block moves to its end (fewer where
+// a range has few).
 struct Walk {
-  // kLeast: units of a range, at least: one sequence of 700 tokens and 16 heads 18.4 us (4: 21.4, 6:
-  // 25), 4 of 3000 23.0 (23.8, 26.2).  kOpen: 32 x 4096 tokens x 128 heads 66 us with 1, 2 and 4; the
+  // kLeast: units of a range, at least: one sequence of 700 tokens and 16 heads 17.4 us (4: 20.5, 6:
+  // 24), 4 of 3000 22.4 (23.2, 25.5).  kOpen: 32 x 4096 tokens x 128 heads 66 us with 1, 2 and 4; the
   // drafts above 56, 54, 52.  kFew: 300 x 10-900 tokens x 64 heads 68 us (4: 72).
   static constexpr int kLeast = 3, kOpen = 4, kFew = 2;
   int used;           // ranges that have any units
@@ -89,44 +90,21 @@ struct Walk {
   Seq seq;            // what it holds
   int size, live;     // units of a row block that has rows; such row blocks
 
-  __device__ __forceinline__ static int live_of(const LatentArgs& a, int n) { return (n * a.H + a.block_rows - 1) / a.block_rows; }
-  struct Lane {  // a sequence a lane
-    int ctx = 0, count = 0, units = 0, top = 0;
-  };
-  __device__ __forceinline__ static Lane lane_of(const LatentArgs& a, int b) {
-    Lane x;
-    if (b < a.B) {
-      x.ctx = a.ctx[b], x.count = a.counts ? a.counts[b] : a.T;
-      const Seq s = seq_of(a, x.ctx, x.count);
-      const int live = live_of(a, s.n);
-      x.top = kOpen + s.pages;
-      x.units = live * x.top + a.row_blocks - live;
-      if (live < a.row_blocks) x.top = 1 << 29;
-    }
-    return x;
-  }
-  __device__ __forceinline__ void take(const LatentArgs& a, int ctx, int count) {
-    seq = seq_of(a, ctx, count);
-    live = live_of(a, seq.n), size = kOpen + seq.pages;
+  __device__ __forceinline__ static int live_of(const LatentArgs& a, int n) { return (n * a.H + a.block_rows - 1) >> a.block_shift; }
+  __device__ __forceinline__ static int units_of(const LatentArgs& a, const Seq& s) {
+    const int live = live_of(a, s.n);
+    return live * (kOpen + s.pages) + a.row_blocks - live;
   }
   __device__ __forceinline__ int units(const LatentArgs& a) const { return live * size + a.row_blocks - live; }
-  __device__ __forceinline__ void find(const LatentArgs& a, int lane, const Lane& first64, int unit) {
-    base = 0;
-    for (int c = 0;; c += 64) {
-      const Lane x = c == 0 ? first64 : lane_of(a, c + lane);
-      const int sum = scan64(x.units);
-      const uint64_t past = __builtin_amdgcn_ballot_w64(base + sum > unit);
-      if (past || c + 64 >= a.B) {
-        const int i = past ? __builtin_ctzll(past) : (a.B - 1) % 64;
-        b = c + i;
-        take(a, __builtin_amdgcn_readlane(x.ctx, i), __builtin_amdgcn_readlane(x.count, i));
-        base += __builtin_amdgcn_readlane(sum, i) - units(a);
-        return;
-      }
-      base += __builtin_amdgcn_readlane(sum, 63);
+  // A sequence a lane.
+  __device__ __forceinline__ static void lane_of(const LatentArgs& a, int b, int& ctx, int& count, int& units) {
+    ctx = count = units = 0;
+    if (b < a.B) {
+      ctx = a.ctx[b], count = a.counts ? a.counts[b] : a.T;
+      units = units_of(a, seq_of(a, ctx, count));
     }
   }
-  // A bound where it belongs, after find() of it: no piece of few pages.
+  // A bound where it belongs, in its sequence: no piece of few pages.
   __device__ __forceinline__ int placed(int unit, int few) const {
     const int in = unit - base;
     if (in >= live * size) return unit;
@@ -134,45 +112,49 @@ struct Walk {
     const int g0 = unit - at, g1 = g0 + size;
     return at - kOpen <= few ? g0 : g1 - unit <= few ? g1 : unit;
   }
-  // This workgroup's range; -1: none.  Those that follow one another run in one XCD.
+  // This workgroup's range; -1: none.  Those that follow one another run in one XCD.  (Loops
+  // and one copy of each step: what a kernel runs once, it waits for to be fetched.)
   __device__ __forceinline__ int start(const LatentArgs& a, int lane) {
-    const Lane x = lane_of(a, lane);
-    int total = 0, largest = 0;
+    int total = 0, ctx, count, sum;
+#pragma unroll 1
     for (int c = 0; c < a.B; c += 64) {
-      const Lane y = c == 0 ? x : lane_of(a, c + lane);
-      total += y.units, largest = max(largest, y.top);
+      lane_of(a, c + lane, ctx, count, sum);
+      sum = scan64(sum);
+      total += __builtin_amdgcn_readlane(sum, 63);
     }
-    total = __builtin_amdgcn_readlane(scan64(total), 63), largest = max64(largest);
-    const int per = max(static_cast<int>(fdiv(total, a.by_ranges)), kLeast);
-    // Where a whole number of row blocks to a range is within an eighth of it, none is cut.
-    const bool uncut = a.each > 0 && static_cast<int64_t>(largest) * a.each <= per + per / 8;
-    used = uncut ? a.ranges : min(max(total / kLeast, 1), a.ranges);
+    const bool many = total >= kLeast * a.ranges;
+    used = many ? a.ranges : max(total / kLeast, 1);
     const int xcd = blockIdx.x & 7, i = blockIdx.x >> 3;
     if (i >= used / 8 + (xcd < used % 8)) return -1;
     const int r = xcd * (used / 8) + min(xcd, used % 8) + i;
-    if (uncut) {
-      const int first = r * a.each, at = static_cast<int>(fdiv(first, a.by_blocks));
-      base = 0;
-      for (int c = 0; c <= at; c += 64) {
-        const Lane y = c == 0 ? x : lane_of(a, c + lane);
-        base += __builtin_amdgcn_readlane(scan64(c + lane < at ? y.units : 0), 63);
+    const int share = many ? static_cast<int>(fdiv(total, a.by_ranges)) : kLeast, rest = many ? total - share * a.ranges : 0;
+#pragma unroll 1
+    for (int k = 1; k >= 0; --k) {
+      int unit = (r + k) * share + static_cast<int>(fdiv((r + k) * rest, a.by_ranges));
+      if (r + k == used) unit = total;
+      if (unit < total) {
+        base = 0;
+#pragma unroll 1
+        for (int c = 0;; c += 64) {
+          if (a.B > 64) {
+            lane_of(a, c + lane, ctx, count, sum);
+            sum = scan64(sum);
+          }
+          const uint64_t past = __builtin_amdgcn_ballot_w64(base + sum > unit);
+          if (past || c + 64 >= a.B) {
+            const int l = past ? __builtin_ctzll(past) : (a.B - 1) % 64;
+            b = c + l;
+            seq = seq_of(a, __builtin_amdgcn_readlane(ctx, l), __builtin_amdgcn_readlane(count, l));
+            live = live_of(a, seq.n), size = kOpen + seq.pages;
+            base += __builtin_amdgcn_readlane(sum, l) - units(a);
+            break;
+          }
+          base += __builtin_amdgcn_readlane(sum, 63);
+        }
+        unit = placed(unit, min(max(share - kOpen, 0) / 2, kFew));
       }
-      b = at;
-      take(a, __builtin_amdgcn_readfirstlane(a.ctx[b]), a.counts ? __builtin_amdgcn_readfirstlane(a.counts[b]) : a.T);
-      u = end = base + (first - at * a.row_blocks) * size;
-      for (int k = 0; k < a.each; ++k) end += kOpen + seq_at(a, static_cast<int>(fdiv(first + k, a.by_blocks))).pages;
-      return r;
+      (k ? end : u) = unit;
     }
-    // (total below 2^30: products of 40 bits)
-    u = static_cast<int>(static_cast<int64_t>(total) * r / used);
-    end = static_cast<int>(static_cast<int64_t>(total) * (r + 1) / used);
-    const int few = min(max(per - kOpen, 0) / 2, kFew);
-    if (end < total) {
-      find(a, lane, x, end);
-      end = placed(end, few);
-    }
-    find(a, lane, x, u);
-    u = placed(u, few);
     if (u < end && u == base + units(a)) next_sequence(a);
     return r;
   }
@@ -282,6 +264,27 @@ __device__ __forceinline__ int key_of(int t) { return (t & 2) << 1 | (t & 4) >> 
 // That of the weights' rows, whose reads are 32 rows x 2 units.
 __device__ __forceinline__ int row_key(int r) { return (r & 2) << 1 | ((r >> 2) & 3); }
 
+// The rows' queries on their way into LDS at `to`, 8 rows to a wavefront: the latent features
+// [rows][RANK], then the rotated ones, unit u of row r at u ^ (r & 15), u ^ (r / 2 & 7).  Offsets are
+// those from the first row's token, 31 bits.  Rows that are not there have the last one's: what they
+// get is given up.
+template <int RANK, int WAVES>
+__device__ __forceinline__ void load_queries(const LatentArgs& a, int b, int n, int row0, int wave, int lane, uint32_t to) {
+  const int last = min(a.rows, n * a.H) - 1, i0 = static_cast<int>(fdiv(row0, a.by_h));
+  const dma_rsrc q = dma_buffer(a.q + b * a.q_sb + i0 * a.q_st, 0x7fffff00), qr = dma_buffer(a.qr + b * a.qr_sb + i0 * a.qr_st, 0x7fffff00);
+  auto from = [&](int r, int64_t st, int64_t sh) {
+    const int row = min(row0 + r, last), i = static_cast<int>(fdiv(row, a.by_h));
+    return 2 * (static_cast<uint32_t>(i - i0) * static_cast<uint32_t>(st) + static_cast<uint32_t>(row - i * a.H) * static_cast<uint32_t>(sh));
+  };
+#pragma unroll 1
+  for (int k = 0; k < 8; ++k) {
+    const int r = k * WAVES + wave;
+    if (lane < RANK / 8) dma16(q, to + r * RANK * 2, (lane ^ (r & 15)) * 16, from(r, a.q_st, a.q_sh));
+  }
+  const int r = 8 * wave + lane / 8;
+  dma16(qr, to + WAVES * 8 * RANK * 2 + wave * 1024, from(r, a.qr_st, a.qr_sh) + ((lane & 7) ^ (r / 2 & 7)) * 16, 0);
+}
+
 // Up to 32 rows: four wavefronts, each a SIMD's alone, have 32 rows x 16 tokens of a page of scores,
 // and then all 64 tokens of 32 rows x a quarter of O's features, which stay in 64 registers.
 template <int RANK>
@@ -360,27 +363,12 @@ __global__ __launch_bounds__(kParts * 64, 1) void latent_kernel(LatentArgs a) {
       load(page, p, buf, std::integral_constant<int, OS>{}, OS * part, 0, One{});
       load(page, p, buf, One{}, NS - 1, wave, Shared{});
     };
-    // Queries, whole rows into the second buffer: the latent features [ROWS][RANK], then the
-    // rotated ones, unit u of row r at u ^ (r & 15), u ^ (r / 2 & 7); rows that are not there
-    // are zeros.
     auto token_of_row = [&](int row) {  // its new token; sq.n or more: none
       return row < a.rows ? static_cast<int>(fdiv(row, a.by_h)) : sq.n;
     };
     int64_t next = 0;  // the page after the ones on their way
     if (p0 < p1) {
-#pragma unroll 2
-      for (int k = 0; k < ROWS / WAVES; ++k) {
-        const int r = k * WAVES + wave, row = row0 + r, i = token_of_row(row);
-        const int64_t h = row - i * a.H;
-        const bool there = i < sq.n;
-        if (lane < RANK / 8)
-          dma16(dma_buffer(a.q + (there ? b * a.q_sb + i * a.q_st + h * a.q_sh : 0), RANK * 2), lds0 + BUF + r * RANK * 2,
-                there ? (lane ^ (r & 15)) * 16 : RANK * 2, 0);
-        if (lane < kRope / 8)
-          dma16(dma_buffer(a.qr + (there ? b * a.qr_sb + i * a.qr_st + h * a.qr_sh : 0), kRope * 2),
-                lds0 + BUF + ROWS * RANK * 2 + r * kRope * 2,
-                there ? (lane ^ (r / 2 & 7)) * 16 : kRope * 2, 0);
-      }
+      load_queries<RANK, WAVES>(a, b, sq.n, row0, wave, lane, lds0 + BUF);
       load_page(pages.at(p0), p0, 0);
       if (p0 + 1 < p1) next = pages.at(p0 + 1);
       wait_loads<SHARE>();
@@ -718,23 +706,9 @@ __global__ __launch_bounds__(2 * kParts * 64, 2) void latent_rows_kernel(LatentA
 #pragma unroll
         for (int k = 0; k < LOADS; ++k) dma16(r, to + k * STICK, off, k * kStick + at * 128);
     };
-    // Queries, whole rows into the last two buffers: the latent features [ROWS][RANK], then the
-    // rotated ones, unit u of row r at u ^ (r & 15), u ^ (r / 2 & 7); rows that are not there
-    // are zeros.
-    constexpr int Q_AT = 2 * TILE;
+    constexpr int Q_AT = 2 * TILE;  // the queries: in the last two buffers
     if (n > 0) {
-#pragma unroll 2
-      for (int k = 0; k < ROWS / WAVES; ++k) {
-        const int r = k * WAVES + wave, row = row0 + r, i = token_of_row(row);
-        const int64_t h = row - i * a.H;
-        const bool there = i < sq.n;
-        if (lane < RANK / 8)
-          dma16(dma_buffer(a.q + (there ? b * a.q_sb + i * a.q_st + h * a.q_sh : 0), RANK * 2), lds0 + Q_AT + r * RANK * 2,
-                there ? (lane ^ (r & 15)) * 16 : RANK * 2, 0);
-        if (lane < kRope / 8)
-          dma16(dma_buffer(a.qr + (there ? b * a.qr_sb + i * a.qr_st + h * a.qr_sh : 0), kRope * 2),
-                lds0 + Q_AT + ROWS * RANK * 2 + r * kRope * 2, there ? (lane ^ (r / 2 & 7)) * 16 : kRope * 2, 0);
-      }
+      load_queries<RANK, WAVES>(a, b, sq.n, row0, wave, lane, lds0 + Q_AT);
       load_tile(0);
       if (n > 1) load_tile(1);
     }
@@ -1090,6 +1064,11 @@ extern "C" int spyre_paged_latent_attn(const void* q, const int64_t* q_strides, 
   for (int i = 0; i < 3; ++i)
     SPYRE_REQUIRE(q_strides[i] % 8 == 0 && q_rope_strides[i] % 8 == 0, SPYRE_EINVAL, "q strides must be multiples of 8 elements");
   const Plan p = plan_of(B, T, H, rank, max_context_len + T);
+  // The rows of a workgroup are addressed from the first one's token, in 31 bits.
+  const int tokens = std::min(T - 1, (p.block_rows + H - 2) / H);
+  for (const int64_t* st : {q_strides, q_rope_strides})
+    SPYRE_REQUIRE(st[1] >= 0 && st[2] >= 0 && static_cast<double>(tokens) * st[1] + static_cast<double>(H - 1) * st[2] < (1 << 30) - rank,
+                  SPYRE_EUNSUPPORTED, "strides of q and q_rope are too large");
   SPYRE_REQUIRE(workspace && workspace_bytes >= p.ws_bytes && aligned(workspace), SPYRE_ENOSPC,
                 "workspace holds %zu bytes, need %zu (16-byte aligned)", workspace ? workspace_bytes : 0, p.ws_bytes);
   LatentArgs a{};
@@ -1104,13 +1083,10 @@ extern "C" int spyre_paged_latent_attn(const void* q, const int64_t* q_strides, 
   a.B = B, a.T = T, a.H = H, a.rows = T * H;
   a.max_ctx = max_context_len, a.scale_log2 = scale * kLog2e;
   a.row_blocks = p.row_blocks, a.block_rows = p.block_rows;
-  a.ranges = p.ranges;
-  const int64_t of_all = static_cast<int64_t>(B) * p.row_blocks;
-  a.each = of_all % p.ranges == 0 ? static_cast<int>(of_all / p.ranges) : 0;
-  SPYRE_REQUIRE(static_cast<double>(of_all) * (pages_of(max_context_len + T) + Walk::kOpen + 1) < (1 << 30), SPYRE_EUNSUPPORTED,
-                "too many pages or rows");
-  a.by_h = make_fastdiv(static_cast<uint32_t>(H));
-  a.by_blocks = make_fastdiv(static_cast<uint32_t>(p.row_blocks)), a.by_ranges = make_fastdiv(static_cast<uint32_t>(p.ranges));
+  a.block_shift = p.groups == 1 ? 5 : 6, a.ranges = p.ranges;
+  SPYRE_REQUIRE(static_cast<double>(B) * p.row_blocks * (pages_of(max_context_len + T) + Walk::kOpen + 1) < (1 << 30),
+                SPYRE_EUNSUPPORTED, "too many pages or rows");
+  a.by_h = make_fastdiv(static_cast<uint32_t>(H)), a.by_ranges = make_fastdiv(static_cast<uint32_t>(p.ranges));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid(static_cast<uint32_t>((p.ranges + 7) / 8 * 8));
   rank == 512 ? launch<512>(a, p.groups, grid, st) : launch<256>(a, p.groups, grid, st);
