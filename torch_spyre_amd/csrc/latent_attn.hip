@@ -995,7 +995,7 @@ __global__ __launch_bounds__(256) void latent_join_kernel(LatentArgs a) {
   if (row >= a.rows) return;
   float M = -INFINITY, L = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  merge_parts(range, min(last, used - 1), M, L, acc, [&](int p, float& m, float& l, f32x4& x) {
+  merge_parts_once(range, __builtin_amdgcn_readfirstlane(min(last, used - 1)), M, L, acc, [&](int p, float& m, float& l, f32x4& x) {
     const float* slot = slot_of(a, 2 * p + (p == range ? 1 : 0), RANK);
     const float* ml = slot + ROWS * RANK + r * 2;
     m = ml[0], l = ml[1];

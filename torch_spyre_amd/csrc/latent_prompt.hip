@@ -366,7 +366,7 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a) {
   const int d = 4 * static_cast<int>(u % (D / 4));
   float M = -INFINITY, L = 0.f;
   f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-  merge_parts(0, a.splits - 1, M, L, acc, [&](int s, float& m, float& l, f32x4_t& x) {
+  merge_parts_once(0, a.splits - 1, M, L, acc, [&](int s, float& m, float& l, f32x4_t& x) {
     const float* ml = a.ws + a.splits * rows * D + (s * rows + at) * 2;
     m = ml[0], l = ml[1];
     x = *reinterpret_cast<const f32x4_t*>(a.ws + (s * rows + at) * D + d);

@@ -303,4 +303,33 @@ __device__ __forceinline__ void merge_parts(int r0, int r1, float& M, float& L, 
   }
 }
 
+// The same where r0 and r1 are the wavefront's: no part is loaded twice (latent attention of 64 x
+// 128-16384 tokens 123.8 us, so 122.9; 600 x 10-900 93.9, 93.3).
+template <typename Load>
+__device__ __forceinline__ void merge_parts_once(int r0, int r1, float& M, float& L, f32x4_t& acc, Load load) {
+  constexpr int G = 4;
+  for (int c = r0; c <= r1; c += G) {
+    float m[G], l[G];
+    f32x4_t x[G];
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+      m[k] = -INFINITY, l[k] = 0.f, x[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      if (c + k <= r1) load(c + k, m[k], l[k], x[k]);
+    }
+    float mc = M;
+#pragma unroll
+    for (int k = 0; k < G; ++k) mc = fmaxf(mc, m[k]);
+    const float f0 = M == -INFINITY ? 0.f : exp2_of(M - mc);
+    L *= f0;
+    acc *= f0;
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+      const float f = m[k] == -INFINITY ? 0.f : exp2_of(m[k] - mc);
+      L += m[k] == -INFINITY ? l[k] : l[k] * f;  // l without a reference is 0, or NaN
+      if (m[k] != -INFINITY) acc += x[k] * f;
+    }
+    M = mc;
+  }
+}
+
 }  // namespace spyre_hip
