@@ -418,3 +418,20 @@ def test_too_few_keys_are_nan(cuda):
     none = tsa.latent_attention(q[..., :64], q[..., 64:], k[:, :0], kr[:, :0], k[:, :0], torch.zeros(3, dtype=torch.int32, device=cuda),
                                 torch.zeros(3, dtype=torch.int32, device=cuda))
     assert none.shape == (3, 20, 2, 64) and not none.any()
+
+
+@pytest.mark.parametrize("H", [16, 33])
+def test_one_token_that_its_mask_leaves_out(cuda, H):
+    """A decode step's own token, masked, holds NaN: the row attends its context alone."""
+    import torch_spyre_amd as tsa
+
+    cache, table = randn((6, 5, 64, 64), cuda, SEED + 80), torch.tensor([[2, 0], [4, 1]], dtype=torch.int32, device=cuda)
+    ctx = torch.tensor([70, 0], dtype=torch.int32, device=cuda)
+    cache[0, :, 70 - 64] = float("nan")
+    cache[4, :, 0] = float("inf")
+    q, qr = randn((2, 1, H, 256), cuda, SEED + 81), randn((2, 1, H, 64), cuda, SEED + 82)
+    mask = torch.zeros((1, 1), dtype=torch.bool, device=cuda)
+    out, lse = tsa.paged_latent_attention(q, qr, cache, table, ctx, 0.05, mask, max_context_len=70, return_lse=True)
+    clean = cache.clone()
+    clean[0, :, 70 - 64] = clean[4, :, 0] = 0
+    check_paged(out, lse, q, qr, clean, table, [70, 0], [1, 1], 0.05, mask.view(1, 1, 1).cpu().numpy())

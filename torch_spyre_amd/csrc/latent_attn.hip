@@ -413,7 +413,7 @@ __global__ __launch_bounds__(kParts * 64, 1) void latent_kernel(LatentArgs a) {
       const bool more = p + 2 < p1;
       if (more) next = pages.at(p + 2);
       uint32_t odd = 0;                            // of this wavefront's tokens, new ones that hold a NaN or an infinity
-      if (EDGE && a.T > 1) {
+      if (EDGE && (a.T > 1 || a.mask)) {
         // What a row does not attend must not meet its weight of 0: such tokens become
         // zeros, and the rows that attend them NaN.
         constexpr int PER = WAVES * 64 / kPage;  // threads of a token
@@ -759,7 +759,7 @@ __global__ __launch_bounds__(2 * kParts * 64, 2) void latent_rows_kernel(LatentA
       auto step = [&](int i, auto edge_tag) {
         constexpr bool EDGE = decltype(edge_tag)::value;
         uint32_t odd = 0;
-        if (EDGE && a.T > 1) odd = odd_of(i);
+        if (EDGE && (a.T > 1 || a.mask)) odd = odd_of(i);
         // The scores: sc[x] of row 16 part + l16, token tok(x).
         auto tok = [&](int x, int ln) { return 16 * (x / 4) + 4 * (ln / 16) + x % 4; };
         float sc[8];
@@ -873,13 +873,13 @@ __global__ __launch_bounds__(2 * kParts * 64, 2) void latent_rows_kernel(LatentA
 #pragma unroll
           for (int x = 0; x < 16; ++x) o[g][dt][x] = 0.f;
       if (n > 0) {
-        if (edge_at(0) && a.T > 1) odd_of(0);
+        if (edge_at(0) && (a.T > 1 || a.mask)) odd_of(0);
         if (n > 2) load_tile(2);
         n > 2 ? wait_loads<LOADS>() : wait_loads<0>();  // tile 1 is there
         __syncthreads();
       }
       for (int i = 1; i <= n; ++i) {
-        if (i < n && edge_at(i) && a.T > 1) odd_of(i);
+        if (i < n && edge_at(i) && (a.T > 1 || a.mask)) odd_of(i);
         const bool more = i + 2 < n;
         {
           const int j = i - 1, ln = here(lane), c = ln % 32;
