@@ -28,8 +28,13 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 
 // Lane l's 16 bytes at byte voff + soff of the buffer go to LDS byte dst + 16 l (dst,
 // soff wave-uniform); where voff is not within the buffer they are zeros.
+// A memory instruction that reads a scalar register needs 5 wait states after a vector
+// instruction that wrote it, and one that uses m0 needs 1 after its write; the hardware
+// checks neither, and for a load in assembly the compiler does not either (a spilled soff
+// comes back by v_readlane right before it).  s_mov and s_nop 3 are 1 + 4.
 __device__ __forceinline__ void dma16(dma_rsrc r, uint32_t dst, uint32_t voff, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(dst), "v"(voff), "s"(r), "s"(soff) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(dst), "v"(voff), "s"(r), "s"(soff)
+               : "memory", "m0");
 }
 
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
