@@ -586,8 +586,9 @@ int spyre_paged_latent_attn(const void* q, const int64_t* q_strides, const void*
  * new_lens[b] (NULL: T) queries, query i < n attends keys t <= context_lens[b] + i:
  *   out = softmax(scale (q . k + q_rope . k_rope)) v,  lse the logarithm of its sum
  * Rows i >= n are zeros with lse -inf; keys from context_lens[b] + n on, and keys
- * that a row does not attend, do not reach it.  A sequence whose lengths exceed
- * `keys` is NaN.
+ * that a row does not attend, do not reach it.  A NaN or an infinity in a value
+ * reaches that feature of the rows that attend it, and no lse.  A sequence whose
+ * lengths exceed `keys` is NaN.
  *   q [B, T, H, D], q_rope [B, T, H, 64], k, v : fp16, feature stride 1, strides {b, t, h},
  *   k_rope {b, t}; multiples of 8 elements, 16-byte aligned; token strides of k, k_rope
  *   and v below 2^23

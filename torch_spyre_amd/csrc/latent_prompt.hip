@@ -265,6 +265,40 @@ __global__ __launch_bounds__(W * 64, 2) void prompt_kernel(PromptArgs a) {
     }
   };
 
+  // What a row does not attend must not meet its weight of 0 in the second product.  So numbers of
+  // such values (`odd`: keys of tile t that hold any) that are a NaN or an infinity are added by
+  // themselves to the rows that attend them, and are zeros in LDS from then on.
+  auto reach = [&](int t, uint64_t odd) {
+    const int ln = here(lane), last = min(ctx + row0 + ln % 32, total - 1) - t * kKeys;
+#pragma unroll 1
+    for (; odd; odd &= odd - 1) {
+      const int tok = __builtin_ctzll(odd), x = 16 * (tok / 32) + tok % 16;
+      float p = 0.f;  // the key's weight: in one half of the wavefront
+#pragma unroll
+      for (int y = 0; y < 32; ++y) p = y == x ? static_cast<float>(w[y / 8][y % 8]) : p;
+      p = __shfl(p, ln % 32 + (tok & 16) * 2, 64);
+      const uint8_t* v = s_mem + V_AT + (t & 1) * V_TILE + tok * 128 + 8 * (ln / 32);
+#pragma unroll
+      for (int y = 0; y < 4 * DT; ++y) {
+        const f16x4 z = *reinterpret_cast<const f16x4*>(v + y / 8 * kStick + ((y % 8) ^ key_of(tok)) * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float f = static_cast<float>(z[e]);
+          o[y / 4][4 * (y % 4) + e] += tok <= last && !(__builtin_fabsf(f) < INFINITY) ? p * f : 0.f;
+        }
+      }
+    }
+  };
+  auto clear = [&](int t, uint64_t odd) {
+    const int tok = here(lane);
+    if (!((odd >> tok) & 1)) return;
+#pragma unroll 1
+    for (int u = 0; u < VS * 64; ++u) {
+      uint16_t* x = reinterpret_cast<uint16_t*>(s_mem + V_AT + (t & 1) * V_TILE + tok * 128 + u / 64 * kStick) + u % 64;
+      if ((*x & 0x7c00) == 0x7c00) *x = 0;
+    }
+  };
+
   for (int t = first; t < tiles; ++t) {
     dma_wait();
     __syncthreads();  // K of t + 1 and V of t are there (at first K of t, too); their places of before are read
@@ -275,10 +309,9 @@ __global__ __launch_bounds__(W * 64, 2) void prompt_kernel(PromptArgs a) {
     if (t == first) __syncthreads();
     uint64_t odd = 0;  // keys whose values hold a NaN or an infinity, of those that not all rows attend
     if (t * kKeys + kKeys > all) {
-      // What a row does not attend must not meet its weight of 0: such values become zeros, and
-      // the rows that attend them NaN.  Every wavefront looks at all 64 rows, one a lane.
+      // Every wavefront looks at all 64 rows, one a lane.
       const int tok = here(lane), at = t * kKeys + tok;
-      uint8_t* x = s_mem + V_AT + (t & 1) * V_TILE + tok * 128;
+      const uint8_t* x = s_mem + V_AT + (t & 1) * V_TILE + tok * 128;
       uint32_t found = 0;
       if (at >= all && at < total)
         for (int s = 0; s < VS; ++s)
@@ -288,35 +321,24 @@ __global__ __launch_bounds__(W * 64, 2) void prompt_kernel(PromptArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) found |= (y[e] & 0x7c007c00u) + 0x04000400u;
           }
-      const bool drop = (found & 0x80008000u) != 0;
-      odd = __ballot(drop);
-      if (odd) {  // the same for all wavefronts
-        __syncthreads();
-        if (drop && wave == 0)
-          for (int s = 0; s < VS; ++s)
-#pragma unroll
-            for (int u = 0; u < 8; ++u) *reinterpret_cast<u32x4*>(x + s * kStick + u * 16) = u32x4{0, 0, 0, 0};
-        __syncthreads();
-      }
-    }
-    if (t >= mine) {  // none of its rows' keys (the barriers above are all of a step's)
-      load_k(t + 2);
-      load_v(t + 1);
-      continue;
+      odd = __ballot((found & 0x80008000u) != 0);
     }
     const bool more = t + 1 < mine;
-    if (more)
+    if (t >= mine) {  // none of its rows' keys (the barriers are all of a step's)
+      load_k(t + 2);
+      load_v(t + 1);
+    } else if (more) {
       products_and_weights(t + 1, yes, yes);
-    else
+    } else {
       products_and_weights(t + 1, no, yes);
-    if (odd) {
-      const int ln = here(lane), last = min(ctx + row0 + ln % 32, total - 1) - t * kKeys - 16 * (ln / 32);
-#pragma unroll
-      for (int x = 0; x < 32; ++x) {
-        const int tok = 32 * (x / 16) + x % 16;
-        if (tok <= last && (odd >> (tok + 16 * (ln / 32))) & 1) w[x / 8][x % 8] = static_cast<_Float16>(NAN), l = NAN;
-      }
     }
+    if (odd) {  // the same for all wavefronts
+      if (t < mine) reach(t, odd);
+      __syncthreads();
+      if (wave == 0) clear(t, odd);
+      __syncthreads();
+    }
+    if (t >= mine) continue;
     if (more)
       settle(t + 1, second(t, yes, yes));
     else

@@ -101,8 +101,9 @@ def latent_attention(q: torch.Tensor, q_rope: torch.Tensor, k: torch.Tensor, k_r
 
     Returns out [B, T, H, D] and, with ``return_lse``, the fp32 logsumexp [B, T, H].  Rows
     i >= new_lens[b] are zeros with logsumexp -inf; what a row does not attend does not
-    reach it, keys behind the sequence's last among it.  A sequence with more context
-    and queries than there are keys is NaN."""
+    reach it, keys behind the sequence's last among it, and a NaN or an infinity in a
+    value reaches only that feature of the rows that attend it.  A sequence with more
+    context and queries than there are keys is NaN."""
     try:
         o, lse = _EXPANDED(q, q_rope, k, k_rope, v, context_lens, new_lens, None if scale is None else float(scale))
     except RuntimeError as e:
