@@ -112,3 +112,29 @@ def test_values_that_keys_weigh_nothing(cuda, D):
     assert out[0, at:, 0, 5:7].isnan().all()
     out[0, at:, 0, 5:7] = torch.from_numpy(ref[0][at:, 5:7]).to(out)
     close(out[0, :, 0], lse[0, :, 0], ref, T, 8.0)
+
+
+@pytest.mark.parametrize("rank", [256, 512])
+@pytest.mark.parametrize("H", [16, 33, 64])
+@pytest.mark.parametrize("bad", [NAN, INF, -INF])
+@pytest.mark.parametrize("where", ["latent", "last latent", "rotated"])
+def test_own_token_of_a_decode_step(cuda, rank, H, bad, where):
+    """It makes the sequence NaN with and without a mask, whatever the score's sign; sequences that have no new token,
+    and those beside it, do not notice."""
+    import torch_spyre_amd as tsa
+
+    ctx, counts = [0, 63, 64, 100, 2000, 70, 31], [1, 1, 1, 1, 1, 0, 1]
+    B, W = len(ctx), 33
+    cache = randn((B * W, (rank + 64) // 64, 64, 64), cuda, SEED + H)
+    table = torch.randperm(B * W, generator=torch.Generator().manual_seed(SEED)).view(B, W).to(torch.int32).to(cuda)
+    q, qr = randn((B, 1, H, rank), cuda, SEED + 1, 0.5), randn((B, 1, H, 64), cuda, SEED + 2)
+    lens, new = (torch.tensor(x, dtype=torch.int32, device=cuda) for x in (ctx, counts))
+    call = lambda mask: tsa.paged_latent_attention(q, qr, cache, table, lens, 0.07, mask, new, max_context_len=2000, return_lse=True)  # noqa: E731
+    clean = call(None)
+    stick, feature = {"latent": (1, 7), "last latent": (rank // 64 - 1, 63), "rotated": (rank // 64, 13)}[where]
+    for b in range(B - 1):  # the last one stays as it is
+        cache[table[b, ctx[b] // 64], stick, ctx[b] % 64, feature] = bad
+    for mask in (None, torch.ones((1, 1), dtype=torch.bool, device=cuda)):
+        out, lse = call(mask)
+        assert out[:5].isnan().all() and lse[:5].isnan().all()
+        assert torch.equal(out[5:], clean[0][5:]) and torch.equal(lse[5:], clean[1][5:])

@@ -285,6 +285,21 @@ __device__ __forceinline__ void load_queries(const LatentArgs& a, int b, int n, 
   dma16(qr, to + WAVES * 8 * RANK * 2 + wave * 1024, from(r, a.qr_st, a.qr_sh) + ((lane & 7) ^ (r / 2 & 7)) * 16, 0);
 }
 
+// Whether a token in LDS, NS sticks of 128 bytes `stride` apart, holds a NaN or an infinity: a decode
+// step's own one, which every row attends, so that the rows are NaN.
+template <int NS>
+__device__ __forceinline__ bool token_odd(const uint8_t* token, int stride, int lane) {
+  uint32_t found = 0;
+#pragma unroll
+  for (int u = 0; u < 8 * NS; u += 64)
+    if (u + lane < 8 * NS) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(token + (u + lane) / 8 * stride + (u + lane) % 8 * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) found |= (w[e] & 0x7c007c00u) + 0x04000400u;
+    }
+  return __ballot((found & 0x80008000u) != 0) != 0;
+}
+
 // Up to 32 rows: four wavefronts, each a SIMD's alone, have 32 rows x 16 tokens of a page of scores,
 // and then all 64 tokens of 32 rows x a quarter of O's features, which stay in 64 registers.
 template <int RANK>
@@ -441,6 +456,8 @@ __global__ __launch_bounds__(kParts * 64, 1) void latent_kernel(LatentArgs a) {
         if (lane == 0) s_odd[wave] = bits;
         __syncthreads();
         odd = s_odd[wave];  // (wavefront w looked at tokens 16 w ..)
+      } else if (EDGE && sq.n > 0) {
+        pages.poisoned |= token_odd<NS>(s_mem + buf * BUF + sq.ctx % kPage * 128, kStick, here(lane));
       }
 
       // The scores: sc[n][x] of row 16 (NR rq + n) + l16, token 16 TB tg + tok(x).
@@ -759,7 +776,10 @@ __global__ __launch_bounds__(2 * kParts * 64, 2) void latent_rows_kernel(LatentA
       auto step = [&](int i, auto edge_tag) {
         constexpr bool EDGE = decltype(edge_tag)::value;
         uint32_t odd = 0;
-        if (EDGE && (a.T > 1 || a.mask)) odd = odd_of(i);
+        if (EDGE && (a.T > 1 || a.mask))
+          odd = odd_of(i);
+        else if (EDGE && sq.n > 0)
+          pages.poisoned |= token_odd<NS>(s_mem + (i & 3) * TILE + sq.ctx % TOKS * 128, STICK, here(lane));
         // The scores: sc[x] of row 16 part + l16, token tok(x).
         auto tok = [&](int x, int ln) { return 16 * (x / 4) + 4 * (ln / 16) + x % 4; };
         float sc[8];
