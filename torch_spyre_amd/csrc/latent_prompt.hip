@@ -100,7 +100,7 @@ __global__ __launch_bounds__(W * 64, 2) void prompt_kernel(PromptArgs a) {
   const int raw = __builtin_amdgcn_readfirstlane(a.ctx[b]);
   const int n = a.counts ? min(max(__builtin_amdgcn_readfirstlane(a.counts[b]), 0), a.T) : a.T;
   const int ctx = min(max(raw, 0), a.keys), total = min(ctx + n, a.keys);
-  const bool bad = raw > a.keys - n;  // fewer keys than the lengths say
+  const bool bad = max(raw, 0) > a.keys - n;  // fewer keys than the lengths say
   const int row0 = block0 + wave * kRows;
   // Keys of the workgroup's rows, of this wavefront's, and those that all rows of
   // the workgroup attend; tiles [first, tiles) of the split, up to `mine` of this wavefront.
