@@ -54,3 +54,25 @@ def test_queries_far_apart(cuda, far, H):
     wide.copy_(x)
     out, lse = call(q, wide) if "rotated" in far else call(wide, qr)
     assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+@pytest.mark.parametrize("far", [0, 1, 2])
+@pytest.mark.parametrize("step", [(1 << 23) - 8, 1 << 23, (1 << 24) + 8])
+def test_keys_far_apart(cuda, far, step):
+    """Tokens of keys, rotated keys or values beyond the kernels' 31 bits, as [keys, B, H, D] has them."""
+    import torch_spyre_amd as tsa
+
+    T, keys, H, D = 5, 70, 2, 64
+    k, v, kr = randn((1, keys, H, D), cuda, SEED), randn((1, keys, H, D), cuda, SEED + 1), randn((1, keys, 64), cuda, SEED + 2)
+    q, ctx = randn((1, T, H, D + 64), cuda, SEED + 3), torch.tensor([keys - T], dtype=torch.int32, device=cuda)
+    call = lambda k, kr, v: tsa.latent_attention(q[..., :D], q[..., D:], k, kr, v, ctx, return_lse=True)  # noqa: E731
+    want = call(k, kr, v)
+    x = [k, kr, v]
+    like = x[far]
+    room = torch.empty(keys * step, dtype=torch.float16, device=cuda)
+    x[far] = room.as_strided(like.shape, (8, step) + like.stride()[2:])
+    x[far].copy_(like)
+    out, lse = call(*x)
+    assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+    none = call(*(y[:, :0] for y in x)) if far == 0 else None  # no keys: the strides do not matter
+    assert none is None or none[0].isnan().all()

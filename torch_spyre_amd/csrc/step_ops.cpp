@@ -269,12 +269,16 @@ std::tuple<at::Tensor, at::Tensor> paged_latent_attention(const at::Tensor& quer
   return {out, lse};
 }
 
+// Keys or values [B, keys, H, D] whose tokens are less than the 2^23 elements apart that the kernel
+// takes (those of a tile in 31 bits): of [keys, B, H, D] with B H D beyond, a copy.
+at::Tensor near_keys(const at::Tensor& t) { return t.stride(1) < (1 << 23) ? t : t.clone(at::MemoryFormat::Contiguous); }
+
 std::tuple<at::Tensor, at::Tensor> latent_attention(const at::Tensor& query, const at::Tensor& query_rope, const at::Tensor& key,
                                                     const at::Tensor& key_rope, const at::Tensor& value,
                                                     const at::Tensor& context_lens, const std::optional<at::Tensor>& new_lens,
                                                     std::optional<double> scale) {
   const at::Tensor q = rows_operand(query, "q"), qr = rows_operand(query_rope, "q_rope");
-  const at::Tensor k = rows_operand(key, "k"), v = rows_operand(value, "v");
+  const at::Tensor k = near_keys(rows_operand(key, "k")), v = near_keys(rows_operand(value, "v"));
   const auto dev = q.device();
   const int64_t B = q.size(0), T = q.size(1), H = q.size(2), D = q.size(3), n = k.size(1);
   require_on(qr, dev, "q_rope");
@@ -290,7 +294,7 @@ std::tuple<at::Tensor, at::Tensor> latent_attention(const at::Tensor& query, con
   check_lens(context_lens, B, dev, "context_lens");
   if (new_lens.has_value()) check_lens(*new_lens, B, dev, "new_lens");
   const c10::OptionalDeviceGuard guard(dev);
-  const at::Tensor kr = rows_operand(key_rope.unsqueeze(2), "k_rope");
+  const at::Tensor kr = near_keys(rows_operand(key_rope.unsqueeze(2), "k_rope"));
   const double s = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(D + kRope));
   at::Tensor out = at::empty({B, T, H, D}, q.options());
   at::Tensor lse = at::empty({B, T, H}, q.options().dtype(at::kFloat));
