@@ -41,11 +41,14 @@ def plan_pages(block_table: torch.Tensor, held: torch.Tensor, context_lens: torc
     sequence after sequence, and written behind the held ones in block_table
     (int32 [B, W]), in one launch.
 
-    With ``length`` positions and slots are [B, length], rows as the appends and
-    ``rotary_embedding`` take them (-1 from new_lens[b] on); with ``tokens`` they
+    With ``length`` positions and slots are [B, length] (-1 from new_lens[b] on):
+    ``rotary_embedding`` takes the positions, ``latent_append`` the slots, and the
+    appends that take a sequence's own slots, ``kv_append_quantized`` and (a column at
+    a time) ``kv_append``, torch.where(slots < 0, -1, positions).  With ``tokens`` they
     are [tokens], the sequences' tokens one after the other (-1 behind the
     last).  Where the ring or the table's row has no page left, slots are -1 and
-    held[b] falls short; nothing else fails.  held and cursor are left as they
+    held[b] falls short; nothing else fails, but the table's entries from held[b] on are
+    stale: no position there may be written or attended.  held and cursor are left as they
     are: keep the plan's for the next call (a captured loop copies them back).
     At most 4096 sequences."""
     if (length is None) == (tokens is None):
