@@ -560,9 +560,9 @@ int spyre_latent_read_f16(const void* cache, const int32_t* block_table, int64_t
  * draft_lens[b] (NULL: T) new ones; query i < n attends the context and the new
  * tokens j < n with mask[b, i, j] (NULL: j <= i):
  *   out = softmax(scale (q . c + q_rope . r)) c,  lse the logarithm of its sum
- * Rows that attend nothing and rows i >= n are zeros with lse -inf.  What a row
- * does not attend does not reach it, whatever it holds; a row that attends a new
- * token with a NaN or an infinity is NaN.
+ * Rows that attend nothing (or only scores of -inf) and rows i >= n are zeros with
+ * lse -inf.  What a row does not attend does not reach it, whatever it holds; a row
+ * that attends a new token with a NaN or an infinity is NaN.
  *   q [B, T, H, rank], q_rope [B, T, H, 64] : fp16, feature stride 1, strides {b, t, h}
  *           multiples of 8 elements, 16-byte aligned; {t, h} not negative, 64 of a
  *           sequence's (t, h) within 2^30 elements
@@ -585,10 +585,10 @@ int spyre_paged_latent_attn(const void* q, const int64_t* q_strides, const void*
  * share; v [B, keys, H, D].  Sequence b has context_lens[b] keys before its n =
  * new_lens[b] (NULL: T) queries, query i < n attends keys t <= context_lens[b] + i:
  *   out = softmax(scale (q . k + q_rope . k_rope)) v,  lse the logarithm of its sum
- * Rows i >= n are zeros with lse -inf; keys from context_lens[b] + n on, and keys
- * that a row does not attend, do not reach it.  A NaN or an infinity in a value
- * reaches that feature of the rows that attend it, and no lse.  A sequence whose
- * lengths exceed `keys` is NaN.
+ * Rows i >= n, and rows whose scores are all -inf, are zeros with lse -inf; keys from
+ * context_lens[b] + n on, and keys that a row does not attend, do not reach it.  A NaN
+ * or an infinity in a value reaches that feature of the rows that attend it, and no
+ * lse.  A sequence whose lengths exceed `keys` is NaN.
  *   q [B, T, H, D], q_rope [B, T, H, 64], k, v : fp16, feature stride 1, strides {b, t, h},
  *   k_rope {b, t}; multiples of 8 elements, 16-byte aligned; token strides of k, k_rope
  *   and v below 2^23

@@ -138,3 +138,51 @@ def test_own_token_of_a_decode_step(cuda, rank, H, bad, where):
         out, lse = call(mask)
         assert out[:5].isnan().all() and lse[:5].isnan().all()
         assert torch.equal(out[5:], clean[0][5:]) and torch.equal(lse[5:], clean[1][5:])
+
+
+RUNS = [(400, [(0, 32)]), (400, [(0, 64)]), (400, [(0, 150)]), (400, [(32, 64)]), (90, [(0, 90)]), (3000, [(0, 600), (900, 1700)])]
+
+
+@pytest.mark.parametrize("rank", [256, 512])
+@pytest.mark.parametrize("T,H", [(1, 16), (1, 64), (3, 8), (7, 32)])
+@pytest.mark.parametrize("ctx,runs", RUNS)
+def test_runs_that_score_minus_infinity(cuda, rank, T, H, ctx, runs):
+    """Runs of tokens whose keys hold infinities (and whose values do not) weigh nothing, wherever a run begins."""
+    import torch_spyre_amd as tsa
+
+    W = (ctx + T + 63) // 64
+    cache = randn((W, rank // 64 + 1, 64, 64), cuda, SEED + 1)
+    table = torch.randperm(W, generator=torch.Generator().manual_seed(SEED)).view(1, W).to(torch.int32).to(cuda)
+    q, qr = randn((1, T, H, rank), cuda, SEED + 2, 0.5), randn((1, T, H, 64), cuda, SEED + 3)
+    qr[..., 0] = qr[..., 0].abs() + 0.125
+    rows = cache[table[0].long()].double().cpu().numpy().transpose(0, 2, 1, 3).reshape(W * 64, -1)[:ctx + T]
+    keep = keep_of(T, H, ctx, T)
+    for first, end in runs:
+        keep[:, first:end] = False
+        for t in range(first, end):
+            cache[table[0, t // 64], rank // 64, t % 64, 0] = -INF
+    out, lse = tsa.paged_latent_attention(q, qr, cache, table, torch.tensor([ctx], dtype=torch.int32, device=cuda), 0.07,
+                                          max_context_len=ctx, return_lse=True)
+    ref = O.attend(torch.cat((q, qr), -1).double().cpu().numpy().reshape(T * H, -1), rows, rows[:, :rank], keep, 0.07)
+    close(out, lse, ref, ctx + T, np.abs(rows).max())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,ctx,runs", [(300, 0, [(0, 40)]), (300, 0, [(64, 128)]), (300, 0, [(100, 290)]), (70, 60, [(0, 125)]),
+                                        (2, 3000, [(0, 600), (900, 1700)])])
+def test_prompt_runs_that_score_minus_infinity(cuda, D, T, ctx, runs):
+    """The same of prompts; rows that attend nothing else are zeros."""
+    import torch_spyre_amd as tsa
+
+    n = ctx + T
+    kv, kr, q = randn((1, n, 1, 2 * D), cuda, SEED), randn((1, n, 64), cuda, SEED + 1), randn((1, T, 1, D + 64), cuda, SEED + 2)
+    q[..., 1] = q[..., 1].abs() + 0.125
+    K = torch.cat((kv[:, :, 0, :D], kr), -1)[0].double().cpu().numpy()
+    keep = keep_of(T, 1, ctx, T)
+    for first, end in runs:
+        keep[:, first:end] = False
+        kv[0, first:end, 0, 1] = -INF
+    out, lse = tsa.latent_attention(q[..., :D], q[..., D:], kv[..., :D], kr, kv[..., D:], torch.tensor([ctx], dtype=torch.int32, device=cuda),
+                                    return_lse=True)
+    ref = O.attend(q[0, :, 0].double().cpu().numpy(), K, kv[0, :, 0, D:].double().cpu().numpy(), keep, (D + 64) ** -0.5)
+    close(out[0, :, 0], lse[0, :, 0], ref, n, 8.0)

@@ -70,11 +70,11 @@ def paged_latent_attention(q: torch.Tensor, q_rope: torch.Tensor, cache: torch.T
 
     scale is that of the expanded keys, usually (D + 64)^-1/2.  Returns out [B, T, H,
     rank] and, with ``return_lse``, the fp32 logsumexp [B, T, H].  Rows i >=
-    draft_lens[b], and rows that attend nothing, are zeros with logsumexp -inf; what a
-    row does not attend does not reach it; a row that attends a new token with a NaN or
-    an infinity is NaN.  ``max_context_len`` bounds context_lens (if omitted it is
-    read from them, which synchronises); longer contexts, and pages that the block
-    table does not name validly, make the sequence NaN."""
+    draft_lens[b], and rows that attend nothing (or only scores of -inf), are zeros with
+    logsumexp -inf; what a row does not attend does not reach it; a row that attends a
+    new token with a NaN or an infinity is NaN.  ``max_context_len`` bounds context_lens
+    (if omitted it is read from them, which synchronises); longer contexts, and pages
+    that the block table does not name validly, make the sequence NaN."""
     one = q.dim() == 3
     if one:
         q, q_rope = q.unsqueeze(1), q_rope.unsqueeze(1)
@@ -100,10 +100,10 @@ def latent_attention(q: torch.Tensor, q_rope: torch.Tensor, k: torch.Tensor, k_r
     to (D + 64)^-1/2; D is 64 or 128.
 
     Returns out [B, T, H, D] and, with ``return_lse``, the fp32 logsumexp [B, T, H].  Rows
-    i >= new_lens[b] are zeros with logsumexp -inf; what a row does not attend does not
-    reach it, keys behind the sequence's last among it, and a NaN or an infinity in a
-    value reaches only that feature of the rows that attend it.  A sequence with more
-    context and queries than there are keys is NaN."""
+    i >= new_lens[b], and rows whose scores are all -inf, are zeros with logsumexp -inf;
+    what a row does not attend does not reach it, keys behind the sequence's last among
+    it, and a NaN or an infinity in a value reaches only that feature of the rows that
+    attend it.  A sequence with more context and queries than there are keys is NaN."""
     try:
         o, lse = _EXPANDED(q, q_rope, k, k_rope, v, context_lens, new_lens, None if scale is None else float(scale))
     except RuntimeError as e:
