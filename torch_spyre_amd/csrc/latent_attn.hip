@@ -18,11 +18,14 @@
 // tokens of them, come into LDS while the ones before are used.  The first product has 16 x 16 tiles
 // with Q in registers, the weights meet in LDS, and the second has 32 x 32 tiles of O in registers.
 //
-// Measured, rank 512: 32 sequences x 4096 tokens x 128 heads 67 us (36.5 GFLOP, 550 TFLOP/s; 32
-// tokens of 64 rows take 0.85 us, of which the matrix cores 0.45 and the loads' way into LDS as much;
-// the start of a range 6 us, the parts' way to memory and back with the second launch 17); 64 x
-// 128-16384 tokens x 16 heads 125 us (629 MB, 5.0 TB/s: memory); 16 x 500-6000 tokens x 1-7 new x 32
-// heads 52; 1 x 700 x 16 heads 17.4, of which two launches 9.
+// Measured, rank 512 (a pass among others, from device to device): 32 sequences x 4096 tokens x 128
+// heads 62-65 us (36.5 GFLOP, 560-590 TFLOP/s; the first kernel 52-58, the join 9.8).  That kernel has
+// wavefronts on the device for 93000 cycles: 32.5 tiles of 32 tokens x 64 rows of 2130 each (0.85 us,
+// of which the matrix cores 0.45 and the loads' way into LDS as much), the start of a range 6 us, the
+// parts; the matrix cores are busy for 38 % of them.  What the rest of its time goes to, or whether the
+// clock falls, is not established.  16 x 500-6000 tokens x 1-7 new x 32 heads 46-48 (39-42 and 9.0;
+// 72000 cycles, 29 % busy); 64 x 128-16384 tokens x 16 heads 124 (629 MB; 117, 5.4 TB/s, and 7.3);
+// 1 x 700 x 16 heads 17.1-17.4: latency.
 
 #include <hip/hip_runtime.h>
 
@@ -394,7 +397,7 @@ __global__ __launch_bounds__(kParts * 64, 1) void latent_kernel(LatentArgs a) {
     for (int n = 0; n < NR; ++n)
 #pragma unroll
       for (int s = 0; s < NQ; ++s) {
-        const int r = 16 * (n) + here(l16);
+        const int r = 16 * n + here(l16);
         const int at = 32 * s < RANK ? r * RANK * 2 + ((4 * s + g16) ^ (r & 15)) * 16
                                      : ROWS * RANK * 2 + r * kRope * 2 + ((4 * s - RANK / 8 + g16) ^ (r / 2 & 7)) * 16;
         qf[n][s] = *reinterpret_cast<const f16x8*>(s_mem + BUF + at);
@@ -460,7 +463,7 @@ __global__ __launch_bounds__(kParts * 64, 1) void latent_kernel(LatentArgs a) {
         pages.poisoned |= token_odd<NS>(s_mem + buf * BUF + sq.ctx % kPage * 128, kStick, here(lane));
       }
 
-      // The scores: sc[n][x] of row 16 (NR rq + n) + l16, token 16 TB tg + tok(x).
+      // The scores: sc[n][x] of row 16 n + l16, token 16 part + tok(x).
       float sc[NR][NT];
       auto tok = [&](int x, int ln) { return 16 * (x / 4) + 4 * (ln / 16) + x % 4; };
       {
@@ -493,7 +496,7 @@ __global__ __launch_bounds__(kParts * 64, 1) void latent_kernel(LatentArgs a) {
         uint32_t seen = ~0u;
         if constexpr (EDGE) {
           const int j0 = p * kPage + 16 * part - sq.ctx;
-          const int i = min(token_of_row(row0 + 16 * (n) + ln % 16), sq.n - 1);
+          const int i = min(token_of_row(row0 + 16 * n + ln % 16), sq.n - 1);
           seen = 0;
           if (a.mask) {
             const uint8_t* mask = a.mask + b * a.m_sb + max(i, 0) * a.m_si;
@@ -519,7 +522,7 @@ __global__ __launch_bounds__(kParts * 64, 1) void latent_kernel(LatentArgs a) {
           mx = fmaxf(mx, v);
         }
         mx = xor32_max(xor16_max(mx));
-        if (ln / 16 == n) s_max[part * ROWS + 16 * (n) + ln % 16] = mx;
+        if (ln / 16 == n) s_max[part * ROWS + 16 * n + ln % 16] = mx;
       }
       // Weights relative to the reference as it is.  They round to fp16 for the product (a
       // relative 2^-12 on average); their sum stays in fp32.
@@ -529,7 +532,7 @@ __global__ __launch_bounds__(kParts * 64, 1) void latent_kernel(LatentArgs a) {
         for (int n = 0; n < NR; ++n) {
           const float mu = m[n] == -INFINITY ? 0.f : m[n];  // a row that has attended nothing yet: weights 0
           add[n] = 0.f;
-          const int row = 16 * (n) + ln % 16;
+          const int row = 16 * n + ln % 16;
 #pragma unroll
           for (int x = 0; x < NT; x += 4) {
             f16x4 w4;
@@ -566,7 +569,7 @@ __global__ __launch_bounds__(kParts * 64, 1) void latent_kernel(LatentArgs a) {
           for (int x = 0; x < 16; ++x) o[dt][x] *= alpha;
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-          const float to = ref_of(16 * (n) + ln % 16);
+          const float to = ref_of(16 * n + ln % 16);
           l[n] *= factor(m[n], to);
           m[n] = to;
         }
@@ -613,7 +616,7 @@ __global__ __launch_bounds__(kParts * 64, 1) void latent_kernel(LatentArgs a) {
     for (int p = whole; p < p1; ++p) step(p, std::true_type{});
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      const int r = 16 * (n) + here(l16);
+      const int r = 16 * n + here(l16);
       const bool live = token_of_row(row0 + r) < sq.n;
       l[n] = xor32_sum(xor16_sum(l[n]));
       if (!live) l[n] = 0.f;

@@ -16,10 +16,11 @@
 // the next one between the second products of this one.  K is a tile ahead of V for it.
 // Few rows with many keys are split over the keys and joined by a second kernel.
 //
-// Measured: 4096 tokens x 32 heads x 128 features 215 us, 4 x 512 rows over 2000-8000 keys
-// 335 us, both 790 TFLOP/s.  A tile of 256 rows takes 2.2 us (1220 TFLOP/s) while some CUs are idle
-// and 2.5 with all at work: power bounds it (the same on zeros 169 and 265 us), then the
-// 9 us until a row block's first products.
+// Measured: 4096 tokens x 32 heads x 128 features 215 us, 4 x 512 rows over 2000-8000 keys 328-345
+// us, from device to device (770-810 TFLOP/s).  Counters of the latter: of the cycles in which the device has
+// any wavefronts the matrix cores are busy for 37 %, of those in which a SIMD has its own for 49 %
+// (row blocks end at different times: 77 %); wavefronts wait in 36 % of their cycles and have an instruction
+// that cannot issue in 24 %, 3 % for LDS.
 
 #include <hip/hip_runtime.h>
 
@@ -91,7 +92,7 @@ __global__ __launch_bounds__(W * 64, 2) void prompt_kernel(PromptArgs a) {
   // A (sequence, head) stays in one XCD, the row blocks of most keys first: begun last, they
   // would run on alone (4096 tokens x 32 heads 215 us; one (sequence, head) after the other 285).
   // Equal shares of all tiles, cut within row blocks and joined, measured no better (4 x 512 rows
-  // over 2000-8000 keys 338 us, this 335; 4096 tokens 240): with every CU at work the clock falls.
+  // over 2000-8000 keys 338 us, this 335; 4096 tokens 240): a tile then took longer.
   const uint32_t js = blockIdx.x >> 3, j = fdiv(js, a.by_splits), split = js - j * a.splits;
   const uint32_t block = fdiv(j, a.by_octets), pair = (j - block * ((a.pairs + 7) / 8)) * 8 + (blockIdx.x & 7);
   if (pair >= static_cast<uint32_t>(a.pairs)) return;

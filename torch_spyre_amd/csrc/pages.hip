@@ -12,9 +12,10 @@
 // Nothing that a call reads is written by it (fresh entries of the table lie
 // behind those that it reads), so a call is one launch: every workgroup sums the
 // sequences for itself and takes its share of the tokens and of the pages.
-// What bounds it: latency (lengths, sums, a table entry, a store) where tokens
-// are few; else its 12 bytes a token.  Measured: 64 sequences x 25 tokens 3.7 us, their
-// pages back 2.9; 256 prompts of 128 to 8192 tokens 10.5 (13 MB).
+// What bounds it: latency (lengths, sums, a table entry, a store).  Measured: 64 sequences x
+// 25 tokens 3.7 us, their pages back 2.9; 256 prompts of 128 to 8192 tokens 10.5 (13 MB, 2.6 at
+// a copy's rate): the sums of all lengths, and then for each token the sequence's lengths again before
+// its table or ring entry, four rounds of them to a thread.
 
 #include <hip/hip_runtime.h>
 

@@ -21,8 +21,8 @@
 // A workgroup that finds all flags finds the run and then the token where the sums pass
 // the limit: one launch, and no row is read twice but for that run.  What bounds it: one
 // row of the vocabulary a sequence (two with q), and for few sequences the chain of
-// loads.  Measured: 64 x 128000 fp32 tokens with q 22 us (65 MB, 3 TB/s), 1 x 32000 11 us,
-// trees of 25 over 16 x 100003 bf16 14 us.
+// loads.  Measured: 64 x 128000 fp32 tokens with q 22 us (65 MB, 3 TB/s, by loads of 4 bytes a
+// lane; wider ones were not tried), 1 x 32000 11 us, trees of 25 over 16 x 100003 bf16 14 us.
 
 #include <hip/hip_runtime.h>
 
