@@ -19,13 +19,13 @@
 // with Q in registers, the weights meet in LDS, and the second has 32 x 32 tiles of O in registers.
 //
 // Measured, rank 512 (a pass among others, from device to device): 32 sequences x 4096 tokens x 128
-// heads 62-65 us (36.5 GFLOP, 560-590 TFLOP/s; the first kernel 52-58, the join 9.8).  That kernel has
+// heads 61-65 us (36.5 GFLOP, 560-600 TFLOP/s; the first kernel 52-58, the join 9.8).  That kernel has
 // wavefronts on the device for 93000 cycles: 32.5 tiles of 32 tokens x 64 rows of 2130 each (0.85 us,
 // of which the matrix cores 0.45 and the loads' way into LDS as much), the start of a range 6 us, the
 // parts; the matrix cores are busy for 38 % of them.  What the rest of its time goes to, or whether the
 // clock falls, is not established.  16 x 500-6000 tokens x 1-7 new x 32 heads 46-48 (39-42 and 9.0;
 // 72000 cycles, 29 % busy); 64 x 128-16384 tokens x 16 heads 124 (629 MB; 117, 5.4 TB/s, and 7.3);
-// 1 x 700 x 16 heads 17.1-17.4: latency.
+// 1 x 700 x 16 heads 17.1-17.5: latency.
 
 #include <hip/hip_runtime.h>
 
